@@ -1,0 +1,64 @@
+/*
+ * oscar_operators.h -- C ABI of the operators around the OSCAR INT2 cache that have no
+ * counterpart in the reference, beside oscar_amd.h and in its manner: device pointers,
+ * strides, shapes and a HIP stream passed as void*; arguments are validated on the host;
+ * launches are asynchronous on `stream`; nothing is allocated; 0 or a negative errno-style
+ * status is returned, with the message in oscar_last_error().
+ *
+ * All entry points may be captured into a HIP graph.
+ */
+#ifndef OSCAR_OPERATORS_H
+#define OSCAR_OPERATORS_H
+
+#include "oscar_amd.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* ---- RMS norm of every query and key head with the position rotation ----------------
+ * For each row x of head_dim values (a token's head):
+ *   y = x / sqrt(mean(x^2) + eps) * (w + weight_offset)          (w = 1 where NULL)
+ * then, over its first rotary_dim values, pairs (a, b) turn by the token's angles:
+ *   (a, b) -> (a cos - b sin, b cos + a sin),
+ * a pair being (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when interleaved.  fp32
+ * throughout, rounded once to the rows' type. */
+typedef struct oscarop_norm_rope_args_v1 {
+  const void* q;                /* [num_tokens, num_q_heads, head_dim] */
+  int64_t q_stride_token;       /* elements; heads are head_dim apart */
+  int64_t num_q_heads;          /* 0: no queries */
+  const void* k;                /* [num_tokens, num_kv_heads, head_dim] */
+  int64_t k_stride_token;
+  int64_t num_kv_heads;         /* 0: no keys */
+  int64_t num_tokens;
+  int64_t head_dim;             /* 128 or 256 */
+  int32_t dtype;                /* enum oscar_dtype of q, k and the outputs */
+  const void* q_weight;         /* [head_dim], or NULL */
+  const void* k_weight;
+  int32_t weight_dtype;
+  float weight_offset;          /* 1 for weights stored around zero */
+  float eps;
+  const void* positions;        /* [num_tokens] device */
+  int32_t positions_int64;      /* 0: int32 */
+  /* [cos_sin_rows, rotary_dim], contiguous: row p holds the rotary_dim / 2 cosines of
+   * position p, then its sines.  A token whose position lies outside [0, cos_sin_rows)
+   * gets NaN rows. */
+  const void* cos_sin;
+  int32_t cos_sin_dtype;
+  int32_t interleaved;
+  int64_t cos_sin_rows;
+  int64_t rotary_dim;           /* a multiple of 16, <= head_dim */
+  /* outputs; q_out == q and k_out == k (with the same strides) work in place, any other
+   * overlap of inputs and outputs does not */
+  void* q_out;
+  int64_t q_out_stride_token;
+  void* k_out;
+  int64_t k_out_stride_token;
+} oscarop_norm_rope_args_v1;
+
+int oscarop_norm_rope_v1(const oscarop_norm_rope_args_v1* args, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* OSCAR_OPERATORS_H */

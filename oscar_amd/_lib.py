@@ -100,6 +100,18 @@ class StepArgs(C.Structure):
     ]
 
 
+class NormRopeArgs(C.Structure):
+    _fields_ = [
+        ("q", vp), ("q_stride_token", i64), ("num_q_heads", i64),
+        ("k", vp), ("k_stride_token", i64), ("num_kv_heads", i64),
+        ("num_tokens", i64), ("head_dim", i64), ("dtype", i32),
+        ("q_weight", vp), ("k_weight", vp), ("weight_dtype", i32), ("weight_offset", f32), ("eps", f32),
+        ("positions", vp), ("positions_int64", i32),
+        ("cos_sin", vp), ("cos_sin_dtype", i32), ("interleaved", i32), ("cos_sin_rows", i64), ("rotary_dim", i64),
+        ("q_out", vp), ("q_out_stride_token", i64), ("k_out", vp), ("k_out_stride_token", i64),
+    ]
+
+
 STEP_NOT_DECODE = 1
 
 # name -> (restype, argtypes); every symbol declared in include/oscar_amd.h
@@ -125,6 +137,11 @@ SIGNATURES = {
     "oscar_decode_step_v1": (C.c_int, [vp, C.POINTER(StepArgs), vp]),
 }
 
+# every symbol declared in include/oscar_operators.h
+OPERATOR_SIGNATURES = {
+    "oscarop_norm_rope_v1": (C.c_int, [C.POINTER(NormRopeArgs), vp]),
+}
+
 _LIB = None
 
 
@@ -142,7 +159,7 @@ def load() -> C.CDLL:
             f"{LIB_PATH} is missing: build it with `python -m oscar_amd.build` "
             "(no CPU fallback exists for the OSCAR HIP path)")
     lib = C.CDLL(str(LIB_PATH))
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in {**SIGNATURES, **OPERATOR_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

@@ -43,6 +43,26 @@ def _require_cuda(*tensors) -> None:
             raise RuntimeError("OSCAR HIP ops need device tensors (no CPU fallback)")
 
 
+def _one_device(*tensors) -> torch.device:
+    """The device that all the tensors given are on."""
+    _require_cuda(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise ValueError(f"OSCAR HIP ops need all tensors on one device, got {sorted(map(str, devices))}")
+    return devices.pop()
+
+
+def _launch(name: str, device: torch.device, *args) -> None:
+    """Call the entry point `name` on the device's current stream, with the device made the
+    current one (the library launches there)."""
+    call = getattr(_lib.load(), name)
+    if device.index is None or device.index == torch.cuda.current_device():
+        _lib.check(call(*args, C.c_void_p(_stream(device))), name)
+        return
+    with torch.cuda.device(device):
+        _lib.check(call(*args, C.c_void_p(_stream(device))), name)
+
+
 def cache_struct(k_cache: torch.Tensor, v_cache: torch.Tensor, head_dim: int) -> _lib.Cache:
     """Byte view of a packed cache pair [num_blocks, block_size, Hk, D] (int8 or bf16)."""
     k8, v8 = k_cache.view(torch.uint8), v_cache.view(torch.uint8)
@@ -317,6 +337,87 @@ def rotate(x: torch.Tensor, r: torch.Tensor, *, transpose=False, out_dtype=None,
     lib = _lib.load()
     _lib.check(lib.oscar_rotate_v1(C.byref(a), C.c_void_p(_stream(x.device))), "oscar_rotate_v1")
     return out
+
+
+# ------------------------------------------------------------------------ head norms and rotation
+def _aligned(x: torch.Tensor) -> torch.Tensor:
+    """x contiguous and 16-byte aligned."""
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
+def _head_rows(x: torch.Tensor, name: str) -> torch.Tensor:
+    """x [N, H, D] as the kernel reads it: heads next to each other, 16-byte aligned rows."""
+    if x.ndim != 3 or x.shape[2] not in (128, 256):
+        raise ValueError(f"{name} must be [tokens, heads, 128 or 256]")
+    size = x.element_size()
+    if x.stride(2) != 1 or x.shape[1] > 1 and x.stride(1) != x.shape[2] or x.data_ptr() % 16 \
+            or x.shape[0] > 1 and x.stride(0) * size % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def norm_rope(q, k, positions, cos_sin, *, q_weight=None, k_weight=None, eps=1e-6, weight_offset=0.0,
+              interleaved=False, q_out=None, k_out=None):
+    """RMS norm of every query and key head, then the position rotation, in one launch.
+
+    q [N, Hq, D] and k [N, Hk, D] of one type (bf16 / fp16 / fp32; either may be None), as
+    views of the projection's rows if they are.  positions [N] int32 or int64; cos_sin
+    [P, R]: row p holds the R / 2 cosines of position p, then its sines (R a multiple of
+    16, at most D; values past R are only normed).  Per row of D values
+    y = x / sqrt(mean(x^2) + eps) * (weight + weight_offset), weights [D] or None (no
+    gain); pairs (i, i + R / 2), or (2 i, 2 i + 1) if interleaved, turn by the angles.
+    fp32 throughout, rounded once.  A position outside the table gives NaN rows.
+
+    Returns (q_out, k_out): new tensors, or the ones given; q_out=q and k_out=k work in
+    place.
+    """
+    given = [t for t in (q, k) if t is not None]
+    if not given:
+        raise ValueError("norm_rope needs queries or keys")
+    dev = _one_device(q, k, positions, cos_sin, q_weight, k_weight, q_out, k_out)
+    dtype, n, d = given[0].dtype, given[0].shape[0], given[0].shape[-1]
+    if dtype not in _DTYPES or any(t.dtype != dtype or t.shape[0] != n or t.shape[-1] != d for t in given):
+        raise ValueError("q and k must share a float dtype, the token count and the head width")
+    if positions.shape != (n,) or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError("positions must be [tokens] int32 or int64")
+    if cos_sin.ndim != 2 or cos_sin.dtype not in _DTYPES or cos_sin.shape[1] % 16 or not 16 <= cos_sin.shape[1] <= d:
+        raise ValueError("cos_sin must be a float [positions, R] table, R a multiple of 16 up to the head width")
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    if any(w.shape != (d,) or w.dtype not in _DTYPES or w.dtype != weights[0].dtype for w in weights):
+        raise ValueError("the norm weights must be [head width] of one float dtype")
+    positions, cos_sin = positions.contiguous(), _aligned(cos_sin)
+    a = _lib.NormRopeArgs()
+    outs, keep = [], [positions, cos_sin]
+    for name, x, weight, out in (("q", q, q_weight, q_out), ("k", k, k_weight, k_out)):
+        if x is None:
+            outs.append(None)
+            continue
+        rows = _head_rows(x, name)
+        if out is None:
+            out = torch.empty(x.shape, dtype=dtype, device=dev)
+        elif out.shape != x.shape or out.dtype != dtype or _head_rows(out, name) is not out:
+            raise ValueError(f"{name}_out must have {name}'s shape and type, its heads next to each other and "
+                             "16-byte aligned rows")
+        if weight is not None:
+            weight = _aligned(weight)
+            setattr(a, f"{name}_weight", weight.data_ptr())
+        heads = "num_q_heads" if name == "q" else "num_kv_heads"
+        setattr(a, name, rows.data_ptr())
+        setattr(a, f"{name}_stride_token", rows.stride(0) if n > 1 else x.shape[1] * d)
+        setattr(a, heads, x.shape[1])
+        setattr(a, f"{name}_out", out.data_ptr())
+        setattr(a, f"{name}_out_stride_token", out.stride(0) if n > 1 else x.shape[1] * d)
+        outs.append(out)
+        keep += [rows, weight]
+    a.num_tokens, a.head_dim, a.dtype = n, d, _DTYPES[dtype]
+    a.weight_dtype = _DTYPES[weights[0].dtype] if weights else OSCAR_F32
+    a.weight_offset, a.eps = float(weight_offset), float(eps)
+    a.positions, a.positions_int64 = positions.data_ptr(), int(positions.dtype == torch.int64)
+    a.cos_sin, a.cos_sin_dtype, a.interleaved = cos_sin.data_ptr(), _DTYPES[cos_sin.dtype], int(bool(interleaved))
+    a.cos_sin_rows, a.rotary_dim = cos_sin.shape
+    _launch("oscarop_norm_rope_v1", dev, C.byref(a))
+    return tuple(outs)
 
 
 # ------------------------------------------------------------------------ decode attention
