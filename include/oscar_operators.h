@@ -5,7 +5,7 @@
  * launches are asynchronous on `stream`; nothing is allocated; 0 or a negative errno-style
  * status is returned, with the message in oscar_last_error().
  *
- * All entry points may be captured into a HIP graph.
+ * All entry points but oscarop_decode_step_v1 may be captured into a HIP graph.
  */
 #ifndef OSCAR_OPERATORS_H
 #define OSCAR_OPERATORS_H
@@ -15,6 +15,24 @@
 #ifdef __cplusplus
 extern "C" {
 #endif
+
+/* ---- attention scores ----------------------------------------------------------------
+ * The score of key t for a query at position p (0-based in its request) and head h, where
+ * s = scale q.k is the plain one:
+ *   s' = soft_cap tanh(s / soft_cap) + alibi_slopes[h] (t - p)
+ * soft_cap 0 leaves s as it is, a NULL alibi_slopes adds nothing.  Keys a query does not
+ * see stay unseen whatever their score. */
+typedef struct oscarop_score_v1 {
+  float soft_cap;               /* finite, >= 0 */
+  const float* alibi_slopes;    /* [num_q_heads] fp32 device, or NULL */
+} oscarop_score_v1;
+
+/* oscar_attn_decode_v1, oscar_attn_prefill_v1 and oscar_decode_step_v1 with these scores
+ * (score == NULL, or no cap and no slopes: the plain calls).  out, lse and every rule of
+ * the plain calls are the same otherwise. */
+int oscarop_attn_decode_v1(const oscar_attn_args_v1* args, const oscarop_score_v1* score, void* stream);
+int oscarop_attn_prefill_v1(const oscar_prefill_args_v1* args, const oscarop_score_v1* score, void* stream);
+int oscarop_decode_step_v1(oscar_context_v1* ctx, oscar_step_args_v1* args, const oscarop_score_v1* score, void* stream);
 
 /* ---- RMS norm of every query and key head with the position rotation ----------------
  * For each row x of head_dim values (a token's head):

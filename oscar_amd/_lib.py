@@ -100,6 +100,10 @@ class StepArgs(C.Structure):
     ]
 
 
+class Score(C.Structure):
+    _fields_ = [("soft_cap", f32), ("alibi_slopes", vp)]
+
+
 class NormRopeArgs(C.Structure):
     _fields_ = [
         ("q", vp), ("q_stride_token", i64), ("num_q_heads", i64),
@@ -139,6 +143,9 @@ SIGNATURES = {
 
 # every symbol declared in include/oscar_operators.h
 OPERATOR_SIGNATURES = {
+    "oscarop_attn_decode_v1": (C.c_int, [C.POINTER(AttnArgs), C.POINTER(Score), vp]),
+    "oscarop_attn_prefill_v1": (C.c_int, [C.POINTER(PrefillArgs), C.POINTER(Score), vp]),
+    "oscarop_decode_step_v1": (C.c_int, [vp, C.POINTER(StepArgs), C.POINTER(Score), vp]),
     "oscarop_norm_rope_v1": (C.c_int, [C.POINTER(NormRopeArgs), vp]),
 }
 

@@ -215,6 +215,19 @@ class OscarAttentionBackendImpl(BaseAttentionImpl):  # type: ignore[misc,valid-t
     def _oscar(self) -> OscarConfig:
         return self._oscar_cfg
 
+    # ------------------------------------------------------------------ scores
+    def _score_args(self, device) -> dict:
+        """The cap and the distance bias that the model gives this layer (the impl's own
+        logits_soft_cap and alibi_slopes; empty for the plain product).  The slopes move to
+        the device as fp32 once."""
+        cap = getattr(self, "logits_soft_cap", None) or 0.0
+        slopes = getattr(self, "alibi_slopes", None)
+        if not cap and slopes is None:
+            return {}
+        if slopes is not None:
+            slopes = self.alibi_slopes = torch.as_tensor(slopes, dtype=torch.float32, device=device).contiguous()
+        return dict(soft_cap=float(cap), alibi_slopes=slopes)
+
     # ------------------------------------------------------------------ geometry
     def _set_caches(self, kv_cache) -> None:
         """Take the (K, V) pair or a stacked [2, ...] tensor; check the slot geometry
@@ -395,7 +408,10 @@ class OscarAttentionBackendImpl(BaseAttentionImpl):  # type: ignore[misc,valid-t
         ctx = ops.DeviceContext.get(query.device)
         ws = scratch.step_workspace(0)  # shared by every layer: the stream's current buffer
         a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        rc = ops.decode_step(ctx, a, stream, scratch)
+        score = self._score_args(query.device)
+        if score:
+            score = ops.score_struct(score["soft_cap"], score["alibi_slopes"], hq, query.device)
+        rc = ops.decode_step(ctx, a, stream, scratch, score or None)
         if rc != 0:
             return False
         if n < query.shape[0]:
@@ -550,9 +566,10 @@ class OscarAttentionBackendImpl(BaseAttentionImpl):  # type: ignore[misc,valid-t
         if actual == 0:
             return output
         out3 = output.view(-1, hq, d)
+        score = self._score_args(dev)
         for i in batch.fresh:
             a, b = batch.qsl[i], batch.qsl[i + 1]
-            ops.attention_prefill(q3[a:b], k3[a:b], v3[a:b], self.scale, head_dim=d, out=out3[a:b])
+            ops.attention_prefill(q3[a:b], k3[a:b], v3[a:b], self.scale, head_dim=d, out=out3[a:b], **score)
         if not (batch.short or batch.long):
             return output
         rk, rv = self._layer_rots(layer, dev)
@@ -571,19 +588,19 @@ class OscarAttentionBackendImpl(BaseAttentionImpl):  # type: ignore[misc,valid-t
         if plan is not None:
             if route["identity"]:
                 ops.attention_decode(q_rot, k_rot, v_rot, self.key_cache, self.value_cache, table,
-                                     plan, self.scale, stage, head_dim=d, out_rot=out_rot, lse=lse)
+                                     plan, self.scale, stage, head_dim=d, out_rot=out_rot, lse=lse, **score)
             elif route["span"] is not None:
                 i0, i1, a, b = route["span"]
                 cut = (lambda t: None if t is None else t[a:b])
                 ops.attention_decode(cut(q_rot), cut(k_rot), cut(v_rot), self.key_cache,
                                      self.value_cache, table[i0:i1], plan, self.scale, stage,
-                                     head_dim=d, out_rot=out_rot[a:b], lse=lse[a:b])
+                                     head_dim=d, out_rot=out_rot[a:b], lse=lse[a:b], **score)
             else:
                 ids, req = route["index_dev"]
                 pick = (lambda t: None if t is None else torch.index_select(t, 0, ids))
                 o, l_ = ops.attention_decode(pick(q_rot), pick(k_rot), pick(v_rot), self.key_cache,
                                              self.value_cache, torch.index_select(table, 0, req),
-                                             plan, self.scale, stage, head_dim=d)
+                                             plan, self.scale, stage, head_dim=d, **score)
                 out_rot.index_copy_(0, ids, o)
                 lse.index_copy_(0, ids, l_)
         if has_new:
@@ -592,7 +609,7 @@ class OscarAttentionBackendImpl(BaseAttentionImpl):  # type: ignore[misc,valid-t
                 ops.attention_prefill(q_rot[a:b], k_rot[a:b], v_rot[a:b], self.scale, head_dim=d,
                                       history=batch.seqs[i] - (b - a), k_cache=self.key_cache,
                                       v_cache=self.value_cache, block_table_row=table[i],
-                                      stage=stage, out=out_rot[a:b], lse=lse[a:b])
+                                      stage=stage, out=out_rot[a:b], lse=lse[a:b], **score)
         if batch.decode_only:
             ops.rotate(out_rot, rv, transpose=True, out_dtype=query.dtype, out=out3[:actual])
         elif cached_span is not None:

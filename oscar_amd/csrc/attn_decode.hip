@@ -53,6 +53,7 @@
 #include <vector>
 
 #include "common.h"
+#include "score.h"
 #include "store_quant.h"
 
 namespace oscar {
@@ -94,6 +95,7 @@ struct AttnParams {
   int group;     // Hq / Hk
   float* part_o;   // [num_items][32 * D] in MFMA register order
   float* part_lse; // [num_items][32]
+  Score sc;        // SC != 0
 };
 
 __device__ __forceinline__ f16x8 as_f16x8(u32x4 v) { return __builtin_bit_cast(f16x8, v); }
@@ -245,7 +247,10 @@ struct TileRegs {
   int blk;              // physical block of the tile (0 off the history)
 };
 
-template <int D, int QT>
+// SC: the score function (score.h).  Distance-biased scores grow towards the query, so the
+// scored variants walk an item's tiles from its last to its first: the reference maximum
+// of a row settles on the near tiles instead of moving (and O with it) tile by tile.
+template <int D, int QT, int SC>
 __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   using C = Cfg<D>;
   using QV = typename QVec<QT>::type;  // one MFMA operand in the query dtype
@@ -282,7 +287,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   }
   const int lim0 = seq - nq + 1;                              // first key masked for a row
   const int fast_end = hist < lim0 ? hist : lim0;             // fast tiles end at or before
-  auto tile_t0 = [&](int j) { return (first + stride * j) * kTile; };  // first key of item tile j
+  // first key of item tile j
+  auto tile_t0 = [&](int j) { return (first + stride * (SC ? count - 1 - j : j)) * kTile; };
 
   // LDS
   __shared__ int32_t s_blk[kMaxPages];                 // block ids of the item's pages
@@ -422,6 +428,14 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
     }
   }
   const float c_score = A.scale * kLog2e;  // scores in log2 units
+  // SC: this lane's row's slope, and its distance to key 4 g (register r's key of a tile at
+  // t0 lies out_tok(r, 0) + t0 further)
+  float slope2 = 0.f;
+  int near = 0;
+  if constexpr (SC != 0) {
+    slope2 = slope2_of(P.sc, kvh * G + (row_ok ? n % G : 0));
+    near = 4 * g - (seq - nq + (row_ok ? n / G : 0));
+  }
   __syncthreads();
   // Q^T operands are read from LDS at each use (volatile: kept out of registers)
   auto qop = [&](int j) { return __builtin_bit_cast(QV, *(const volatile u32x4*)&s_q[j][lane]); };
@@ -628,7 +642,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
         for (int r = 0; r < 16; ++r) {
           const int tp = t0 + out_tok(r, g);
           const bool vis = row_ok && tp < limit;  // limit <= seq
-          xs[r] = vis ? S[r] * c_score : -INFINITY;
+          if constexpr (SC == 0) xs[r] = vis ? S[r] * c_score : -INFINITY;
+          else xs[r] = vis ? score2<SC>(P.sc, S[r], slope2, (float)(near + t0) + out_tok(r, 0)) : -INFINITY;
           mx = fmaxf(mx, xs[r]);
         }
         mx = fmaxf(mx, swap_halves(mx));
@@ -715,13 +730,19 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   // O^T += V^T P'^T.
   // P' = p * s_V (fp16) is the B operand; V^T comes from LDS by transpose reads as
   // the subnormals c * 2^(2k-24); sum p and sum p * z_V accumulate on the VALU.
-  auto pv_tile = [&](const f32x16& S) {
+  auto pv_tile = [&](f32x16& S, int t0) {
+    if constexpr (SC != 0) {
+#pragma unroll
+      for (int r2 = 0; r2 < 16; ++r2)
+        S[r2] = score2<SC>(P.sc, S[r2], slope2, (float)(near + t0) + out_tok(r2, 0));
+    }
     wait_lds();
     __builtin_amdgcn_wave_barrier();
     float mx = -INFINITY;
 #pragma unroll
     for (int r2 = 0; r2 < 16; ++r2) mx = fmaxf(mx, S[r2]);
-    mx = fmaxf(mx, swap_halves(mx)) * c_score;  // c_score > 0
+    mx = fmaxf(mx, swap_halves(mx));
+    if constexpr (SC == 0) mx *= c_score;  // c_score > 0
     update_max(mx);
     const float nm = -m_run;
     u32x4 pb[2];
@@ -734,8 +755,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
       for (int i = 0; i < 4; i += 2) {
         const int r0 = 4 * q4 + i;
         // p <= 2^kLazy: no range reduction needed for v_exp_f32
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(S[r0], c_score, nm));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(S[r0 + 1], c_score, nm));
+        const float p0 = __builtin_amdgcn_exp2f(SC ? S[r0] + nm : fmaf(S[r0], c_score, nm));
+        const float p1 = __builtin_amdgcn_exp2f(SC ? S[r0 + 1] + nm : fmaf(S[r0 + 1], c_score, nm));
         lsum += p0 + p1;
         zsum = fmaf(p0, zv[i], fmaf(p1, zv[i + 1], zsum));
         const f16x2 h = {(_Float16)(p0 * sv[i]), (_Float16)(p1 * sv[i + 1])};
@@ -812,17 +833,19 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
     {
       const bool fast = jA < count && !slow_bit(jA);
       f32x16 S;
+      const int t0 = tile_t0(jA);
       if (fast) qk_tile(RA, S);
       jA = take();
       load_next(jA, RA);
-      if (fast) pv_tile(S);
+      if (fast) pv_tile(S, t0);
     }
     const bool fast = jB < count && !slow_bit(jB);
     f32x16 S;
+    const int t0 = tile_t0(jB);
     if (fast) qk_tile(RB, S);
     jB = take();
     load_next(jB, RB);
-    if (fast) pv_tile(S);
+    if (fast) pv_tile(S, t0);
   }
 
   // ---- fast-tile accumulators to value units: O = O * 2^(24-2k) / v_fac + z
@@ -1048,12 +1071,13 @@ __global__ __launch_bounds__(kMergeWaves * 64) void attn_merge_kernel(AttnParams
 }
 
 template <int D>
-int launch_decode(const AttnParams& p, hipStream_t s, const StoreParams& sp) {
+int launch_decode(const AttnParams& p, int sc, hipStream_t s, const StoreParams& sp) {
   if (p.a.phases != 2) {
-    if (p.a.q_dtype == OSCAR_F16)
-      hipLaunchKernelGGL((attn_main_kernel<D, OSCAR_F16>), dim3(p.a.num_items), dim3(kThreads), 0, s, p);
-    else
-      hipLaunchKernelGGL((attn_main_kernel<D, OSCAR_BF16>), dim3(p.a.num_items), dim3(kThreads), 0, s, p);
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(p.a.num_items), dim3(kThreads), 0, s, p); };
+    const bool f16 = p.a.q_dtype == OSCAR_F16;
+    if (sc == 0) f16 ? launch(attn_main_kernel<D, OSCAR_F16, 0>) : launch(attn_main_kernel<D, OSCAR_BF16, 0>);
+    else if (sc == 1) f16 ? launch(attn_main_kernel<D, OSCAR_F16, 1>) : launch(attn_main_kernel<D, OSCAR_BF16, 1>);
+    else f16 ? launch(attn_main_kernel<D, OSCAR_F16, 2>) : launch(attn_main_kernel<D, OSCAR_BF16, 2>);
     OSCAR_CHECK_LAUNCH("attn_main_kernel");
   }
   if (p.a.phases != 1) {
@@ -1381,8 +1405,12 @@ int check_args(const oscar_attn_args_v1& a, const char* name) {
 // store enqueued once the decode's arguments have passed, deferred (its quantization in
 // the merge launch) when it is a small call.
 int launch_checked(const oscar_attn_args_v1& a, const char* name, void* partials, int64_t partial_bytes,
-                   hipStream_t s, const oscar_store_args_v1* store = nullptr, const MetaCopy* meta = nullptr) {
+                   hipStream_t s, const oscarop_score_v1* score = nullptr, const oscar_store_args_v1* store = nullptr,
+                   const MetaCopy* meta = nullptr) {
   const int64_t D = a.cache.head_dim;
+  AttnParams p{};
+  const int sc = score_of(score, a.scale, &p.sc);
+  if (sc < 0) return fail(-22, "%s: soft_cap must be a finite number, 0 for none", name);
   if (D != 128 && D != 256) return fail(-22, "%s: head_dim %lld unsupported", name, (long long)D);
   if (a.num_items <= 0 || a.num_groups <= 0) {
     StoreParams sp{};
@@ -1394,7 +1422,6 @@ int launch_checked(const oscar_attn_args_v1& a, const char* name, void* partials
   if (partial_bytes < need)
     return fail(-22, "%s: workspace of %lld bytes < %lld for %d items", name, (long long)partial_bytes,
                 (long long)need, a.num_items);
-  AttnParams p{};
   p.a = a;
   p.has_stage = a.staging != nullptr;
   if (a.staging) p.st = *a.staging;
@@ -1409,7 +1436,7 @@ int launch_checked(const oscar_attn_args_v1& a, const char* name, void* partials
     const int rc = store_launch(store, s, a.phases == 0, name, &sp, meta);
     if (rc != 0) return rc;
   }
-  return D == 256 ? launch_decode<256>(p, s, sp) : launch_decode<128>(p, s, sp);
+  return D == 256 ? launch_decode<256>(p, sc, s, sp) : launch_decode<128>(p, sc, s, sp);
 }
 
 // ---- the entry point that allocates nothing: item partials in a file-scope device
@@ -1453,17 +1480,23 @@ extern "C" int oscar_attn_decode_v1(const oscar_attn_args_v1* args, void* stream
                         (hipStream_t)stream);
 }
 
-int oscar::decode_write_launch(const oscar_store_args_v1& store, const oscar_attn_args_v1& attn, const MetaCopy* meta,
-                               void* stream) {
+extern "C" int oscarop_attn_decode_v1(const oscar_attn_args_v1* args, const oscarop_score_v1* score, void* stream) {
+  if (!args) return fail(-22, "oscarop_attn_decode_v1: null args");
+  return launch_checked(*args, "oscarop_attn_decode_v1", args->workspace, args->workspace_bytes, (hipStream_t)stream,
+                        score);
+}
+
+int oscar::decode_write_launch(const oscar_store_args_v1& store, const oscar_attn_args_v1& attn,
+                               const oscarop_score_v1* score, const MetaCopy* meta, void* stream) {
   return launch_checked(attn, "oscar_decode_write_v1", attn.workspace, attn.workspace_bytes, (hipStream_t)stream,
-                        &store, meta);
+                        score, &store, meta);
 }
 
 extern "C" int oscar_decode_write_v1(const oscar_store_args_v1* store, const oscar_attn_args_v1* attn,
                                      void* stream) {
   if (!store || !attn) return fail(-22, "oscar_decode_write_v1: null args");
   return launch_checked(*attn, "oscar_decode_write_v1", attn->workspace, attn->workspace_bytes, (hipStream_t)stream,
-                        store);
+                        nullptr, store);
 }
 
 extern "C" int oscar_attn_decode_static_v1(const oscar_attn_args_v1* args, void* stream) {

@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "score.h"
 
 namespace oscar {
 
@@ -120,6 +121,7 @@ struct PrefillParams {
   float* part_o;       // [slot][Hk][kRows / 32][D / 32][4][64][4] normalised partial O of the split tiles'
                        // chunks, as the MFMA results lie (32 rows x 32 columns per 4 x 64 x 4)
   float* part_lse;     // [slot][Hk][kRows] log2-domain LSE of each partial
+  Score sc;            // SC != 0
 };
 
 // key tiles seen by the last query of a tile ending at chunk token q1
@@ -313,7 +315,9 @@ __device__ __forceinline__ void hold_acc(f32x16 (&o)[N]) {
 // other launches: 1880 us before (four waves of 32 rows, tiles through registers, one phase
 // after the other), 1155 to 1200 us now, 0.98 PFLOP/s; a large library bf16 product reaches
 // 1.2 to 1.36 on this card.
-template <int D, int QT, int NB>
+// SC: the score function (score.h); its work per score, three times the plain product's,
+// takes the room beside the PV MFMAs that the second row block would need.
+template <int D, int QT, int NB, int SC>
 __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(PrefillParams P) {
   using QV = typename QVec<QT>::type;    // one MFMA operand in the query dtype
   const oscar_prefill_args_v1& A = P.a;
@@ -479,6 +483,23 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
       qreg[nb][j] = __builtin_bit_cast(QV, r.ok ? *(const u32x4*)(qrow + 16 * j + 8 * g) : u32x4{0u, 0u, 0u, 0u});
   }
   const float c = A.scale * kLog2e;
+  // SC: the rows' slopes (log2 units) and positions, and the bias of a tile's first key
+  float slope2[NB] = {}, row_pos[NB] = {}, bias0[NB] = {};
+  if constexpr (SC != 0) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const Row r = row_of(nb);
+      slope2[nb] = slope2_of(P.sc, r.head);
+      row_pos[nb] = (float)(hist + r.qi);
+    }
+  }
+  auto at_tile = [&](int kt) __attribute__((always_inline)) {
+    if constexpr (SC != 0) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+        bias0[nb] = slope2[nb] * ((float)(kt * kKeys + 4 * (int)(ulane >> 5)) - row_pos[nb]);
+    }
+  };
 
   float m_run[NB], l_run[NB];
   f32x16 O[NB][D / 32];
@@ -581,8 +602,11 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) asm volatile("s_nop 15" : "+v"(S[nb]));
   };
-  // masked keys get -inf scores (boundary tiles only).  Padding rows have zero queries
-  // and are never written, so they need no mask.
+  // masked keys get -inf scores (boundary tiles only); before a cap, which would make a
+  // finite score of it, the lowest number stands for that (a product that overflows is -inf
+  // and capped).
+  constexpr float kMasked = SC == 2 ? -3.402823466e38f : -INFINITY;
+  // Padding rows have zero queries and are never written, so they need no mask.
   const int all_see = (int)(hist + q0 + 1);  // keys visible to every row of the wave's tile
   auto mask = [&](int kt) __attribute__((always_inline)) {
     const int k0 = kt * kKeys;
@@ -592,18 +616,31 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
     for (int nb = 0; nb < NB; ++nb) {
       const int lim = (int)(hist + row_of(nb).qi + 1) - k0 - 4 * ml;  // keys of the tile visible to this row
 #pragma unroll
-      for (int r = 0; r < 16; ++r) S[nb][r] = 8 * (r >> 2) + (r & 3) >= lim ? -INFINITY : S[nb][r];
+      for (int r = 0; r < 16; ++r) S[nb][r] = 8 * (r >> 2) + (r & 3) >= lim ? kMasked : S[nb][r];
     }
   };
   // p = 2^(S c - m) of element r (exp2 of -inf is 0; rows with no key yet have m = -inf and p = 0)
-  auto prob = [&](int nb, int r, float nm) __attribute__((always_inline)) { return __builtin_amdgcn_exp2f(fmaf(S[nb][r], c, nm)); };
+  // SC: the score of element r (log2 units; -inf where masked) plus x
+  auto score = [&](int nb, int r, float x) __attribute__((always_inline)) {
+    const float b = fmaf(slope2[nb], (float)(8 * (r >> 2) + (r & 3)), bias0[nb] + x);
+    if constexpr (SC == 1) return fmaf(S[nb][r], P.sc.scale2, b);
+    const float y = capped2(P.sc, S[nb][r]) + b;
+    return S[nb][r] == kMasked ? -INFINITY : y;
+  };
+  auto prob = [&](int nb, int r, float nm) __attribute__((always_inline)) {
+    if constexpr (SC != 0) return __builtin_amdgcn_exp2f(score(nb, r, nm));
+    else return __builtin_amdgcn_exp2f(fmaf(S[nb][r], c, nm));
+  };
   auto neg_m = [&](int nb) __attribute__((always_inline)) { return m_run[nb] == -INFINITY ? 0.f : -m_run[nb]; };
   auto row_max = [&](int nb) __attribute__((always_inline)) {  // of the scores, over both halves of the row
     float mx = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[nb][r]);
+    for (int r = 0; r < 16; ++r) {
+      if constexpr (SC != 0) mx = fmaxf(mx, score(nb, r, 0.f));
+      else mx = fmaxf(mx, S[nb][r]);
+    }
     auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-    return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * c;  // c > 0
+    return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * (SC ? 1.f : c);  // c > 0
   };
   auto put_p = [&](int nb, int r, float p0, float p1) __attribute__((always_inline)) {
     unsigned w = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{p0, p1}, f16x2));
@@ -680,6 +717,7 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
   k_ahead(k_tile(0));
   qk(kb, k_tile(0), v_tile(0), v_tile(0), Tile{}, std::integral_constant<bool, QT == OSCAR_BF16>{}, std::false_type{});
   mask(kb);
+  at_tile(kb);
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) m_run[nb] = row_max(nb);
   softmax();
@@ -711,6 +749,7 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
     // landed (kt + 2's DMAs are outstanding)
     tile_barrier<2 * NDMA>();
     mask(kt);
+    at_tile(kt);
     pv(v_tile(vr), k_tile(next(k1, NK)), std::true_type{});
     kr = k1;
     vr = v1;
@@ -872,14 +911,14 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams P) {
 // there.
 constexpr int64_t kPairUnits = kSplitCUs + kSplitCUs / 8;
 template <int D, int QT>
-void launch_prefill(const PrefillParams& p, dim3 grid, bool pairs, hipStream_t s) {
+void launch_prefill(const PrefillParams& p, int sc, dim3 grid, bool pairs, hipStream_t s) {
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, p); };
+  if (sc == 1) return launch(prefill_kernel<D, QT, 1, 1>);
+  if (sc == 2) return launch(prefill_kernel<D, QT, 1, 2>);
   if constexpr (D == 256) {
-    if (pairs) {
-      hipLaunchKernelGGL((prefill_kernel<D, QT, 2>), grid, dim3(kThreads), 0, s, p);
-      return;
-    }
+    if (pairs) return launch(prefill_kernel<D, QT, 2, 0>);
   }
-  hipLaunchKernelGGL((prefill_kernel<D, QT, 1>), grid, dim3(kThreads), 0, s, p);
+  launch(prefill_kernel<D, QT, 1, 0>);
 }
 
 }  // namespace
@@ -914,39 +953,53 @@ extern "C" int oscar_prefill_plan_v1(int64_t history, int64_t num_tokens, int64_
   return 0;
 }
 
+static int prefill_launch(const oscar_prefill_args_v1* args, const oscarop_score_v1* score, const char* name,
+                          void* stream);
+
 extern "C" int oscar_attn_prefill_v1(const oscar_prefill_args_v1* args, void* stream) {
-  if (!args) return fail(-22, "oscar_attn_prefill_v1: null args");
+  return prefill_launch(args, nullptr, "oscar_attn_prefill_v1", stream);
+}
+
+extern "C" int oscarop_attn_prefill_v1(const oscar_prefill_args_v1* args, const oscarop_score_v1* score, void* stream) {
+  return prefill_launch(args, score, "oscarop_attn_prefill_v1", stream);
+}
+
+static int prefill_launch(const oscar_prefill_args_v1* args, const oscarop_score_v1* score, const char* name,
+                          void* stream) {
+  if (!args) return fail(-22, "%s: null args", name);
   const oscar_prefill_args_v1& a = *args;
   if (a.num_tokens == 0) return 0;
   const int64_t D = a.head_dim;
-  if (D != 128 && D != 256) return fail(-22, "oscar_attn_prefill_v1: head_dim %lld unsupported", (long long)D);
+  if (D != 128 && D != 256) return fail(-22, "%s: head_dim %lld unsupported", name, (long long)D);
   if (!a.q || !a.k || !a.v || !a.out || a.num_tokens < 0 || a.num_kv_heads < 1 ||
       a.num_q_heads % a.num_kv_heads)
-    return fail(-22, "oscar_attn_prefill_v1: invalid arguments");
+    return fail(-22, "%s: invalid arguments", name);
   if (a.q_dtype != OSCAR_BF16 && a.q_dtype != OSCAR_F16)
-    return fail(-22, "oscar_attn_prefill_v1: q_dtype must be OSCAR_BF16 or OSCAR_F16");
+    return fail(-22, "%s: q_dtype must be OSCAR_BF16 or OSCAR_F16", name);
   const int G = (int)(a.num_q_heads / a.num_kv_heads);
-  if (G > kRows) return fail(-22, "oscar_attn_prefill_v1: more than %d query heads per KV head", kRows);
-  if (a.history < 0) return fail(-22, "oscar_attn_prefill_v1: negative history");
+  if (G > kRows) return fail(-22, "%s: more than %d query heads per KV head", name, kRows);
+  if (a.history < 0) return fail(-22, "%s: negative history", name);
   if (a.history > 0 && (!a.cache.k || !a.cache.v || !a.block_table_row || a.cache.head_dim != D ||
                         a.cache.block_size < 1))
-    return fail(-22, "oscar_attn_prefill_v1: history needs the cache and the block-table row");
+    return fail(-22, "%s: history needs the cache and the block-table row", name);
   // streaming_attention.py:51-53
   if (a.history > 0 && (a.history + a.cache.block_size - 1) / a.cache.block_size > a.block_table_cols)
-    return fail(-22, "oscar_attn_prefill_v1: Block table cannot cover the history");
+    return fail(-22, "%s: Block table cannot cover the history", name);
   // q/k/v rows and the history workspace are read as 16-byte vectors
   if ((((uintptr_t)a.q) & 15) || (((uintptr_t)a.k) & 15) || (((uintptr_t)a.v) & 15) ||
       ((a.q_stride_token * 2) & 15) || ((a.kv_stride_token * 2) & 15))
-    return fail(-22, "oscar_attn_prefill_v1: q/k/v rows must be 16-byte aligned");
+    return fail(-22, "%s: q/k/v rows must be 16-byte aligned", name);
   // the prefill kernel addresses history and chunk rows with 32-bit element offsets
   if ((a.history + 64) * a.num_kv_heads * D >= (1ll << 31) ||
       (a.num_tokens + 64) * a.kv_stride_token >= (1ll << 31))
-    return fail(-22, "oscar_attn_prefill_v1: history or chunk too large for one call");
+    return fail(-22, "%s: history or chunk too large for one call", name);
   const int64_t need = oscar_prefill_workspace_bytes_v1(a.history, a.num_kv_heads, D);
   if (a.history > 0 &&
       (a.workspace == nullptr || a.workspace_bytes < need || (((uintptr_t)a.workspace) & 15)))
-    return fail(-22, "oscar_attn_prefill_v1: 16-byte aligned workspace of %lld bytes required", (long long)need);
+    return fail(-22, "%s: 16-byte aligned workspace of %lld bytes required", name, (long long)need);
   PrefillParams p{};
+  const int sc = score_of(score, a.scale, &p.sc);
+  if (sc < 0) return fail(-22, "%s: soft_cap must be a finite number, 0 for none", name);
   p.a = a;
   p.has_stage = a.staging != nullptr;
   if (a.staging) p.st = *a.staging;
@@ -983,16 +1036,16 @@ extern "C" int oscar_attn_prefill_v1(const oscar_prefill_args_v1* args, void* st
     OSCAR_CHECK_LAUNCH("history_bf16_kernel");
   }
   const int units = p.split ? sp.units : p.ntq;
-  const bool pairs = D == 256 && units * a.num_kv_heads > kPairUnits;
+  const bool pairs = D == 256 && sc == 0 && units * a.num_kv_heads > kPairUnits;
   for (int c = 0; c < p.chunks; ++c) p.pbase[c + 1] = p.pbase[c] + (sp.base[c + 1] - sp.base[c] + 1) / 2;
   const int wgs = !pairs ? units : p.split ? p.pbase[p.chunks] : (p.ntq + 1) / 2;
   const dim3 grid((unsigned)wgs, (unsigned)a.num_kv_heads);
   if (a.q_dtype == OSCAR_F16) {
-    if (D == 256) launch_prefill<256, OSCAR_F16>(p, grid, pairs, s);
-    else launch_prefill<128, OSCAR_F16>(p, grid, pairs, s);
+    if (D == 256) launch_prefill<256, OSCAR_F16>(p, sc, grid, pairs, s);
+    else launch_prefill<128, OSCAR_F16>(p, sc, grid, pairs, s);
   } else {
-    if (D == 256) launch_prefill<256, OSCAR_BF16>(p, grid, pairs, s);
-    else launch_prefill<128, OSCAR_BF16>(p, grid, pairs, s);
+    if (D == 256) launch_prefill<256, OSCAR_BF16>(p, sc, grid, pairs, s);
+    else launch_prefill<128, OSCAR_BF16>(p, sc, grid, pairs, s);
   }
   OSCAR_CHECK_LAUNCH("prefill_kernel");
   if (p.split) {

@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "common.h"
+#include "score.h"
 #include "store_quant.h"
 
 namespace oscar {
@@ -113,9 +114,17 @@ extern "C" int64_t oscar_step_workspace_bytes_v1(int64_t num_tokens, int64_t num
 }
 
 extern "C" int oscar_decode_step_v1(oscar_context_v1* ctx, oscar_step_args_v1* args, void* stream) {
+  return oscarop_decode_step_v1(ctx, args, nullptr, stream);
+}
+
+extern "C" int oscarop_decode_step_v1(oscar_context_v1* ctx, oscar_step_args_v1* args, const oscarop_score_v1* score,
+                                      void* stream) {
   if (!ctx || !args) return fail(-22, "oscar_decode_step_v1: null context or args");
   oscar_step_args_v1& a = *args;
   a.workspace_needed = 0;
+  Score checked;
+  if (score_of(score, a.scale, &checked) < 0)
+    return fail(-22, "oscarop_decode_step_v1: soft_cap must be a finite number, 0 for none");
   const int64_t n = a.num_tokens, hq = a.num_q_heads, hk = a.cache.num_kv_heads, d = a.cache.head_dim;
   const int B = a.num_reqs;
   if (n <= 0 || B <= 0 || hk < 1 || hq % hk || !a.host_query_start_loc || !a.host_seq_lens || !a.query ||
@@ -301,7 +310,9 @@ extern "C" int oscar_decode_step_v1(oscar_context_v1* ctx, oscar_step_args_v1* a
     at.q_dtype = a.q_dtype;
     // with new tokens: the store and the decode in one call (a small store's
     // quantization and slot / window writes ride in the decode's merge launch)
-    rc = has_new ? decode_write_launch(st, at, &meta, stream) : oscar_attn_decode_v1(&at, stream);
+    rc = has_new ? decode_write_launch(st, at, score, &meta, stream)
+         : score ? oscarop_attn_decode_v1(&at, score, stream)
+                 : oscar_attn_decode_v1(&at, stream);
   }
   if (rc == 0) {
     oscar_rotate_args_v1 ro{};

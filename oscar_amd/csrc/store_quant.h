@@ -7,6 +7,8 @@
 
 #include "common.h"
 
+#include "../../include/oscar_operators.h"
+
 namespace oscar {
 
 enum Kind { KIND_K = 0, KIND_V = 1, KIND_Q = 2 };
@@ -357,9 +359,10 @@ __device__ void quant_vector(const StoreParams& p, int kind, int64_t t, int64_t 
 int store_launch(const oscar_store_args_v1* args, void* stream, bool defer, const char* fn, StoreParams* out,
                  const MetaCopy* meta = nullptr);
 
-// oscar_decode_write_v1 whose integer arrays (attn and store point at their device copies)
-// are still on the host: `meta` rides on the store's launch (small stores; empty: nothing)
-int decode_write_launch(const oscar_store_args_v1& store, const oscar_attn_args_v1& attn, const MetaCopy* meta,
-                        void* stream);
+// oscar_decode_write_v1, with a score function (or null), whose integer arrays (attn and
+// store point at their device copies) are still on the host: `meta` rides on the store's
+// launch (small stores; empty: nothing)
+int decode_write_launch(const oscar_store_args_v1& store, const oscar_attn_args_v1& attn,
+                        const oscarop_score_v1* score, const MetaCopy* meta, void* stream);
 
 }  // namespace oscar

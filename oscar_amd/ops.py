@@ -223,10 +223,28 @@ class DeviceContext:
         return ctx
 
 
-def decode_step(ctx: DeviceContext, args: "_lib.StepArgs", stream: int, scratch: DeviceScratch) -> int:
-    """oscar_decode_step_v1; grows the stream's step workspace and retries once when it
-    is too small.  Returns 0, or STEP_NOT_DECODE when the batch needs the general path."""
+def score_struct(soft_cap, alibi_slopes, num_q_heads: int, device) -> _lib.Score | None:
+    """The score function of an attention call as a C struct; None for the plain product."""
+    if alibi_slopes is not None:
+        if alibi_slopes.dtype != torch.float32 or alibi_slopes.shape != (num_q_heads,) \
+                or not alibi_slopes.is_contiguous():
+            raise ValueError(f"alibi_slopes must be a contiguous fp32 [{num_q_heads}] tensor")
+        if alibi_slopes.device != device:
+            raise ValueError(f"alibi_slopes are on {alibi_slopes.device}, the queries on {device}")
+    if not 0 <= soft_cap < math.inf:
+        raise ValueError("soft_cap must be a finite number, 0 for none")
+    if soft_cap == 0 and alibi_slopes is None:
+        return None
+    return _lib.Score(float(soft_cap), _ptr(alibi_slopes))
+
+
+def decode_step(ctx: DeviceContext, args: "_lib.StepArgs", stream: int, scratch: DeviceScratch, score=None) -> int:
+    """oscar_decode_step_v1 (oscarop_decode_step_v1 with a score function); grows the
+    stream's step workspace and retries once when it is too small.  Returns 0, or
+    STEP_NOT_DECODE when the batch needs the general path."""
     lib = _lib.load()
+    if score is not None:
+        return _scored_step(lib, ctx, args, stream, scratch, score)
     rc = lib.oscar_decode_step_v1(ctx.ptr, C.byref(args), C.c_void_p(stream))
     if rc == -28 and args.workspace_needed > args.workspace_bytes:
         ws = scratch.step_workspace(args.workspace_needed)
@@ -234,6 +252,18 @@ def decode_step(ctx: DeviceContext, args: "_lib.StepArgs", stream: int, scratch:
         rc = lib.oscar_decode_step_v1(ctx.ptr, C.byref(args), C.c_void_p(stream))
     if rc < 0:
         _lib.check(rc, "oscar_decode_step_v1")
+    return rc
+
+
+def _scored_step(lib, ctx, args, stream, scratch, score) -> int:
+    for _ in range(2):
+        rc = lib.oscarop_decode_step_v1(ctx.ptr, C.byref(args), C.byref(score), C.c_void_p(stream))
+        if rc != -28 or args.workspace_needed <= args.workspace_bytes:
+            break
+        ws = scratch.step_workspace(args.workspace_needed)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
+    if rc < 0:
+        _lib.check(rc, "oscarop_decode_step_v1")
     return rc
 
 
@@ -516,17 +546,23 @@ def _check_table(table: torch.Tensor, plan: DecodePlan, block_size: int) -> None
 
 def attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, plan: DecodePlan, scale,
                      stage=None, *, head_dim, out_rot=None, lse=None, phases=0, static_scratch=False,
-                     store=None):
+                     store=None, soft_cap=0.0, alibi_slopes=None):
     """Rotated-domain attention over INT2 history (+ current chunk): (out_rot fp32, lse fp32).
 
     q (and k_new / v_new) are bf16 or fp16; history values are rounded q_dtype(fp16(x)).
     static_scratch: call oscar_attn_decode_static_v1 (item partials in the library's
     static device array, no workspace).  store: store_args(...) of the step's write, whose
     rotated outputs are q / k_new / v_new: one oscar_decode_write_v1 call runs the store
-    and the decode (a small store's quantization then rides in the merge launch)."""
+    and the decode (a small store's quantization then rides in the merge launch).
+    soft_cap, alibi_slopes [Hq] fp32: a score s (scaled) of key t for a query at position p
+    becomes soft_cap tanh(s / soft_cap) + alibi_slopes[h] (t - p); 0 and None leave it.  The
+    position is that in the cache, so tokens that were evicted do not count."""
     _require_cuda(q, k_cache, v_cache, block_table)
     if store is not None and static_scratch:
         raise ValueError("store= goes with the workspace decode only")
+    score = score_struct(soft_cap, alibi_slopes, q.shape[1], q.device)
+    if score is not None and (store is not None or static_scratch):
+        raise ValueError("soft_cap and alibi_slopes go with the plain workspace decode")
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("OSCAR HIP attention requires bf16 or fp16 queries")
     n, hq, _ = q.shape
@@ -577,6 +613,9 @@ def attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, plan: Decod
     a.phases = int(phases)
     a.q_dtype = _DTYPES[q.dtype]
     lib = _lib.load()
+    if score is not None:
+        _launch("oscarop_attn_decode_v1", dev, C.byref(a), C.byref(score))
+        return out_rot, lse
     if store is not None:
         _lib.check(lib.oscar_decode_write_v1(C.byref(store[0]), C.byref(a), C.c_void_p(_stream(dev))),
                    "oscar_decode_write_v1")
@@ -588,7 +627,8 @@ def attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, plan: Decod
 
 # ------------------------------------------------------------------------ prefill
 def attention_prefill(q, k, v, scale, *, head_dim, history=0, k_cache=None, v_cache=None,
-                      block_table_row=None, stage=None, out=None, lse=None, split=True):
+                      block_table_row=None, stage=None, out=None, lse=None, split=True, soft_cap=0.0,
+                      alibi_slopes=None):
     """Causal GQA prefill of one request.
 
     q/k/v are bf16 or fp16 (history values rounded q_dtype(fp16(x))).
@@ -597,8 +637,10 @@ def attention_prefill(q, k, v, scale, *, head_dim, history=0, k_cache=None, v_ca
     (and fills lse [n, Hq] when given).
     split: cut the query tiles' key ranges into balanced chunks (a larger workspace for
     their partials and one merge launch); False runs one workgroup per query tile.
+    soft_cap, alibi_slopes: as in attention_decode.
     """
     _require_cuda(q, k, v)
+    score = score_struct(soft_cap, alibi_slopes, q.shape[1], q.device)
     if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("OSCAR HIP prefill requires bf16 or fp16 q/k/v of one dtype")
     n, hq, _ = q.shape
@@ -641,5 +683,8 @@ def attention_prefill(q, k, v, scale, *, head_dim, history=0, k_cache=None, v_ca
         # grown past v1's size: the call would then split)
         ws = DeviceScratch.get(q.device).prefill_workspace(need)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    if score is not None:
+        _launch("oscarop_attn_prefill_v1", q.device, C.byref(a), C.byref(score))
+        return out
     _lib.check(lib.oscar_attn_prefill_v1(C.byref(a), C.c_void_p(_stream(q.device))), "oscar_attn_prefill_v1")
     return out

@@ -18,13 +18,15 @@ layer's FP32 window arena):
   (None without a window) because they are mutated.
 * ``attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, query_start_loc,
   seq_lens, scale, head_dim, stage_k, stage_v, owner, sink_tokens_eff, recent_tokens)
-  -> (out_rot, lse)``: plan + split-K decode + merge (``oscar_attn_plan_v1`` /
+  soft_cap, alibi_slopes) -> (out_rot, lse)``: plan + split-K decode + merge (``oscar_attn_plan_v1`` /
   ``oscar_attn_decode_v1``; slab_attention.py:23-92,376-476); the request lists are
   host integers.
 * ``attention_prefill(q, k, v, scale, head_dim, history, k_cache, v_cache,
-  block_table_row, stage_k, stage_v, owner) -> (out, lse)``: fresh-only (history 0,
+  block_table_row, stage_k, stage_v, owner, soft_cap, alibi_slopes) -> (out, lse)``: fresh-only (history 0,
   output in q's dtype, lse empty) or continuation prefill (fp32 rotated output and LSE)
   (``oscar_attn_prefill_v1``; prefill.py:69-72, slab_attention.py:376-476).
+* ``norm_rope(q, k, positions, cos_sin, q_weight, k_weight, eps, weight_offset,
+  interleaved) -> (q, k)``: head norms with the position rotation (``oscarop_norm_rope_v1``).
 """
 from __future__ import annotations
 
@@ -84,19 +86,20 @@ def attention_decode(q: torch.Tensor, k_new: torch.Tensor | None, v_new: torch.T
                      query_start_loc: list[int], seq_lens: list[int], scale: float, head_dim: int,
                      stage_k: torch.Tensor | None = None, stage_v: torch.Tensor | None = None,
                      owner: torch.Tensor | None = None, sink_tokens_eff: int = 0,
-                     recent_tokens: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+                     recent_tokens: int = 0, soft_cap: float = 0.0,
+                     alibi_slopes: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     hq, hk = q.shape[1], k_cache.shape[2]
     stage = _stage(stage_k, stage_v, owner)
     window = (sink_tokens_eff, recent_tokens) if stage is not None else (0, 0)
     plan = ops.plan_decode(list(query_start_loc), list(seq_lens), has_new=k_new is not None,
                            num_kv_heads=hk, group=hq // hk, head_dim=head_dim, device=q.device, window=window)
     return ops.attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, plan, scale, stage,
-                                head_dim=head_dim)
+                                head_dim=head_dim, soft_cap=soft_cap, alibi_slopes=alibi_slopes)
 
 
 @attention_decode.register_fake
 def _(q, k_new, v_new, k_cache, v_cache, block_table, query_start_loc, seq_lens, scale, head_dim,
-      stage_k=None, stage_v=None, owner=None, sink_tokens_eff=0, recent_tokens=0):
+      stage_k=None, stage_v=None, owner=None, sink_tokens_eff=0, recent_tokens=0, soft_cap=0.0, alibi_slopes=None):
     n, hq = q.shape[0], q.shape[1]
     return (q.new_empty((n, hq, head_dim), dtype=torch.float32), q.new_empty((n, hq), dtype=torch.float32))
 
@@ -107,19 +110,35 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
                       history: int = 0, k_cache: torch.Tensor | None = None,
                       v_cache: torch.Tensor | None = None, block_table_row: torch.Tensor | None = None,
                       stage_k: torch.Tensor | None = None, stage_v: torch.Tensor | None = None,
-                      owner: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+                      owner: torch.Tensor | None = None, soft_cap: float = 0.0,
+                      alibi_slopes: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     n, hq = q.shape[0], q.shape[1]
     lse = torch.empty((n, hq) if history > 0 else (0,), dtype=torch.float32, device=q.device)
     out = ops.attention_prefill(q, k, v, scale, head_dim=head_dim, history=history, k_cache=k_cache,
                                 v_cache=v_cache, block_table_row=block_table_row,
-                                stage=_stage(stage_k, stage_v, owner), lse=lse if history > 0 else None)
+                                stage=_stage(stage_k, stage_v, owner), lse=lse if history > 0 else None,
+                                soft_cap=soft_cap, alibi_slopes=alibi_slopes)
     return out, lse
 
 
 @attention_prefill.register_fake
 def _(q, k, v, scale, head_dim, history=0, k_cache=None, v_cache=None, block_table_row=None,
-      stage_k=None, stage_v=None, owner=None):
+      stage_k=None, stage_v=None, owner=None, soft_cap=0.0, alibi_slopes=None):
     n, hq = q.shape[0], q.shape[1]
     if history > 0:
         return (q.new_empty((n, hq, head_dim), dtype=torch.float32), q.new_empty((n, hq), dtype=torch.float32))
     return q.new_empty((n, hq, head_dim)), q.new_empty((0,), dtype=torch.float32)
+
+
+# ------------------------------------------------------------------ head norms and rotation
+@torch.library.custom_op(f"{_LIB}::norm_rope", mutates_args=(), device_types="cuda")
+def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+              q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+              weight_offset: float = 0.0, interleaved: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    return ops.norm_rope(q, k, positions, cos_sin, q_weight=q_weight, k_weight=k_weight, eps=eps,
+                         weight_offset=weight_offset, interleaved=interleaved)
+
+
+@norm_rope.register_fake
+def _(q, k, positions, cos_sin, q_weight=None, k_weight=None, eps=1e-6, weight_offset=0.0, interleaved=False):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
