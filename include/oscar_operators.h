@@ -76,6 +76,52 @@ typedef struct oscarop_norm_rope_args_v1 {
 
 int oscarop_norm_rope_v1(const oscarop_norm_rope_args_v1* args, void* stream);
 
+/* ---- the attention weight that each cached token received -----------------------------
+ * weights[r][h][t] += sum over request r's queries and the query heads of KV head h of
+ * exp(s' - lse), s' being the row's score of key t (unseen keys: nothing) and lse its
+ * log-sum-exp as the attention call over the same batch wrote it; a row with lse = -inf
+ * saw no key and adds nothing.  Keys as oscar_attn_decode_v1 reads them: request r's
+ * queries are rows [query_start_loc[r], query_start_loc[r + 1]) of q, its length
+ * seq_lens[r] includes the current chunk when k_new is given, and query i of n_q sees keys
+ * [0, seq - n_q + i + 1).  With history 0 and k_new the rows may be unrotated ones.  No
+ * rounding below fp32; the order of the sums is fixed.  A request that does not fit
+ * (queries past num_tokens, a length past weights_cols, a history past the block table)
+ * reads nothing and its weights become NaN. */
+typedef struct oscarop_weights_args_v1 {
+  const void* q;                /* [num_tokens, num_q_heads, D] in q_dtype */
+  int64_t num_tokens;
+  int64_t num_q_heads;
+  int64_t q_stride_token;       /* elements */
+  const void* k_new;            /* [num_tokens, Hk, D] current chunk, or NULL (cache only) */
+  int64_t k_new_stride_token;
+  oscar_cache_v1 cache;         /* the v side is not read */
+  const int32_t* block_table;   /* [block_table_rows, block_table_cols] */
+  int64_t block_table_stride;
+  int64_t block_table_rows;
+  int64_t block_table_cols;
+  const int32_t* query_start_loc; /* device [num_reqs + 1] */
+  const int32_t* seq_lens;        /* device [num_reqs] */
+  int32_t num_reqs;
+  int32_t q_dtype;              /* OSCAR_BF16 or OSCAR_F16 */
+  /* the longest length and the most queries of a request: they size the launch, and any
+   * batch gives the same results */
+  int64_t max_seq_len;
+  int64_t max_query_len;
+  const oscar_staging_v1* staging; /* NULL = no window; its v side is not read */
+  float scale;
+  const float* lse;             /* [num_tokens, num_q_heads] */
+  float* weights;               /* [num_reqs][Hk][weights_cols], strides in elements */
+  int64_t weights_stride_request;
+  int64_t weights_stride_head;
+  int64_t weights_cols;
+  void* workspace;              /* >= oscarop_attn_weights_workspace_bytes_v1(args), 16-byte aligned */
+  int64_t workspace_bytes;
+} oscarop_weights_args_v1;
+
+/* reads the sizes of *args alone; -22 for sizes that the call would refuse */
+int64_t oscarop_attn_weights_workspace_bytes_v1(const oscarop_weights_args_v1* args);
+int oscarop_attn_weights_v1(const oscarop_weights_args_v1* args, const oscarop_score_v1* score, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -116,6 +116,18 @@ class NormRopeArgs(C.Structure):
     ]
 
 
+class WeightsArgs(C.Structure):
+    _fields_ = [
+        ("q", vp), ("num_tokens", i64), ("num_q_heads", i64), ("q_stride_token", i64),
+        ("k_new", vp), ("k_new_stride_token", i64), ("cache", Cache),
+        ("block_table", vp), ("block_table_stride", i64), ("block_table_rows", i64), ("block_table_cols", i64),
+        ("query_start_loc", vp), ("seq_lens", vp), ("num_reqs", i32), ("q_dtype", i32),
+        ("max_seq_len", i64), ("max_query_len", i64), ("staging", C.POINTER(Staging)), ("scale", f32), ("lse", vp),
+        ("weights", vp), ("weights_stride_request", i64), ("weights_stride_head", i64), ("weights_cols", i64),
+        ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
 STEP_NOT_DECODE = 1
 
 # name -> (restype, argtypes); every symbol declared in include/oscar_amd.h
@@ -146,6 +158,8 @@ OPERATOR_SIGNATURES = {
     "oscarop_attn_decode_v1": (C.c_int, [C.POINTER(AttnArgs), C.POINTER(Score), vp]),
     "oscarop_attn_prefill_v1": (C.c_int, [C.POINTER(PrefillArgs), C.POINTER(Score), vp]),
     "oscarop_decode_step_v1": (C.c_int, [vp, C.POINTER(StepArgs), C.POINTER(Score), vp]),
+    "oscarop_attn_weights_workspace_bytes_v1": (i64, [C.POINTER(WeightsArgs)]),
+    "oscarop_attn_weights_v1": (C.c_int, [C.POINTER(WeightsArgs), C.POINTER(Score), vp]),
     "oscarop_norm_rope_v1": (C.c_int, [C.POINTER(NormRopeArgs), vp]),
 }
 

@@ -688,3 +688,104 @@ def attention_prefill(q, k, v, scale, *, head_dim, history=0, k_cache=None, v_ca
         return out
     _lib.check(lib.oscar_attn_prefill_v1(C.byref(a), C.c_void_p(_stream(q.device))), "oscar_attn_prefill_v1")
     return out
+
+
+# ------------------------------------------------------------------------ accumulated weights
+@dataclass
+class WeightsPlan:
+    """The requests of a batch, on the host and on the device, as accumulate_weights takes
+    them (a DecodePlan of the same batch serves as well)."""
+    host_qsl: list
+    host_seqs: list
+    has_new: bool
+    qsl: torch.Tensor    # device int32
+    seqs: torch.Tensor
+
+
+def _request_lists(qsl, seqs, has_new) -> tuple[list, list]:
+    qsl, seqs = [int(x) for x in qsl], [int(x) for x in seqs]
+    if len(qsl) != len(seqs) + 1 or qsl[0] < 0 or any(b < a for a, b in zip(qsl, qsl[1:])):
+        raise ValueError("query starts must be one more than the lengths and must not decrease")
+    if any(s < 0 or has_new and s < b - a for a, b, s in zip(qsl, qsl[1:], seqs)):
+        raise ValueError("Sequence length must cover its query chunk")
+    return qsl, seqs
+
+
+def plan_weights(qsl, seqs, *, has_new: bool, device) -> WeightsPlan:
+    """The lists of a batch (query starts, lengths) for accumulate_weights, uploaded once for
+    all layers."""
+    qsl, seqs = _request_lists(qsl, seqs, has_new)
+    dev = upload([np.asarray(qsl, np.int32), np.asarray(seqs or [0], np.int32)], device)
+    return WeightsPlan(qsl, seqs, bool(has_new), *dev)
+
+
+def accumulate_weights(q, k_new, k_cache, v_cache, block_table, plan, scale, lse, weights, stage=None, *, head_dim,
+                       soft_cap=0.0, alibi_slopes=None):
+    """Add to weights [requests, Hk, columns] (fp32) the attention weight that each token of
+    each request received: weights[r, h, t] += sum over r's queries and the query heads of
+    KV head h of exp(score - lse).
+
+    q, k_new, the caches, block_table, scale, stage, soft_cap and alibi_slopes as
+    attention_decode took them for this batch, lse [n, Hq] (fp32) as it returned it (a row
+    with -inf adds nothing).  After a fresh prompt's attention_prefill(lse=...), history 0:
+    its unrotated q and k.  plan: plan_weights(...) or the batch's plan_decode(...).  Request
+    r is row r of block_table and of weights; weights is updated in place and returned, the
+    same bits whatever runs beside it.
+    """
+    dev = _one_device(q, k_new, k_cache, v_cache, block_table, lse, weights, plan.qsl, plan.seqs)
+    score = score_struct(soft_cap, alibi_slopes, q.shape[1], q.device)
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("OSCAR HIP attention requires bf16 or fp16 queries")
+    if plan.qsl is None:
+        raise ValueError("the plan has not been uploaded")
+    n, hq, _ = q.shape
+    hk, reqs = k_cache.shape[2], len(plan.host_seqs)
+    if plan.has_new != (k_new is not None):
+        raise ValueError("plan and call disagree on the presence of current K")
+    if plan.host_qsl[-1] > n:
+        raise ValueError("the plan has more queries than the call")
+    if q.shape[2] != head_dim or q.stride(2) != 1 or q.stride(1) != head_dim:
+        if q.shape[2] != head_dim:
+            raise ValueError("q must be [tokens, heads, head_dim]")
+        q = q.contiguous()
+    if k_new is not None:
+        if k_new.dtype != q.dtype or k_new.shape[1:] != (hk, head_dim) or k_new.shape[0] < plan.host_qsl[-1]:
+            raise ValueError("Current K must match the queries' type and the cache's heads")
+        k_new = k_new.contiguous()
+    if lse.dtype != torch.float32 or lse.shape != (n, hq):
+        raise ValueError("lse must be fp32 [tokens, query heads]")
+    longest = max((s for a, b, s in zip(plan.host_qsl, plan.host_qsl[1:], plan.host_seqs) if b > a), default=0)
+    if weights.dtype != torch.float32 or weights.ndim != 3 or weights.shape[0] < reqs or weights.shape[1] != hk \
+            or weights.stride(2) != 1 and weights.shape[2] > 1:
+        raise ValueError("weights must be fp32 [requests, KV heads, columns], columns next to each other")
+    if longest > weights.shape[2]:
+        raise ValueError(f"weights have {weights.shape[2]} columns for {longest} tokens")
+    if reqs == 0 or n == 0 or longest == 0:
+        return weights
+    table = block_table.to(dtype=torch.int32)
+    if table.stride(-1) != 1:
+        table = table.contiguous()
+    _check_table(table, plan, k_cache.shape[1])
+    st = staging_struct(stage, k_cache, head_dim)
+    lse = lse.contiguous()
+    a = _lib.WeightsArgs()
+    a.q, a.num_tokens, a.num_q_heads, a.q_stride_token = q.data_ptr(), n, hq, q.stride(0)
+    if k_new is not None:
+        a.k_new, a.k_new_stride_token = k_new.data_ptr(), k_new.stride(0)
+    a.cache = cache_struct(k_cache, v_cache, head_dim)
+    a.block_table, a.block_table_stride = table.data_ptr(), table.stride(0)
+    a.block_table_rows, a.block_table_cols = table.shape
+    a.query_start_loc, a.seq_lens, a.num_reqs = plan.qsl.data_ptr(), plan.seqs.data_ptr(), reqs
+    a.q_dtype, a.scale, a.lse = _DTYPES[q.dtype], float(scale), lse.data_ptr()
+    a.max_seq_len, a.max_query_len = longest, max(b - c for c, b in zip(plan.host_qsl, plan.host_qsl[1:]))
+    if st is not None:
+        a.staging = C.pointer(st)
+    a.weights, a.weights_cols = weights.data_ptr(), weights.shape[2]
+    a.weights_stride_head = weights.stride(1) if hk > 1 else weights.shape[2]
+    a.weights_stride_request = weights.stride(0) if reqs > 1 else hk * a.weights_stride_head
+    need = _lib.load().oscarop_attn_weights_workspace_bytes_v1(C.byref(a))
+    if need > 0:
+        ws = DeviceScratch.get(dev).attn_workspace(need)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    _launch("oscarop_attn_weights_v1", dev, C.byref(a), None if score is None else C.byref(score))
+    return weights
