@@ -122,6 +122,45 @@ typedef struct oscarop_weights_args_v1 {
 int64_t oscarop_attn_weights_workspace_bytes_v1(const oscarop_weights_args_v1* args);
 int oscarop_attn_weights_v1(const oscarop_weights_args_v1* args, const oscarop_score_v1* score, void* stream);
 
+/* ---- eviction by accumulated weight ----------------------------------------------------
+ * Of request r's tokens [sink, tail) the `drop` of least weight leave the cache, for each KV
+ * head its own (equal weights: the later token first; NaN counts as the largest).  The kept
+ * tokens of [tail - drop, tail) move into the places of the dropped ones of
+ * [sink, tail - drop), the i-th into the i-th, with slot bytes and weights; a place that is
+ * written loses its FP32 window copy.  The tokens [tail, seq) stay in their pages, so that
+ * with tail and drop whole pages the request's pages [(tail - drop) / block_size,
+ * tail / block_size) are free afterwards and its length is seq - drop: the caller takes them
+ * out of the block table (the call leaves it alone, since the layers of a model share it).
+ * No page of [sink, tail) may belong to another request or come twice. */
+typedef struct oscarop_evict_args_v1 {
+  const float* weights;         /* [num_reqs][Hk][weights_cols], strides in elements */
+  int64_t weights_stride_request;
+  int64_t weights_stride_head;
+  int64_t weights_cols;
+  /* the weights by new position, zero from the new length on; no overlap with weights */
+  float* weights_out;
+  int64_t out_stride_request;
+  int64_t out_stride_head;
+  oscar_cache_v1 cache;
+  const int32_t* block_table;   /* [block_table_rows, block_table_cols] */
+  int64_t block_table_stride;
+  int64_t block_table_rows;
+  int64_t block_table_cols;
+  /* device [num_reqs][4]: seq, sink, tail, drop.  A request that does not fit (0 <= sink,
+   * 0 <= drop <= tail - sink, tail <= seq <= weights_cols, drop <= max_drop, pages within
+   * the table) keeps its cache, and its weights are copied. */
+  const int32_t* requests;
+  int32_t num_reqs;
+  int32_t reserved;
+  int64_t max_drop;             /* the largest drop: whole pages */
+  const oscar_staging_v1* staging; /* NULL = no window; only its owner tags are used */
+  void* workspace;              /* >= oscarop_evict_workspace_bytes_v1(...), 16-byte aligned */
+  int64_t workspace_bytes;
+} oscarop_evict_args_v1;
+
+int64_t oscarop_evict_workspace_bytes_v1(int64_t num_reqs, int64_t num_kv_heads, int64_t max_drop);
+int oscarop_evict_v1(const oscarop_evict_args_v1* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -128,6 +128,16 @@ class WeightsArgs(C.Structure):
     ]
 
 
+class EvictArgs(C.Structure):
+    _fields_ = [
+        ("weights", vp), ("weights_stride_request", i64), ("weights_stride_head", i64), ("weights_cols", i64),
+        ("weights_out", vp), ("out_stride_request", i64), ("out_stride_head", i64), ("cache", Cache),
+        ("block_table", vp), ("block_table_stride", i64), ("block_table_rows", i64), ("block_table_cols", i64),
+        ("requests", vp), ("num_reqs", i32), ("reserved", i32), ("max_drop", i64), ("staging", C.POINTER(Staging)),
+        ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
 STEP_NOT_DECODE = 1
 
 # name -> (restype, argtypes); every symbol declared in include/oscar_amd.h
@@ -160,6 +170,8 @@ OPERATOR_SIGNATURES = {
     "oscarop_decode_step_v1": (C.c_int, [vp, C.POINTER(StepArgs), C.POINTER(Score), vp]),
     "oscarop_attn_weights_workspace_bytes_v1": (i64, [C.POINTER(WeightsArgs)]),
     "oscarop_attn_weights_v1": (C.c_int, [C.POINTER(WeightsArgs), C.POINTER(Score), vp]),
+    "oscarop_evict_workspace_bytes_v1": (i64, [i64, i64, i64]),
+    "oscarop_evict_v1": (C.c_int, [C.POINTER(EvictArgs), vp]),
     "oscarop_norm_rope_v1": (C.c_int, [C.POINTER(NormRopeArgs), vp]),
 }
 

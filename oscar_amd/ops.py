@@ -789,3 +789,117 @@ def accumulate_weights(q, k_new, k_cache, v_cache, block_table, plan, scale, lse
         a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
     _launch("oscarop_attn_weights_v1", dev, C.byref(a), None if score is None else C.byref(score))
     return weights
+
+
+# ------------------------------------------------------------------------ eviction
+@dataclass
+class EvictPlan:
+    """How many pages each request of a batch gives up, for all layers of a model.
+
+    seq_lens: the lengths afterwards.  freed[r]: the columns (first, last + 1) of request r's
+    row of table(...) that hold its free pages."""
+    seq_lens: list
+    freed: list
+    lengths: list        # before
+    max_drop: int        # tokens
+    block_size: int
+    requests: torch.Tensor   # device int32 [requests, 4]: length, sink, tail, dropped tokens
+
+    def table(self, block_table: torch.Tensor) -> torch.Tensor:
+        """The block table after the last layer's evict: each request's kept pages in their
+        order, then its free ones."""
+        length, _, tail, drop = self.requests.to(torch.int64).t()[..., None]
+        bs, many = self.block_size, len(self.lengths)
+        pages, end, gone = -(-length // bs), (tail - drop) // bs, drop // bs
+        col = torch.arange(block_table.shape[1], device=block_table.device)
+        source = torch.where(col < end, col, torch.where(col < pages - gone, col + gone,
+                                                         torch.where(col < pages, col - pages + gone + end, col)))
+        out = block_table.clone()
+        out[:many] = torch.gather(block_table[:many], 1, source)
+        return out
+
+
+def plan_evict(seq_lens, drop_pages, *, block_size: int, sink_tokens: int = 0, recent_tokens: int = 0, device) -> EvictPlan:
+    """Plan to take drop_pages[r] whole pages out of request r of length seq_lens[r] (host
+    lists; 0: the request keeps all).  The first sink_tokens and the last recent_tokens stay,
+    the latter with all of their pages; a request that has too little between them is refused."""
+    lengths, pages = [int(x) for x in seq_lens], [int(x) for x in drop_pages]
+    if len(lengths) != len(pages):
+        raise ValueError("one page count for each length")
+    if block_size < 1 or sink_tokens < 0 or recent_tokens < 0:
+        raise ValueError("block size, sink and recent tokens must not be negative")
+    records, freed = [], []
+    for r, (length, many) in enumerate(zip(lengths, pages)):
+        if length < 0 or many < 0:
+            raise ValueError(f"request {r}: negative length or page count")
+        tail = max(length - recent_tokens, 0) // block_size * block_size
+        if many and tail - sink_tokens < many * block_size:
+            raise ValueError(f"request {r}: {many} pages of {block_size} to drop, {max(tail - sink_tokens, 0)} tokens "
+                             "between its first and its last ones")
+        drop = many * block_size
+        records.append([length, sink_tokens, tail, drop] if many else [length, 0, 0, 0])
+        freed.append((-(-length // block_size) - many, -(-length // block_size)))
+    dev, = upload([np.asarray(records, np.int32).reshape(-1)], device)
+    return EvictPlan([n - q[3] for n, q in zip(lengths, records)], freed, lengths, max((q[3] for q in records), default=0),
+                     int(block_size), dev.view(-1, 4))
+
+
+def evict(plan: EvictPlan, weights, k_cache, v_cache, block_table, *, head_dim, stage=None, weights_out=None):
+    """Drop the tokens of least accumulated weight from one layer's cache, whole pages at a
+    time; returns the weights by new position ([requests, Hk, columns], zero from the new
+    length on; weights_out if given, which must not overlap weights).
+
+    plan: plan_evict(...) of the batch.  Per request and KV head the plan's tokens of least
+    weight between the first and the last ones go (equal weights: the later token first; NaN
+    counts as the largest); the kept tokens of the last pages before the recent ones move
+    into their places (keys of attention have no order; with alibi_slopes they have one, and
+    distances then count what is left).  A place that is written loses its FP32 window copy.
+    The caches and the owner tags of `stage` change in place, block_table does not: after the
+    last layer plan.table(block_table) is the new one, plan.seq_lens the new lengths.  The
+    pages between must be the request's own.
+    """
+    dev = _one_device(weights, k_cache, v_cache, block_table, weights_out, plan.requests)
+    cache = cache_struct(k_cache, v_cache, head_dim)
+    reqs, hk, bs = len(plan.lengths), k_cache.shape[2], k_cache.shape[1]
+    if plan.block_size != bs:
+        raise ValueError(f"the plan is for pages of {plan.block_size} tokens, the cache has {bs}")
+    if weights_out is None:
+        weights_out = torch.empty(weights.shape, dtype=torch.float32, device=dev)
+    for name, w in (("weights", weights), ("weights_out", weights_out)):
+        if w.dtype != torch.float32 or w.ndim != 3 or w.shape[0] < reqs or w.shape[1] != hk \
+                or w.stride(2) != 1 and w.shape[2] > 1:
+            raise ValueError(f"{name} must be fp32 [requests, KV heads, columns], columns next to each other")
+    if weights.shape != weights_out.shape:
+        raise ValueError("weights_out must have the shape of weights")
+    longest = max(plan.lengths, default=0)
+    if longest > weights.shape[2]:
+        raise ValueError(f"weights have {weights.shape[2]} columns for {longest} tokens")
+    if reqs < weights.shape[0]:
+        weights_out[reqs:].copy_(weights[reqs:])
+    if reqs == 0 or weights.shape[2] == 0:
+        return weights_out
+    table = block_table.to(dtype=torch.int32)
+    if table.ndim != 2 or table.shape[0] < reqs:
+        raise ValueError("Missing request block-table rows")
+    if -(-longest // bs) > table.shape[1]:
+        raise ValueError("Block table cannot cover the history")
+    if table.stride(1) != 1:
+        table = table.contiguous()
+    st = staging_struct(stage, k_cache, head_dim)
+    a = _lib.EvictArgs()
+    a.weights, a.weights_cols, a.weights_out = weights.data_ptr(), weights.shape[2], weights_out.data_ptr()
+    for name, w in (("weights", weights), ("out", weights_out)):
+        head = w.stride(1) if hk > 1 else w.shape[2]
+        setattr(a, f"{name}_stride_head", head)
+        setattr(a, f"{name}_stride_request", w.stride(0) if reqs > 1 else hk * head)
+    a.cache = cache
+    a.block_table, a.block_table_stride = table.data_ptr(), table.stride(0)
+    a.block_table_rows, a.block_table_cols = table.shape
+    a.requests, a.num_reqs, a.max_drop = plan.requests.data_ptr(), reqs, plan.max_drop
+    if st is not None:
+        a.staging = C.pointer(st)
+    need = _lib.load().oscarop_evict_workspace_bytes_v1(reqs, hk, plan.max_drop)
+    ws = DeviceScratch.get(dev).attn_workspace(need)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    _launch("oscarop_evict_v1", dev, C.byref(a))
+    return weights_out
