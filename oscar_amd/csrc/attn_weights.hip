@@ -4,16 +4,23 @@
 // attention call left it.  Keys are those the attention reads: the packed INT2 history, FP32
 // window copies where the owner tag matches, and the current chunk's rows.
 //
-// A wave holds the K operands of one 32-token tile in registers for all rows and adds up
-// probabilities per key, lane by lane (lane l: row l % 32 of a row block), so that the sum
-// over the rows crosses lanes once, at the end.  The query operands of a block of 32 rows
-// go through LDS, shared by the workgroup's waves.  Every weight has one owner, so nothing
-// is atomic and results do not depend on the order of workgroups.
+// Probabilities are added up per key, lane by lane (lane l: row l % 32 of a row block), so
+// that the sum over the rows crosses lanes once per key, at the end.  Every number has one
+// owner, so nothing is atomic and results do not depend on the order of workgroups.
+//
+//   weights_few_kernel   a batch of at most 32 rows per KV head (decode, verification): the
+//                        queries stay in LDS and every wave streams key tiles past them, the
+//                        next tile's codes in flight; bound by the lookups of the K operands
+//   weights_many_kernel  more rows: a wave holds the K operands of two tiles in registers and
+//                        the row blocks go past, through LDS and shared by the workgroup's
+//                        waves; where the keys alone do not fill the chip the rows are cut
+//                        into chunks, whose sums weights_sum_kernel adds in their order
 #include <type_traits>
 
 #include "common.h"
 #include "int2_tile.h"
 #include "score.h"
+#include "store_quant.h"
 
 #include "../../include/oscar_operators.h"
 
@@ -24,141 +31,401 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr int kTile = 32;
+constexpr int kFewRows = 32;                           // of a KV head, for weights_few_kernel
+constexpr int kKeyTiles = 2;                           // per wave of weights_many_kernel
+constexpr int kGroupKeys = kWaves * kKeyTiles * kTile;  // per workgroup
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct WeightsParams {
   oscarop_weights_args_v1 a;
   oscar_staging_v1 st;
   int has_stage;
-  int group;  // Hq / Hk
+  FastDiv group;  // Hq / Hk
   Score sc;
+  int chunks;        // row chunks (1: sums go to the weights)
+  int chunk_blocks;  // row blocks of a chunk; the last one takes what is left
+  float* part;       // [num_reqs][chunks][Hk][weights_cols]
 };
 
-template <int D, int QT, int SC>
-__global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams P) {
-  constexpr int NCH = D / 32;  // 16-element chunks per lane half
+// The row chunks of the requests' key groups.  A key group's rows begin with the first that
+// sees one of its keys.
+struct Rows {
+  int first, end;  // row blocks
+};
+__device__ __forceinline__ Rows rows_of(const WeightsParams& P, int chunk, int tb, int before, int nrows) {
+  const int from = tb > before ? (int)(((int64_t)(tb - before) * P.group.d) / 32) : 0, blocks = (nrows + 31) / 32;
+  const int a = chunk * P.chunk_blocks;
+  Rows r;
+  r.first = a > from ? a : from;
+  r.end = chunk == P.chunks - 1 || blocks < a + P.chunk_blocks ? blocks : a + P.chunk_blocks;
+  return r;
+}
+
+// a request that does not fit the call's arrays
+__device__ __forceinline__ bool misfit(const oscarop_weights_args_v1& A, int qa, int nq, int seq) {
+  const int hist = A.k_new != nullptr ? seq - nq : seq;
+  return qa < 0 || (int64_t)qa + nq > A.num_tokens || hist < 0 || seq > A.weights_cols ||
+         (hist > 0 && (hist - 1) / (int)A.cache.block_size >= A.block_table_cols);
+}
+
+// What a request's workgroups share.
+struct Span {
+  int qa, nq, seq, hist, before;  // first query, queries, length, cached tokens; query i sees keys [0, before + i + 1)
+};
+__device__ __forceinline__ Span span_of(const oscarop_weights_args_v1& A, int req) {
+  Span x;
+  x.qa = A.query_start_loc[req];
+  x.nq = A.query_start_loc[req + 1] - x.qa;
+  x.seq = A.seq_lens[req];
+  x.before = x.seq - x.nq;
+  x.hist = A.k_new != nullptr ? x.before : x.seq;
+  return x;
+}
+
+// Row n of a request under KV head kvh: its token (0-based in the request) and query head.
+struct RowRef {
+  int tok, head;
+  bool ok;
+};
+__device__ __forceinline__ RowRef row_of(const WeightsParams& P, int n, int nrows, int kvh) {
+  RowRef r;
+  r.ok = n < nrows;
+  r.tok = (int)fdiv((uint32_t)(r.ok ? n : 0), P.group);
+  r.head = kvh * (int)P.group.d + ((r.ok ? n : 0) - r.tok * (int)P.group.d);
+  return r;
+}
+
+// One lane's token of a key tile: token t0 + lane % 32, half lane / 32 of its elements.
+enum KeyKind { kNone = 0, kCodes = 1, kStaged = 2, kCurrent = 3 };  // past the length; history; its window copy; the chunk
+template <int D>
+struct KeyRegs {
+  u32x4 word[D / 128];  // history: its half of the codes
+  unsigned meta;        // history: scale and zero
+  int kind;
+  int64_t at;           // window copy, chunk: its first element
+};
+
+template <int D>
+__device__ __forceinline__ void load_keys(const WeightsParams& P, const Span& x, int req, int kvh, int t0, KeyRegs<D>& k) {
   const oscarop_weights_args_v1& A = P.a;
-  const int tid = threadIdx.x, lane = tid & 63, m = lane & 31, g = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int req = blockIdx.z, kvh = blockIdx.y, G = P.group;
-  const int qa = A.query_start_loc[req], nq = A.query_start_loc[req + 1] - qa, seq = A.seq_lens[req];
-  if (nq < 1) return;
-  const bool has_new = A.k_new != nullptr;
-  const int hist = has_new ? seq - nq : seq;
-  const int before = seq - nq;  // query i sees keys [0, before + i + 1)
-  const int bs = (int)A.cache.block_size;
-  const int64_t hk = A.cache.num_kv_heads;
-  float* out = A.weights + req * A.weights_stride_request + kvh * A.weights_stride_head;
-  // a request that does not fit the call's arrays reads nothing and turns its weights, as
-  // far as there are any, into NaN
-  const bool bad = qa < 0 || (int64_t)qa + nq > A.num_tokens || hist < 0 || seq > A.weights_cols ||
-                   (hist > 0 && (hist - 1) / bs >= A.block_table_cols);
-  if (bad) {
-    for (int64_t t = (int64_t)blockIdx.x * kThreads + tid; t < A.weights_cols && t < seq; t += (int64_t)gridDim.x * kThreads)
-      out[t] = NAN;
+  const int lane = threadIdx.x & 63, t = t0 + (lane & 31), g = lane >> 5, bs = (int)A.cache.block_size;
+  k.kind = kNone;
+  k.at = 0;
+  if (t0 < x.hist) {
+    int64_t blk = A.block_table[req * A.block_table_stride + t0 / bs];
+    blk = blk < 0 || blk >= A.cache.num_blocks ? 0 : blk;  // a bad id must not fault
+    const int off = t0 % bs + (lane & 31);
+    const uint8_t* slot = A.cache.k + blk * A.cache.k_stride[0] + off * A.cache.k_stride[1] + kvh * A.cache.k_stride[2];
+    k.meta = *(const unsigned*)slot;  // (pages hold whole tiles: also where t is past the history)
+#pragma unroll
+    for (int i = 0; i < D / 128; ++i) k.word[i] = *(const u32x4*)(slot + 32 + g * (D / 8) + 16 * i);
+    if (t < x.hist) k.kind = kCodes;
+    if (P.has_stage) {
+      const int64_t seat = (unsigned)blk % (unsigned)P.st.rows * bs + off;
+      if (P.st.owner[seat] == blk && t < x.hist) {
+        k.kind = kStaged;
+        k.at = (seat * A.cache.num_kv_heads + kvh) * D + g * (D / 2);
+      }
+    }
+  }
+  if (A.k_new != nullptr && t >= x.hist && t < x.seq) {
+    k.kind = kCurrent;
+    k.at = (int64_t)(x.qa + t - x.hist) * A.k_new_stride_token + kvh * D + g * (D / 2);
+  }
+}
+
+// The K operands of the lane's half, 16 elements (two operands) at a time: use(c, a, b).
+template <int D, int QT, class Use>
+__device__ __forceinline__ void key_operands(const WeightsParams& P, const KeyRegs<D>& k, Use use) {
+  constexpr int NCH = D / 32;
+  if (__all(k.kind == kCodes)) {
+    unsigned t_lo, t_hi;
+    byte_tables<QT>(k.meta, t_lo, t_hi);
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      unsigned o[8];
+      lut16(k.word[c >> 2][c & 3], t_lo, t_hi, o);
+      use(c, u32x4{o[0], o[1], o[2], o[3]}, u32x4{o[4], o[5], o[6], o[7]});
+    }
     return;
   }
-  __shared__ __attribute__((aligned(16))) u32x4 s_q[2 * NCH][64];  // Q^T operands of a row block
-  const int nrows = nq * G;
-  for (int tb = blockIdx.x * (kWaves * kTile); tb < seq; tb += gridDim.x * (kWaves * kTile)) {
-    // ---- this wave's tile: lane (token m, half g) holds the K operands of its half
-    const int t0 = tb + wave * kTile, t = t0 + m;
-    u32x4 kop[2 * NCH];
-    {
-      int64_t blk = 0;
-      bool staged = false;
-      int64_t seat = 0;
-      const int off = t % bs;
-      if (t0 < hist) {
-        blk = A.block_table[req * A.block_table_stride + t0 / bs];
-        blk = blk < 0 || blk >= A.cache.num_blocks ? 0 : blk;  // a bad id must not fault
-        if (P.has_stage && t < hist) {
-          seat = blk % P.st.rows * bs + off;
-          staged = P.st.owner[seat] == blk;
-        }
+  unsigned t_lo = 0, t_hi = 0;
+  if (k.kind == kCodes) byte_tables<QT>(k.meta, t_lo, t_hi);
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    unsigned o[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+    if (k.kind == kCodes) {
+      lut16(k.word[c >> 2][c & 3], t_lo, t_hi, o);
+    } else if (k.kind == kStaged) {
+      const float* fp = P.st.stage_k + k.at + 16 * c;
+      f32x4 f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = *(const f32x4*)(fp + 4 * i);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[i] = hist_pair<QT>(f[0][i], f[1][i]);
+        o[4 + i] = hist_pair<QT>(f[2][i], f[3][i]);
       }
-      const bool codes = t < hist && !staged, cur = has_new && t >= hist && t < seq;
-      const uint8_t* slot = A.cache.k + blk * A.cache.k_stride[0] + off * A.cache.k_stride[1] + kvh * A.cache.k_stride[2];
-      unsigned t_lo = 0, t_hi = 0;
-      if (codes) byte_tables<QT>(*(const unsigned*)slot, t_lo, t_hi);
-      const float* fp = P.st.stage_k + (seat * hk + kvh) * D + g * (D / 2);
-      const uint16_t* row = (const uint16_t*)A.k_new + (int64_t)(qa + (cur ? t - hist : 0)) * A.k_new_stride_token + kvh * D +
-                            g * (D / 2);
-#pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        unsigned o[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-        if (codes) {
-          lut16(*(const unsigned*)(slot + 32 + g * (D / 8) + 4 * c), t_lo, t_hi, o);
-        } else if (staged) {
-          f32x4 f[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) f[x] = *(const f32x4*)(fp + 16 * c + 4 * x);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            o[x] = hist_pair<QT>(f[0][x], f[1][x]);
-            o[4 + x] = hist_pair<QT>(f[2][x], f[3][x]);
-          }
-        } else if (cur) {
-          kpairs16(*(const u32x4*)(row + 16 * c), *(const u32x4*)(row + 16 * c + 8), o);
-        }
-        kop[2 * c] = u32x4{o[0], o[1], o[2], o[3]};
-        kop[2 * c + 1] = u32x4{o[4], o[5], o[6], o[7]};
-      }
+    } else if (k.kind == kCurrent) {
+      const uint16_t* row = (const uint16_t*)P.a.k_new + k.at + 16 * c;
+      kpairs16(*(const u32x4*)row, *(const u32x4*)(row + 8), o);
     }
-    float acc[16] = {};
-    // ---- all rows that see the workgroup's first key
-    const int first = tb > before ? (tb - before) * G : 0;
-    for (int rb = first / 32; rb * 32 < nrows; ++rb) {
-      const int n = 32 * rb + m;
-      const bool row_ok = n < nrows;
-      const int tok = row_ok ? n / G : 0, head = kvh * G + (row_ok ? n - tok * G : 0);
-      const uint16_t* q = (const uint16_t*)A.q + (int64_t)(qa + tok) * A.q_stride_token + (int64_t)head * D + g * (D / 2);
-      __syncthreads();  // the block before has been read
-#pragma unroll
-      for (int c = wave; c < NCH; c += kWaves) {
-        unsigned o[8];
-        kpairs16(*(const u32x4*)(q + 16 * c), *(const u32x4*)(q + 16 * c + 8), o);
-        s_q[2 * c][lane] = u32x4{o[0], o[1], o[2], o[3]};
-        s_q[2 * c + 1][lane] = u32x4{o[4], o[5], o[6], o[7]};
-      }
-      const float lse = A.lse[(int64_t)(qa + tok) * A.num_q_heads + head];
-      __syncthreads();
-      f32x16 S = {};
-#pragma unroll
-      for (int j = 0; j < 2 * NCH; ++j) S = mma16<QT>(kop[j], s_q[j][lane], S);
-      // exp(s' - lse) = 2^(s2 - lse2) f, f the rest of lse's conversion to log2 units (a
-      // rounding of up to 2^-20 there would show in every weight of the row)
-      const float lse2 = lse * kScoreLog2e;
-      const float f = fabsf(lse) < INFINITY ? 1.f - kLn2 * fmaf(lse, kScoreLog2e, -lse2) : 1.f;
-      const float slope2 = SC ? slope2_of(P.sc, head) : 0.f;
-      // keys of the lane's half that the row sees (none of a row that saw no key at all)
-      const int limit = row_ok && lse != -INFINITY ? before + tok + 1 - t0 - 4 * g : 0;
-      const float near = (float)(t0 + 4 * g - (before + tok));
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = out_tok(r, 0);
-        float x;
-        if constexpr (SC == 0) x = fmaf(S[r], P.sc.scale2, -lse2);
-        else x = fmaf(slope2, near + key, (SC == 2 ? capped2_fine(P.sc, S[r]) : S[r] * P.sc.scale2) - lse2);
-        const float p = key < limit ? __builtin_amdgcn_exp2f(x) : 0.f;
-        acc[r] = fmaf(p, f, acc[r]);
-      }
-    }
-    // ---- over the rows: the 32 lanes of each half
-    float sum = 0.f;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float x = acc[r];
-      x += dpp_row<kDppXor1>(x);
-      x += dpp_row<kDppXor2>(x);
-      x += dpp_row<kDppHalfMirror>(x);
-      x += dpp_row<kDppMirror>(x);
-      x += swizzle_xor16(x);
-      if (m == r) sum = x;
-    }
-    const int mine = t0 + out_tok(m, g);  // lane m < 16 of each half
-    if (m < 16 && mine < seq) out[mine] += sum;
+    use(c, u32x4{o[0], o[1], o[2], o[3]}, u32x4{o[4], o[5], o[6], o[7]});
   }
+}
+
+// What a lane's row needs to turn products into weights: exp(s' - lse) = 2^(s2 - lse2) f, f
+// the rest of lse's conversion to log2 units (a rounding of up to 2^-20 there would show in
+// every weight of the row).
+struct RowScore {
+  float lse2, f, slope2;
+  int sees, pos;  // keys that the row sees (none of a row that saw no key at all), its position
+};
+template <int SC>
+__device__ __forceinline__ RowScore row_score(const WeightsParams& P, const Span& x, const RowRef& r, float lse) {
+  RowScore s;
+  s.lse2 = lse * kScoreLog2e;
+  s.f = fabsf(lse) < INFINITY ? 1.f - kLn2 * fmaf(lse, kScoreLog2e, -s.lse2) : 1.f;
+  s.slope2 = SC ? slope2_of(P.sc, r.head) : 0.f;
+  s.pos = x.before + r.tok;
+  s.sees = r.ok && lse != -INFINITY ? s.pos + 1 : 0;
+  return s;
+}
+
+// acc += the weights of the 16 keys of this lane's half of the tile at t0
+template <int SC>
+__device__ __forceinline__ void add_weights(const WeightsParams& P, const RowScore& s, int t0, const f32x16& S, float (&acc)[16]) {
+  const int g = (threadIdx.x & 63) >> 5;
+  const float near = (float)(t0 + 4 * g - s.pos);
+  auto prob = [&](int e) {
+    if constexpr (SC == 0) return __builtin_amdgcn_exp2f(fmaf(S[e], P.sc.scale2, -s.lse2));
+    const float y = SC == 2 ? capped2_fine(P.sc, S[e]) : S[e] * P.sc.scale2;
+    return __builtin_amdgcn_exp2f(fmaf(s.slope2, near + out_tok(e, 0), y - s.lse2));
+  };
+  const int limit = s.sees - t0 - 4 * g;  // keys of the lane's half that the row sees
+  if (__all(limit >= kTile)) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = fmaf(prob(e), s.f, acc[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float p = out_tok(e, 0) < limit ? prob(e) : 0.f;
+      acc[e] = fmaf(p, s.f, acc[e]);
+    }
+  }
+}
+
+// over the rows (the 32 lanes of each half): lane m < 16 gets the sum of key out_tok(m, g)
+__device__ __forceinline__ float sum_rows(const float (&acc)[16]) {
+  const int m = threadIdx.x & 31;
+  float sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    float x = acc[r];
+    x += dpp_row<kDppXor1>(x);
+    x += dpp_row<kDppXor2>(x);
+    x += dpp_row<kDppHalfMirror>(x);
+    x += dpp_row<kDppMirror>(x);
+    x += swizzle_xor16(x);
+    if (m == r) sum = x;
+  }
+  return sum;
+}
+
+// the weights of a request that does not fit: nothing is read, they become NaN as far as
+// there are any
+__device__ __forceinline__ void poison(const oscarop_weights_args_v1& A, float* out, int seq, int part, int parts) {
+  for (int64_t t = (int64_t)part * kThreads + threadIdx.x; t < A.weights_cols && t < seq; t += (int64_t)parts * kThreads) out[t] = NAN;
+}
+
+template <int D, int QT, int SC>
+__global__ __launch_bounds__(kThreads, 2) void weights_few_kernel(WeightsParams P) {
+  constexpr int NCH = D / 32, NQ = NCH / kWaves;  // 16-element chunks per lane half
+  const oscarop_weights_args_v1& A = P.a;
+  const int lane = threadIdx.x & 63, m = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int req = blockIdx.z, kvh = blockIdx.y;
+  const Span x = span_of(A, req);
+  if (x.nq < 1) return;
+  float* out = A.weights + req * A.weights_stride_request + kvh * A.weights_stride_head;
+  if (misfit(A, x.qa, x.nq, x.seq)) return poison(A, out, x.seq, blockIdx.x, gridDim.x);
+  const int step = gridDim.x * kWaves * kTile, t_first = (blockIdx.x * kWaves + wave) * kTile;
+  if ((int)(blockIdx.x * kWaves * kTile) >= x.seq) return;
+  __shared__ __attribute__((aligned(16))) u32x4 s_q[2 * NCH][64];  // Q^T operands of a row block
+  const int nrows = x.nq * (int)P.group.d;
+  for (int n0 = 0; n0 < nrows; n0 += 32) {  // once, unless the batch outgrew the call's max_query_len
+    KeyRegs<D> next;
+    load_keys<D>(P, x, req, kvh, t_first, next);
+    const RowRef r = row_of(P, n0 + m, nrows, kvh);
+    const uint16_t* q = (const uint16_t*)A.q + (int64_t)(x.qa + r.tok) * A.q_stride_token + (int64_t)r.head * D + g * (D / 2);
+    const float lse = A.lse[(int64_t)(x.qa + r.tok) * A.num_q_heads + r.head];
+    if (n0) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      const int c = wave + kWaves * i;
+      unsigned o[8];
+      kpairs16(*(const u32x4*)(q + 16 * c), *(const u32x4*)(q + 16 * c + 8), o);
+      s_q[2 * c][lane] = u32x4{o[0], o[1], o[2], o[3]};
+      s_q[2 * c + 1][lane] = u32x4{o[4], o[5], o[6], o[7]};
+    }
+    const RowScore s = row_score<SC>(P, x, r, lse);
+    __syncthreads();
+    for (int t0 = t_first; t0 < x.seq; t0 += step) {
+      const KeyRegs<D> k = next;
+      if (t0 + step < x.seq) load_keys<D>(P, x, req, kvh, t0 + step, next);
+      // two accumulators, of half the contraction each: the partial sums stay smaller and
+      // fewer roundings follow on each other (the error of one request's weights is 5e-7 so,
+      // 1.2e-6 with one)
+      f32x16 S = {}, S2 = {};
+      key_operands<D, QT>(P, k, [&](int c, u32x4 a, u32x4 b) {
+        f32x16& T = c < NCH / 2 ? S : S2;
+        T = mma16<QT>(a, s_q[2 * c][lane], T);
+        T = mma16<QT>(b, s_q[2 * c + 1][lane], T);
+      });
+      S += S2;
+      float acc[16] = {};
+      add_weights<SC>(P, s, t0, S, acc);
+      const float sum = sum_rows(acc);
+      const int mine = t0 + out_tok(m, g);
+      if (m < 16 && mine < x.seq) out[mine] += sum;
+    }
+  }
+}
+
+template <int D, int QT, int SC>
+__global__ __launch_bounds__(kThreads, 2) void weights_many_kernel(WeightsParams P) {
+  constexpr int NCH = D / 32, NQ = NCH / kWaves;
+  const oscarop_weights_args_v1& A = P.a;
+  const int lane = threadIdx.x & 63, m = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int req = blockIdx.z, kvh = blockIdx.y;
+  const int chunk = blockIdx.x % P.chunks, group0 = blockIdx.x / P.chunks, groups = gridDim.x / P.chunks;
+  const Span x = span_of(A, req);
+  if (x.nq < 1) return;
+  float* out = P.chunks > 1 ? P.part + (((int64_t)req * P.chunks + chunk) * A.cache.num_kv_heads + kvh) * A.weights_cols
+                            : A.weights + req * A.weights_stride_request + kvh * A.weights_stride_head;
+  if (misfit(A, x.qa, x.nq, x.seq)) {
+    if (P.chunks == 1) poison(A, out, x.seq, group0, groups);
+    return;
+  }
+  __shared__ __attribute__((aligned(16))) u32x4 s_q[2][2 * NCH][64];  // Q^T operands of a row block
+  const int nrows = x.nq * (int)P.group.d;
+  for (int tb = group0 * kGroupKeys; tb < x.seq; tb += groups * kGroupKeys) {
+    const Rows rows = rows_of(P, chunk, tb, x.before, nrows);
+    if (rows.first >= rows.end) continue;
+    u32x4 qv[NQ][2];
+    float lse_next;
+    auto load_rows = [&](int rb) {  // this wave's share: chunks wave, wave + kWaves, ...
+      const RowRef r = row_of(P, 32 * rb + m, nrows, kvh);
+      const uint16_t* q = (const uint16_t*)A.q + (int64_t)(x.qa + r.tok) * A.q_stride_token + (int64_t)r.head * D + g * (D / 2);
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        qv[i][0] = *(const u32x4*)(q + 16 * (wave + kWaves * i));
+        qv[i][1] = *(const u32x4*)(q + 16 * (wave + kWaves * i) + 8);
+      }
+      lse_next = A.lse[(int64_t)(x.qa + r.tok) * A.num_q_heads + r.head];
+    };
+    load_rows(rows.first);
+    const int wave_t0 = tb + wave * kKeyTiles * kTile;
+    u32x4 kop[kKeyTiles][2 * NCH];
+#pragma unroll
+    for (int i = 0; i < kKeyTiles; ++i) {
+      KeyRegs<D> k;
+      load_keys<D>(P, x, req, kvh, wave_t0 + i * kTile, k);
+      key_operands<D, QT>(P, k, [&](int c, u32x4 a, u32x4 b) {
+        kop[i][2 * c] = a;
+        kop[i][2 * c + 1] = b;
+      });
+    }
+    float acc[kKeyTiles][16] = {};
+    for (int rb = rows.first; rb < rows.end; ++rb) {
+      const int buf = (rb - rows.first) & 1;
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        const int c = wave + kWaves * i;
+        unsigned o[8];
+        kpairs16(qv[i][0], qv[i][1], o);
+        s_q[buf][2 * c][lane] = u32x4{o[0], o[1], o[2], o[3]};
+        s_q[buf][2 * c + 1][lane] = u32x4{o[4], o[5], o[6], o[7]};
+      }
+      const RowScore s = row_score<SC>(P, x, row_of(P, 32 * rb + m, nrows, kvh), lse_next);
+      if (rb + 1 < rows.end) load_rows(rb + 1);
+      // one barrier a block: the buffer written next was read before the last barrier
+      __syncthreads();
+      f32x16 S[kKeyTiles] = {};
+#pragma unroll
+      for (int j = 0; j < 2 * NCH; ++j) {
+        const u32x4 qop = s_q[buf][j][lane];
+#pragma unroll
+        for (int i = 0; i < kKeyTiles; ++i) S[i] = mma16<QT>(kop[i][j], qop, S[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kKeyTiles; ++i) add_weights<SC>(P, s, wave_t0 + i * kTile, S[i], acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kKeyTiles; ++i) {
+      const float sum = sum_rows(acc[i]);
+      const int mine = wave_t0 + i * kTile + out_tok(m, g);
+      if (m < 16 && mine < x.seq) out[mine] = P.chunks > 1 ? sum : out[mine] + sum;
+    }
+    __syncthreads();  // the next key group's first block goes over a buffer still being read
+  }
+}
+
+// weights += the chunks' sums, in a fixed order: 32 keys per workgroup, the chunks dealt to
+// eight lanes of each
+__global__ __launch_bounds__(256) void weights_sum_kernel(WeightsParams P) {
+  const oscarop_weights_args_v1& A = P.a;
+  const int req = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+  const Span x = span_of(A, req);
+  if (x.nq < 1) return;
+  float* out = A.weights + req * A.weights_stride_request + kvh * A.weights_stride_head;
+  if (misfit(A, x.qa, x.nq, x.seq)) return poison(A, out, x.seq, blockIdx.x, gridDim.x);
+  __shared__ float s_sum[8][32];
+  const int64_t pitch = A.cache.num_kv_heads * A.weights_cols;
+  const float* p = P.part + ((int64_t)req * P.chunks * A.cache.num_kv_heads + kvh) * A.weights_cols;
+  for (int t0 = blockIdx.x * 32; t0 < x.seq; t0 += gridDim.x * 32) {
+    const int t = t0 + lane;
+    float sum = 0.f;
+    if (t < x.seq)
+      for (int c = part; c < P.chunks; c += 8) {
+        const Rows r = rows_of(P, c, t / kGroupKeys * kGroupKeys, x.before, x.nq * (int)P.group.d);
+        sum += r.first < r.end ? p[c * pitch + t] : 0.f;
+      }
+    __syncthreads();
+    s_sum[part][lane] = sum;
+    __syncthreads();
+    if (part == 0 && t < x.seq) {
+#pragma unroll
+      for (int i = 1; i < 8; ++i) sum += s_sum[i][lane];
+      out[t] += sum;
+    }
+  }
+}
+
+// Workgroups of weights_few_kernel that the chip holds, and key tiles of a wave at most.
+constexpr int64_t kFewWorkgroups = 1024;
+constexpr int64_t kFewTiles = 8;
+
+// Row chunks of a call.  A workgroup's key operands cost about as much to load as four row
+// blocks, and one round of the chip is two workgroups per compute unit.
+constexpr int64_t kUnits = 512;
+constexpr int64_t kMinBlocks = 4;
+constexpr int64_t kMaxPart = 256ll << 20;  // bytes of partial sums
+struct Chunks {
+  int64_t count, blocks;
+};
+Chunks chunks_of(const oscarop_weights_args_v1& a) {
+  const int64_t hk = a.cache.num_kv_heads, rows = a.max_query_len * (a.num_q_heads / hk);
+  const int64_t blocks = (rows + 31) / 32, units = a.num_reqs * hk * ((a.max_seq_len + kGroupKeys - 1) / kGroupKeys);
+  if (units < 1 || rows <= kFewRows || blocks < 2 * kMinBlocks || units >= kUnits) return {1, 1 << 30};
+  int64_t count = (kUnits + units - 1) / units;
+  if (count > blocks / kMinBlocks) count = blocks / kMinBlocks;
+  const int64_t most = kMaxPart / (a.num_reqs * hk * a.weights_cols * (int64_t)sizeof(float));
+  if (count > most) count = most;
+  if (count < 2) return {1, 1 << 30};
+  const int64_t per = (blocks + count - 1) / count;
+  return {(blocks + per - 1) / per, per};
 }
 
 }  // namespace
@@ -168,7 +435,11 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams P) {
 using namespace oscar;
 
 extern "C" int64_t oscarop_attn_weights_workspace_bytes_v1(const oscarop_weights_args_v1* args) {
-  return args ? 0 : -22;
+  if (!args || args->num_reqs < 0 || args->max_seq_len < 0 || args->max_query_len < 0 || args->cache.num_kv_heads < 1 ||
+      args->num_q_heads < 1 || args->num_q_heads % args->cache.num_kv_heads || args->weights_cols < 1)
+    return -22;
+  const Chunks c = chunks_of(*args);
+  return c.count > 1 ? args->num_reqs * c.count * args->cache.num_kv_heads * args->weights_cols * (int64_t)sizeof(float) : 0;
 }
 
 extern "C" int oscarop_attn_weights_v1(const oscarop_weights_args_v1* args, const oscarop_score_v1* score, void* stream) {
@@ -209,16 +480,29 @@ extern "C" int oscarop_attn_weights_v1(const oscarop_weights_args_v1* args, cons
   p.a = a;
   p.has_stage = a.staging != nullptr;
   if (a.staging) p.st = *a.staging;
-  p.group = (int)(a.num_q_heads / a.cache.num_kv_heads);
+  p.group = FastDiv::of(a.num_q_heads / a.cache.num_kv_heads);
+  const Chunks chunks = chunks_of(a);
+  const int64_t need = oscarop_attn_weights_workspace_bytes_v1(&a);
+  if (need > 0 && (!a.workspace || a.workspace_bytes < need || (((uintptr_t)a.workspace) & 15)))
+    return fail(-22, "%s: 16-byte aligned workspace of %lld bytes required", name, (long long)need);
+  p.chunks = (int)chunks.count;
+  p.chunk_blocks = (int)chunks.blocks;
+  p.part = (float*)a.workspace;
   hipStream_t s = (hipStream_t)stream;
-  const int64_t per = kWaves * kTile;
-  const dim3 grid((unsigned)((a.max_seq_len + per - 1) / per), (unsigned)a.cache.num_kv_heads, (unsigned)a.num_reqs);
+  const unsigned hk = (unsigned)a.cache.num_kv_heads, reqs = (unsigned)a.num_reqs;
+  const bool few = a.max_query_len * (int64_t)p.group.d <= kFewRows;
+  // key tiles per wave: as many as leave the chip its waves
+  const int64_t tiles = (a.max_seq_len + kTile - 1) / kTile, wgs = (tiles + kWaves - 1) / kWaves;
+  int64_t per_wave = wgs * hk * reqs / kFewWorkgroups;
+  per_wave = per_wave < 1 ? 1 : per_wave > kFewTiles ? kFewTiles : per_wave;
+  const dim3 grid(few ? (unsigned)((wgs + per_wave - 1) / per_wave)
+                      : (unsigned)((a.max_seq_len + kGroupKeys - 1) / kGroupKeys * chunks.count),
+                  hk, reqs);
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, p); };
   auto by_score = [&](auto d, auto qt) {
     constexpr int DD = decltype(d)::value, QT = decltype(qt)::value;
-    if (sc == 0) launch(weights_kernel<DD, QT, 0>);
-    else if (sc == 1) launch(weights_kernel<DD, QT, 1>);
-    else launch(weights_kernel<DD, QT, 2>);
+    if (few) sc == 0 ? launch(weights_few_kernel<DD, QT, 0>) : sc == 1 ? launch(weights_few_kernel<DD, QT, 1>) : launch(weights_few_kernel<DD, QT, 2>);
+    else sc == 0 ? launch(weights_many_kernel<DD, QT, 0>) : sc == 1 ? launch(weights_many_kernel<DD, QT, 1>) : launch(weights_many_kernel<DD, QT, 2>);
   };
   using std::integral_constant;
   if (D == 256) {
@@ -228,6 +512,11 @@ extern "C" int oscarop_attn_weights_v1(const oscarop_weights_args_v1* args, cons
     if (a.q_dtype == OSCAR_F16) by_score(integral_constant<int, 128>{}, integral_constant<int, OSCAR_F16>{});
     else by_score(integral_constant<int, 128>{}, integral_constant<int, OSCAR_BF16>{});
   }
-  OSCAR_CHECK_LAUNCH("weights_kernel");
+  OSCAR_CHECK_LAUNCH(few ? "weights_few_kernel" : "weights_many_kernel");
+  if (p.chunks > 1) {
+    const dim3 sums((unsigned)tiles, hk, reqs);
+    hipLaunchKernelGGL(weights_sum_kernel, sums, dim3(256), 0, s, p);
+    OSCAR_CHECK_LAUNCH("weights_sum_kernel");
+  }
   return 0;
 }
