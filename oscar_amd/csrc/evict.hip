@@ -9,10 +9,15 @@
 // ascending, so that the result is fixed.
 //
 //   evict_select_kernel  one workgroup per (request, KV head): the drop-th smallest weight by
-//                        radix selection, then the lists of places and movers and the new
-//                        weights
-//   evict_move_kernel    the slots' bytes and weights from mover to place, and the places'
-//                        window tags
+//                        radix selection, then the lists of places and movers, and the new
+//                        weights up to the new end
+//   evict_move_kernel    the slots' bytes and weights from mover to place, the places' window
+//                        tags, and the new weights from the new end on
+//
+// The selection is bound by what one compute unit issues, some forty instructions a token
+// in all, not by the 4 bytes per token it reads: the weights lie in LDS as ordered numbers and
+// every thread takes a run of consecutive tokens, so that marks and lists are counted without
+// talk between lanes and only a thread's totals are scanned.
 #include "common.h"
 
 #include "../../include/oscar_operators.h"
@@ -21,7 +26,14 @@ namespace oscar {
 
 namespace {
 
-constexpr int kSelect = 1024;  // threads of a selecting workgroup
+constexpr int kSelect = 1024;          // threads of a selecting workgroup
+constexpr int kSelectWaves = kSelect / 64;
+constexpr int kRun = 32;               // consecutive tokens of a thread at most
+constexpr int kStep = 4;               // of them at a time; a run is a multiple of it
+constexpr int kFew = 256;              // candidates whose ranks are counted pair by pair
+constexpr int kBlock = kSelect * kRun; // tokens held at a time; longer lists are read again in every step
+constexpr int kDigit = 11;             // bits of a digit: the first holds sign, exponent and two more
+constexpr int kBins = 1 << kDigit;     // two a thread
 constexpr int kMove = 256;
 
 struct EvictParams {
@@ -58,31 +70,37 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 }
 
 // exclusive prefix sum over the workgroup of one number per thread; *total gets the sum
-__device__ __forceinline__ int scan(int x, int* total, int* s_part) {
+__device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t* total, uint32_t* s_part) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int v = x;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int y = __shfl_up(v, d);
-    v += lane >= d ? y : 0;
-  }
+  // over the wave: within rows of 16 lanes by row_shr 1, 2, 4, 8, then the rows' last lanes
+  // to the rows behind them (row_bcast 15, 31)
+  uint32_t v = x;
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
   __syncthreads();  // s_part of the call before has been read
   if (lane == 63) s_part[wave] = v;
   __syncthreads();
-  int before = 0, sum = 0;
+  uint32_t before = 0, sum = 0;
 #pragma unroll
-  for (int w = 0; w < kSelect / 64; ++w) {
-    const int p = s_part[w];
-    before += w < wave ? p : 0;
-    sum += p;
+  for (int w = 0; w < kSelectWaves; ++w) {
+    before += w < wave ? s_part[w] : 0;
+    sum += s_part[w];
   }
   *total = sum;
   return before + v - x;
 }
 
+// where number i of a block lies in s_buf: a word is left out every 32, so that the threads'
+// runs start in different banks
+__device__ __forceinline__ int place_of(int i) { return i + i / 32; }
+
 __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
   const oscarop_evict_args_v1& A = P.a;
-  const int tid = threadIdx.x, h = blockIdx.x, r = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.x, r = blockIdx.y;
   const int64_t hk = A.cache.num_kv_heads;
   const Request q = request_of(A, r);
   const float* w = A.weights + r * A.weights_stride_request + h * A.weights_stride_head;
@@ -94,96 +112,269 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
     return;
   }
   const int end = q.tail - q.drop;  // where the tail goes
-  // the tail's weights, then zeros
-  for (int64_t t = end + tid; t < A.weights_cols; t += kSelect) out[t] = t < q.seq - q.drop ? w[t + q.drop] : 0.f;
-  __shared__ int s_hist[256];
-  __shared__ int s_part[kSelect / 64];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_left;
-  // ---- the drop-th smallest: byte by byte from the top, `left` = its rank among those that
-  // share the bytes found so far
+  if (q.drop == 0) {
+    for (int t = tid; t < end; t += kSelect) out[t] = w[t];
+    if (tid == 0) P.counts[list] = 0;
+    return;
+  }
+  for (int t = tid; t < q.sink; t += kSelect) out[t] = w[t];
+  const int n = q.tail - q.sink;  // token sink + i, i < n
+  __shared__ uint32_t s_buf[kBlock + kBlock / 32];
+  __shared__ int s_bin[kBins];
+  __shared__ uint32_t s_part[kSelectWaves];
+  __shared__ uint32_t s_prefix, s_low, s_high;
+  __shared__ int s_left, s_equal, s_places, s_few;
+  __shared__ uint32_t s_cand[kFew];
+  for (int i = tid; i < kBins; i += kSelect) s_bin[i] = 0;
+  if (tid == 0) {
+    s_low = 0xffffffffu;
+    s_high = 0;
+    s_few = 0;
+  }
+  // ---- blocks of the list; thread t has the tokens base + t per + b, b < mine, of a block,
+  // `per` being a multiple of kStep
+  int base = 0, per = 0, mine = 0;
+  auto load = [&](int at, bool copy) __attribute__((always_inline)) {
+    const int many = n - at < kBlock ? n - at : kBlock;
+    base = at;
+    per = (many + kSelect * kStep - 1) / (kSelect * kStep) * kStep;
+    mine = many - tid * per;
+    mine = mine < 0 ? 0 : mine < per ? mine : per;
+    __syncthreads();  // s_buf of the block before has been read
+    for (int b = 0; b < per; b += kStep) {
+      float x[kStep];
+#pragma unroll
+      for (int u = 0; u < kStep; ++u) {
+        const int i = (b + u) * kSelect + tid;
+        x[u] = i < many ? w[q.sink + at + i] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < kStep; ++u) {
+        const int i = (b + u) * kSelect + tid;
+        s_buf[place_of(i)] = i < many ? order_of(x[u]) : 0xffffffffu;
+        // (places get their movers' weights later)
+        if (copy && i < many && q.sink + at + i < end) out[q.sink + at + i] = x[u];
+      }
+    }
+    __syncthreads();
+  };
+  auto each = [&](auto use) __attribute__((always_inline)) {  // use(b, key): of every thread at once, b < mine or not
+    for (int b = 0; b < per; b += kStep) {
+      uint32_t k[kStep];
+#pragma unroll
+      for (int u = 0; u < kStep; ++u) k[u] = s_buf[place_of(tid * per + b + u)];
+#pragma unroll
+      for (int u = 0; u < kStep; ++u) use(b + u, k[u]);
+    }
+  };
+  const bool one = n <= kBlock;
+  auto blocks = [&](auto step) __attribute__((always_inline)) {
+    if (one) return step();
+    for (int at = 0; at < n; at += kBlock) {
+      load(at, false);
+      step();
+    }
+  };
+  // ---- the drop-th smallest, digit by digit from the top.  The bin of the digit that holds
+  // rank `left` among those that share the digits found so far:
   uint32_t prefix = 0;
-  int left = q.drop;  // drop the `left` smallest
-  if (q.drop > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kSelect) s_hist[i] = 0;
-      __syncthreads();
-      for (int t = q.sink + tid; t < q.tail; t += kSelect) {
-        const uint32_t u = order_of(w[t]);
-        if (shift == 24 || (u >> (shift + 8)) == prefix) atomicAdd(&s_hist[(u >> shift) & 255], 1);
+  int left = q.drop, equal = 0;
+  auto find = [&](int bits) __attribute__((always_inline)) {
+    __syncthreads();
+    const uint32_t b0 = s_bin[2 * tid], b1 = s_bin[2 * tid + 1];
+    uint32_t all;
+    const uint32_t before = scan(b0 + b1, &all, s_part);
+    if (before < (uint32_t)left && (uint32_t)left <= before + b0 + b1) {
+      const bool second = (uint32_t)left > before + b0;
+      s_prefix = prefix << bits | (uint32_t)(2 * tid + second);
+      s_left = left - (int)(before + (second ? b0 : 0));
+      s_equal = second ? b1 : b0;
+    }
+    s_bin[2 * tid] = s_bin[2 * tid + 1] = 0;
+    __syncthreads();
+    prefix = s_prefix;
+    left = s_left;
+    equal = s_equal;
+  };
+  auto first_digit = [&]() __attribute__((always_inline)) {
+    each([&](int b, uint32_t k) __attribute__((always_inline)) {
+      // where many lanes have the first one's digit (equal weights) they count as one
+      const int digit = (int)(k >> (32 - kDigit)), first = __builtin_amdgcn_readfirstlane(digit);
+      const uint64_t same = __ballot(b < mine && digit == first);
+      if (b < mine && digit != first) atomicAdd(&s_bin[digit], 1);
+      if (lane == 0 && same) atomicAdd(&s_bin[first], __popcll(same));
+    });
+  };
+  for (int at = 0; at < n; at += kBlock) {
+    load(at, true);
+    first_digit();
+  }
+  find(0);
+  // few candidates: every one's rank among them, pair by pair
+  auto finish = [&](int shift) __attribute__((always_inline)) {
+    blocks([&]() __attribute__((always_inline)) {
+      each([&](int b, uint32_t k) __attribute__((always_inline)) {
+        if (b < mine && k >> shift == prefix) s_cand[atomicAdd(&s_few, 1)] = k;
+      });
+    });
+    __syncthreads();
+    if (tid < equal) {
+      const uint32_t k = s_cand[tid];
+      int below = 0, same = 0;
+      for (int i = 0; i < equal; ++i) {
+        below += s_cand[i] < k;
+        same += s_cand[i] == k;
       }
-      __syncthreads();
-      if (tid == 0) {
-        int b = 0, sum = 0;
-        while (sum + s_hist[b] < left) sum += s_hist[b++];
-        s_prefix = prefix << 8 | b;
-        s_left = left - sum;
+      if (below < left && left <= below + same) {  // equal candidates write the same
+        s_prefix = k;
+        s_left = left - below;
+        s_equal = same;
       }
-      __syncthreads();
-      prefix = s_prefix;
-      left = s_left;
+    }
+    __syncthreads();
+    prefix = s_prefix;
+    left = s_left;
+    equal = s_equal;
+  };
+  constexpr int kShift1 = 32 - kDigit, kShift2 = 32 - 2 * kDigit;
+  if (equal <= kFew) {
+    finish(kShift1);
+  } else {
+    // one value in the bin (equal weights) needs no further digits
+    uint32_t low = 0xffffffffu, high = 0;
+    blocks([&]() __attribute__((always_inline)) {
+      each([&](int b, uint32_t k) __attribute__((always_inline)) {
+        const bool in = b < mine && k >> kShift1 == prefix;
+        low = in && k < low ? k : low;
+        high = in && k > high ? k : high;
+      });
+    });
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) {
+      const uint32_t y = __shfl_xor(low, d), z = __shfl_xor(high, d);
+      low = y < low ? y : low;
+      high = z > high ? z : high;
+    }
+    if (lane == 0 && low <= high) {
+      atomicMin(&s_low, low);
+      atomicMax(&s_high, high);
+    }
+    __syncthreads();
+    auto digit = [&](int shift, int bits) __attribute__((always_inline)) {
+      blocks([&]() __attribute__((always_inline)) {
+        each([&](int b, uint32_t k) __attribute__((always_inline)) {
+          if (b < mine && k >> (shift + bits) == prefix) atomicAdd(&s_bin[(k >> shift) & ((1u << bits) - 1u)], 1);
+        });
+      });
+      find(bits);
+    };
+    if (s_low == s_high) {
+      prefix = s_low;
+    } else {
+      digit(kShift2, kDigit);
+      if (equal <= kFew) finish(kShift2);
+      else digit(0, kShift2);
     }
   }
-  // weights below `prefix` go, and of those equal to it the last `left`: those whose rank
-  // among the equal ones is at least equal - left
-  int equal = 0;
-  if (q.drop > 0) {
-    int mine = 0;
-    for (int t = q.sink + tid; t < q.tail; t += kSelect) mine += order_of(w[t]) == prefix;
-    scan(mine, &equal, s_part);
-  }
-  int32_t* places = P.places + list * P.pairs;
-  int32_t* movers = P.movers + list * P.pairs;
-  for (int t = tid; t < q.sink && t < end; t += kSelect) out[t] = w[t];
-  int n_equal = 0, n_place = 0, n_mover = 0, total;
-  for (int t0 = q.sink; t0 < q.tail; t0 += kSelect) {
-    const int t = t0 + tid;
-    const bool in = t < q.tail;
-    const float x = in ? w[t] : 0.f;
-    const uint32_t u = order_of(x);
-    const bool same = in && q.drop > 0 && u == prefix;
-    const int rank = n_equal + scan(same, &total, s_part);
-    n_equal += total;
-    const bool gone = in && q.drop > 0 && (u < prefix || (same && rank >= equal - left));
-    const bool place = gone && t < end, mover = in && !gone && t >= end;
-    const int at = n_place + scan(place, &total, s_part);
-    n_place += total;
-    const int from = n_mover + scan(mover, &total, s_part);
-    n_mover += total;
-    if (place) places[at] = t;
-    if (mover) movers[from] = t;
-    if (in && !gone && t < end) out[t] = x;
-  }
-  if (tid == 0) P.counts[list] = n_place;
+  // ---- weights below `prefix` go, and of those equal to it the last `left`: those with
+  // `keep` of them before.  Of the tokens before one, L are below and E equal: L +
+  // max(0, E - keep) of them go.
+  const int keep = equal - left;
+  auto gone_before = [&](int below, int same) __attribute__((always_inline)) { return below + (same > keep ? same - keep : 0); };
+  // a thread's tokens' totals, and those of the tokens before its first
+  auto totals = [&](int& below, int& same, int carry_below, int carry_same, int* all_below, int* all_same) __attribute__((always_inline)) {
+    uint32_t mine_both = 0, all;  // below in the low half, equal in the high one: a block has 2^15 tokens
+    each([&](int b, uint32_t k) __attribute__((always_inline)) {
+      mine_both += k < prefix ? 1u : b < mine && k == prefix ? 0x10000u : 0u;
+    });
+    const uint32_t before = scan(mine_both, &all, s_part);
+    below = carry_below + (int)(before & 0xffffu);
+    same = carry_same + (int)(before >> 16);
+    *all_below = carry_below + (int)(all & 0xffffu);
+    *all_same = carry_same + (int)(all >> 16);
+  };
+  // how many go before the new end: the thread that has its token counts on from its own
+  int below = 0, same = 0, all_below = 0, all_same = 0;
+  blocks([&]() __attribute__((always_inline)) {
+    totals(below, same, all_below, all_same, &all_below, &all_same);
+    const int to = end - q.sink - base - tid * per;  // this thread's tokens before the end
+    if (to >= 0 && to < mine) {
+      int l = below, e = same;
+      each([&](int b, uint32_t k) __attribute__((always_inline)) {
+        l += b < to && k < prefix;
+        e += b < to && b < mine && k == prefix;
+      });
+      s_places = gone_before(l, e);
+    }
+  });
+  __syncthreads();
+  const int places = s_places;
+  // ---- the lists: a key's place gets the tokens that go before its own, and whether that
+  // goes; then the block's tokens in order, so that the lists' parts are written side by side
+  int32_t* place_list = P.places + list * P.pairs;
+  int32_t* mover_list = P.movers + list * P.pairs;
+  all_below = all_same = 0;
+  blocks([&]() __attribute__((always_inline)) {
+    if (!one) totals(below, same, all_below, all_same, &all_below, &all_same);
+    int l = below, e = same;
+    each([&](int b, uint32_t k) __attribute__((always_inline)) {
+      const bool equal_one = b < mine && k == prefix, gone = k < prefix || (equal_one && e >= keep);
+      s_buf[place_of(tid * per + b)] = (uint32_t)gone_before(l, e) | (gone ? 0x80000000u : 0u);
+      l += k < prefix;
+      e += equal_one;
+    });
+    __syncthreads();
+    const int many = n - base < kBlock ? n - base : kBlock;
+    for (int i0 = 0; i0 < many; i0 += kStep * kSelect) {
+      uint32_t m[kStep];
+#pragma unroll
+      for (int u = 0; u < kStep; ++u) m[u] = s_buf[place_of(i0 + u * kSelect + tid)];
+#pragma unroll
+      for (int u = 0; u < kStep; ++u) {
+        const int i = i0 + u * kSelect + tid, t = q.sink + base + i, g = (int)(m[u] & 0x7fffffffu);
+        const bool gone = m[u] >> 31;
+        if (i < many && gone && t < end) place_list[g] = t;
+        if (i < many && !gone && t >= end) mover_list[t - end - (g - places)] = t;
+      }
+    }
+  });
+  if (tid == 0) P.counts[list] = places;
 }
 
+// A group of D / 16 lanes per move: 8 bytes of constants and the codes of K and V, 16 bytes a
+// lane (five lanes of eight at head dim 128, nine of sixteen at 256).  Bound by the lines that
+// the scattered slots touch, two read and two written for each move: 128000 moves at head dim
+// 128 15 us, 65 MB.  (Four moves of a group in flight: 17 us.)
+template <int D>
 __global__ __launch_bounds__(kMove) void evict_move_kernel(EvictParams P) {
+  constexpr int L = D / 16, W = D / 64;  // lanes of a move; 16-byte parts of a side's codes
   const oscarop_evict_args_v1& A = P.a;
   const int h = blockIdx.y, r = blockIdx.z;
   const int64_t hk = A.cache.num_kv_heads, list = (int64_t)r * hk + h;
-  const int many = P.counts[list];
-  const int bs = (int)A.cache.block_size, words = (int)A.cache.head_dim / 16;  // 4-byte words of codes
+  const int many = P.counts[list], bs = (int)A.cache.block_size;
   const int32_t* row = A.block_table + (int64_t)r * A.block_table_stride;
-  // 32 lanes per move: two words of constants and `words` of codes for K, then for V
-  const int lane = threadIdx.x & 31;
-  for (int i = (blockIdx.x * kMove + threadIdx.x) / 32; i < many; i += gridDim.x * (kMove / 32)) {
+  const float* w = A.weights + r * A.weights_stride_request + h * A.weights_stride_head;
+  float* out = A.weights_out + r * A.out_stride_request + h * A.out_stride_head;
+  // the tail's weights, then zeros
+  if (const Request q = request_of(A, r); q.ok) {
+    for (int64_t t = q.tail - q.drop + (int64_t)blockIdx.x * kMove + threadIdx.x; t < A.weights_cols; t += (int64_t)gridDim.x * kMove)
+      out[t] = t < q.seq - q.drop ? w[t + q.drop] : 0.f;
+  }
+  const int lane = threadIdx.x % L;
+  const bool v_side = lane > W;
+  const int64_t* stride = v_side ? A.cache.v_stride : A.cache.k_stride;
+  const int64_t s0 = stride[0], s1 = stride[1];
+  uint8_t* base = (v_side ? A.cache.v : A.cache.k) + h * stride[2] + (lane == 0 ? 0 : v_side ? 16 * (lane - 1 - W) : 32 + 16 * (lane - 1));
+  for (int i = (blockIdx.x * kMove + threadIdx.x) / L; i < many; i += gridDim.x * (kMove / L)) {
     const int to = P.places[list * P.pairs + i], from = P.movers[list * P.pairs + i];
     const int64_t bt = row[to / bs], bf = row[from / bs];
-    if (lane == 0)
-      A.weights_out[r * A.out_stride_request + h * A.out_stride_head + to] =
-          A.weights[r * A.weights_stride_request + h * A.weights_stride_head + from];
+    if (lane == L - 1) out[to] = w[from];
     if (bt < 0 || bt >= A.cache.num_blocks || bf < 0 || bf >= A.cache.num_blocks) continue;  // never out of the cache
-    auto move = [&](uint8_t* base, const int64_t* stride, int at) {
-      const int64_t head = h * stride[2] + at;
-      *(uint32_t*)(base + bt * stride[0] + to % bs * stride[1] + head) =
-          *(const uint32_t*)(base + bf * stride[0] + from % bs * stride[1] + head);
-    };
-    for (int x = lane; x < 2 + 2 * words; x += 32) {
-      if (x < 2) move(A.cache.k, A.cache.k_stride, 4 * x);
-      else if (x < 2 + words) move(A.cache.k, A.cache.k_stride, 32 + 4 * (x - 2));
-      else move(A.cache.v, A.cache.v_stride, 4 * (x - 2 - words));
-    }
-    if (lane == 0 && P.has_stage) {
+    uint8_t* dst = base + bt * s0 + to % bs * s1;
+    const uint8_t* src = base + bf * s0 + from % bs * s1;
+    if (lane == 0) *(u32x2*)dst = *(const u32x2*)src;
+    else if (lane <= 2 * W) *(u32x4*)dst = *(const u32x4*)src;
+    if (lane == L - 2 && P.has_stage) {
       int64_t* tag = P.st.owner + bt % P.st.rows * bs + to % bs;
       if (*tag == bt) *tag = -1;
     }
@@ -216,10 +407,9 @@ extern "C" int oscarop_evict_v1(const oscarop_evict_args_v1* args, void* stream)
   if (bs < 1 || bs > (1 << 20) || a.max_drop % bs) return fail(-22, "%s: max_drop must be whole pages", name);
   if (a.block_table_rows < a.num_reqs || a.block_table_cols < 1 || a.block_table_stride < a.block_table_cols)
     return fail(-22, "%s: Missing request block-table rows", name);
-  for (int i = 0; i < 3; ++i)
-    if ((a.cache.k_stride[i] & 3) || (a.cache.v_stride[i] & 3)) return fail(-22, "%s: cache slots must be 4-byte aligned", name);
-  if ((((uintptr_t)a.cache.k) & 3) || (((uintptr_t)a.cache.v) & 3))
-    return fail(-22, "%s: cache slots must be 4-byte aligned", name);
+  if ((a.cache.k_stride[0] & 15) || (a.cache.k_stride[1] & 15) || (a.cache.k_stride[2] & 15) || (((uintptr_t)a.cache.k) & 15) ||
+      (a.cache.v_stride[0] & 15) || (a.cache.v_stride[1] & 15) || (a.cache.v_stride[2] & 15) || (((uintptr_t)a.cache.v) & 15))
+    return fail(-22, "%s: cache slots must be 16-byte aligned", name);
   auto overlap = [&](int64_t head, int64_t request) {
     return (hk > 1 && head < a.weights_cols) || (a.num_reqs > 1 && request < (hk - 1) * head + a.weights_cols);
   };
@@ -244,12 +434,13 @@ extern "C" int oscarop_evict_v1(const oscarop_evict_args_v1* args, void* stream)
   p.places = p.counts + a.num_reqs * hk;
   p.movers = p.places + a.num_reqs * hk * p.pairs;
   hipStream_t s = (hipStream_t)stream;
-  hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)hk, (unsigned)a.num_reqs), dim3(kSelect), 0, s, p);
+  const dim3 lists((unsigned)hk, (unsigned)a.num_reqs);
+  hipLaunchKernelGGL(evict_select_kernel, lists, dim3(kSelect), 0, s, p);
   OSCAR_CHECK_LAUNCH("evict_select_kernel");
-  if (a.max_drop == 0) return 0;
-  const int64_t per = kMove / 32, wgs = (a.max_drop + per - 1) / per;
-  hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)(wgs < 256 ? wgs : 256), (unsigned)hk, (unsigned)a.num_reqs), dim3(kMove), 0, s,
-                     p);
+  const int64_t per = kMove / (D / 16), wgs = (a.max_drop + per - 1) / per;
+  const dim3 grid((unsigned)(wgs < 1 ? 1 : wgs < 256 ? wgs : 256), (unsigned)hk, (unsigned)a.num_reqs);
+  if (D == 256) hipLaunchKernelGGL(evict_move_kernel<256>, grid, dim3(kMove), 0, s, p);
+  else hipLaunchKernelGGL(evict_move_kernel<128>, grid, dim3(kMove), 0, s, p);
   OSCAR_CHECK_LAUNCH("evict_move_kernel");
   return 0;
 }

@@ -40,7 +40,7 @@ def args(**changes):
     (dict(cache_num_kv_heads=0), "out of range"),
     (dict(max_drop=100), "whole pages"),
     (dict(block_table_rows=1), "block-table rows"),
-    (dict(cache_k=(1 << 20) + 2), "4-byte aligned"),
+    (dict(cache_k=(1 << 20) + 2), "16-byte aligned"),
     (dict(weights_stride_head=200), "overlap"),
     (dict(out_stride_request=500), "overlap"),
     (dict(weights_out=(1 << 12) + 4796), "weights_out overlaps"),
