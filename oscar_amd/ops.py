@@ -43,39 +43,46 @@ def _require_cuda(*tensors) -> None:
             raise RuntimeError("OSCAR HIP ops need device tensors (no CPU fallback)")
 
 
-def _one_device(*tensors) -> torch.device:
-    """The device that all the tensors given are on."""
-    _require_cuda(*tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) != 1:
-        raise ValueError(f"OSCAR HIP ops need all tensors on one device, got {sorted(map(str, devices))}")
-    return devices.pop()
+_get_device = getattr(torch._C, "_cuda_getDevice", None)  # the current device's index, as above
 
 
-def _launch(name: str, device: torch.device, *args) -> None:
+def _device_index(*tensors) -> int:
+    """The index of the device that all the tensors given (None: none) are on."""
+    index = None
+    for t in tensors:
+        if t is not None:
+            i = t.get_device()
+            if i != index:
+                if i < 0:
+                    raise RuntimeError("OSCAR HIP ops need device tensors (no CPU fallback)")
+                if index is not None:
+                    raise ValueError(f"OSCAR HIP ops need all tensors on one device, got {index} and {i}")
+                index = i
+    return index
+
+
+def _launch(name: str, index: int, *args) -> None:
     """Call the entry point `name` on the device's current stream, with the device made the
     current one (the library launches there)."""
     call = getattr(_lib.load(), name)
-    if device.index is None or device.index == torch.cuda.current_device():
-        _lib.check(call(*args, C.c_void_p(_stream(device))), name)
-        return
-    with torch.cuda.device(device):
-        _lib.check(call(*args, C.c_void_p(_stream(device))), name)
+    if index == _get_device():
+        status = call(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = call(*args, _raw_stream(index))
+    if status:
+        _lib.check(status, name)
 
 
 def cache_struct(k_cache: torch.Tensor, v_cache: torch.Tensor, head_dim: int) -> _lib.Cache:
     """Byte view of a packed cache pair [num_blocks, block_size, Hk, D] (int8 or bf16)."""
-    k8, v8 = k_cache.view(torch.uint8), v_cache.view(torch.uint8)
-    if k8.ndim != 4 or v8.ndim != 4 or not k8.is_contiguous() or not v8.is_contiguous():
+    if k_cache.ndim != 4 or v_cache.ndim != 4 or not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise ValueError("OSCAR requires contiguous [blocks, tokens, heads, bytes] caches")
-    c = _lib.Cache()
-    c.k, c.v = k8.data_ptr(), v8.data_ptr()
-    c.num_blocks, c.block_size, c.num_kv_heads = k8.shape[0], k8.shape[1], k8.shape[2]
-    c.head_dim = head_dim
-    for i in range(3):
-        c.k_stride[i] = k8.stride(i)
-        c.v_stride[i] = v8.stride(i)
-    return c
+    blocks, tokens, heads, _ = k_cache.shape
+    (k0, k1, k2, _), ks = k_cache.stride(), k_cache.element_size()
+    (v0, v1, v2, _), vs = v_cache.stride(), v_cache.element_size()
+    return _lib.Cache(k_cache.data_ptr(), v_cache.data_ptr(), blocks, tokens, heads, head_dim,
+                      (k0 * ks, k1 * ks, k2 * ks), (v0 * vs, v1 * vs, v2 * vs))
 
 
 def staging_struct(stage, k_cache: torch.Tensor | None = None, head_dim: int | None = None) -> _lib.Staging | None:
@@ -92,11 +99,9 @@ def staging_struct(stage, k_cache: torch.Tensor | None = None, head_dim: int | N
     if k_cache is not None:
         rows = owner.shape[0] if owner.ndim == 2 else 0
         want = (rows, k_cache.shape[1], k_cache.shape[2], head_dim)
-        if rows < 1 or tuple(owner.shape) != want[:2] or tuple(sk.shape) != want or tuple(sv.shape) != want:
+        if rows < 1 or owner.shape != want[:2] or sk.shape != want or sv.shape != want:
             raise ValueError("Invalid streaming staging geometry")
-    s = _lib.Staging()
-    s.stage_k, s.stage_v, s.owner, s.rows = sk.data_ptr(), sv.data_ptr(), owner.data_ptr(), owner.shape[0]
-    return s
+    return _lib.Staging(sk.data_ptr(), sv.data_ptr(), owner.data_ptr(), owner.shape[0])
 
 
 def upload(parts, device) -> list:
@@ -360,12 +365,12 @@ def rotate(x: torch.Tensor, r: torch.Tensor, *, transpose=False, out_dtype=None,
     if out is None:
         out = torch.empty(*x.shape[:-1], d, dtype=out_dtype, device=x.device)
     o2 = out.reshape(rows, d)
-    a = _lib.RotateArgs()
-    a.x, a.x_dtype, a.rows, a.x_stride_row = x2.data_ptr(), _DTYPES[x2.dtype], rows, x2.stride(0)
-    a.r, a.transpose = r.contiguous().data_ptr(), int(bool(transpose))
-    a.out, a.out_dtype, a.out_stride_row, a.head_dim = o2.data_ptr(), _DTYPES[out_dtype], o2.stride(0), d
-    lib = _lib.load()
-    _lib.check(lib.oscar_rotate_v1(C.byref(a), C.c_void_p(_stream(x.device))), "oscar_rotate_v1")
+    r = r.contiguous()
+    a = _lib.RotateArgs(x2.data_ptr(), _DTYPES[x2.dtype], rows, x2.stride(0), r.data_ptr(), int(bool(transpose)),
+                        o2.data_ptr(), _DTYPES[out_dtype], o2.stride(0), d)
+    status = _lib.load().oscar_rotate_v1(C.byref(a), _stream(x.device))
+    if status:
+        _lib.check(status, "oscar_rotate_v1")
     return out
 
 
@@ -376,15 +381,16 @@ def _aligned(x: torch.Tensor) -> torch.Tensor:
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
-def _head_rows(x: torch.Tensor, name: str) -> torch.Tensor:
-    """x [N, H, D] as the kernel reads it: heads next to each other, 16-byte aligned rows."""
-    if x.ndim != 3 or x.shape[2] not in (128, 256):
-        raise ValueError(f"{name} must be [tokens, heads, 128 or 256]")
-    size = x.element_size()
-    if x.stride(2) != 1 or x.shape[1] > 1 and x.stride(1) != x.shape[2] or x.data_ptr() % 16 \
-            or x.shape[0] > 1 and x.stride(0) * size % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
+def _row_stride(x: torch.Tensor) -> int | None:
+    """The token stride of x [N, H, D] if the kernel reads it as it lies: heads next to each
+    other, rows 16-byte aligned."""
+    n, h, d = x.shape
+    s0, s1, s2 = x.stride()
+    if n == 1:
+        s0 = h * d
+    if s2 != 1 or h > 1 and s1 != d or x.data_ptr() % 16 or s0 * x.element_size() % 16:
+        return None
+    return s0
 
 
 def norm_rope(q, k, positions, cos_sin, *, q_weight=None, k_weight=None, eps=1e-6, weight_offset=0.0,
@@ -402,52 +408,48 @@ def norm_rope(q, k, positions, cos_sin, *, q_weight=None, k_weight=None, eps=1e-
     Returns (q_out, k_out): new tensors, or the ones given; q_out=q and k_out=k work in
     place.
     """
-    given = [t for t in (q, k) if t is not None]
-    if not given:
+    x = k if q is None else q
+    if x is None:
         raise ValueError("norm_rope needs queries or keys")
-    dev = _one_device(q, k, positions, cos_sin, q_weight, k_weight, q_out, k_out)
-    dtype, n, d = given[0].dtype, given[0].shape[0], given[0].shape[-1]
-    if dtype not in _DTYPES or any(t.dtype != dtype or t.shape[0] != n or t.shape[-1] != d for t in given):
+    index = _device_index(q, k, positions, cos_sin, q_weight, k_weight, q_out, k_out)
+    dtype, code = x.dtype, _DTYPES.get(x.dtype)
+    if x.ndim != 3 or x.shape[2] not in (128, 256):
+        raise ValueError("q and k must be [tokens, heads, 128 or 256]")
+    n, _, d = x.shape
+    if code is None or k is not None and k is not x and (k.dtype != dtype or k.ndim != 3 or k.shape[0] != n or k.shape[2] != d):
         raise ValueError("q and k must share a float dtype, the token count and the head width")
-    if positions.shape != (n,) or positions.dtype not in (torch.int32, torch.int64):
+    if positions.shape != (n,) or positions.dtype not in (torch.int64, torch.int32):
         raise ValueError("positions must be [tokens] int32 or int64")
-    if cos_sin.ndim != 2 or cos_sin.dtype not in _DTYPES or cos_sin.shape[1] % 16 or not 16 <= cos_sin.shape[1] <= d:
+    rows, rotary = cos_sin.shape if cos_sin.ndim == 2 else (0, 0)
+    if cos_sin.dtype not in _DTYPES or rotary % 16 or not 16 <= rotary <= d:
         raise ValueError("cos_sin must be a float [positions, R] table, R a multiple of 16 up to the head width")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    if any(w.shape != (d,) or w.dtype not in _DTYPES or w.dtype != weights[0].dtype for w in weights):
-        raise ValueError("the norm weights must be [head width] of one float dtype")
-    positions, cos_sin = positions.contiguous(), _aligned(cos_sin)
-    a = _lib.NormRopeArgs()
-    outs, keep = [], [positions, cos_sin]
-    for name, x, weight, out in (("q", q, q_weight, q_out), ("k", k, k_weight, k_out)):
-        if x is None:
-            outs.append(None)
+    positions, cos_sin, wtype, sides = positions.contiguous(), _aligned(cos_sin), None, []
+    for name, y, weight, out in (("q", q, q_weight, q_out), ("k", k, k_weight, k_out)):
+        if y is None:
+            sides.append((None, 0, 0, None, None, None, 0, None))
             continue
-        rows = _head_rows(x, name)
+        stride = _row_stride(y)
+        if stride is None:
+            y = y.clone(memory_format=torch.contiguous_format)
+            stride = y.shape[1] * d
         if out is None:
-            out = torch.empty(x.shape, dtype=dtype, device=dev)
-        elif out.shape != x.shape or out.dtype != dtype or _head_rows(out, name) is not out:
-            raise ValueError(f"{name}_out must have {name}'s shape and type, its heads next to each other and "
-                             "16-byte aligned rows")
+            out, out_stride = torch.empty(y.shape, dtype=dtype, device=y.device), y.shape[1] * d
+        else:
+            out_stride = _row_stride(out) if out.shape == y.shape and out.dtype == dtype else None
+            if out_stride is None:
+                raise ValueError(f"{name}_out must have {name}'s shape and type, its heads next to each other and "
+                                 "16-byte aligned rows")
         if weight is not None:
-            weight = _aligned(weight)
-            setattr(a, f"{name}_weight", weight.data_ptr())
-        heads = "num_q_heads" if name == "q" else "num_kv_heads"
-        setattr(a, name, rows.data_ptr())
-        setattr(a, f"{name}_stride_token", rows.stride(0) if n > 1 else x.shape[1] * d)
-        setattr(a, heads, x.shape[1])
-        setattr(a, f"{name}_out", out.data_ptr())
-        setattr(a, f"{name}_out_stride_token", out.stride(0) if n > 1 else x.shape[1] * d)
-        outs.append(out)
-        keep += [rows, weight]
-    a.num_tokens, a.head_dim, a.dtype = n, d, _DTYPES[dtype]
-    a.weight_dtype = _DTYPES[weights[0].dtype] if weights else OSCAR_F32
-    a.weight_offset, a.eps = float(weight_offset), float(eps)
-    a.positions, a.positions_int64 = positions.data_ptr(), int(positions.dtype == torch.int64)
-    a.cos_sin, a.cos_sin_dtype, a.interleaved = cos_sin.data_ptr(), _DTYPES[cos_sin.dtype], int(bool(interleaved))
-    a.cos_sin_rows, a.rotary_dim = cos_sin.shape
-    _launch("oscarop_norm_rope_v1", dev, C.byref(a))
-    return tuple(outs)
+            if weight.shape != (d,) or weight.dtype not in _DTYPES or wtype not in (None, weight.dtype):
+                raise ValueError("the norm weights must be [head width] of one float dtype")
+            weight, wtype = _aligned(weight), weight.dtype
+        sides.append((y.data_ptr(), stride, y.shape[1], _ptr(weight), out, out.data_ptr(), out_stride, (y, weight)))
+    (qp, qs, hq, qw, q_out, qo, qos, _), (kp, ks, hk, kw, k_out, ko, kos, _) = sides
+    a = _lib.NormRopeArgs(qp, qs, hq, kp, ks, hk, n, d, code, qw, kw, OSCAR_F32 if wtype is None else _DTYPES[wtype],
+                          weight_offset, eps, positions.data_ptr(), positions.dtype == torch.int64, cos_sin.data_ptr(),
+                          _DTYPES[cos_sin.dtype], bool(interleaved), rows, rotary, qo, qos, ko, kos)
+    _launch("oscarop_norm_rope_v1", index, C.byref(a))
+    return q_out, k_out
 
 
 # ------------------------------------------------------------------------ decode attention
@@ -534,14 +536,32 @@ def cu_count(device) -> int:
     return _CU_COUNT[key]
 
 
+def _plan_sizes(plan, block_size: int) -> tuple:
+    """Of a plan's requests with queries: (pages of the longest history, longest length, most
+    queries), worked out once for a plan and page size."""
+    sizes = getattr(plan, "_sizes", None)
+    if sizes is None or sizes[0] != block_size:
+        pages = longest = most = 0
+        for a, b, seq in zip(plan.host_qsl, plan.host_qsl[1:], plan.host_seqs):
+            if b > a:
+                pages = max(pages, -(-(seq - (b - a) if plan.has_new else seq) // block_size))
+                longest, most = max(longest, seq), max(most, b - a)
+        sizes = plan._sizes = (block_size, pages, longest, most)
+    return sizes[1:]
+
+
+def _covers(plan: DecodePlan, n: int) -> bool:
+    """The plan's requests tile the rows [0, n)."""
+    qsl = plan.host_qsl
+    return qsl[0] == 0 and qsl[-1] == n and all(a <= b for a, b in zip(qsl, qsl[1:]))
+
+
 def _check_table(table: torch.Tensor, plan: DecodePlan, block_size: int) -> None:
     """streaming_attention.py:48-53: the block table must cover every history."""
     if table.ndim != 2 or table.shape[0] < len(plan.host_seqs):
         raise ValueError("Missing request block-table rows")
-    for a, b, seq in zip(plan.host_qsl, plan.host_qsl[1:], plan.host_seqs):
-        hist = seq - (b - a) if plan.has_new else seq
-        if b > a and math.ceil(hist / block_size) > table.shape[1]:
-            raise ValueError("Block table cannot cover the history")
+    if _plan_sizes(plan, block_size)[0] > table.shape[1]:
+        raise ValueError("Block table cannot cover the history")
 
 
 def attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, plan: DecodePlan, scale,
@@ -567,10 +587,15 @@ def attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, plan: Decod
         raise ValueError("OSCAR HIP attention requires bf16 or fp16 queries")
     n, hq, _ = q.shape
     dev = q.device
-    if out_rot is None:
-        out_rot = torch.zeros(n, hq, head_dim, dtype=torch.float32, device=dev)
-    if lse is None:
-        lse = torch.full((n, hq), -math.inf, dtype=torch.float32, device=dev)
+    if out_rot is None or lse is None:
+        # rows of no request stay zero (lse -inf); the merge writes every row of a request
+        all_rows = phases == 0 and plan.num_items > 0 and _covers(plan, n)
+        if out_rot is None:
+            out_rot = (torch.empty if all_rows else torch.zeros)(n, hq, head_dim, dtype=torch.float32, device=dev)
+        if lse is None:
+            lse = torch.empty(n, hq, dtype=torch.float32, device=dev)
+            if not all_rows:
+                lse.fill_(-math.inf)
     if plan.num_items == 0 or n == 0:
         if store is not None:
             _lib.check(_lib.load().oscar_store_v1(C.byref(store[0]), C.c_void_p(_stream(dev))), "oscar_store_v1")
@@ -583,8 +608,8 @@ def attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, plan: Decod
         if k_new.dtype != q.dtype or v_new.dtype != q.dtype:
             raise ValueError("Current K/V must match the query dtype")
         k_new, v_new = k_new.contiguous(), v_new.contiguous()
-    table = block_table.to(device=dev, dtype=torch.int32)
-    if table.stride(1) != 1:
+    table = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
+    if table.stride(-1) != 1:
         table = table.contiguous()
     if plan.has_new != (k_new is not None):
         raise ValueError("plan and call disagree on the presence of current K/V")
@@ -592,36 +617,24 @@ def attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, plan: Decod
         raise ValueError("the decode plan has not been uploaded")
     _check_table(table, plan, k_cache.shape[1])
     st = staging_struct(stage, k_cache, head_dim)
-    a = _lib.AttnArgs()
-    a.q, a.num_tokens, a.num_q_heads, a.q_stride_token = q.data_ptr(), n, hq, q.stride(0)
-    if k_new is not None:
-        a.k_new, a.v_new, a.kv_new_stride_token = k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0)
-    a.cache = cache_struct(k_cache, v_cache, head_dim)
-    a.block_table, a.block_table_stride = table.data_ptr(), table.stride(0)
-    a.block_table_rows, a.block_table_cols = table.shape
-    a.query_start_loc, a.seq_lens, a.num_reqs = plan.qsl.data_ptr(), plan.seqs.data_ptr(), plan.seqs.numel()
-    if st is not None:
-        a.staging = C.pointer(st)
-    a.scale = float(scale)
-    a.items, a.num_items = plan.items.data_ptr(), plan.num_items
-    a.groups, a.num_groups = plan.groups.data_ptr(), plan.num_groups
+    ws, ws_bytes = None, 0
     if not static_scratch:
         ws = DeviceScratch.get(dev).attn_workspace(plan.partial_bytes)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    a.max_group_items = plan.max_group_items
-    a.out_rot, a.lse = out_rot.data_ptr(), lse.data_ptr()
-    a.phases = int(phases)
-    a.q_dtype = _DTYPES[q.dtype]
-    lib = _lib.load()
+        ws, ws_bytes = ws.data_ptr(), ws.numel()
+    has_new = k_new is not None
+    a = _lib.AttnArgs(q.data_ptr(), n, hq, q.stride(0), _ptr(k_new), _ptr(v_new), k_new.stride(0) if has_new else 0,
+                      cache_struct(k_cache, v_cache, head_dim), table.data_ptr(), table.stride(0), plan.qsl.data_ptr(),
+                      plan.seqs.data_ptr(), plan.seqs.numel(), None if st is None else C.pointer(st), scale,
+                      plan.items.data_ptr(), plan.num_items, plan.groups.data_ptr(), plan.num_groups, ws, ws_bytes,
+                      plan.max_group_items, out_rot.data_ptr(), lse.data_ptr(), phases, _DTYPES[q.dtype], *table.shape)
+    lib, stream = _lib.load(), _stream(dev)
     if score is not None:
-        _launch("oscarop_attn_decode_v1", dev, C.byref(a), C.byref(score))
-        return out_rot, lse
-    if store is not None:
-        _lib.check(lib.oscar_decode_write_v1(C.byref(store[0]), C.byref(a), C.c_void_p(_stream(dev))),
-                   "oscar_decode_write_v1")
-        return out_rot, lse
-    entry = "oscar_attn_decode_static_v1" if static_scratch else "oscar_attn_decode_v1"
-    _lib.check(getattr(lib, entry)(C.byref(a), C.c_void_p(_stream(dev))), entry)
+        _launch("oscarop_attn_decode_v1", q.get_device(), C.byref(a), C.byref(score))
+    elif store is not None:
+        _lib.check(lib.oscar_decode_write_v1(C.byref(store[0]), C.byref(a), stream), "oscar_decode_write_v1")
+    else:
+        entry = "oscar_attn_decode_static_v1" if static_scratch else "oscar_attn_decode_v1"
+        _lib.check(getattr(lib, entry)(C.byref(a), stream), entry)
     return out_rot, lse
 
 
@@ -684,7 +697,7 @@ def attention_prefill(q, k, v, scale, *, head_dim, history=0, k_cache=None, v_ca
         ws = DeviceScratch.get(q.device).prefill_workspace(need)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
     if score is not None:
-        _launch("oscarop_attn_prefill_v1", q.device, C.byref(a), C.byref(score))
+        _launch("oscarop_attn_prefill_v1", q.get_device(), C.byref(a), C.byref(score))
         return out
     _lib.check(lib.oscar_attn_prefill_v1(C.byref(a), C.c_void_p(_stream(q.device))), "oscar_attn_prefill_v1")
     return out
@@ -732,63 +745,61 @@ def accumulate_weights(q, k_new, k_cache, v_cache, block_table, plan, scale, lse
     r is row r of block_table and of weights; weights is updated in place and returned, the
     same bits whatever runs beside it.
     """
-    dev = _one_device(q, k_new, k_cache, v_cache, block_table, lse, weights, plan.qsl, plan.seqs)
-    score = score_struct(soft_cap, alibi_slopes, q.shape[1], q.device)
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError("OSCAR HIP attention requires bf16 or fp16 queries")
     if plan.qsl is None:
         raise ValueError("the plan has not been uploaded")
+    index = _device_index(q, k_new, k_cache, v_cache, block_table, lse, weights, plan.qsl, plan.seqs)
+    score = score_struct(soft_cap, alibi_slopes, q.shape[1], q.device)
+    code = _DTYPES.get(q.dtype)
+    if code is None or code == OSCAR_F32:
+        raise ValueError("OSCAR HIP attention requires bf16 or fp16 queries")
+    if q.ndim != 3 or q.shape[2] != head_dim:
+        raise ValueError("q must be [tokens, heads, head_dim]")
     n, hq, _ = q.shape
-    hk, reqs = k_cache.shape[2], len(plan.host_seqs)
+    hk, reqs, bs = k_cache.shape[2], len(plan.host_seqs), k_cache.shape[1]
     if plan.has_new != (k_new is not None):
         raise ValueError("plan and call disagree on the presence of current K")
     if plan.host_qsl[-1] > n:
         raise ValueError("the plan has more queries than the call")
-    if q.shape[2] != head_dim or q.stride(2) != 1 or q.stride(1) != head_dim:
-        if q.shape[2] != head_dim:
-            raise ValueError("q must be [tokens, heads, head_dim]")
-        q = q.contiguous()
     if k_new is not None:
         if k_new.dtype != q.dtype or k_new.shape[1:] != (hk, head_dim) or k_new.shape[0] < plan.host_qsl[-1]:
             raise ValueError("Current K must match the queries' type and the cache's heads")
         k_new = k_new.contiguous()
     if lse.dtype != torch.float32 or lse.shape != (n, hq):
         raise ValueError("lse must be fp32 [tokens, query heads]")
-    longest = max((s for a, b, s in zip(plan.host_qsl, plan.host_qsl[1:], plan.host_seqs) if b > a), default=0)
-    if weights.dtype != torch.float32 or weights.ndim != 3 or weights.shape[0] < reqs or weights.shape[1] != hk \
-            or weights.stride(2) != 1 and weights.shape[2] > 1:
-        raise ValueError("weights must be fp32 [requests, KV heads, columns], columns next to each other")
-    if longest > weights.shape[2]:
-        raise ValueError(f"weights have {weights.shape[2]} columns for {longest} tokens")
+    _, longest, most = _plan_sizes(plan, bs)
+    head_stride, request_stride = _weight_strides("weights", weights, reqs, hk, longest)
     if reqs == 0 or n == 0 or longest == 0:
         return weights
-    table = block_table.to(dtype=torch.int32)
+    table = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
     if table.stride(-1) != 1:
         table = table.contiguous()
-    _check_table(table, plan, k_cache.shape[1])
+    _check_table(table, plan, bs)
+    if q.stride(2) != 1 or q.stride(1) != head_dim:
+        q = q.contiguous()
     st = staging_struct(stage, k_cache, head_dim)
     lse = lse.contiguous()
-    a = _lib.WeightsArgs()
-    a.q, a.num_tokens, a.num_q_heads, a.q_stride_token = q.data_ptr(), n, hq, q.stride(0)
-    if k_new is not None:
-        a.k_new, a.k_new_stride_token = k_new.data_ptr(), k_new.stride(0)
-    a.cache = cache_struct(k_cache, v_cache, head_dim)
-    a.block_table, a.block_table_stride = table.data_ptr(), table.stride(0)
-    a.block_table_rows, a.block_table_cols = table.shape
-    a.query_start_loc, a.seq_lens, a.num_reqs = plan.qsl.data_ptr(), plan.seqs.data_ptr(), reqs
-    a.q_dtype, a.scale, a.lse = _DTYPES[q.dtype], float(scale), lse.data_ptr()
-    a.max_seq_len, a.max_query_len = longest, max(b - c for c, b in zip(plan.host_qsl, plan.host_qsl[1:]))
-    if st is not None:
-        a.staging = C.pointer(st)
-    a.weights, a.weights_cols = weights.data_ptr(), weights.shape[2]
-    a.weights_stride_head = weights.stride(1) if hk > 1 else weights.shape[2]
-    a.weights_stride_request = weights.stride(0) if reqs > 1 else hk * a.weights_stride_head
+    a = _lib.WeightsArgs(q.data_ptr(), n, hq, q.stride(0), _ptr(k_new), 0 if k_new is None else k_new.stride(0),
+                         cache_struct(k_cache, v_cache, head_dim), table.data_ptr(), table.stride(0), *table.shape,
+                         plan.qsl.data_ptr(), plan.seqs.data_ptr(), reqs, code, longest, most,
+                         None if st is None else C.pointer(st), scale, lse.data_ptr(), weights.data_ptr(), request_stride,
+                         head_stride, weights.shape[2], None, 0)
     need = _lib.load().oscarop_attn_weights_workspace_bytes_v1(C.byref(a))
     if need > 0:
-        ws = DeviceScratch.get(dev).attn_workspace(need)
+        ws = DeviceScratch.get(q.device).attn_workspace(need)
         a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    _launch("oscarop_attn_weights_v1", dev, C.byref(a), None if score is None else C.byref(score))
+    _launch("oscarop_attn_weights_v1", index, C.byref(a), None if score is None else C.byref(score))
     return weights
+
+
+def _weight_strides(name: str, w: torch.Tensor, reqs: int, hk: int, longest: int) -> tuple:
+    """(head, request) strides of weights for at least reqs requests of up to `longest` tokens."""
+    if w.dtype != torch.float32 or w.ndim != 3 or w.shape[0] < reqs or w.shape[1] != hk \
+            or w.stride(2) != 1 and w.shape[2] > 1:
+        raise ValueError(f"{name} must be fp32 [requests, KV heads, columns], columns next to each other")
+    if longest > w.shape[2]:
+        raise ValueError(f"{name} has {w.shape[2]} columns for {longest} tokens")
+    head = w.stride(1) if hk > 1 else w.shape[2]
+    return head, w.stride(0) if reqs > 1 else hk * head
 
 
 # ------------------------------------------------------------------------ eviction
@@ -801,6 +812,7 @@ class EvictPlan:
     seq_lens: list
     freed: list
     lengths: list        # before
+    longest: int         # of them
     max_drop: int        # tokens
     block_size: int
     requests: torch.Tensor   # device int32 [requests, 4]: length, sink, tail, dropped tokens
@@ -840,7 +852,7 @@ def plan_evict(seq_lens, drop_pages, *, block_size: int, sink_tokens: int = 0, r
         records.append([length, sink_tokens, tail, drop] if many else [length, 0, 0, 0])
         freed.append((-(-length // block_size) - many, -(-length // block_size)))
     dev, = upload([np.asarray(records, np.int32).reshape(-1)], device)
-    return EvictPlan([n - q[3] for n, q in zip(lengths, records)], freed, lengths, max((q[3] for q in records), default=0),
+    return EvictPlan([n - q[3] for n, q in zip(lengths, records)], freed, lengths, max(lengths, default=0), max((q[3] for q in records), default=0),
                      int(block_size), dev.view(-1, 4))
 
 
@@ -858,27 +870,22 @@ def evict(plan: EvictPlan, weights, k_cache, v_cache, block_table, *, head_dim, 
     last layer plan.table(block_table) is the new one, plan.seq_lens the new lengths.  The
     pages between must be the request's own.
     """
-    dev = _one_device(weights, k_cache, v_cache, block_table, weights_out, plan.requests)
+    index = _device_index(weights, k_cache, v_cache, block_table, weights_out, plan.requests)
     cache = cache_struct(k_cache, v_cache, head_dim)
-    reqs, hk, bs = len(plan.lengths), k_cache.shape[2], k_cache.shape[1]
+    reqs, hk, bs, longest = len(plan.lengths), cache.num_kv_heads, cache.block_size, plan.longest
     if plan.block_size != bs:
         raise ValueError(f"the plan is for pages of {plan.block_size} tokens, the cache has {bs}")
     if weights_out is None:
-        weights_out = torch.empty(weights.shape, dtype=torch.float32, device=dev)
-    for name, w in (("weights", weights), ("weights_out", weights_out)):
-        if w.dtype != torch.float32 or w.ndim != 3 or w.shape[0] < reqs or w.shape[1] != hk \
-                or w.stride(2) != 1 and w.shape[2] > 1:
-            raise ValueError(f"{name} must be fp32 [requests, KV heads, columns], columns next to each other")
+        weights_out = torch.empty(weights.shape, dtype=torch.float32, device=weights.device)
+    head, request = _weight_strides("weights", weights, reqs, hk, longest)
+    out_head, out_request = _weight_strides("weights_out", weights_out, reqs, hk, longest)
     if weights.shape != weights_out.shape:
         raise ValueError("weights_out must have the shape of weights")
-    longest = max(plan.lengths, default=0)
-    if longest > weights.shape[2]:
-        raise ValueError(f"weights have {weights.shape[2]} columns for {longest} tokens")
     if reqs < weights.shape[0]:
         weights_out[reqs:].copy_(weights[reqs:])
     if reqs == 0 or weights.shape[2] == 0:
         return weights_out
-    table = block_table.to(dtype=torch.int32)
+    table = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
     if table.ndim != 2 or table.shape[0] < reqs:
         raise ValueError("Missing request block-table rows")
     if -(-longest // bs) > table.shape[1]:
@@ -886,20 +893,10 @@ def evict(plan: EvictPlan, weights, k_cache, v_cache, block_table, *, head_dim, 
     if table.stride(1) != 1:
         table = table.contiguous()
     st = staging_struct(stage, k_cache, head_dim)
-    a = _lib.EvictArgs()
-    a.weights, a.weights_cols, a.weights_out = weights.data_ptr(), weights.shape[2], weights_out.data_ptr()
-    for name, w in (("weights", weights), ("out", weights_out)):
-        head = w.stride(1) if hk > 1 else w.shape[2]
-        setattr(a, f"{name}_stride_head", head)
-        setattr(a, f"{name}_stride_request", w.stride(0) if reqs > 1 else hk * head)
-    a.cache = cache
-    a.block_table, a.block_table_stride = table.data_ptr(), table.stride(0)
-    a.block_table_rows, a.block_table_cols = table.shape
-    a.requests, a.num_reqs, a.max_drop = plan.requests.data_ptr(), reqs, plan.max_drop
-    if st is not None:
-        a.staging = C.pointer(st)
-    need = _lib.load().oscarop_evict_workspace_bytes_v1(reqs, hk, plan.max_drop)
-    ws = DeviceScratch.get(dev).attn_workspace(need)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    _launch("oscarop_evict_v1", dev, C.byref(a))
+    ws = DeviceScratch.get(weights.device).attn_workspace(
+        _lib.load().oscarop_evict_workspace_bytes_v1(reqs, hk, plan.max_drop))
+    a = _lib.EvictArgs(weights.data_ptr(), request, head, weights.shape[2], weights_out.data_ptr(), out_request, out_head,
+                       cache, table.data_ptr(), table.stride(0), *table.shape, plan.requests.data_ptr(), reqs, 0,
+                       plan.max_drop, None if st is None else C.pointer(st), ws.data_ptr(), ws.numel())
+    _launch("oscarop_evict_v1", index, C.byref(a))
     return weights_out
