@@ -4,7 +4,10 @@
 // turn by the token's angles.  A row (one head of one token) lies in head_dim / 8 lanes,
 // 16 bytes of a 16-bit type each, so that its sum of squares is a reduction within 16 or
 // 32 lanes and the other half of a rotated pair, rotary_dim / 2 values away, is whole lanes
-// away.
+// away.  Lanes take HPG heads of their token one after the other: the angles are loaded once
+// for all of them and their rows are in flight together.  Bound by the rows' bytes.
+#include <type_traits>
+
 #include "common.h"
 #include "store_quant.h"
 
@@ -15,18 +18,40 @@ namespace oscar {
 namespace {
 
 constexpr int kThreads = 256;
+// Four heads per lane group from this many bytes of rows on: fewer, longer waves, which cost
+// more while there is one round of them or two and save once memory is the bound.  One head /
+// four, us: 600 tokens of 28 heads of 128 bf16 4.7 / 7.9, 5000 19.1 / 22.0, 15361 (110 MB)
+// 59.1 / 54.3 (48.7 with interleaved pairs, 4.7 TB/s in and out; a large copy reaches 5.1);
+// 10000 of 7 heads of 256 20.6 / 21.7; 5000 of 7 of 256 fp32 (36 MB) 16.7 / 16.0.  Two heads
+// lie between.
+constexpr int64_t kManyBytes = 40 << 20;
 
 struct NormRopeParams {
   oscarop_norm_rope_args_v1 a;
-  FastDiv div_heads;  // num_q_heads + num_kv_heads
-  uint32_t rows;      // tokens x heads
+  FastDiv div_units;  // units of a token: HPG heads each
+  uint32_t units;     // of all tokens
+  int heads;          // num_q_heads + num_kv_heads
 };
 
-// 8 elements at i of an array whose type is known at run time (uniform)
+// 8 (or 4) elements at i of an array whose type is known at run time (uniform)
 __device__ __forceinline__ void load8_of(const void* base, int32_t dtype, int64_t i, float* v) {
   if (dtype == OSCAR_BF16) load8<OSCAR_BF16>(base, i, v);
   else if (dtype == OSCAR_F16) load8<OSCAR_F16>(base, i, v);
   else load8<OSCAR_F32>(base, i, v);
+}
+__device__ __forceinline__ void load4_of(const void* base, int32_t dtype, int64_t i, float* v) {
+  if (dtype == OSCAR_F32) {
+    const f32x4 x = *(const f32x4*)((const float*)base + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = x[e];
+  } else {
+    const u32x2 x = *(const u32x2*)((const uint16_t*)base + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const unsigned short b = (unsigned short)(x[e / 2] >> (16 * (e & 1)));
+      v[e] = dtype == OSCAR_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
+    }
+  }
 }
 
 template <int DT>
@@ -47,81 +72,91 @@ __device__ __forceinline__ void store8(void* base, int64_t i, const float* v) {
   }
 }
 
-template <int D, int DT>
+template <int D, int DT, int HPG>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeParams P) {
   constexpr int L = D / 8;  // lanes of a row
   const oscarop_norm_rope_args_v1& A = P.a;
   const int lane = threadIdx.x & 63, e0 = 8 * (lane % L);
-  const uint32_t row = (uint32_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
-  const bool live = row < P.rows;  // whole lane groups; all lanes stay for the exchanges
-  const uint32_t t = fdiv(live ? row : 0, P.div_heads);
-  const int head = (int)((live ? row : 0) - t * P.div_heads.d);
-  const bool is_q = head < A.num_q_heads;
-  const int64_t in = is_q ? t * A.q_stride_token + (int64_t)head * D
-                          : t * A.k_stride_token + (int64_t)(head - A.num_q_heads) * D;
-  float x[8], w[8];
-  load8<DT>(is_q ? A.q : A.k, in + e0, x);
+  const uint32_t unit = (uint32_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
+  const bool live = unit < P.units;  // whole lane groups; all lanes stay for the exchanges
+  const uint32_t t = fdiv(live ? unit : 0, P.div_units);
+  const int head0 = (int)((live ? unit : 0) - t * P.div_units.d) * HPG;
+  float x[HPG][8];
+#pragma unroll
+  for (int i = 0; i < HPG; ++i) {
+    const int head = head0 + i < P.heads ? head0 + i : head0;
+    if (head < A.num_q_heads) load8<DT>(A.q, t * A.q_stride_token + (int64_t)head * D + e0, x[i]);
+    else load8<DT>(A.k, t * A.k_stride_token + (int64_t)(head - A.num_q_heads) * D + e0, x[i]);
+  }
   const int64_t pos = A.positions_int64 ? ((const int64_t*)A.positions)[t] : ((const int32_t*)A.positions)[t];
   const bool known = pos >= 0 && pos < A.cos_sin_rows;
-  const void* weight = is_q ? A.q_weight : A.k_weight;
-  if (weight != nullptr) {
-    load8_of(weight, A.weight_dtype, e0, w);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] += A.weight_offset;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = 1.f;
-  }
-  float sum = 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
-  sum += dpp_row<kDppXor1>(sum);
-  sum += dpp_row<kDppXor2>(sum);
-  sum += dpp_row<kDppHalfMirror>(sum);
-  sum += dpp_row<kDppMirror>(sum);
-  if constexpr (L == 32) sum += swizzle_xor16(sum);
-  const float r = 1.f / sqrtf(sum * (1.f / D) + A.eps);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
+  // ---- this lane's angles: c and s of its 8 values' pairs (4 when interleaved), 1 and 0 past
+  // the rotated ones
   const int half = (int)A.rotary_dim / 2;
+  const bool turns = e0 < 2 * half, low = e0 < half;
   const int64_t table = (known ? pos : 0) * A.rotary_dim;
-  float y[8];
-  if (A.interleaved) {
-    if (e0 < 2 * half) {
-      float c[4], s[4];
+  float c[8], s[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        c[e] = load_elem(A.cos_sin, A.cos_sin_dtype, table + e0 / 2 + e);
-        s[e] = load_elem(A.cos_sin, A.cos_sin_dtype, table + half + e0 / 2 + e);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[2 * e] = fmaf(x[2 * e], c[e], -(x[2 * e + 1] * s[e]));
-        y[2 * e + 1] = fmaf(x[2 * e + 1], c[e], x[2 * e] * s[e]);
-      }
-    }
-  } else {
-    const bool low = e0 < half;
-    const int other = lane + (low ? half / 8 : -(half / 8));  // a lane of the same row where e0 < rotary_dim
-    float p[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = __shfl(x[e], e0 < 2 * half ? other : lane);
-    if (e0 < 2 * half) {
-      float c[8], s[8];
+  for (int e = 0; e < 8; ++e) {
+    c[e] = 1.f;
+    s[e] = 0.f;
+  }
+  if (turns) {
+    if (A.interleaved) {
+      load4_of(A.cos_sin, A.cos_sin_dtype, table + e0 / 2, c);
+      load4_of(A.cos_sin, A.cos_sin_dtype, table + half + e0 / 2, s);
+    } else {
       load8_of(A.cos_sin, A.cos_sin_dtype, table + (low ? e0 : e0 - half), c);
       load8_of(A.cos_sin, A.cos_sin_dtype, table + half + (low ? e0 : e0 - half), s);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = fmaf(x[e], c[e], (low ? -p[e] : p[e]) * s[e]);
+      for (int e = 0; e < 8; ++e) s[e] = low ? -s[e] : s[e];
     }
   }
-  if (!live) return;
+  const int other = !turns ? lane : low ? lane + half / 8 : lane - half / 8;  // the lane of the pairs' other values
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    y[e] = e0 < 2 * half ? y[e] : x[e];
-    y[e] = known ? y[e] : NAN;
+  for (int i = 0; i < HPG; ++i) {
+    const int head = head0 + i;
+    const bool is_q = head < A.num_q_heads;
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fmaf(x[i][e], x[i][e], sum);
+    sum += dpp_row<kDppXor1>(sum);
+    sum += dpp_row<kDppXor2>(sum);
+    sum += dpp_row<kDppHalfMirror>(sum);
+    sum += dpp_row<kDppMirror>(sum);
+    if constexpr (L == 32) sum += swizzle_xor16(sum);
+    const float r = 1.f / sqrtf(sum * (1.f / D) + A.eps);
+    float w[8], y[8];
+    const void* weight = is_q ? A.q_weight : A.k_weight;
+    if (weight != nullptr) {
+      load8_of(weight, A.weight_dtype, e0, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] += A.weight_offset;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = 1.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[i][e] = x[i][e] * r * w[e];
+    if (A.interleaved) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        y[2 * e] = fmaf(x[i][2 * e], c[e], -(x[i][2 * e + 1] * s[e]));
+        y[2 * e + 1] = fmaf(x[i][2 * e + 1], c[e], x[i][2 * e] * s[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = fmaf(x[i][e], c[e], __shfl(x[i][e], other) * s[e]);
+    }
+    if (!live || head >= P.heads) continue;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      y[e] = turns ? y[e] : x[i][e];  // (0 times an infinity beside it would be NaN)
+      y[e] = known ? y[e] : NAN;
+    }
+    if (is_q) store8<DT>(A.q_out, t * A.q_out_stride_token + (int64_t)head * D + e0, y);
+    else store8<DT>(A.k_out, t * A.k_out_stride_token + (int64_t)(head - A.num_q_heads) * D + e0, y);
   }
-  if (is_q) store8<DT>(A.q_out, t * A.q_out_stride_token + (int64_t)head * D + e0, y);
-  else store8<DT>(A.k_out, t * A.k_out_stride_token + (int64_t)(head - A.num_q_heads) * D + e0, y);
 }
 
 bool aligned16(const void* p) { return (((uintptr_t)p) & 15) == 0; }
@@ -163,21 +198,26 @@ extern "C" int oscarop_norm_rope_v1(const oscarop_norm_rope_args_v1* args, void*
     return fail(-22, "%s: output tokens overlap", name);
   NormRopeParams p{};
   p.a = a;
-  p.div_heads = FastDiv::of(heads);
-  p.rows = (uint32_t)(a.num_tokens * heads);
-  const int64_t per = kThreads / (D / 8);
-  const dim3 grid((unsigned)((p.rows + per - 1) / per));
+  const int hpg = a.num_tokens * heads * D * (16 / v) >= kManyBytes ? 4 : 1;
+  const int64_t units = (heads + hpg - 1) / hpg, per = kThreads / (D / 8);
+  p.div_units = FastDiv::of(units);
+  p.units = (uint32_t)(a.num_tokens * units);
+  p.heads = (int)heads;
+  const dim3 grid((unsigned)((p.units + per - 1) / per));
   hipStream_t s = (hipStream_t)stream;
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, p); };
-  if (D == 256) {
-    if (a.dtype == OSCAR_BF16) launch(norm_rope_kernel<256, OSCAR_BF16>);
-    else if (a.dtype == OSCAR_F16) launch(norm_rope_kernel<256, OSCAR_F16>);
-    else launch(norm_rope_kernel<256, OSCAR_F32>);
-  } else {
-    if (a.dtype == OSCAR_BF16) launch(norm_rope_kernel<128, OSCAR_BF16>);
-    else if (a.dtype == OSCAR_F16) launch(norm_rope_kernel<128, OSCAR_F16>);
-    else launch(norm_rope_kernel<128, OSCAR_F32>);
-  }
+  auto by_heads = [&](auto d, auto dt) {
+    constexpr int DD = decltype(d)::value, DT = decltype(dt)::value;
+    hpg == 4 ? launch(norm_rope_kernel<DD, DT, 4>) : launch(norm_rope_kernel<DD, DT, 1>);
+  };
+  using std::integral_constant;
+  auto by_type = [&](auto d) {
+    if (a.dtype == OSCAR_BF16) by_heads(d, integral_constant<int, OSCAR_BF16>{});
+    else if (a.dtype == OSCAR_F16) by_heads(d, integral_constant<int, OSCAR_F16>{});
+    else by_heads(d, integral_constant<int, OSCAR_F32>{});
+  };
+  if (D == 256) by_type(integral_constant<int, 256>{});
+  else by_type(integral_constant<int, 128>{});
   OSCAR_CHECK_LAUNCH("norm_rope_kernel");
   return 0;
 }

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from dataclasses import dataclass
 
 import numpy as np
@@ -74,15 +75,17 @@ def _launch(name: str, index: int, *args) -> None:
         _lib.check(status, name)
 
 
+_CACHE = struct.Struct("=QQ10q").pack  # _lib.Cache's fields
+
+
 def cache_struct(k_cache: torch.Tensor, v_cache: torch.Tensor, head_dim: int) -> _lib.Cache:
     """Byte view of a packed cache pair [num_blocks, block_size, Hk, D] (int8 or bf16)."""
     if k_cache.ndim != 4 or v_cache.ndim != 4 or not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise ValueError("OSCAR requires contiguous [blocks, tokens, heads, bytes] caches")
-    blocks, tokens, heads, _ = k_cache.shape
-    (k0, k1, k2, _), ks = k_cache.stride(), k_cache.element_size()
-    (v0, v1, v2, _), vs = v_cache.stride(), v_cache.element_size()
-    return _lib.Cache(k_cache.data_ptr(), v_cache.data_ptr(), blocks, tokens, heads, head_dim,
-                      (k0 * ks, k1 * ks, k2 * ks), (v0 * vs, v1 * vs, v2 * vs))
+    blocks, tokens, heads, width = k_cache.shape
+    k2, v2 = width * k_cache.element_size(), v_cache.shape[3] * v_cache.element_size()
+    return _lib.Cache.from_buffer_copy(_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), blocks, tokens, heads, head_dim,
+                                              tokens * heads * k2, heads * k2, k2, tokens * heads * v2, heads * v2, v2))
 
 
 def staging_struct(stage, k_cache: torch.Tensor | None = None, head_dim: int | None = None) -> _lib.Staging | None:
@@ -381,14 +384,15 @@ def _aligned(x: torch.Tensor) -> torch.Tensor:
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
-def _row_stride(x: torch.Tensor) -> int | None:
-    """The token stride of x [N, H, D] if the kernel reads it as it lies: heads next to each
-    other, rows 16-byte aligned."""
-    n, h, d = x.shape
+def _row_stride(x: torch.Tensor, address: int, heads: int, d: int) -> int | None:
+    """The token stride of x [N, heads, d] if the kernel reads it as it lies: heads next to
+    each other, rows 16-byte aligned."""
+    if address % 16:
+        return None
+    if x.is_contiguous():
+        return heads * d
     s0, s1, s2 = x.stride()
-    if n == 1:
-        s0 = h * d
-    if s2 != 1 or h > 1 and s1 != d or x.data_ptr() % 16 or s0 * x.element_size() % 16:
+    if s2 != 1 or heads > 1 and s1 != d or s0 * x.element_size() % 16:
         return None
     return s0
 
@@ -412,42 +416,54 @@ def norm_rope(q, k, positions, cos_sin, *, q_weight=None, k_weight=None, eps=1e-
     if x is None:
         raise ValueError("norm_rope needs queries or keys")
     index = _device_index(q, k, positions, cos_sin, q_weight, k_weight, q_out, k_out)
-    dtype, code = x.dtype, _DTYPES.get(x.dtype)
-    if x.ndim != 3 or x.shape[2] not in (128, 256):
+    dtype = x.dtype
+    code = _DTYPES.get(dtype)
+    if x.ndim != 3:
         raise ValueError("q and k must be [tokens, heads, 128 or 256]")
     n, _, d = x.shape
-    if code is None or k is not None and k is not x and (k.dtype != dtype or k.ndim != 3 or k.shape[0] != n or k.shape[2] != d):
+    if d != 256 and d != 128:
+        raise ValueError("q and k must be [tokens, heads, 128 or 256]")
+    if code is None or k is not x and k is not None and (k.dtype != dtype or k.ndim != 3 or k.shape[::2] != (n, d)):
         raise ValueError("q and k must share a float dtype, the token count and the head width")
-    if positions.shape != (n,) or positions.dtype not in (torch.int64, torch.int32):
+    wide = positions.dtype == torch.int64
+    if not wide and positions.dtype != torch.int32 or positions.shape != (n,):
         raise ValueError("positions must be [tokens] int32 or int64")
     rows, rotary = cos_sin.shape if cos_sin.ndim == 2 else (0, 0)
-    if cos_sin.dtype not in _DTYPES or rotary % 16 or not 16 <= rotary <= d:
+    cs_code = _DTYPES.get(cos_sin.dtype)
+    if cs_code is None or rotary % 16 or not 16 <= rotary <= d:
         raise ValueError("cos_sin must be a float [positions, R] table, R a multiple of 16 up to the head width")
     positions, cos_sin, wtype, sides = positions.contiguous(), _aligned(cos_sin), None, []
     for name, y, weight, out in (("q", q, q_weight, q_out), ("k", k, k_weight, k_out)):
         if y is None:
             sides.append((None, 0, 0, None, None, None, 0, None))
             continue
-        stride = _row_stride(y)
+        heads, address = y.shape[1], y.data_ptr()
+        stride = _row_stride(y, address, heads, d)
         if stride is None:
             y = y.clone(memory_format=torch.contiguous_format)
-            stride = y.shape[1] * d
+            stride, address = heads * d, y.data_ptr()
         if out is None:
-            out, out_stride = torch.empty(y.shape, dtype=dtype, device=y.device), y.shape[1] * d
+            out = torch.empty(n, heads, d, dtype=dtype, device=y.device)
+            out_address, out_stride = out.data_ptr(), heads * d
         else:
-            out_stride = _row_stride(out) if out.shape == y.shape and out.dtype == dtype else None
+            out_address = out.data_ptr()
+            out_stride = _row_stride(out, out_address, heads, d) if out.dtype == dtype and out.shape == y.shape else None
             if out_stride is None:
                 raise ValueError(f"{name}_out must have {name}'s shape and type, its heads next to each other and "
                                  "16-byte aligned rows")
+        gain = None
         if weight is not None:
-            if weight.shape != (d,) or weight.dtype not in _DTYPES or wtype not in (None, weight.dtype):
+            if wtype is None:
+                wtype = weight.dtype
+            if weight.dtype != wtype or weight.shape != (d,) or wtype not in _DTYPES:
                 raise ValueError("the norm weights must be [head width] of one float dtype")
-            weight, wtype = _aligned(weight), weight.dtype
-        sides.append((y.data_ptr(), stride, y.shape[1], _ptr(weight), out, out.data_ptr(), out_stride, (y, weight)))
+            weight = _aligned(weight)
+            gain = weight.data_ptr()
+        sides.append((address, stride, heads, gain, out, out_address, out_stride, (y, weight)))
     (qp, qs, hq, qw, q_out, qo, qos, _), (kp, ks, hk, kw, k_out, ko, kos, _) = sides
     a = _lib.NormRopeArgs(qp, qs, hq, kp, ks, hk, n, d, code, qw, kw, OSCAR_F32 if wtype is None else _DTYPES[wtype],
-                          weight_offset, eps, positions.data_ptr(), positions.dtype == torch.int64, cos_sin.data_ptr(),
-                          _DTYPES[cos_sin.dtype], bool(interleaved), rows, rotary, qo, qos, ko, kos)
+                          weight_offset, eps, positions.data_ptr(), wide, cos_sin.data_ptr(), cs_code,
+                          bool(interleaved), rows, rotary, qo, qos, ko, kos)
     _launch("oscarop_norm_rope_v1", index, C.byref(a))
     return q_out, k_out
 

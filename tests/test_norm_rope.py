@@ -113,6 +113,9 @@ CASES = [
     (301, 3, 5, 128, torch.float32, 16, True, 0.0, "same", torch.float32),
     (129, 1, 1, 128, torch.float32, 48, False, 0.0, "none", torch.bfloat16),
     (4099, 7, 3, 256, torch.bfloat16, 32, True, 1.0, "fp32", torch.float32),
+    # four heads per lane group (rows of 40 MB and more), seven and nine heads of a token
+    (12001, 5, 2, 256, torch.float16, 64, False, 0.0, "same", torch.float32),
+    (9999, 8, 1, 128, torch.float32, 128, True, 0.0, "fp32", torch.float16),
 ]
 
 
