@@ -608,9 +608,9 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
   constexpr float kMasked = SC == 2 ? -3.402823466e38f : -INFINITY;
   // Padding rows have zero queries and are never written, so they need no mask.
   const int all_see = (int)(hist + q0 + 1);  // keys visible to every row of the wave's tile
-  auto mask = [&](int kt) __attribute__((always_inline)) {
+  auto mask = [&](int kt) __attribute__((always_inline)) {  // whether there are any
     const int k0 = kt * kKeys;
-    if (__builtin_expect(k0 + kKeys <= all_see, 1)) return;
+    if (__builtin_expect(k0 + kKeys <= all_see, 1)) return false;
     const int ml = (int)(fresh(ulane) >> 5);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -618,6 +618,7 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
 #pragma unroll
       for (int r = 0; r < 16; ++r) S[nb][r] = 8 * (r >> 2) + (r & 3) >= lim ? kMasked : S[nb][r];
     }
+    return true;
   };
   // p = 2^(S c - m) of element r (exp2 of -inf is 0; rows with no key yet have m = -inf and p = 0)
   // SC: the score of element r (log2 units; -inf where masked) plus x
@@ -626,6 +627,12 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
     if constexpr (SC == 1) return fmaf(S[nb][r], P.sc.scale2, b);
     const float y = capped2(P.sc, S[nb][r]) + b;
     return S[nb][r] == kMasked ? -INFINITY : y;
+  };
+  // SC == 2: the probability of element r from 1 / (1 + e^2u); of a masked one that of -cap,
+  // which the loop puts right
+  auto cap_prob = [&](int nb, int r, float rcp, float nm) __attribute__((always_inline)) {
+    const float b = fmaf(slope2[nb], (float)(8 * (r >> 2) + (r & 3)), bias0[nb] + nm + P.sc.cap2);
+    return __builtin_amdgcn_exp2f(fmaf(-2.f * P.sc.cap2, rcp, b));
   };
   auto prob = [&](int nb, int r, float nm) __attribute__((always_inline)) {
     if constexpr (SC != 0) return __builtin_amdgcn_exp2f(score(nb, r, nm));
@@ -672,6 +679,7 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
     constexpr int NPV = D / 16;   // steps
     constexpr int EPS = 16 / NPV; // elements of S per row block and step
     float nm[NB], pe[NB][2];
+    float cap_e[NB] = {}, cap_r[NB] = {};  // SC == 2: the element before in its second step, the one before that
     u32x4 seen[2] = {};  // all ones where the step's V operand is of a key of this wave's tile
     if constexpr (SM) {
 #pragma unroll
@@ -702,12 +710,30 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
 #pragma unroll
           for (int e = 0; e < EPS; ++e) {
             const int r = EPS * i + e;
-            if (r % 2 == 0 && r > 0) pair_done(nb, r - 1);
-            pe[nb][r & 1] = prob(nb, r, nm[nb]);
-            if (r == 15) pair_done(nb, r);
+            if constexpr (SC != 2) {
+              if (r % 2 == 0 && r > 0) pair_done(nb, r - 1);
+              pe[nb][r & 1] = prob(nb, r, nm[nb]);
+              if (r == 15) pair_done(nb, r);
+            } else {
+              // a capped score is a chain of three steps (e^2u, 1 / (1 + e^2u), the
+              // probability), one a step for three elements at a time
+              if (r >= 4 && r % 2 == 0) pair_done(nb, r - 3);
+              if (r >= 2) pe[nb][r & 1] = cap_prob(nb, r - 2, cap_r[nb], nm[nb]);
+              if (r >= 1) cap_r[nb] = __builtin_amdgcn_rcpf(cap_e[nb] + 1.f);
+              cap_e[nb] = __builtin_amdgcn_exp2f(S[nb][r] * P.sc.exp2_scale);
+            }
           }
         }
         __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if constexpr (SM && SC == 2) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        pair_done(nb, 13);
+        pe[nb][0] = cap_prob(nb, 14, cap_r[nb], nm[nb]);
+        pe[nb][1] = cap_prob(nb, 15, __builtin_amdgcn_rcpf(cap_e[nb] + 1.f), nm[nb]);
+        pair_done(nb, 15);
       }
     }
   };
@@ -748,12 +774,12 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
     // every wave is past QK of kt and PV of kt - 2; kt's V is in its format; kt + 1 has
     // landed (kt + 2's DMAs are outstanding)
     tile_barrier<2 * NDMA>();
-    mask(kt);
+    const bool masked = mask(kt);
     at_tile(kt);
     pv(v_tile(vr), k_tile(next(k1, NK)), std::true_type{});
     kr = k1;
     vr = v1;
-    bool moved = false;
+    bool moved = SC == 2 && masked;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) moved = moved || lsum[nb] > (float)(1 << kLazy) || m_run[nb] == -INFINITY;
     if (__builtin_expect(__any(moved), 0)) {
