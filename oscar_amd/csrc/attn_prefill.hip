@@ -501,6 +501,36 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
     }
   };
 
+  // With a distance bias a row's maximum lies near its own position, and a reference that
+  // starts at the unit's first keys would move, and all of O with it, in every tile of a
+  // steep head.  It starts at the score of the row's own key instead, which it sees in any
+  // case: what is so far below that its probability rounds to nothing in fp16 is below 2^-24
+  // of the row's sum.
+  float m_own[NB];
+  const bool own_first = SC != 0 && P.sc.slopes != nullptr;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) m_own[nb] = -INFINITY;
+  if (own_first) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const Row r = row_of(nb);
+      const uint16_t* krow = (const uint16_t*)cur_k + (r.ok ? r.qi : 0) * A.kv_stride_token;
+      float dot = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        float qf[8], kf[8];
+        load8<QT>(krow, 16 * j + 8 * g, kf);
+        const u32x4 qw = __builtin_bit_cast(u32x4, qreg[nb][j]);
+        load8<QT>(&qw, 0, qf);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot = fmaf(qf[e], kf[e], dot);
+      }
+      auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(dot), __float_as_uint(dot), false, false);
+      dot = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+      m_own[nb] = SC == 2 ? capped2(P.sc, dot) : dot * P.sc.scale2;
+    }
+  }
+
   float m_run[NB], l_run[NB];
   f32x16 O[NB][D / 32];
 #pragma unroll
@@ -745,7 +775,7 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
   mask(kb);
   at_tile(kb);
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) m_run[nb] = row_max(nb);
+  for (int nb = 0; nb < NB; ++nb) m_run[nb] = SC ? fmaxf(row_max(nb), m_own[nb]) : row_max(nb);
   softmax();
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) l_run[nb] = lsum[nb];
@@ -846,8 +876,11 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
     const int rg = (int)(fresh(ulane) >> 5);
     if (!row.ok) continue;
     // O back from the PV scale of bf16 V values (a power of two: exact)
-    const float inv = (l_tot > 0.f) ? (QT == OSCAR_F16 ? 1.f : (float)(1 << kVShift)) / l_tot : 0.f;
-    const float lse2 = (l_tot > 0.f) ? m_run[nb] + log2f(l_tot) : -INFINITY;
+    // (a chunk far from the row's own key, which the reference may be: below 2^-64 of the row
+    // it counts as empty, its reciprocal could overflow)
+    const bool some = l_tot > (SC ? 0x1p-64f : 0.f);
+    const float inv = some ? (QT == OSCAR_F16 ? 1.f : (float)(1 << kVShift)) / l_tot : 0.f;
+    const float lse2 = some ? m_run[nb] + log2f(l_tot) : -INFINITY;
     if (slot >= 0) {
       // a chunk of a split tile: normalised O and its log2-domain LSE (-inf: no key of
       // the chunk visible to the row) for prefill_merge_kernel
@@ -869,7 +902,7 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
       for (int r = 0; r < 16; r += 4)
         store_out<QT>(A, obase + 32 * b + 8 * (r >> 2) + 4 * rg,
                       f32x4{O[nb][b][r] * inv, O[nb][b][r + 1] * inv, O[nb][b][r + 2] * inv, O[nb][b][r + 3] * inv});
-    if (A.lse != nullptr && rg == 0) A.lse[row.qi * A.num_q_heads + row.head] = l_tot > 0.f ? lse2 * kLn2 : -INFINITY;
+    if (A.lse != nullptr && rg == 0) A.lse[row.qi * A.num_q_heads + row.head] = some ? lse2 * kLn2 : -INFINITY;
   }
 }
 
