@@ -29,6 +29,11 @@ constexpr int kKeys = 32;
 constexpr int kRows = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+// SC: how far above the first maximum known the softmax reference of a row starts (log2).  A
+// larger score moves it, and O with it, only from kMargin + kLazy above that maximum on, and
+// the largest probability, 2^-kMargin, still has eight binary orders of normal fp16 below it.
+// 1600 tokens over 8000, capped, us: margin 0 184, 4 172, 6 169.
+constexpr float kMargin = 6.f;
 constexpr int kLazy = 10;     // log2 of the largest row sum of a tile's probabilities before O is rescaled
 // workgroups per CU the register budget of prefill_kernel<D> is set for
 constexpr int prefill_wgs(int D) { return D == 256 ? 1 : 2; }
@@ -483,6 +488,41 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
       qreg[nb][j] = __builtin_bit_cast(QV, r.ok ? *(const u32x4*)(qrow + 16 * j + 8 * g) : u32x4{0u, 0u, 0u, 0u});
   }
   const float c = A.scale * kLog2e;
+  // With a distance bias a row's maximum lies near its own position, and a reference that
+  // starts at the unit's first keys would move, and all of O with it, in every tile of a
+  // steep head.  It starts at the score of the row's own key instead, which it sees in any
+  // case: what is so far below that its probability rounds to nothing in fp16 is below 2^-24
+  // of the row's sum.  (2047 fresh tokens, slopes from 0.4 down: 66 us before, 58 us so.)
+  float m_own[NB];
+  const bool own_first = SC != 0 && P.sc.slopes != nullptr;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) m_own[nb] = -INFINITY;
+  if (own_first) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const Row r = row_of(nb);
+      const uint16_t* krow = (const uint16_t*)cur_k + (r.ok ? r.qi : 0) * A.kv_stride_token;
+      u32x4 kw[D / 16];
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) kw[j] = *(const u32x4*)(krow + 16 * j + 8 * g);
+      __builtin_amdgcn_sched_barrier(0);  // all of them in flight at once
+      float dots[4] = {};
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        float qf[8], kf[8];
+        load8<QT>(&kw[j], 0, kf);
+        const u32x4 qw = __builtin_bit_cast(u32x4, qreg[nb][j]);
+        load8<QT>(&qw, 0, qf);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dots[e & 3] = fmaf(qf[e], kf[e], dots[e & 3]);
+      }
+      float dot = (dots[0] + dots[1]) + (dots[2] + dots[3]);
+      auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(dot), __float_as_uint(dot), false, false);
+      dot = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+      m_own[nb] = (SC == 2 ? capped2(P.sc, dot) : dot * P.sc.scale2) + kMargin;
+    }
+  }
+
   // SC: the rows' slopes (log2 units) and positions, and the bias of a tile's first key
   float slope2[NB] = {}, row_pos[NB] = {}, bias0[NB] = {};
   if constexpr (SC != 0) {
@@ -500,36 +540,6 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
         bias0[nb] = slope2[nb] * ((float)(kt * kKeys + 4 * (int)(ulane >> 5)) - row_pos[nb]);
     }
   };
-
-  // With a distance bias a row's maximum lies near its own position, and a reference that
-  // starts at the unit's first keys would move, and all of O with it, in every tile of a
-  // steep head.  It starts at the score of the row's own key instead, which it sees in any
-  // case: what is so far below that its probability rounds to nothing in fp16 is below 2^-24
-  // of the row's sum.
-  float m_own[NB];
-  const bool own_first = SC != 0 && P.sc.slopes != nullptr;
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) m_own[nb] = -INFINITY;
-  if (own_first) {
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const Row r = row_of(nb);
-      const uint16_t* krow = (const uint16_t*)cur_k + (r.ok ? r.qi : 0) * A.kv_stride_token;
-      float dot = 0.f;
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
-        float qf[8], kf[8];
-        load8<QT>(krow, 16 * j + 8 * g, kf);
-        const u32x4 qw = __builtin_bit_cast(u32x4, qreg[nb][j]);
-        load8<QT>(&qw, 0, qf);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dot = fmaf(qf[e], kf[e], dot);
-      }
-      auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(dot), __float_as_uint(dot), false, false);
-      dot = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-      m_own[nb] = SC == 2 ? capped2(P.sc, dot) : dot * P.sc.scale2;
-    }
-  }
 
   float m_run[NB], l_run[NB];
   f32x16 O[NB][D / 32];
@@ -775,7 +785,7 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
   mask(kb);
   at_tile(kb);
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) m_run[nb] = SC ? fmaxf(row_max(nb), m_own[nb]) : row_max(nb);
+  for (int nb = 0; nb < NB; ++nb) m_run[nb] = SC ? fmaxf(row_max(nb) + (own_first ? 0.f : kMargin), m_own[nb]) : row_max(nb);
   softmax();
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) l_run[nb] = lsum[nb];
