@@ -4,9 +4,10 @@
 // attention call left it.  Keys are those the attention reads: the packed INT2 history, FP32
 // window copies where the owner tag matches, and the current chunk's rows.
 //
-// Probabilities are added up per key, lane by lane (lane l: row l % 32 of a row block), so
-// that the sum over the rows crosses lanes once per key, at the end.  Every number has one
-// owner, so nothing is atomic and results do not depend on the order of workgroups.
+// S = Q K^T of 32 rows and 32 keys leaves a key's scores in one lane pair (lane % 32: the key;
+// registers: the rows), so that the sum over the rows is a sum over registers and crosses
+// lanes once.  Every number has one owner, so nothing is atomic and results do not depend on
+// the order of workgroups.
 //
 //   weights_few_kernel   a batch of at most 32 rows per KV head (decode, verification): the
 //                        queries stay in LDS and every wave streams key tiles past them, the
@@ -174,62 +175,74 @@ __device__ __forceinline__ void key_operands(const WeightsParams& P, const KeyRe
   }
 }
 
-// What a lane's row needs to turn products into weights: exp(s' - lse) = 2^(s2 - lse2) f, f
-// the rest of lse's conversion to log2 units (a rounding of up to 2^-20 there would show in
-// every weight of the row).
-struct RowScore {
-  float lse2, f, slope2;
-  int sees, pos;  // keys that the row sees (none of a row that saw no key at all), its position
+// What the rows of a block need to turn products into weights, in LDS by row:
+// exp(s' - lse) = 2^(s2 - lse2) f, f being the rest of lse's conversion to log2 units (a
+// rounding of up to 2^-20 there would show in every weight of the row).  Rows past the last
+// and rows that saw no key have lse2 = inf and f = 0 (and zero queries).
+struct RowConst {
+  float lse2, f, slope2, tok;
+};
+struct BlockConst {
+  __attribute__((aligned(16))) float lse2[32], f[32], slope2[32], tok[32];
 };
 template <int SC>
-__device__ __forceinline__ RowScore row_score(const WeightsParams& P, const Span& x, const RowRef& r, float lse) {
-  RowScore s;
-  s.lse2 = lse * kScoreLog2e;
-  s.f = fabsf(lse) < INFINITY ? 1.f - kLn2 * fmaf(lse, kScoreLog2e, -s.lse2) : 1.f;
-  s.slope2 = SC ? slope2_of(P.sc, r.head) : 0.f;
-  s.pos = x.before + r.tok;
-  s.sees = r.ok && lse != -INFINITY ? s.pos + 1 : 0;
-  return s;
+__device__ __forceinline__ RowConst row_const(const WeightsParams& P, const RowRef& r, float lse) {
+  const bool sees = r.ok && lse != -INFINITY;
+  RowConst c;
+  c.lse2 = sees ? lse * kScoreLog2e : INFINITY;
+  c.f = !sees ? 0.f : fabsf(lse) < INFINITY ? 1.f - kLn2 * fmaf(lse, kScoreLog2e, -c.lse2) : 1.f;
+  c.slope2 = SC ? slope2_of(P.sc, r.head) : 0.f;
+  c.tok = (float)r.tok;
+  return c;
+}
+__device__ __forceinline__ void put_row(BlockConst& b, int row, const RowConst& c) {
+  b.lse2[row] = c.lse2;
+  b.f[row] = c.f;
+  b.slope2[row] = c.slope2;
+  b.tok[row] = c.tok;
 }
 
-// acc += the weights of the 16 keys of this lane's half of the tile at t0
+// The sum over `rows` rows of the weights of this lane's key of a tile (both lanes of the key
+// get it): register 4 q + i holds row 8 q + 4 g + i.  near: the key's distance to the
+// request's first query; full: every row sees every key of the tile.
 template <int SC>
-__device__ __forceinline__ void add_weights(const WeightsParams& P, const RowScore& s, int t0, const f32x16& S, float (&acc)[16]) {
+__device__ __forceinline__ float sum_weights(const WeightsParams& P, const BlockConst& b, int rows, const f32x16& S, float near,
+                                             bool full) {
   const int g = (threadIdx.x & 63) >> 5;
-  const float near = (float)(t0 + 4 * g - s.pos);
-  auto prob = [&](int e) {
-    if constexpr (SC == 0) return __builtin_amdgcn_exp2f(fmaf(S[e], P.sc.scale2, -s.lse2));
-    const float y = SC == 2 ? capped2_fine(P.sc, S[e]) : S[e] * P.sc.scale2;
-    return __builtin_amdgcn_exp2f(fmaf(s.slope2, near + out_tok(e, 0), y - s.lse2));
-  };
-  const int limit = s.sees - t0 - 4 * g;  // keys of the lane's half that the row sees
-  if (__all(limit >= kTile)) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e] = fmaf(prob(e), s.f, acc[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float p = out_tok(e, 0) < limit ? prob(e) : 0.f;
-      acc[e] = fmaf(p, s.f, acc[e]);
-    }
-  }
-}
-
-// over the rows (the 32 lanes of each half): lane m < 16 gets the sum of key out_tok(m, g)
-__device__ __forceinline__ float sum_rows(const float (&acc)[16]) {
-  const int m = threadIdx.x & 31;
   float sum = 0.f;
+  auto add = [&](auto all, auto fine) __attribute__((always_inline)) {
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    float x = acc[r];
-    x += dpp_row<kDppXor1>(x);
-    x += dpp_row<kDppXor2>(x);
-    x += dpp_row<kDppHalfMirror>(x);
-    x += dpp_row<kDppMirror>(x);
-    x += swizzle_xor16(x);
-    if (m == r) sum = x;
+    for (int q = 0; q < 4; ++q) {
+      if (8 * q >= rows) break;
+      const f32x4 lse2 = *(const f32x4*)&b.lse2[8 * q + 4 * g], f = *(const f32x4*)&b.f[8 * q + 4 * g];
+      f32x4 slope2 = {}, tok = {};
+      if constexpr (SC != 0) slope2 = *(const f32x4*)&b.slope2[8 * q + 4 * g];
+      if constexpr (SC != 0 || !decltype(all)::value) tok = *(const f32x4*)&b.tok[8 * q + 4 * g];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float s = S[4 * q + i];
+        float x;
+        if constexpr (SC == 0) x = fmaf(s, P.sc.scale2, -lse2[i]);
+        else x = fmaf(slope2[i], near - tok[i], (SC == 1 ? s * P.sc.scale2 : decltype(fine)::value ? capped2_small(P.sc, s) : capped2_fine(P.sc, s)) - lse2[i]);
+        float p = __builtin_amdgcn_exp2f(x);
+        if constexpr (!decltype(all)::value) p = near <= tok[i] ? p : 0.f;
+        sum = fmaf(p, f[i], sum);
+      }
+    }
+  };
+  using std::false_type;
+  using std::true_type;
+  if constexpr (SC == 2) {
+    // the whole tile's scores small against the cap, as they are for most: the series alone
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(S[e]));
+    if (__all(top * fabsf(P.sc.over_cap) < kSmallTanh)) full ? add(true_type{}, true_type{}) : add(false_type{}, true_type{});
+    else full ? add(true_type{}, false_type{}) : add(false_type{}, false_type{});
+  } else {
+    full ? add(true_type{}, false_type{}) : add(false_type{}, false_type{});
   }
-  return sum;
+  return sum + swap_halves(sum);
 }
 
 // the weights of a request that does not fit: nothing is read, they become NaN as far as
@@ -238,11 +251,47 @@ __device__ __forceinline__ void poison(const oscarop_weights_args_v1& A, float* 
   for (int64_t t = (int64_t)part * kThreads + threadIdx.x; t < A.weights_cols && t < seq; t += (int64_t)parts * kThreads) out[t] = NAN;
 }
 
+// This wave's part of a row block's queries, as MFMA operands: chunks wave, wave + kWaves, ...
+template <int D>
+struct QueryRegs {
+  u32x4 v[D / 32 / kWaves][2];
+  float lse;
+  RowRef row;
+};
+template <int D>
+__device__ __forceinline__ void load_queries(const WeightsParams& P, const Span& x, int kvh, int n0, QueryRegs<D>& q) {
+  const oscarop_weights_args_v1& A = P.a;
+  const int lane = threadIdx.x & 63, g = lane >> 5, wave = threadIdx.x >> 6;
+  q.row = row_of(P, n0 + (lane & 31), x.nq * (int)P.group.d, kvh);
+  const uint16_t* p = (const uint16_t*)A.q + (int64_t)(x.qa + q.row.tok) * A.q_stride_token + (int64_t)q.row.head * D + g * (D / 2);
+#pragma unroll
+  for (int i = 0; i < D / 32 / kWaves; ++i) {
+    q.v[i][0] = *(const u32x4*)(p + 16 * (wave + kWaves * i));
+    q.v[i][1] = *(const u32x4*)(p + 16 * (wave + kWaves * i) + 8);
+  }
+  q.lse = A.lse[(int64_t)(x.qa + q.row.tok) * A.num_q_heads + q.row.head];
+}
+template <int D, int SC>
+__device__ __forceinline__ void put_queries(const WeightsParams& P, const QueryRegs<D>& q, u32x4 (*s_q)[64], BlockConst& s_row) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const bool sees = q.row.ok && q.lse != -INFINITY;
+#pragma unroll
+  for (int i = 0; i < D / 32 / kWaves; ++i) {
+    const int c = wave + kWaves * i;
+    unsigned o[8];
+    kpairs16(q.v[i][0], q.v[i][1], o);
+    const u32x4 a = {o[0], o[1], o[2], o[3]}, b = {o[4], o[5], o[6], o[7]}, zero = {0u, 0u, 0u, 0u};
+    s_q[2 * c][lane] = sees ? a : zero;
+    s_q[2 * c + 1][lane] = sees ? b : zero;
+  }
+  if (threadIdx.x < 32) put_row(s_row, threadIdx.x, row_const<SC>(P, q.row, q.lse));
+}
+
 template <int D, int QT, int SC>
 __global__ __launch_bounds__(kThreads, 2) void weights_few_kernel(WeightsParams P) {
-  constexpr int NCH = D / 32, NQ = NCH / kWaves;  // 16-element chunks per lane half
+  constexpr int NCH = D / 32;  // 16-element chunks per lane half
   const oscarop_weights_args_v1& A = P.a;
-  const int lane = threadIdx.x & 63, m = lane & 31, g = lane >> 5;
+  const int lane = threadIdx.x & 63, m = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int req = blockIdx.z, kvh = blockIdx.y;
   const Span x = span_of(A, req);
@@ -251,52 +300,47 @@ __global__ __launch_bounds__(kThreads, 2) void weights_few_kernel(WeightsParams 
   if (misfit(A, x.qa, x.nq, x.seq)) return poison(A, out, x.seq, blockIdx.x, gridDim.x);
   const int step = gridDim.x * kWaves * kTile, t_first = (blockIdx.x * kWaves + wave) * kTile;
   if ((int)(blockIdx.x * kWaves * kTile) >= x.seq) return;
-  __shared__ __attribute__((aligned(16))) u32x4 s_q[2 * NCH][64];  // Q^T operands of a row block
+  __shared__ __attribute__((aligned(16))) u32x4 s_q[2 * NCH][64];  // query operands of a row block
+  __shared__ BlockConst s_row;
   const int nrows = x.nq * (int)P.group.d;
   for (int n0 = 0; n0 < nrows; n0 += 32) {  // once, unless the batch outgrew the call's max_query_len
     KeyRegs<D> next;
+    float old_next = 0.f;
     load_keys<D>(P, x, req, kvh, t_first, next);
-    const RowRef r = row_of(P, n0 + m, nrows, kvh);
-    const uint16_t* q = (const uint16_t*)A.q + (int64_t)(x.qa + r.tok) * A.q_stride_token + (int64_t)r.head * D + g * (D / 2);
-    const float lse = A.lse[(int64_t)(x.qa + r.tok) * A.num_q_heads + r.head];
+    if (t_first + m < x.seq) old_next = out[t_first + m];
+    QueryRegs<D> q;
+    load_queries<D>(P, x, kvh, n0, q);
     if (n0) __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      const int c = wave + kWaves * i;
-      unsigned o[8];
-      kpairs16(*(const u32x4*)(q + 16 * c), *(const u32x4*)(q + 16 * c + 8), o);
-      s_q[2 * c][lane] = u32x4{o[0], o[1], o[2], o[3]};
-      s_q[2 * c + 1][lane] = u32x4{o[4], o[5], o[6], o[7]};
-    }
-    const RowScore s = row_score<SC>(P, x, r, lse);
+    put_queries<D, SC>(P, q, s_q, s_row);
     __syncthreads();
     for (int t0 = t_first; t0 < x.seq; t0 += step) {
       const KeyRegs<D> k = next;
-      if (t0 + step < x.seq) load_keys<D>(P, x, req, kvh, t0 + step, next);
+      const float old = old_next;
+      if (t0 + step < x.seq) {
+        load_keys<D>(P, x, req, kvh, t0 + step, next);
+        if (t0 + step + m < x.seq) old_next = out[t0 + step + m];
+      }
       // two accumulators, of half the contraction each: the partial sums stay smaller and
       // fewer roundings follow on each other (the error of one request's weights is 5e-7 so,
       // 1.2e-6 with one)
       f32x16 S = {}, S2 = {};
       key_operands<D, QT>(P, k, [&](int c, u32x4 a, u32x4 b) {
         f32x16& T = c < NCH / 2 ? S : S2;
-        T = mma16<QT>(a, s_q[2 * c][lane], T);
-        T = mma16<QT>(b, s_q[2 * c + 1][lane], T);
+        T = mma16<QT>(s_q[2 * c][lane], a, T);
+        T = mma16<QT>(s_q[2 * c + 1][lane], b, T);
       });
       S += S2;
-      float acc[16] = {};
-      add_weights<SC>(P, s, t0, S, acc);
-      const float sum = sum_rows(acc);
-      const int mine = t0 + out_tok(m, g);
-      if (m < 16 && mine < x.seq) out[mine] += sum;
+      const float sum = sum_weights<SC>(P, s_row, nrows - n0, S, (float)(t0 + m - x.before), t0 + kTile - 1 <= x.before);
+      if (lane < 32 && t0 + m < x.seq) out[t0 + m] = old + sum;
     }
   }
 }
 
 template <int D, int QT, int SC>
 __global__ __launch_bounds__(kThreads, 2) void weights_many_kernel(WeightsParams P) {
-  constexpr int NCH = D / 32, NQ = NCH / kWaves;
+  constexpr int NCH = D / 32;
   const oscarop_weights_args_v1& A = P.a;
-  const int lane = threadIdx.x & 63, m = lane & 31, g = lane >> 5;
+  const int lane = threadIdx.x & 63, m = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int req = blockIdx.z, kvh = blockIdx.y;
   const int chunk = blockIdx.x % P.chunks, group0 = blockIdx.x / P.chunks, groups = gridDim.x / P.chunks;
@@ -308,24 +352,14 @@ __global__ __launch_bounds__(kThreads, 2) void weights_many_kernel(WeightsParams
     if (P.chunks == 1) poison(A, out, x.seq, group0, groups);
     return;
   }
-  __shared__ __attribute__((aligned(16))) u32x4 s_q[2][2 * NCH][64];  // Q^T operands of a row block
+  __shared__ __attribute__((aligned(16))) u32x4 s_q[2][2 * NCH][64];  // query operands of a row block
+  __shared__ BlockConst s_row[2];
   const int nrows = x.nq * (int)P.group.d;
   for (int tb = group0 * kGroupKeys; tb < x.seq; tb += groups * kGroupKeys) {
     const Rows rows = rows_of(P, chunk, tb, x.before, nrows);
     if (rows.first >= rows.end) continue;
-    u32x4 qv[NQ][2];
-    float lse_next;
-    auto load_rows = [&](int rb) {  // this wave's share: chunks wave, wave + kWaves, ...
-      const RowRef r = row_of(P, 32 * rb + m, nrows, kvh);
-      const uint16_t* q = (const uint16_t*)A.q + (int64_t)(x.qa + r.tok) * A.q_stride_token + (int64_t)r.head * D + g * (D / 2);
-#pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        qv[i][0] = *(const u32x4*)(q + 16 * (wave + kWaves * i));
-        qv[i][1] = *(const u32x4*)(q + 16 * (wave + kWaves * i) + 8);
-      }
-      lse_next = A.lse[(int64_t)(x.qa + r.tok) * A.num_q_heads + r.head];
-    };
-    load_rows(rows.first);
+    QueryRegs<D> q;
+    load_queries<D>(P, x, kvh, 32 * rows.first, q);
     const int wave_t0 = tb + wave * kKeyTiles * kTile;
     u32x4 kop[kKeyTiles][2 * NCH];
 #pragma unroll
@@ -337,19 +371,11 @@ __global__ __launch_bounds__(kThreads, 2) void weights_many_kernel(WeightsParams
         kop[i][2 * c + 1] = b;
       });
     }
-    float acc[kKeyTiles][16] = {};
+    float acc[kKeyTiles] = {};
     for (int rb = rows.first; rb < rows.end; ++rb) {
       const int buf = (rb - rows.first) & 1;
-#pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        const int c = wave + kWaves * i;
-        unsigned o[8];
-        kpairs16(qv[i][0], qv[i][1], o);
-        s_q[buf][2 * c][lane] = u32x4{o[0], o[1], o[2], o[3]};
-        s_q[buf][2 * c + 1][lane] = u32x4{o[4], o[5], o[6], o[7]};
-      }
-      const RowScore s = row_score<SC>(P, x, row_of(P, 32 * rb + m, nrows, kvh), lse_next);
-      if (rb + 1 < rows.end) load_rows(rb + 1);
+      put_queries<D, SC>(P, q, s_q[buf], s_row[buf]);
+      if (rb + 1 < rows.end) load_queries<D>(P, x, kvh, 32 * (rb + 1), q);
       // one barrier a block: the buffer written next was read before the last barrier
       __syncthreads();
       f32x16 S[kKeyTiles] = {};
@@ -357,16 +383,19 @@ __global__ __launch_bounds__(kThreads, 2) void weights_many_kernel(WeightsParams
       for (int j = 0; j < 2 * NCH; ++j) {
         const u32x4 qop = s_q[buf][j][lane];
 #pragma unroll
-        for (int i = 0; i < kKeyTiles; ++i) S[i] = mma16<QT>(kop[i][j], qop, S[i]);
+        for (int i = 0; i < kKeyTiles; ++i) S[i] = mma16<QT>(qop, kop[i][j], S[i]);
       }
+      const int first_tok = (int)fdiv((uint32_t)(32 * rb), P.group);
 #pragma unroll
-      for (int i = 0; i < kKeyTiles; ++i) add_weights<SC>(P, s, wave_t0 + i * kTile, S[i], acc[i]);
+      for (int i = 0; i < kKeyTiles; ++i) {
+        const int t0 = wave_t0 + i * kTile;
+        acc[i] += sum_weights<SC>(P, s_row[buf], nrows - 32 * rb, S[i], (float)(t0 + m - x.before), t0 + kTile - 1 <= x.before + first_tok);
+      }
     }
 #pragma unroll
     for (int i = 0; i < kKeyTiles; ++i) {
-      const float sum = sum_rows(acc[i]);
-      const int mine = wave_t0 + i * kTile + out_tok(m, g);
-      if (m < 16 && mine < x.seq) out[mine] = P.chunks > 1 ? sum : out[mine] + sum;
+      const int t = wave_t0 + i * kTile + m;
+      if (lane < 32 && t < x.seq) out[t] = P.chunks > 1 ? acc[i] : out[t] + acc[i];
     }
     __syncthreads();  // the next key group's first block goes over a buffer still being read
   }

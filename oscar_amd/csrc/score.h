@@ -49,16 +49,20 @@ __device__ __forceinline__ float capped2(const Score& f, float s) {
 }
 
 // The same with the relative error of a few roundings also where the score is small
-// against the cap, where the form above keeps cap 2^-22: the series of tanh up to u^11
-// below 0.35 (the first term left out is below 2^-25 of it there).
-__device__ __forceinline__ float capped2_fine(const Score& f, float s) {
+// against the cap, where the form above keeps cap 2^-22: the series of tanh up to u^11 for
+// u < kSmallTanh (the first term left out is below 2^-25 of it there).
+constexpr float kSmallTanh = 0.35f;
+__device__ __forceinline__ float capped2_small(const Score& f, float s) {
   const float u = s * f.over_cap, t = u * u;
   float p = fmaf(t, -1382.f / 155925.f, 62.f / 2835.f);
   p = fmaf(t, p, -17.f / 315.f);
   p = fmaf(t, p, 2.f / 15.f);
   p = fmaf(t, p, -1.f / 3.f);
   const float x = s * f.scale2;
-  return t < 0.35f * 0.35f ? fmaf(x * t, p, x) : capped2(f, s);
+  return fmaf(x * t, p, x);
+}
+__device__ __forceinline__ float capped2_fine(const Score& f, float s) {
+  return fabsf(s * f.over_cap) < kSmallTanh ? capped2_small(f, s) : capped2(f, s);
 }
 
 // the score of a raw product s at `distance` = t - position
