@@ -96,50 +96,54 @@ __device__ __forceinline__ RowRef row_of(const WeightsParams& P, int n, int nrow
   return r;
 }
 
-// One lane's token of a key tile: token t0 + lane % 32, half lane / 32 of its elements.
+// One lane's token of a key tile: token t0 + lane % 32, half lane / 32 of its elements, as
+// loaded.  What it is (KeyKind) shows only when the loads are in.
 enum KeyKind { kNone = 0, kCodes = 1, kStaged = 2, kCurrent = 3 };  // past the length; history; its window copy; the chunk
 template <int D>
 struct KeyRegs {
   u32x4 word[D / 128];  // history: its half of the codes
   unsigned meta;        // history: scale and zero
-  int kind;
-  int64_t at;           // window copy, chunk: its first element
+  int tag;              // history: the low word of its seat's owner tag (tags are -1, -2 or block ids < 2^31)
+  int blk, t;           // history: its block; the token
 };
 
+// the block of the history tile at t0 (0 off the history: a place that may be read)
+__device__ __forceinline__ int block_of_tile(const oscarop_weights_args_v1& A, const Span& x, int req, int t0) {
+  if (t0 >= x.hist) return 0;
+  const int blk = A.block_table[req * A.block_table_stride + t0 / (int)A.cache.block_size];
+  return blk < 0 || blk >= A.cache.num_blocks ? 0 : blk;  // a bad id must not fault
+}
+
+// first key of the i-th tile from t0, far past any length where it would overflow
+__device__ __forceinline__ int tile_at(int t0, int i, int step) {
+  const int64_t t = t0 + (int64_t)i * step;
+  return t < 0x7fffffff ? (int)t : 0x7fffffff;
+}
+
+// (pages hold whole tiles: a tile that ends past the history is read within its page)
 template <int D>
-__device__ __forceinline__ void load_keys(const WeightsParams& P, const Span& x, int req, int kvh, int t0, KeyRegs<D>& k) {
+__device__ __forceinline__ void load_keys(const WeightsParams& P, const Span& x, int kvh, int t0, int blk, KeyRegs<D>& k) {
   const oscarop_weights_args_v1& A = P.a;
-  const int lane = threadIdx.x & 63, t = t0 + (lane & 31), g = lane >> 5, bs = (int)A.cache.block_size;
-  k.kind = kNone;
-  k.at = 0;
+  const int lane = threadIdx.x & 63, g = lane >> 5, bs = (int)A.cache.block_size;
+  k.t = t0 + (lane & 31);
+  k.blk = blk;
+  k.tag = -1;
   if (t0 < x.hist) {
-    int64_t blk = A.block_table[req * A.block_table_stride + t0 / bs];
-    blk = blk < 0 || blk >= A.cache.num_blocks ? 0 : blk;  // a bad id must not fault
     const int off = t0 % bs + (lane & 31);
     const uint8_t* slot = A.cache.k + blk * A.cache.k_stride[0] + off * A.cache.k_stride[1] + kvh * A.cache.k_stride[2];
-    k.meta = *(const unsigned*)slot;  // (pages hold whole tiles: also where t is past the history)
+    k.meta = *(const unsigned*)slot;
 #pragma unroll
     for (int i = 0; i < D / 128; ++i) k.word[i] = *(const u32x4*)(slot + 32 + g * (D / 8) + 16 * i);
-    if (t < x.hist) k.kind = kCodes;
-    if (P.has_stage) {
-      const int64_t seat = (unsigned)blk % (unsigned)P.st.rows * bs + off;
-      if (P.st.owner[seat] == blk && t < x.hist) {
-        k.kind = kStaged;
-        k.at = (seat * A.cache.num_kv_heads + kvh) * D + g * (D / 2);
-      }
-    }
-  }
-  if (A.k_new != nullptr && t >= x.hist && t < x.seq) {
-    k.kind = kCurrent;
-    k.at = (int64_t)(x.qa + t - x.hist) * A.k_new_stride_token + kvh * D + g * (D / 2);
+    if (P.has_stage) k.tag = ((const int*)P.st.owner)[2 * ((int64_t)((unsigned)blk % (unsigned)P.st.rows) * bs + off)];
   }
 }
 
 // The K operands of the lane's half, 16 elements (two operands) at a time: use(c, a, b).
 template <int D, int QT, class Use>
-__device__ __forceinline__ void key_operands(const WeightsParams& P, const KeyRegs<D>& k, Use use) {
+__device__ __forceinline__ void key_operands(const WeightsParams& P, const Span& x, int kvh, const KeyRegs<D>& k, Use use) {
   constexpr int NCH = D / 32;
-  if (__all(k.kind == kCodes)) {
+  const int kind = k.t < x.hist ? (k.tag == k.blk ? kStaged : kCodes) : P.a.k_new != nullptr && k.t < x.seq ? kCurrent : kNone;
+  if (__all(kind == kCodes)) {
     unsigned t_lo, t_hi;
     byte_tables<QT>(k.meta, t_lo, t_hi);
 #pragma unroll
@@ -150,28 +154,43 @@ __device__ __forceinline__ void key_operands(const WeightsParams& P, const KeyRe
     }
     return;
   }
+  const int g = (threadIdx.x & 63) >> 5, bs = (int)P.a.cache.block_size;
+  const int64_t seat = (int64_t)((unsigned)k.blk % (unsigned)(P.has_stage ? P.st.rows : 1)) * bs + k.t % bs;
+  const float* staged = P.st.stage_k + (seat * P.a.cache.num_kv_heads + kvh) * D + g * (D / 2);
+  const uint16_t* row = (const uint16_t*)P.a.k_new + (int64_t)(x.qa + k.t - x.hist) * P.a.k_new_stride_token + kvh * D + g * (D / 2);
   unsigned t_lo = 0, t_hi = 0;
-  if (k.kind == kCodes) byte_tables<QT>(k.meta, t_lo, t_hi);
+  if (kind == kCodes) byte_tables<QT>(k.meta, t_lo, t_hi);
+  constexpr int kAhead = 4;  // chunks whose rows are in flight together: a tile is a chain of these
 #pragma unroll
-  for (int c = 0; c < NCH; ++c) {
-    unsigned o[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-    if (k.kind == kCodes) {
-      lut16(k.word[c >> 2][c & 3], t_lo, t_hi, o);
-    } else if (k.kind == kStaged) {
-      const float* fp = P.st.stage_k + k.at + 16 * c;
-      f32x4 f[4];
+  for (int c0 = 0; c0 < NCH; c0 += kAhead) {
+    f32x4 f[kAhead][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = *(const f32x4*)(fp + 4 * i);
+    for (int c = 0; c < kAhead; ++c) {
+      if (kind == kStaged) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o[i] = hist_pair<QT>(f[0][i], f[1][i]);
-        o[4 + i] = hist_pair<QT>(f[2][i], f[3][i]);
+        for (int i = 0; i < 4; ++i) f[c][i] = *(const f32x4*)(staged + 16 * (c0 + c) + 4 * i);
+      } else if (kind == kCurrent) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) f[c][i] = *(const f32x4*)(row + 16 * (c0 + c) + 8 * i);
       }
-    } else if (k.kind == kCurrent) {
-      const uint16_t* row = (const uint16_t*)P.a.k_new + k.at + 16 * c;
-      kpairs16(*(const u32x4*)row, *(const u32x4*)(row + 8), o);
     }
-    use(c, u32x4{o[0], o[1], o[2], o[3]}, u32x4{o[4], o[5], o[6], o[7]});
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = 0; c < kAhead; ++c) {
+      unsigned o[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+      if (kind == kCodes) {
+        lut16(k.word[(c0 + c) >> 2][(c0 + c) & 3], t_lo, t_hi, o);
+      } else if (kind == kStaged) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[i] = hist_pair<QT>(f[c][0][i], f[c][1][i]);
+          o[4 + i] = hist_pair<QT>(f[c][2][i], f[c][3][i]);
+        }
+      } else if (kind == kCurrent) {
+        kpairs16(__builtin_bit_cast(u32x4, f[c][0]), __builtin_bit_cast(u32x4, f[c][1]), o);
+      }
+      use(c0 + c, u32x4{o[0], o[1], o[2], o[3]}, u32x4{o[4], o[5], o[6], o[7]});
+    }
   }
 }
 
@@ -298,33 +317,42 @@ __global__ __launch_bounds__(kThreads, 2) void weights_few_kernel(WeightsParams 
   if (x.nq < 1) return;
   float* out = A.weights + req * A.weights_stride_request + kvh * A.weights_stride_head;
   if (misfit(A, x.qa, x.nq, x.seq)) return poison(A, out, x.seq, blockIdx.x, gridDim.x);
-  const int step = gridDim.x * kWaves * kTile, t_first = (blockIdx.x * kWaves + wave) * kTile;
-  if ((int)(blockIdx.x * kWaves * kTile) >= x.seq) return;
+  // neighbouring tiles go to different workgroups: the window's are slow ones (their rows come
+  // one line a lane), and those of one compute unit would wait for each other
+  const int step = gridDim.x * kWaves * kTile, t_first = (wave * gridDim.x + blockIdx.x) * kTile;
+  if ((int)(blockIdx.x * kTile) >= x.seq) return;
   __shared__ __attribute__((aligned(16))) u32x4 s_q[2 * NCH][64];  // query operands of a row block
   __shared__ BlockConst s_row;
   const int nrows = x.nq * (int)P.group.d;
   for (int n0 = 0; n0 < nrows; n0 += 32) {  // once, unless the batch outgrew the call's max_query_len
+    // lane i: the block of the wave's tile i (and, every 64 tiles, of the next 64)
+    int blocks = block_of_tile(A, x, req, tile_at(t_first, lane, step));
     KeyRegs<D> next;
     float old_next = 0.f;
-    load_keys<D>(P, x, req, kvh, t_first, next);
+    load_keys<D>(P, x, kvh, t_first, __builtin_amdgcn_readlane(blocks, 0), next);
     if (t_first + m < x.seq) old_next = out[t_first + m];
     QueryRegs<D> q;
     load_queries<D>(P, x, kvh, n0, q);
     if (n0) __syncthreads();
     put_queries<D, SC>(P, q, s_q, s_row);
     __syncthreads();
+    int tile = 0;
     for (int t0 = t_first; t0 < x.seq; t0 += step) {
       const KeyRegs<D> k = next;
       const float old = old_next;
       if (t0 + step < x.seq) {
-        load_keys<D>(P, x, req, kvh, t0 + step, next);
+        if (++tile == 64) {
+          tile = 0;
+          blocks = block_of_tile(A, x, req, tile_at(t0 + step, lane, step));
+        }
+        load_keys<D>(P, x, kvh, t0 + step, __builtin_amdgcn_readlane(blocks, tile), next);
         if (t0 + step + m < x.seq) old_next = out[t0 + step + m];
       }
       // two accumulators, of half the contraction each: the partial sums stay smaller and
       // fewer roundings follow on each other (the error of one request's weights is 5e-7 so,
       // 1.2e-6 with one)
       f32x16 S = {}, S2 = {};
-      key_operands<D, QT>(P, k, [&](int c, u32x4 a, u32x4 b) {
+      key_operands<D, QT>(P, x, kvh, k, [&](int c, u32x4 a, u32x4 b) {
         f32x16& T = c < NCH / 2 ? S : S2;
         T = mma16<QT>(s_q[2 * c][lane], a, T);
         T = mma16<QT>(s_q[2 * c + 1][lane], b, T);
@@ -365,8 +393,8 @@ __global__ __launch_bounds__(kThreads, 2) void weights_many_kernel(WeightsParams
 #pragma unroll
     for (int i = 0; i < kKeyTiles; ++i) {
       KeyRegs<D> k;
-      load_keys<D>(P, x, req, kvh, wave_t0 + i * kTile, k);
-      key_operands<D, QT>(P, k, [&](int c, u32x4 a, u32x4 b) {
+      load_keys<D>(P, x, kvh, wave_t0 + i * kTile, block_of_tile(A, x, req, wave_t0 + i * kTile), k);
+      key_operands<D, QT>(P, x, kvh, k, [&](int c, u32x4 a, u32x4 b) {
         kop[i][2 * c] = a;
         kop[i][2 * c + 1] = b;
       });
@@ -433,8 +461,8 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(WeightsParams P) {
 }
 
 // Workgroups of weights_few_kernel that the chip holds, and key tiles of a wave at most.
-constexpr int64_t kFewWorkgroups = 1024;
-constexpr int64_t kFewTiles = 8;
+constexpr int64_t kFewWorkgroups = 768;
+constexpr int64_t kFewTiles = 16;
 
 // Row chunks of a call.  A workgroup's key operands cost about as much to load as four row
 // blocks, and one round of the chip is two workgroups per compute unit.
@@ -520,11 +548,12 @@ extern "C" int oscarop_attn_weights_v1(const oscarop_weights_args_v1* args, cons
   hipStream_t s = (hipStream_t)stream;
   const unsigned hk = (unsigned)a.cache.num_kv_heads, reqs = (unsigned)a.num_reqs;
   const bool few = a.max_query_len * (int64_t)p.group.d <= kFewRows;
-  // key tiles per wave: as many as leave the chip its waves
-  const int64_t tiles = (a.max_seq_len + kTile - 1) / kTile, wgs = (tiles + kWaves - 1) / kWaves;
-  int64_t per_wave = wgs * hk * reqs / kFewWorkgroups;
-  per_wave = per_wave < 1 ? 1 : per_wave > kFewTiles ? kFewTiles : per_wave;
-  const dim3 grid(few ? (unsigned)((wgs + per_wave - 1) / per_wave)
+  // few: a workgroup per key tile as long as the chip holds them all, then more tiles each
+  const int64_t tiles = (a.max_seq_len + kTile - 1) / kTile;
+  int64_t few_wgs = kFewWorkgroups / ((int64_t)hk * reqs);
+  const int64_t least = (tiles + kWaves * kFewTiles - 1) / (kWaves * kFewTiles);
+  few_wgs = few_wgs < least ? least : few_wgs > tiles ? tiles : few_wgs;
+  const dim3 grid(few ? (unsigned)few_wgs
                       : (unsigned)((a.max_seq_len + kGroupKeys - 1) / kGroupKeys * chunks.count),
                   hk, reqs);
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, p); };
