@@ -27,6 +27,13 @@ layer's FP32 window arena):
   (``oscar_attn_prefill_v1``; prefill.py:69-72, slab_attention.py:376-476).
 * ``norm_rope(q, k, positions, cos_sin, q_weight, k_weight, eps, weight_offset,
   interleaved) -> (q, k)``: head norms with the position rotation (``oscarop_norm_rope_v1``).
+* ``accumulate_weights(q, k_new, k_cache, v_cache, block_table, query_start_loc, seq_lens,
+  scale, lse, weights!, head_dim, stage_k, stage_v, owner, soft_cap, alibi_slopes) -> ()``:
+  the attention weight each cached token received (``oscarop_attn_weights_v1``); the request
+  lists are host integers.
+* ``evict(weights, k_cache!, v_cache!, block_table, seq_lens, drop_pages, stage_k, stage_v,
+  owner!, head_dim, sink_tokens, recent_tokens) -> weights``: drops the tokens of
+  least weight, whole pages at a time (``oscarop_evict_v1``).
 """
 from __future__ import annotations
 
@@ -142,3 +149,37 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin
 @norm_rope.register_fake
 def _(q, k, positions, cos_sin, q_weight=None, k_weight=None, eps=1e-6, weight_offset=0.0, interleaved=False):
     return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+# ------------------------------------------------------------------ accumulated weights, eviction
+@torch.library.custom_op(f"{_LIB}::accumulate_weights", mutates_args=("weights",), device_types="cuda")
+def accumulate_weights(q: torch.Tensor, k_new: torch.Tensor | None, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                       block_table: torch.Tensor, query_start_loc: list[int], seq_lens: list[int], scale: float,
+                       lse: torch.Tensor, weights: torch.Tensor, head_dim: int, stage_k: torch.Tensor | None = None,
+                       stage_v: torch.Tensor | None = None, owner: torch.Tensor | None = None, soft_cap: float = 0.0,
+                       alibi_slopes: torch.Tensor | None = None) -> None:
+    plan = ops.plan_weights(query_start_loc, seq_lens, has_new=k_new is not None, device=q.device)
+    ops.accumulate_weights(q, k_new, k_cache, v_cache, block_table, plan, scale, lse, weights,
+                           _stage(stage_k, stage_v, owner), head_dim=head_dim, soft_cap=soft_cap, alibi_slopes=alibi_slopes)
+
+
+@accumulate_weights.register_fake
+def _(q, k_new, k_cache, v_cache, block_table, query_start_loc, seq_lens, scale, lse, weights, head_dim, stage_k=None,
+      stage_v=None, owner=None, soft_cap=0.0, alibi_slopes=None):
+    return None
+
+
+@torch.library.custom_op(f"{_LIB}::evict", mutates_args=("k_cache", "v_cache", "owner"), device_types="cuda")
+def evict(weights: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+          seq_lens: list[int], drop_pages: list[int], stage_k: torch.Tensor | None, stage_v: torch.Tensor | None,
+          owner: torch.Tensor | None, head_dim: int, sink_tokens: int = 0, recent_tokens: int = 0) -> torch.Tensor:
+    plan = ops.plan_evict(seq_lens, drop_pages, block_size=k_cache.shape[1], sink_tokens=sink_tokens,
+                          recent_tokens=recent_tokens, device=weights.device)
+    return ops.evict(plan, weights, k_cache, v_cache, block_table, head_dim=head_dim,
+                     stage=_stage(stage_k, stage_v, owner))
+
+
+@evict.register_fake
+def _(weights, k_cache, v_cache, block_table, seq_lens, drop_pages, stage_k, stage_v, owner, head_dim, sink_tokens=0,
+      recent_tokens=0):
+    return weights.new_empty(weights.shape)
