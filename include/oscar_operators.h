@@ -23,7 +23,7 @@ extern "C" {
  * soft_cap 0 leaves s as it is, a NULL alibi_slopes adds nothing.  Keys a query does not
  * see stay unseen whatever their score. */
 typedef struct oscarop_score_v1 {
-  float soft_cap;               /* finite, >= 0 */
+  float soft_cap;               /* 0, or in [2^-20, 1024] */
   const float* alibi_slopes;    /* [num_q_heads] fp32 device, or NULL */
 } oscarop_score_v1;
 
@@ -89,7 +89,7 @@ int oscarop_norm_rope_v1(const oscarop_norm_rope_args_v1* args, void* stream);
  * reads nothing and its weights become NaN. */
 typedef struct oscarop_weights_args_v1 {
   const void* q;                /* [num_tokens, num_q_heads, D] in q_dtype */
-  int64_t num_tokens;
+  int64_t num_tokens;           /* at most 2^24 */
   int64_t num_q_heads;
   int64_t q_stride_token;       /* elements */
   const void* k_new;            /* [num_tokens, Hk, D] current chunk, or NULL (cache only) */
@@ -105,7 +105,7 @@ typedef struct oscarop_weights_args_v1 {
   int32_t q_dtype;              /* OSCAR_BF16 or OSCAR_F16 */
   /* the longest length and the most queries of a request: they size the launch, and any
    * batch gives the same results */
-  int64_t max_seq_len;
+  int64_t max_seq_len;          /* at most 2^30, as weights_cols */
   int64_t max_query_len;
   const oscar_staging_v1* staging; /* NULL = no window; its v side is not read */
   float scale;

@@ -1316,7 +1316,7 @@ int launch_checked(const oscar_attn_args_v1& a, const char* name, void* partials
   const int64_t D = a.cache.head_dim;
   AttnParams p{};
   const int sc = score_of(score, a.scale, &p.sc);
-  if (sc < 0) return fail(-22, "%s: soft_cap must be a finite number, 0 for none", name);
+  if (sc < 0) return fail(-22, kBadCap, name);
   if (D != 128 && D != 256) return fail(-22, "%s: head_dim %lld unsupported", name, (long long)D);
   if (a.num_items <= 0 || a.num_groups <= 0) {
     StoreParams sp{};

@@ -1068,7 +1068,7 @@ static int prefill_launch(const oscar_prefill_args_v1* args, const oscarop_score
     return fail(-22, "%s: 16-byte aligned workspace of %lld bytes required", name, (long long)need);
   PrefillParams p{};
   const int sc = score_of(score, a.scale, &p.sc);
-  if (sc < 0) return fail(-22, "%s: soft_cap must be a finite number, 0 for none", name);
+  if (sc < 0) return fail(-22, kBadCap, name);
   p.a = a;
   p.has_stage = a.staging != nullptr;
   if (a.staging) p.st = *a.staging;

@@ -22,13 +22,19 @@ struct Score {
 
 constexpr float kScoreLog2e = 1.4426950408889634f;
 
-// 0, 1 or 2 (see above); -22 for a cap that is not a finite number >= 0
+// The caps that are taken: up to 2^10, since a capped score keeps cap 2^-22 (capped2), which
+// has to stay below the roundings of a probability (2^-12 of it); from 2^-20, since scale / cap
+// has to be a finite number.
+constexpr float kLeastCap = 9.5367431640625e-7f, kMostCap = 1024.f;
+constexpr char kBadCap[] = "%s: soft_cap must lie in [2^-20, 1024], 0 for none";
+
+// 0, 1 or 2 (see above); -22 for a cap that is not taken
 inline int score_of(const oscarop_score_v1* score, float scale, Score* out) {
   *out = Score{};
   out->scale2 = scale * kScoreLog2e;
   if (score == nullptr) return 0;
   const float cap = score->soft_cap;
-  if (!(cap >= 0.f && cap <= 3.0e38f)) return -22;
+  if (cap != 0.f && !(cap >= kLeastCap && cap <= kMostCap)) return -22;
   out->slopes = score->alibi_slopes;
   if (cap == 0.f) return out->slopes != nullptr ? 1 : 0;
   out->cap2 = cap * kScoreLog2e;

@@ -124,7 +124,7 @@ extern "C" int oscarop_decode_step_v1(oscar_context_v1* ctx, oscar_step_args_v1*
   a.workspace_needed = 0;
   Score checked;
   if (score_of(score, a.scale, &checked) < 0)
-    return fail(-22, "oscarop_decode_step_v1: soft_cap must be a finite number, 0 for none");
+    return fail(-22, kBadCap, "oscarop_decode_step_v1");
   const int64_t n = a.num_tokens, hq = a.num_q_heads, hk = a.cache.num_kv_heads, d = a.cache.head_dim;
   const int B = a.num_reqs;
   if (n <= 0 || B <= 0 || hk < 1 || hq % hk || !a.host_query_start_loc || !a.host_seq_lens || !a.query ||

@@ -239,8 +239,8 @@ def score_struct(soft_cap, alibi_slopes, num_q_heads: int, device) -> _lib.Score
             raise ValueError(f"alibi_slopes must be a contiguous fp32 [{num_q_heads}] tensor")
         if alibi_slopes.device != device:
             raise ValueError(f"alibi_slopes are on {alibi_slopes.device}, the queries on {device}")
-    if not 0 <= soft_cap < math.inf:
-        raise ValueError("soft_cap must be a finite number, 0 for none")
+    if soft_cap != 0 and not 2.0 ** -20 <= soft_cap <= 1024:
+        raise ValueError(f"soft_cap must lie in [2^-20, 1024], 0 for none, got {soft_cap}")
     if soft_cap == 0 and alibi_slopes is None:
         return None
     return _lib.Score(float(soft_cap), _ptr(alibi_slopes))
@@ -591,8 +591,8 @@ def attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, plan: Decod
     rotated outputs are q / k_new / v_new: one oscar_decode_write_v1 call runs the store
     and the decode (a small store's quantization then rides in the merge launch).
     soft_cap, alibi_slopes [Hq] fp32: a score s (scaled) of key t for a query at position p
-    becomes soft_cap tanh(s / soft_cap) + alibi_slopes[h] (t - p); 0 and None leave it.  The
-    position is that in the cache, so tokens that were evicted do not count."""
+    becomes soft_cap tanh(s / soft_cap) + alibi_slopes[h] (t - p); 0 and None leave it, a cap
+    lies in [2^-20, 1024] (a score keeps 2^-22 of it).  The position is that in the cache, so tokens that were evicted do not count."""
     _require_cuda(q, k_cache, v_cache, block_table)
     if store is not None and static_scratch:
         raise ValueError("store= goes with the workspace decode only")
@@ -624,7 +624,9 @@ def attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, plan: Decod
         if k_new.dtype != q.dtype or v_new.dtype != q.dtype:
             raise ValueError("Current K/V must match the query dtype")
         k_new, v_new = k_new.contiguous(), v_new.contiguous()
-    table = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
+    table = block_table
+    if table.dtype != torch.int32 or table.get_device() != q.get_device():
+        table = table.to(device=dev, dtype=torch.int32)
     if table.stride(-1) != 1:
         table = table.contiguous()
     if plan.has_new != (k_new is not None):
@@ -763,7 +765,7 @@ def accumulate_weights(q, k_new, k_cache, v_cache, block_table, plan, scale, lse
     """
     if plan.qsl is None:
         raise ValueError("the plan has not been uploaded")
-    index = _device_index(q, k_new, k_cache, v_cache, block_table, lse, weights, plan.qsl, plan.seqs)
+    index = _device_index(q, k_new, k_cache, v_cache, block_table, lse, weights, plan.qsl, plan.seqs, *(stage or ()))
     score = score_struct(soft_cap, alibi_slopes, q.shape[1], q.device)
     code = _DTYPES.get(q.dtype)
     if code is None or code == OSCAR_F32:
@@ -794,15 +796,16 @@ def accumulate_weights(q, k_new, k_cache, v_cache, block_table, plan, scale, lse
         q = q.contiguous()
     st = staging_struct(stage, k_cache, head_dim)
     lse = lse.contiguous()
-    a = _lib.WeightsArgs(q.data_ptr(), n, hq, q.stride(0), _ptr(k_new), 0 if k_new is None else k_new.stride(0),
+    rows = n if k_new is None else min(n, k_new.shape[0])  # what a plan's lists on the device may reach
+    a = _lib.WeightsArgs(q.data_ptr(), rows, hq, q.stride(0), _ptr(k_new), 0 if k_new is None else k_new.stride(0),
                          cache_struct(k_cache, v_cache, head_dim), table.data_ptr(), table.stride(0), *table.shape,
                          plan.qsl.data_ptr(), plan.seqs.data_ptr(), reqs, code, longest, most,
                          None if st is None else C.pointer(st), scale, lse.data_ptr(), weights.data_ptr(), request_stride,
                          head_stride, weights.shape[2], None, 0)
     need = _lib.load().oscarop_attn_weights_workspace_bytes_v1(C.byref(a))
     if need > 0:
-        ws = DeviceScratch.get(q.device).attn_workspace(need)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)  # a captured call keeps its own
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
     _launch("oscarop_attn_weights_v1", index, C.byref(a), None if score is None else C.byref(score))
     return weights
 
@@ -836,8 +839,12 @@ class EvictPlan:
     def table(self, block_table: torch.Tensor) -> torch.Tensor:
         """The block table after the last layer's evict: each request's kept pages in their
         order, then its free ones."""
-        length, _, tail, drop = self.requests.to(torch.int64).t()[..., None]
         bs, many = self.block_size, len(self.lengths)
+        if block_table.ndim != 2 or block_table.shape[0] < many:
+            raise ValueError("Missing request block-table rows")
+        if -(-self.longest // bs) > block_table.shape[1]:
+            raise ValueError("Block table cannot cover the history")
+        length, _, tail, drop = self.requests.to(torch.int64).t()[..., None]
         pages, end, gone = -(-length // bs), (tail - drop) // bs, drop // bs
         col = torch.arange(block_table.shape[1], device=block_table.device)
         source = torch.where(col < end, col, torch.where(col < pages - gone, col + gone,
@@ -886,7 +893,7 @@ def evict(plan: EvictPlan, weights, k_cache, v_cache, block_table, *, head_dim, 
     last layer plan.table(block_table) is the new one, plan.seq_lens the new lengths.  The
     pages between must be the request's own.
     """
-    index = _device_index(weights, k_cache, v_cache, block_table, weights_out, plan.requests)
+    index = _device_index(weights, k_cache, v_cache, block_table, weights_out, plan.requests, *(stage or ()))
     cache = cache_struct(k_cache, v_cache, head_dim)
     reqs, hk, bs, longest = len(plan.lengths), cache.num_kv_heads, cache.block_size, plan.longest
     if plan.block_size != bs:
@@ -909,8 +916,8 @@ def evict(plan: EvictPlan, weights, k_cache, v_cache, block_table, *, head_dim, 
     if table.stride(1) != 1:
         table = table.contiguous()
     st = staging_struct(stage, k_cache, head_dim)
-    ws = DeviceScratch.get(weights.device).attn_workspace(
-        _lib.load().oscarop_evict_workspace_bytes_v1(reqs, hk, plan.max_drop))
+    need = _lib.load().oscarop_evict_workspace_bytes_v1(reqs, hk, plan.max_drop)
+    ws = torch.empty(need, dtype=torch.uint8, device=weights.device)  # a captured call keeps its own
     a = _lib.EvictArgs(weights.data_ptr(), request, head, weights.shape[2], weights_out.data_ptr(), out_request, out_head,
                        cache, table.data_ptr(), table.stride(0), *table.shape, plan.requests.data_ptr(), reqs, 0,
                        plan.max_drop, None if st is None else C.pointer(st), ws.data_ptr(), ws.numel())

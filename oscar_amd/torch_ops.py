@@ -17,13 +17,13 @@ layer's FP32 window arena):
   store_kernel.py:54-102, backend.py:130-198,513-555); the arena tensors are passed
   (None without a window) because they are mutated.
 * ``attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, query_start_loc,
-  seq_lens, scale, head_dim, stage_k, stage_v, owner, sink_tokens_eff, recent_tokens)
-  soft_cap, alibi_slopes) -> (out_rot, lse)``: plan + split-K decode + merge (``oscar_attn_plan_v1`` /
-  ``oscar_attn_decode_v1``; slab_attention.py:23-92,376-476); the request lists are
+  seq_lens, scale, head_dim, stage_k, stage_v, owner, sink_tokens_eff, recent_tokens,
+  soft_cap, alibi_slopes) -> (out_rot, lse)``: plan + split-K decode + merge
+  (``oscar_attn_plan_v1`` / ``oscar_attn_decode_v1``; slab_attention.py:23-92,376-476); the request lists are
   host integers.
 * ``attention_prefill(q, k, v, scale, head_dim, history, k_cache, v_cache,
-  block_table_row, stage_k, stage_v, owner, soft_cap, alibi_slopes) -> (out, lse)``: fresh-only (history 0,
-  output in q's dtype, lse empty) or continuation prefill (fp32 rotated output and LSE)
+  block_table_row, stage_k, stage_v, owner, soft_cap, alibi_slopes) -> (out, lse)``:
+  fresh-only (history 0, output in q's dtype, lse empty) or continuation prefill (fp32 rotated output and LSE)
   (``oscar_attn_prefill_v1``; prefill.py:69-72, slab_attention.py:376-476).
 * ``norm_rope(q, k, positions, cos_sin, q_weight, k_weight, eps, weight_offset,
   interleaved) -> (q, k)``: head norms with the position rotation (``oscarop_norm_rope_v1``).

@@ -65,6 +65,9 @@ def args(**changes):
     (dict(lse=None), "missing pointer"),
     (dict(weights=None), "missing pointer"),
     (dict(num_reqs=70000, block_table_rows=70000), "too many"),
+    (dict(num_tokens=(1 << 24) + 1), "too many"),
+    (dict(max_seq_len=(1 << 30) + 1), "too many"),
+    (dict(weights_cols=(1 << 30) + 1, weights_stride_head=1 << 31, weights_stride_request=1 << 31), "too many"),
     (dict(block_table_rows=1), "block-table rows"),
     (dict(block_table_cols=0), "block-table rows"),
     (dict(cache_block_size=48), "block_size"),
@@ -233,6 +236,68 @@ def test_wrapper_refusals_on_the_device(cuda):
     with pytest.raises(ValueError, match="overlap"):
         ops.accumulate_weights(**{**good, "plan": two, "block_table": good["block_table"].repeat(2, 1),
                                   "weights": torch.zeros(1, 1, 303, device=cuda).expand(2, 1, 303)})
+
+
+@pytest.mark.gpu
+def test_current_keys_of_fewer_rows_than_the_queries(cuda):
+    """A padded batch whose keys are not padded: lists on the device that reach past the keys
+    read nothing."""
+    from oscar_amd import ops
+
+    c = cases.make_case([300, 40], [3, 2])
+    q, k = (torch.from_numpy(c[x]).bfloat16().to(cuda) for x in "qk")
+    q = torch.cat([q, torch.full_like(q[:4], math.nan)])
+    kc, vc = (torch.from_numpy(c[x]).view(torch.int8).to(cuda) for x in ("k8", "v8"))
+    bt, lse = torch.from_numpy(c["bt"]).to(cuda), torch.zeros(9, 6, device=cuda)
+    plan = ops.plan_weights(c["qsl"], c["seqs"], has_new=True, device=cuda)
+    call = (lambda: ops.accumulate_weights(q, k, kc, vc, bt, plan, 0.0625, lse, torch.zeros(2, 1, 320, device=cuda), head_dim=256))
+    want = call()
+    assert want.isfinite().all() and (want[1, 0, :40] > 0).all()
+    plan.qsl.copy_(torch.tensor([0, 3, 6], dtype=torch.int32))
+    got = call()
+    assert torch.equal(got[0], want[0]) and got[1, 0, :42].isnan().all()
+
+
+@pytest.mark.gpu
+def test_a_captured_prompt_keeps_its_workspace(cuda):
+    """Row chunks go through a workspace: the captured call's stays its own, whatever sizes run
+    and whatever is allocated afterwards, also under a replay on another stream."""
+    from oscar_amd import ops
+
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    kc = torch.zeros(4, 128, 1, 256, dtype=torch.int8, device=cuda)
+    bt = torch.zeros(1, 40, dtype=torch.int32, device=cuda)
+
+    def prompt(n):
+        q, k = (torch.randn(n, h, 256, generator=gen, device=cuda).bfloat16() for h in (6, 1))
+        lse = torch.full((n, 6), 3.0, device=cuda)
+        plan = ops.plan_weights([0, n], [n], has_new=True, device=cuda)
+        return lambda w: ops.accumulate_weights(q, k, kc, kc, bt, plan, 0.0625, lse, w, head_dim=256)
+
+    small, large = prompt(700), prompt(4000)
+    want, weights = (torch.zeros(1, 1, 4096, device=cuda) for _ in range(2))
+    small(want)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        small(torch.zeros_like(weights))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            small(weights)
+    beside = torch.zeros_like(weights)
+    for step in range(3):
+        weights.zero_()
+        beside.zero_()
+        torch.cuda.synchronize()
+        other = [torch.full((1 << 20,), 7.0, device=cuda) for _ in range(4)]
+        with torch.cuda.stream(side):
+            large(beside)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(weights, want), step
+        if step == 0:
+            first = beside.clone()
+        assert torch.equal(beside, first) and all((x == 7.0).all() for x in other)
 
 
 @pytest.mark.gpu

@@ -88,6 +88,14 @@ def test_plan_of_a_whole_middle(monkeypatch):
     assert plan.table(torch.arange(8)[None])[0].tolist() == [0, 7, 1, 2, 3, 4, 5, 6]
 
 
+def test_tables_that_do_not_hold_the_requests_are_refused(monkeypatch):
+    plan = plan_on_the_cpu(monkeypatch, [1000, 300], [6, 0], block_size=128)
+    for bad in (torch.zeros(2, 7, dtype=torch.int32), torch.zeros(1, 9, dtype=torch.int32), torch.zeros(16, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="(?i)block.table"):
+            plan.table(bad)
+    assert plan.table(torch.zeros(2, 8, dtype=torch.int32)).shape == (2, 8)
+
+
 @pytest.mark.parametrize("lengths,pages,more", [
     ([1000], [7], dict(sink_tokens=128, recent_tokens=100)),
     ([1000], [7], dict(sink_tokens=1)),

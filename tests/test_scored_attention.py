@@ -89,6 +89,18 @@ def test_c_entries_refuse_a_bad_cap(cap):
         assert "soft_cap" in lib.oscar_last_error().decode()
 
 
+@pytest.mark.parametrize("cap", [-0.5, 2.0 ** -21, 1024.5, 1e30, 3.4e38])
+def test_caps_outside_the_range_are_refused(cap):
+    """A large cap would lose the score (it keeps cap 2^-22), a tiny one has no scale / cap."""
+    from oscar_amd import ops
+
+    test_c_entries_refuse_a_bad_cap(cap)
+    with pytest.raises(ValueError, match="soft_cap"):
+        ops.score_struct(cap, None, 6, torch.device("cpu"))
+    for good in (2.0 ** -20, 1024):
+        assert ops.score_struct(good, None, 6, torch.device("cpu")).soft_cap == good
+
+
 def test_score_struct_refusals():
     from oscar_amd import ops
 
@@ -147,6 +159,32 @@ def test_decode(cuda, name, prefixes, lengths, opts, cap, steep, dtype):
         if k is not None:
             hk_, hv = np.concatenate([hk_, k[a:b].float()]), np.concatenate([hv, v[a:b].float()])
         check(out[a:b], lse[a:b], reference(q[a:b].float(), hk_, hv, hist, c["scale"], cap, slopes, seq - (b - a) + 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [2.0 ** -20, 1024.0])
+def test_the_least_and_the_largest_cap(cuda, cap):
+    """Scores within LSE_TOL of the formula's: 1024 2^-22 is 2.5e-4, and products that err by
+    less than 1e-4 here (a query that is not scaled up)."""
+    from oscar_amd import ops
+
+    c = cases.make_case([129, 700, 0], [4, 2, 3])
+    q, k, v = (torch.from_numpy(c[x]).bfloat16() for x in "qkv")
+    kc, vc = (torch.from_numpy(c[x]).view(torch.int8).to(cuda) for x in ("k8", "v8"))
+    stage = tuple(torch.from_numpy(a).to(cuda) for a in c["stage"])
+    bt = torch.from_numpy(c["bt"]).to(cuda)
+    plan = ops.plan_decode(c["qsl"], c["seqs"], has_new=True, num_kv_heads=1, group=6, head_dim=256, device=cuda)
+    out, lse = ops.attention_decode(q.to(cuda), k.to(cuda), v.to(cuda), kc, vc, bt, plan, c["scale"], stage, head_dim=256,
+                                    soft_cap=cap)
+    long = ops.attention_prefill(q[:4].to(cuda), k[:4].to(cuda), v[:4].to(cuda), c["scale"], head_dim=256, history=129,
+                                 k_cache=kc, v_cache=vc, block_table_row=bt[0], stage=stage, soft_cap=cap)
+    for r, (a, b, seq) in enumerate(zip(c["qsl"], c["qsl"][1:], c["seqs"])):
+        hk_, hv = read_history(c["k8"], c["v8"], c["bt"][r], 0, seq - (b - a), 1, 256, c["stage"], "bf16")
+        hk_, hv = np.concatenate([hk_, k[a:b].float()]), np.concatenate([hv, v[a:b].float()])
+        ref = reference(q[a:b].float(), hk_, hv, seq - (b - a), c["scale"], cap, None, seq - (b - a) + 1)
+        check(out[a:b], lse[a:b], ref)
+        if r == 0:
+            check(long, None, ref)
 
 
 @pytest.mark.gpu
