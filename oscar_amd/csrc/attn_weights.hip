@@ -72,7 +72,7 @@ __device__ __forceinline__ Rows rows_of(const WeightsParams& P, int chunk, int t
 // a request that does not fit the call's arrays
 __device__ __forceinline__ bool misfit(const oscarop_weights_args_v1& A, int qa, int nq, int seq) {
   const int hist = A.k_new != nullptr ? seq - nq : seq;
-  return qa < 0 || (int64_t)qa + nq > A.num_tokens || hist < 0 || seq > A.weights_cols ||
+  return qa < 0 || (int64_t)qa + nq > A.num_tokens || seq < 0 || hist < 0 || seq > A.weights_cols ||
          (hist > 0 && (hist - 1) / (int)A.cache.block_size >= A.block_table_cols);
 }
 

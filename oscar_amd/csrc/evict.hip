@@ -56,7 +56,7 @@ __device__ __forceinline__ Request request_of(const oscarop_evict_args_v1& A, in
   const int32_t* q = A.requests + 4 * (int64_t)r;
   Request x{q[0], q[1], q[2], q[3], true};
   const int bs = (int)A.cache.block_size;
-  x.ok = x.sink >= 0 && x.drop >= 0 && x.tail <= x.seq && x.drop <= x.tail - x.sink && x.seq <= A.weights_cols &&
+  x.ok = x.sink >= 0 && x.drop >= 0 && x.sink <= x.tail && x.tail <= x.seq && x.drop <= x.tail - x.sink && x.seq <= A.weights_cols &&
          x.drop <= A.max_drop && (x.seq <= 0 || (x.seq - 1) / bs < A.block_table_cols);
   return x;
 }

@@ -239,6 +239,21 @@ def test_bad_pages_and_records_touch_nothing_else(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("record", [[1000, 10, -2 ** 31, 128], [-2 ** 31, 10, -2 ** 31, 0], [1000, 900, 896, 0], [1000, 2 ** 31 - 1, 896, 128],
+                                    [2 ** 31 - 1, 0, 896, 128], [1000, 0, 896, -2 ** 31]])
+def test_records_at_the_ends_of_the_integers_change_nothing(cuda, record):
+    from oscar_amd import ops
+
+    x = make([1000], 1, 128, 128, 5, "plain")
+    dev = {n: torch.from_numpy(a.copy()).to(cuda) for n, a in x.items()}
+    plan = ops.plan_evict([1000], [3], block_size=128, device=cuda)
+    plan.requests[0] = torch.tensor(record, dtype=torch.int32)
+    before = dev["k"].clone()
+    got = ops.evict(plan, dev["w"], dev["k"].view(torch.int8), dev["v"].view(torch.int8), dev["table"], head_dim=128)
+    assert torch.equal(dev["k"], before) and torch.equal(got, dev["w"])
+
+
+@pytest.mark.gpu
 def test_wrapper_refusals_on_the_device(cuda):
     from oscar_amd import ops
 
