@@ -14,10 +14,13 @@
 //   evict_move_kernel    the slots' bytes and weights from mover to place, the places' window
 //                        tags, and the new weights from the new end on
 //
-// The selection is bound by what one compute unit issues, some forty instructions a token
-// in all, not by the 4 bytes per token it reads: the weights lie in LDS as ordered numbers and
+// The selection is bound by what one compute unit issues, some hundred instructions a token
+// in all, not by the 4 bytes per token it reads (31000 tokens 26 us: 8 the reading with the
+// first digit, 5 the further ones, 3 the counts, 8 the lists): the weights lie in LDS as ordered numbers and
 // every thread takes a run of consecutive tokens, so that marks and lists are counted without
 // talk between lanes and only a thread's totals are scanned.
+#include <type_traits>
+
 #include "common.h"
 
 #include "../../include/oscar_operators.h"
@@ -29,11 +32,14 @@ namespace {
 constexpr int kSelect = 1024;          // threads of a selecting workgroup
 constexpr int kSelectWaves = kSelect / 64;
 constexpr int kRun = 32;               // consecutive tokens of a thread at most
+constexpr int kLoads = 16;             // loads of a thread in flight
 constexpr int kStep = 4;               // of them at a time; a run is a multiple of it
 constexpr int kFew = 256;              // candidates whose ranks are counted pair by pair
 constexpr int kBlock = kSelect * kRun; // tokens held at a time; longer lists are read again in every step
-constexpr int kDigit = 11;             // bits of a digit: the first holds sign, exponent and two more
-constexpr int kBins = 1 << kDigit;     // two a thread
+constexpr int kDigit = 11;             // bits of the second and third digit, two bins a thread
+constexpr int kFirst = 10;             // bits of the first: sign, exponent and one more
+constexpr int kCopies = 4;             // of its bins: most weights share a few exponents, and atomics of one bin take turns
+constexpr int kBins = kCopies << kFirst;
 constexpr int kMove = 256;
 
 struct EvictParams {
@@ -94,6 +100,12 @@ __device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t* total, uint32_t* 
   return before + v - x;
 }
 
+// element i < 2^30 of an array, by an offset of 32 bits
+template <class T>
+__device__ __forceinline__ T* at32(T* p, int i) {
+  return (T*)((std::conditional_t<std::is_const_v<T>, const char*, char*>)p + (uint32_t)i * (uint32_t)sizeof(T));
+}
+
 // where number i of a block lies in s_buf: a word is left out every 32, so that the threads'
 // runs start in different banks
 __device__ __forceinline__ int place_of(int i) { return i + i / 32; }
@@ -117,7 +129,6 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
     if (tid == 0) P.counts[list] = 0;
     return;
   }
-  for (int t = tid; t < q.sink; t += kSelect) out[t] = w[t];
   const int n = q.tail - q.sink;  // token sink + i, i < n
   __shared__ uint32_t s_buf[kBlock + kBlock / 32];
   __shared__ int s_bin[kBins];
@@ -134,26 +145,32 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
   // ---- blocks of the list; thread t has the tokens base + t per + b, b < mine, of a block,
   // `per` being a multiple of kStep
   int base = 0, per = 0, mine = 0;
-  auto load = [&](int at, bool copy) __attribute__((always_inline)) {
+  auto load = [&](int at, auto first) __attribute__((always_inline)) {
+    constexpr bool FIRST = decltype(first)::value;  // the list's first reading: counts the first digit, copies the weights
     const int many = n - at < kBlock ? n - at : kBlock;
     base = at;
     per = (many + kSelect * kStep - 1) / (kSelect * kStep) * kStep;
-    mine = many - tid * per;
-    mine = mine < 0 ? 0 : mine < per ? mine : per;
+    mine = min(max(many - tid * per, 0), per);
     __syncthreads();  // s_buf of the block before has been read
-    for (int b = 0; b < per; b += kStep) {
-      float x[kStep];
+    const int run = per;
+    for (int b = 0; b < run; b += kLoads) {
+      float x[kLoads];
 #pragma unroll
-      for (int u = 0; u < kStep; ++u) {
+      for (int u = 0; u < kLoads; ++u) {
         const int i = (b + u) * kSelect + tid;
-        x[u] = i < many ? w[q.sink + at + i] : 0.f;
+        x[u] = i < many ? *at32(w, q.sink + at + i) : 0.f;
       }
 #pragma unroll
-      for (int u = 0; u < kStep; ++u) {
+      for (int u = 0; u < kLoads; ++u) {
         const int i = (b + u) * kSelect + tid;
-        s_buf[place_of(i)] = i < many ? order_of(x[u]) : 0xffffffffu;
-        // (places get their movers' weights later)
-        if (copy && i < many && q.sink + at + i < end) out[q.sink + at + i] = x[u];
+        if (b + u >= run) break;
+        const uint32_t k = i < many ? order_of(x[u]) : 0xffffffffu;
+        s_buf[place_of(i)] = k;
+        if constexpr (FIRST) {
+          // (places get their movers' weights later)
+          if (i < many && q.sink + at + i < end) *at32(out, q.sink + at + i) = x[u];
+          if (i < many) atomicAdd(&s_bin[kCopies * (k >> (32 - kFirst)) + lane % kCopies], 1);
+        }
       }
     }
     __syncthreads();
@@ -171,7 +188,7 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
   auto blocks = [&](auto step) __attribute__((always_inline)) {
     if (one) return step();
     for (int at = 0; at < n; at += kBlock) {
-      load(at, false);
+      load(at, std::false_type{});
       step();
     }
   };
@@ -179,37 +196,39 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
   // rank `left` among those that share the digits found so far:
   uint32_t prefix = 0;
   int left = q.drop, equal = 0;
-  auto find = [&](int bits) __attribute__((always_inline)) {
+  auto find = [&](int bits, auto first) __attribute__((always_inline)) {
+    constexpr bool FIRST = decltype(first)::value;
+    static_assert(kSelect == 1 << kFirst && 2 * kSelect == 1 << kDigit);
     __syncthreads();
-    const uint32_t b0 = s_bin[2 * tid], b1 = s_bin[2 * tid + 1];
-    uint32_t all;
+    int c[FIRST ? kCopies : 2];
+    int* mine_bins = s_bin + (FIRST ? kCopies : 2) * tid;
+    uint32_t b0 = 0, b1 = 0, all;
+#pragma unroll
+    for (int i = 0; i < (FIRST ? kCopies : 2); ++i) {
+      c[i] = mine_bins[i];
+      mine_bins[i] = 0;
+    }
+    if constexpr (FIRST) {
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) b0 += c[i];
+    } else {
+      b0 = c[0];
+      b1 = c[1];
+    }
     const uint32_t before = scan(b0 + b1, &all, s_part);
     if (before < (uint32_t)left && (uint32_t)left <= before + b0 + b1) {
       const bool second = (uint32_t)left > before + b0;
-      s_prefix = prefix << bits | (uint32_t)(2 * tid + second);
+      s_prefix = prefix << bits | (uint32_t)(FIRST ? tid : 2 * tid + second);
       s_left = left - (int)(before + (second ? b0 : 0));
       s_equal = second ? b1 : b0;
     }
-    s_bin[2 * tid] = s_bin[2 * tid + 1] = 0;
     __syncthreads();
     prefix = s_prefix;
     left = s_left;
     equal = s_equal;
   };
-  auto first_digit = [&]() __attribute__((always_inline)) {
-    each([&](int b, uint32_t k) __attribute__((always_inline)) {
-      // where many lanes have the first one's digit (equal weights) they count as one
-      const int digit = (int)(k >> (32 - kDigit)), first = __builtin_amdgcn_readfirstlane(digit);
-      const uint64_t same = __ballot(b < mine && digit == first);
-      if (b < mine && digit != first) atomicAdd(&s_bin[digit], 1);
-      if (lane == 0 && same) atomicAdd(&s_bin[first], __popcll(same));
-    });
-  };
-  for (int at = 0; at < n; at += kBlock) {
-    load(at, true);
-    first_digit();
-  }
-  find(0);
+  for (int at = 0; at < n; at += kBlock) load(at, std::true_type{});
+  find(0, std::true_type{});
   // few candidates: every one's rank among them, pair by pair
   auto finish = [&](int shift) __attribute__((always_inline)) {
     blocks([&]() __attribute__((always_inline)) {
@@ -236,7 +255,8 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
     left = s_left;
     equal = s_equal;
   };
-  constexpr int kShift1 = 32 - kDigit, kShift2 = 32 - 2 * kDigit;
+  constexpr int kShift1 = 32 - kFirst, kShift2 = kShift1 - kDigit;
+  static_assert(kShift2 == kDigit);
   if (equal <= kFew) {
     finish(kShift1);
   } else {
@@ -266,7 +286,7 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
           if (b < mine && k >> (shift + bits) == prefix) atomicAdd(&s_bin[(k >> shift) & ((1u << bits) - 1u)], 1);
         });
       });
-      find(bits);
+      find(bits, std::false_type{});
     };
     if (s_low == s_high) {
       prefix = s_low;
@@ -282,29 +302,31 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
   const int keep = equal - left;
   auto gone_before = [&](int below, int same) __attribute__((always_inline)) { return below + (same > keep ? same - keep : 0); };
   // a thread's tokens' totals, and those of the tokens before its first
-  auto totals = [&](int& below, int& same, int carry_below, int carry_same, int* all_below, int* all_same) __attribute__((always_inline)) {
+  struct Totals {
+    int below, same;  // of the tokens before the thread's first
+    int all_below, all_same;
+  };
+  auto totals = [&](const Totals& carry) __attribute__((always_inline)) {
     uint32_t mine_both = 0, all;  // below in the low half, equal in the high one: a block has 2^15 tokens
     each([&](int b, uint32_t k) __attribute__((always_inline)) {
       mine_both += k < prefix ? 1u : b < mine && k == prefix ? 0x10000u : 0u;
     });
     const uint32_t before = scan(mine_both, &all, s_part);
-    below = carry_below + (int)(before & 0xffffu);
-    same = carry_same + (int)(before >> 16);
-    *all_below = carry_below + (int)(all & 0xffffu);
-    *all_same = carry_same + (int)(all >> 16);
+    return Totals{carry.all_below + (int)(before & 0xffffu), carry.all_same + (int)(before >> 16),
+                  carry.all_below + (int)(all & 0xffffu), carry.all_same + (int)(all >> 16)};
   };
-  // how many go before the new end: the thread that has its token counts on from its own
-  int below = 0, same = 0, all_below = 0, all_same = 0;
+  // how many go before the new end: the wave that has its token counts on from the thread's own
+  Totals sum{};
   blocks([&]() __attribute__((always_inline)) {
-    totals(below, same, all_below, all_same, &all_below, &all_same);
+    sum = totals(sum);
     const int to = end - q.sink - base - tid * per;  // this thread's tokens before the end
-    if (to >= 0 && to < mine) {
-      int l = below, e = same;
-      each([&](int b, uint32_t k) __attribute__((always_inline)) {
-        l += b < to && k < prefix;
-        e += b < to && b < mine && k == prefix;
-      });
-      s_places = gone_before(l, e);
+    const uint64_t has = __ballot(to >= 0 && to < mine);
+    if (has) {
+      const int from = __builtin_ctzll(has);
+      const int many = __builtin_amdgcn_readlane(to, from), l = __builtin_amdgcn_readlane(sum.below, from), e = __builtin_amdgcn_readlane(sum.same, from);
+      const uint32_t k = s_buf[place_of((tid - lane + from) * per + (lane < many ? lane : 0))];
+      const int more_l = __popcll(__ballot(lane < many && k < prefix)), more_e = __popcll(__ballot(lane < many && k == prefix));
+      if (lane == 0) s_places = gone_before(l + more_l, e + more_e);
     }
   });
   __syncthreads();
@@ -313,10 +335,10 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
   // goes; then the block's tokens in order, so that the lists' parts are written side by side
   int32_t* place_list = P.places + list * P.pairs;
   int32_t* mover_list = P.movers + list * P.pairs;
-  all_below = all_same = 0;
+  if (!one) sum = Totals{};
   blocks([&]() __attribute__((always_inline)) {
-    if (!one) totals(below, same, all_below, all_same, &all_below, &all_same);
-    int l = below, e = same;
+    if (!one) sum = totals(sum);
+    int l = sum.below, e = sum.same;
     each([&](int b, uint32_t k) __attribute__((always_inline)) {
       const bool equal_one = b < mine && k == prefix, gone = k < prefix || (equal_one && e >= keep);
       s_buf[place_of(tid * per + b)] = (uint32_t)gone_before(l, e) | (gone ? 0x80000000u : 0u);
@@ -333,8 +355,8 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
       for (int u = 0; u < kStep; ++u) {
         const int i = i0 + u * kSelect + tid, t = q.sink + base + i, g = (int)(m[u] & 0x7fffffffu);
         const bool gone = m[u] >> 31;
-        if (i < many && gone && t < end) place_list[g] = t;
-        if (i < many && !gone && t >= end) mover_list[t - end - (g - places)] = t;
+        if (i < many && gone && t < end) *at32(place_list, g) = t;
+        if (i < many && !gone && t >= end) *at32(mover_list, t - end - (g - places)) = t;
       }
     }
   });
@@ -355,8 +377,9 @@ __global__ __launch_bounds__(kMove) void evict_move_kernel(EvictParams P) {
   const int32_t* row = A.block_table + (int64_t)r * A.block_table_stride;
   const float* w = A.weights + r * A.weights_stride_request + h * A.weights_stride_head;
   float* out = A.weights_out + r * A.out_stride_request + h * A.out_stride_head;
-  // the tail's weights, then zeros
+  // the first tokens' weights, the tail's, then zeros
   if (const Request q = request_of(A, r); q.ok) {
+    for (int t = blockIdx.x * kMove + threadIdx.x; t < q.sink; t += gridDim.x * kMove) out[t] = w[t];
     for (int64_t t = q.tail - q.drop + (int64_t)blockIdx.x * kMove + threadIdx.x; t < A.weights_cols; t += (int64_t)gridDim.x * kMove)
       out[t] = t < q.seq - q.drop ? w[t + q.drop] : 0.f;
   }
