@@ -19,12 +19,16 @@ namespace {
 
 constexpr int kThreads = 256;
 // Four heads per lane group from this many bytes of rows on: fewer, longer waves, which cost
-// more while there is one round of them or two and save once memory is the bound.  One head /
-// four, us: 600 tokens of 28 heads of 128 bf16 4.7 / 7.9, 5000 19.1 / 22.0, 15361 (110 MB)
-// 59.1 / 54.3 (48.7 with interleaved pairs, 4.7 TB/s in and out; a large copy reaches 5.1);
-// 10000 of 7 heads of 256 20.6 / 21.7; 5000 of 7 of 256 fp32 (36 MB) 16.7 / 16.0.  Two heads
-// lie between.
-constexpr int64_t kManyBytes = 40 << 20;
+// more while there is one round of them and save once instructions and memory are the bound.
+// One head / four, us: 600 tokens of 28 heads of 128 bf16 4.3 / 5.1, 1200 (9 MB) 7.4 / 6.9,
+// 5000 18.8 / 16.7, 15361 (110 MB) 57.0 / 43.3 (5.1 TB/s in and out, a large copy's rate; 40.4 with
+// interleaved pairs); 1200 of 7 heads of 256 4.3 / 5.4, 5000 (18 MB) 12.0 / 11.4;
+// 5000 of 7 of 256 fp32 (36 MB) 17.3 / 15.6.
+constexpr int64_t kManyBytes = 8 << 20;
+
+typedef float __attribute__((ext_vector_type(2))) f32x2;
+typedef __bf16 __attribute__((ext_vector_type(2))) bf16x2;
+typedef _Float16 __attribute__((ext_vector_type(2))) f16x2;
 
 struct NormRopeParams {
   oscarop_norm_rope_args_v1 a;
@@ -62,11 +66,9 @@ __device__ __forceinline__ void store8(void* base, int64_t i, const float* v) {
   } else {
     u32x4 w;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (DT == OSCAR_BF16)
-        w[e] = f32_to_bf16_bits(v[2 * e]) | ((unsigned)f32_to_bf16_bits(v[2 * e + 1]) << 16);
-      else
-        w[e] = f32_to_f16_bits(v[2 * e]) | ((unsigned)f32_to_f16_bits(v[2 * e + 1]) << 16);
+    for (int e = 0; e < 4; ++e) {  // (to nearest even)
+      if constexpr (DT == OSCAR_BF16) w[e] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{v[2 * e], v[2 * e + 1]}, bf16x2));
+      else w[e] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{v[2 * e], v[2 * e + 1]}, f16x2));
     }
     *(u32x4*)((uint16_t*)base + i) = w;
   }
@@ -112,11 +114,24 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeParams P) {
       for (int e = 0; e < 8; ++e) s[e] = low ? -s[e] : s[e];
     }
   }
+  const bool all_turn = 2 * half == D;
   const int other = !turns ? lane : low ? lane + half / 8 : lane - half / 8;  // the lane of the pairs' other values
+  float w[8];
 #pragma unroll
   for (int i = 0; i < HPG; ++i) {
     const int head = head0 + i;
     const bool is_q = head < A.num_q_heads;
+    if (i == 0 || head == A.num_q_heads) {  // another side's weights
+      const void* weight = is_q ? A.q_weight : A.k_weight;
+      if (weight != nullptr) {
+        load8_of(weight, A.weight_dtype, e0, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] += A.weight_offset;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = 1.f;
+      }
+    }
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum = fmaf(x[i][e], x[i][e], sum);
@@ -125,17 +140,8 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeParams P) {
     sum += dpp_row<kDppHalfMirror>(sum);
     sum += dpp_row<kDppMirror>(sum);
     if constexpr (L == 32) sum += swizzle_xor16(sum);
-    const float r = 1.f / sqrtf(sum * (1.f / D) + A.eps);
-    float w[8], y[8];
-    const void* weight = is_q ? A.q_weight : A.k_weight;
-    if (weight != nullptr) {
-      load8_of(weight, A.weight_dtype, e0, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] += A.weight_offset;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = 1.f;
-    }
+    const float r = known ? 1.f / sqrtf(sum * (1.f / D) + A.eps) : NAN;
+    float y[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[i][e] = x[i][e] * r * w[e];
     if (A.interleaved) {
@@ -148,12 +154,11 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeParams P) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = fmaf(x[i][e], c[e], __shfl(x[i][e], other) * s[e]);
     }
-    if (!live || head >= P.heads) continue;
+    if (!all_turn) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      y[e] = turns ? y[e] : x[i][e];  // (0 times an infinity beside it would be NaN)
-      y[e] = known ? y[e] : NAN;
+      for (int e = 0; e < 8; ++e) y[e] = turns ? y[e] : x[i][e];  // (0 times an infinity beside it would be NaN)
     }
+    if (!live || head >= P.heads) continue;
     if (is_q) store8<DT>(A.q_out, t * A.q_out_stride_token + (int64_t)head * D + e0, y);
     else store8<DT>(A.k_out, t * A.k_out_stride_token + (int64_t)(head - A.num_q_heads) * D + e0, y);
   }
