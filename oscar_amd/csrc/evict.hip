@@ -14,11 +14,12 @@
 //   evict_move_kernel    the slots' bytes and weights from mover to place, the places' window
 //                        tags, and the new weights from the new end on
 //
-// The selection is bound by what one compute unit issues, some hundred instructions a token
-// in all, not by the 4 bytes per token it reads (31000 tokens 26 us: 8 the reading with the
-// first digit, 5 the further ones, 3 the counts, 8 the lists): the weights lie in LDS as ordered numbers and
+// The selection is bound by what one compute unit issues, some eighty instructions a token in
+// all, not by the 4 bytes per token it reads (31000 tokens 23 us, a third of it the reading
+// with the first digit and a third the lists): the weights lie in LDS as ordered numbers and
 // every thread takes a run of consecutive tokens, so that marks and lists are counted without
-// talk between lanes and only a thread's totals are scanned.
+// talk between lanes and only a thread's totals are scanned.  (Further compute units a list
+// would have to meet between the digits: four launches more, at 3 to 5 us each.)
 #include <type_traits>
 
 #include "common.h"
@@ -69,10 +70,8 @@ __device__ __forceinline__ Request request_of(const oscarop_evict_args_v1& A, in
 
 // weights in ascending order as unsigned numbers: +0 and -0 alike, NaN above everything
 __device__ __forceinline__ uint32_t order_of(float w) {
-  uint32_t u = __float_as_uint(w);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
-  if (u == 0x80000000u) u = 0;
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t u = __float_as_uint(w + 0.f);  // (-0 becomes +0)
+  return w != w ? 0xffffffffu : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
 // exclusive prefix sum over the workgroup of one number per thread; *total gets the sum
@@ -107,8 +106,10 @@ __device__ __forceinline__ T* at32(T* p, int i) {
 }
 
 // where number i of a block lies in s_buf: a word is left out every 32, so that the threads'
-// runs start in different banks
+// runs start in different banks (four numbers from a multiple of four lie side by side, and
+// 32 n further on is 33 n further on)
 __device__ __forceinline__ int place_of(int i) { return i + i / 32; }
+constexpr int kPitch = kSelect + kSelect / 32;
 
 __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
   const oscarop_evict_args_v1& A = P.a;
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
         const int i = (b + u) * kSelect + tid;
         if (b + u >= run) break;
         const uint32_t k = i < many ? order_of(x[u]) : 0xffffffffu;
-        s_buf[place_of(i)] = k;
+        s_buf[place_of(tid) + (b + u) * kPitch] = k;
         if constexpr (FIRST) {
           // (places get their movers' weights later)
           if (i < many && q.sink + at + i < end) *at32(out, q.sink + at + i) = x[u];
@@ -175,13 +176,13 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
     }
     __syncthreads();
   };
-  auto each = [&](auto use) __attribute__((always_inline)) {  // use(b, key): of every thread at once, b < mine or not
+  auto each = [&](auto use) __attribute__((always_inline)) {  // use(b, key, place): of every thread at once, b < mine or not
     for (int b = 0; b < per; b += kStep) {
       uint32_t k[kStep];
 #pragma unroll
-      for (int u = 0; u < kStep; ++u) k[u] = s_buf[place_of(tid * per + b + u)];
+      for (int u = 0; u < kStep; ++u) k[u] = s_buf[place_of(tid * per + b) + u];
 #pragma unroll
-      for (int u = 0; u < kStep; ++u) use(b + u, k[u]);
+      for (int u = 0; u < kStep; ++u) use(b + u, k[u], place_of(tid * per + b) + u);
     }
   };
   const bool one = n <= kBlock;
@@ -232,7 +233,7 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
   // few candidates: every one's rank among them, pair by pair
   auto finish = [&](int shift) __attribute__((always_inline)) {
     blocks([&]() __attribute__((always_inline)) {
-      each([&](int b, uint32_t k) __attribute__((always_inline)) {
+      each([&](int b, uint32_t k, int) __attribute__((always_inline)) {
         if (b < mine && k >> shift == prefix) s_cand[atomicAdd(&s_few, 1)] = k;
       });
     });
@@ -263,10 +264,10 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
     // one value in the bin (equal weights) needs no further digits
     uint32_t low = 0xffffffffu, high = 0;
     blocks([&]() __attribute__((always_inline)) {
-      each([&](int b, uint32_t k) __attribute__((always_inline)) {
+      each([&](int b, uint32_t k, int) __attribute__((always_inline)) {
         const bool in = b < mine && k >> kShift1 == prefix;
-        low = in && k < low ? k : low;
-        high = in && k > high ? k : high;
+        low = min(low, in ? k : 0xffffffffu);
+        high = max(high, in ? k : 0u);
       });
     });
 #pragma unroll
@@ -282,7 +283,7 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
     __syncthreads();
     auto digit = [&](int shift, int bits) __attribute__((always_inline)) {
       blocks([&]() __attribute__((always_inline)) {
-        each([&](int b, uint32_t k) __attribute__((always_inline)) {
+        each([&](int b, uint32_t k, int) __attribute__((always_inline)) {
           if (b < mine && k >> (shift + bits) == prefix) atomicAdd(&s_bin[(k >> shift) & ((1u << bits) - 1u)], 1);
         });
       });
@@ -308,8 +309,9 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
   };
   auto totals = [&](const Totals& carry) __attribute__((always_inline)) {
     uint32_t mine_both = 0, all;  // below in the low half, equal in the high one: a block has 2^15 tokens
-    each([&](int b, uint32_t k) __attribute__((always_inline)) {
-      mine_both += k < prefix ? 1u : b < mine && k == prefix ? 0x10000u : 0u;
+    each([&](int, uint32_t k, int) __attribute__((always_inline)) {
+      // (numbers past the list, which may equal it, are the last ones)
+      mine_both += k < prefix ? 1u : k == prefix ? 0x10000u : 0u;
     });
     const uint32_t before = scan(mine_both, &all, s_part);
     return Totals{carry.all_below + (int)(before & 0xffffu), carry.all_same + (int)(before >> 16),
@@ -339,9 +341,9 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
   blocks([&]() __attribute__((always_inline)) {
     if (!one) sum = totals(sum);
     int l = sum.below, e = sum.same;
-    each([&](int b, uint32_t k) __attribute__((always_inline)) {
-      const bool equal_one = b < mine && k == prefix, gone = k < prefix || (equal_one && e >= keep);
-      s_buf[place_of(tid * per + b)] = (uint32_t)gone_before(l, e) | (gone ? 0x80000000u : 0u);
+    each([&](int, uint32_t k, int place) __attribute__((always_inline)) {
+      const bool equal_one = k == prefix, gone = k < prefix || (equal_one && e >= keep);
+      s_buf[place] = (uint32_t)gone_before(l, e) | (gone ? 0x80000000u : 0u);
       l += k < prefix;
       e += equal_one;
     });
@@ -350,13 +352,12 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
     for (int i0 = 0; i0 < many; i0 += kStep * kSelect) {
       uint32_t m[kStep];
 #pragma unroll
-      for (int u = 0; u < kStep; ++u) m[u] = s_buf[place_of(i0 + u * kSelect + tid)];
+      for (int u = 0; u < kStep; ++u) m[u] = s_buf[place_of(i0) + place_of(tid) + u * kPitch];
 #pragma unroll
       for (int u = 0; u < kStep; ++u) {
         const int i = i0 + u * kSelect + tid, t = q.sink + base + i, g = (int)(m[u] & 0x7fffffffu);
         const bool gone = m[u] >> 31;
-        if (i < many && gone && t < end) *at32(place_list, g) = t;
-        if (i < many && !gone && t >= end) *at32(mover_list, t - end - (g - places)) = t;
+        if (i < many && gone == (t < end)) *at32(gone ? place_list : mover_list, gone ? g : t - end - (g - places)) = t;
       }
     }
   });
