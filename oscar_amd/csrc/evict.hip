@@ -42,6 +42,9 @@ constexpr int kFirst = 10;             // bits of the first: sign, exponent and 
 constexpr int kCopies = 4;             // of its bins: most weights share a few exponents, and atomics of one bin take turns
 constexpr int kBins = kCopies << kFirst;
 constexpr int kMove = 256;
+// workgroups of evict_move_kernel: about one per 32 moves of a large call, since fewer than
+// max_drop tokens move (128000 moves in 8192 / 4096 / 2048 workgroups: 14.9 / 13.6 / 14.5 us)
+constexpr int64_t kMoveWorkgroups = 4096;
 
 struct EvictParams {
   oscarop_evict_args_v1 a;
@@ -367,7 +370,7 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
 // A group of D / 16 lanes per move: 8 bytes of constants and the codes of K and V, 16 bytes a
 // lane (five lanes of eight at head dim 128, nine of sixteen at 256).  Bound by the lines that
 // the scattered slots touch, two read and two written for each move: 128000 moves at head dim
-// 128 15 us, 65 MB.  (Four moves of a group in flight: 17 us.)
+// 128 14 us, 43 MB between the L2 and memory.  (Four moves of a group in flight: 17 us.)
 template <int D>
 __global__ __launch_bounds__(kMove) void evict_move_kernel(EvictParams P) {
   constexpr int L = D / 16, W = D / 64;  // lanes of a move; 16-byte parts of a side's codes
@@ -462,7 +465,8 @@ extern "C" int oscarop_evict_v1(const oscarop_evict_args_v1* args, void* stream)
   hipLaunchKernelGGL(evict_select_kernel, lists, dim3(kSelect), 0, s, p);
   OSCAR_CHECK_LAUNCH("evict_select_kernel");
   const int64_t per = kMove / (D / 16), wgs = (a.max_drop + per - 1) / per;
-  const dim3 grid((unsigned)(wgs < 1 ? 1 : wgs < 256 ? wgs : 256), (unsigned)hk, (unsigned)a.num_reqs);
+  const int64_t most = (kMoveWorkgroups + hk * a.num_reqs - 1) / (hk * a.num_reqs);
+  const dim3 grid((unsigned)(wgs < 1 ? 1 : wgs < most ? wgs : most), (unsigned)hk, (unsigned)a.num_reqs);
   if (D == 256) hipLaunchKernelGGL(evict_move_kernel<256>, grid, dim3(kMove), 0, s, p);
   else hipLaunchKernelGGL(evict_move_kernel<128>, grid, dim3(kMove), 0, s, p);
   OSCAR_CHECK_LAUNCH("evict_move_kernel");
