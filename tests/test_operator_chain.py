@@ -61,6 +61,32 @@ def test_torch_operators_match_the_wrappers(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cap,steep", [(0.0, 0.0), (20.0, 1.0)])
+@pytest.mark.parametrize("n", [1, 33, 700, 2500])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_fresh_prompt_and_its_weights(cuda, n, dtype, cap, steep):
+    """The LSE of a fresh prefill (within 4e-4 of the formula's) with the prompt's own rows: every
+    query gives one in all, to within that LSE, the weights' own products (3e-4) and their 1e-4."""
+    from oscar_amd import ops
+
+    gen = torch.Generator().manual_seed(n)
+    q, k, v = (torch.randn(n, h, D, generator=gen).to(dtype) for h in (HQ, HK, HK))
+    slopes = torch.tensor([steep * 2.0 ** (-8.0 * (h + 1) / HQ) for h in range(HQ)]) if steep else None
+    score = dict(soft_cap=cap, alibi_slopes=None if slopes is None else slopes.to(cuda))
+    lse = torch.full((n, HQ), 77.0, device=cuda)
+    ops.attention_prefill(q.to(cuda), k.to(cuda), v.to(cuda), SCALE, head_dim=D, lse=lse, **score)
+    _, want, _ = reference(q.float(), k.float(), v.float(), 0, SCALE, cap, slopes, 1)
+    assert (lse.double().cpu() - want).abs().max() <= 4e-4
+    kc = torch.zeros(1, BS, HK, D, dtype=torch.int8, device=cuda)
+    table = torch.zeros(1, -(-n // BS), dtype=torch.int32, device=cuda)
+    weights = torch.zeros(1, HK, n, device=cuda)
+    ops.accumulate_weights(q.to(cuda), k.to(cuda), kc, kc, table, ops.plan_weights([0, n], [n], has_new=True, device=cuda), SCALE,
+                           lse, weights, head_dim=D, **score)
+    assert (weights.double().sum(-1) / (n * HQ / HK) - 1).abs().max() <= 8e-4
+    assert (weights >= 0).all()
+
+
+@pytest.mark.gpu
 def test_a_serving_loop(cuda):
     """Two requests: prompts, decode steps whose weights add up, an eviction, and a step over
     what is left.  Each attention is checked against a 64-bit evaluation of the cache as it
