@@ -19,7 +19,7 @@
 //                        waves; where the keys alone do not fill the chip the rows are cut
 //                        into chunks, whose sums weights_sum_kernel adds in their order.  A
 //                        block of 32 rows against 256 keys takes 2.1 us a workgroup with two
-//                        of them on a compute unit.  2500 fresh tokens of 6 heads: 35 us and
+//                        of them on a compute unit.  2500 fresh tokens of 6 heads: 29 us and
 //                        5 us for the sums, of which the keys' way into registers is 6 us
 //                        (eight waves of one tile each, their rows reordered through LDS
 //                        instead of loaded one a lane, took as long in all)
@@ -42,6 +42,7 @@ constexpr int kTile = 32;
 constexpr int kFewRows = 32;                           // of a KV head, for weights_few_kernel
 constexpr int kKeyTiles = 2;                           // per wave of weights_many_kernel
 constexpr int kGroupKeys = kWaves * kKeyTiles * kTile;  // per workgroup
+constexpr int kTable = 128;
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct WeightsParams {
@@ -53,6 +54,10 @@ struct WeightsParams {
   int chunks;        // row chunks (1: sums go to the weights)
   int chunk_blocks;  // row blocks of a chunk; the last one takes what is left
   float* part;       // [num_reqs][chunks][Hk][weights_cols]
+  // the chunks with rows of the key groups before one, and of all; plain_order: the groups do
+  // not fit here, and workgroups lie in the order of the groups
+  int first[kTable];
+  int plain_order;
 };
 
 // The row chunks of the requests' key groups.  A key group's rows begin with the first that
@@ -67,6 +72,35 @@ __device__ __forceinline__ Rows rows_of(const WeightsParams& P, int chunk, int t
   r.first = a > from ? a : from;
   r.end = chunk == P.chunks - 1 || blocks < a + P.chunk_blocks ? blocks : a + P.chunk_blocks;
   return r;
+}
+
+// Which request, KV head, key group and row chunk a workgroup takes.  Where there are several
+// chunks the workgroups lie along one axis, and those that have rows in a batch of the call's
+// largest sizes come first and side by side: workgroups go to the dies and their shader engines
+// in turn, and one with more than its share would need a second round (6000 fresh tokens of 6
+// heads on 1: 118 us in the order of the groups, 85 so).
+struct Unit {
+  int req, kvh, group, chunk, groups;
+};
+__device__ __forceinline__ Unit unit_of(const WeightsParams& P) {
+  if (P.chunks == 1) return {(int)blockIdx.z, (int)blockIdx.y, (int)blockIdx.x, 0, (int)gridDim.x};
+  const int hk = (int)P.a.cache.num_kv_heads, lists = P.a.num_reqs * hk, list = blockIdx.x % lists;
+  const int i = blockIdx.x / lists, groups = gridDim.x / (lists * P.chunks);
+  Unit u{list / hk, list % hk, i / P.chunks, i % P.chunks, groups};
+  if (P.plain_order) return u;
+  const int lane = threadIdx.x & 63, total = P.first[groups];
+  // entries of a table that lie at or below x, less one; they ascend, past `groups` they do not count
+  auto last = [&](int x, auto entry) __attribute__((always_inline)) {
+    return __popcll(__ballot(lane < groups && entry(lane) <= x)) + __popcll(__ballot(64 + lane < groups && entry(64 + lane) <= x)) - 1;
+  };
+  if (i < total) {
+    u.group = last(i, [&](int g) __attribute__((always_inline)) { return P.first[g]; });
+    u.chunk = P.chunks - (P.first[u.group + 1] - i);
+  } else {
+    u.group = last(i - total, [&](int g) __attribute__((always_inline)) { return g * P.chunks - P.first[g]; });
+    u.chunk = i - total - (u.group * P.chunks - P.first[u.group]);
+  }
+  return u;
 }
 
 // a request that does not fit the call's arrays
@@ -377,8 +411,7 @@ __global__ __launch_bounds__(kThreads, 2) void weights_many_kernel(WeightsParams
   const oscarop_weights_args_v1& A = P.a;
   const int lane = threadIdx.x & 63, m = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int req = blockIdx.z, kvh = blockIdx.y;
-  const int chunk = blockIdx.x % P.chunks, group0 = blockIdx.x / P.chunks, groups = gridDim.x / P.chunks;
+  const auto [req, kvh, group0, chunk, groups] = unit_of(P);
   const Span x = span_of(A, req);
   if (x.nq < 1) return;
   float* out = P.chunks > 1 ? P.part + (((int64_t)req * P.chunks + chunk) * A.cache.num_kv_heads + kvh) * A.weights_cols
@@ -471,25 +504,45 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(WeightsParams P) {
 constexpr int64_t kFewWorkgroups = 768;
 constexpr int64_t kFewTiles = 16;
 
-// Row chunks of a call.  A workgroup's key operands cost about as much to load as four row
-// blocks, and one round of the chip is two workgroups per compute unit.
+// Row chunks of a call: as many as leave the workgroups with any rows within one round of the
+// chip, two per compute unit (the rows that see a key group's first key begin later in every
+// group of a fresh prompt, and the chunks before them are empty).  A workgroup's key operands
+// cost about as much to load as four row blocks.
 constexpr int64_t kUnits = 512;
 constexpr int64_t kMinBlocks = 4;
 constexpr int64_t kMaxPart = 256ll << 20;  // bytes of partial sums
 struct Chunks {
   int64_t count, blocks;
 };
+// chunks of `per` blocks before key group g's first one with rows
+int64_t empty_chunks(const oscarop_weights_args_v1& a, int64_t g, int64_t per, int64_t count) {
+  const int64_t tokens = g * kGroupKeys - (a.max_seq_len - a.max_query_len);
+  const int64_t none = tokens <= 0 ? 0 : tokens * (a.num_q_heads / a.cache.num_kv_heads) / 32 / per;
+  return none < count ? none : count;
+}
 Chunks chunks_of(const oscarop_weights_args_v1& a) {
-  const int64_t hk = a.cache.num_kv_heads, rows = a.max_query_len * (a.num_q_heads / hk);
-  const int64_t blocks = (rows + 31) / 32, units = a.num_reqs * hk * ((a.max_seq_len + kGroupKeys - 1) / kGroupKeys);
-  if (units < 1 || rows <= kFewRows || blocks < 2 * kMinBlocks || units >= kUnits) return {1, 1 << 30};
-  int64_t count = (kUnits + units - 1) / units;
-  if (count > blocks / kMinBlocks) count = blocks / kMinBlocks;
-  const int64_t most = kMaxPart / (a.num_reqs * hk * a.weights_cols * (int64_t)sizeof(float));
-  if (count > most) count = most;
-  if (count < 2) return {1, 1 << 30};
-  const int64_t per = (blocks + count - 1) / count;
-  return {(blocks + per - 1) / per, per};
+  const Chunks one = {1, 1 << 30};
+  const int64_t hk = a.cache.num_kv_heads, rows = a.max_query_len * (a.num_q_heads / hk), blocks = (rows + 31) / 32;
+  const int64_t groups = (a.max_seq_len + kGroupKeys - 1) / kGroupKeys, lists = a.num_reqs * hk;
+  if (groups * lists < 1 || rows <= kFewRows || blocks < 2 * kMinBlocks || groups * lists >= kUnits) return one;
+  const int64_t before = a.max_seq_len - a.max_query_len;
+  const int64_t all = before < 0 ? 0 : before / kGroupKeys + 1;  // key groups that every row block sees
+  auto fits = [&](int64_t per) {
+    const int64_t count = (blocks + per - 1) / per;
+    int64_t sum = all * count;
+    for (int64_t g = all; g < groups; ++g) sum += count - empty_chunks(a, g, per, count);
+    return sum * lists <= kUnits;
+  };
+  const int64_t most = kMaxPart / (lists * a.weights_cols * (int64_t)sizeof(float));
+  if (most < 2) return one;
+  int64_t low = (blocks + most - 1) / most, high = blocks;  // the fewest blocks a chunk that fit
+  if (low < kMinBlocks) low = kMinBlocks;
+  while (low < high) {
+    const int64_t per = (low + high) / 2;
+    if (fits(per)) high = per;
+    else low = per + 1;
+  }
+  return low < blocks ? Chunks{(blocks + low - 1) / low, low} : one;
 }
 
 }  // namespace
@@ -555,6 +608,11 @@ extern "C" int oscarop_attn_weights_v1(const oscarop_weights_args_v1* args, cons
   p.chunks = (int)chunks.count;
   p.chunk_blocks = (int)chunks.blocks;
   p.part = (float*)a.workspace;
+  const int64_t key_groups = (a.max_seq_len + kGroupKeys - 1) / kGroupKeys;
+  p.plain_order = key_groups >= kTable;
+  if (p.chunks > 1 && !p.plain_order)
+    for (int64_t g = 0; g < key_groups; ++g)
+      p.first[g + 1] = p.first[g] + p.chunks - (int)empty_chunks(a, g, p.chunk_blocks, p.chunks);
   hipStream_t s = (hipStream_t)stream;
   const unsigned hk = (unsigned)a.cache.num_kv_heads, reqs = (unsigned)a.num_reqs;
   const bool few = a.max_query_len * (int64_t)p.group.d <= kFewRows;
@@ -563,9 +621,8 @@ extern "C" int oscarop_attn_weights_v1(const oscarop_weights_args_v1* args, cons
   int64_t few_wgs = kFewWorkgroups / ((int64_t)hk * reqs);
   const int64_t least = (tiles + kWaves * kFewTiles - 1) / (kWaves * kFewTiles);
   few_wgs = few_wgs < least ? least : few_wgs > tiles ? tiles : few_wgs;
-  const dim3 grid(few ? (unsigned)few_wgs
-                      : (unsigned)((a.max_seq_len + kGroupKeys - 1) / kGroupKeys * chunks.count),
-                  hk, reqs);
+  const unsigned units = (unsigned)(few ? few_wgs : key_groups * chunks.count);
+  const dim3 grid = chunks.count > 1 ? dim3(units * hk * reqs) : dim3(units, hk, reqs);
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, p); };
   auto by_score = [&](auto d, auto qt) {
     constexpr int DD = decltype(d)::value, QT = decltype(qt)::value;

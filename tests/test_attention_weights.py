@@ -173,6 +173,37 @@ def test_values(cuda, name, prefixes, lengths, opts, cap, steep, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("name,prefixes,lengths,opts", [
+    ("more_key_groups_than_the_table", [33000], [200], {"window": False}),
+    ("prompts_beside_each_other", [0, 0, 300], [1500, 700, 1000], {"d": 128, "hk": 2, "group": 4}),
+])
+def test_values_of_many_row_chunks(cuda, name, prefixes, lengths, opts):
+    test_values(cuda, name, prefixes, lengths, opts, 30.0, 1.0, torch.bfloat16)
+
+
+@pytest.mark.gpu
+def test_lists_of_another_batch_than_the_call_is_sized_for(cuda):
+    """Row chunks and their order come from the largest sizes alone: the device's lists may hold
+    any other requests within them."""
+    from oscar_amd import ops
+
+    c = cases.make_case([900, 0, 5], [1200, 700, 1], window=False)
+    q, k = (torch.from_numpy(c[x]).bfloat16().to(cuda) for x in "qk")
+    kc, vc = (torch.from_numpy(c[x]).view(torch.int8).to(cuda) for x in ("k8", "v8"))
+    bt, lse = torch.from_numpy(c["bt"]).to(cuda), torch.full((1901, 6), 5.0, device=cuda)
+    bt = torch.cat([bt, bt.new_zeros(3, 20 - bt.shape[1])], 1) if bt.shape[1] < 20 else bt
+    own = ops.plan_weights(c["qsl"], c["seqs"], has_new=True, device=cuda)
+    call = (lambda plan: ops.accumulate_weights(q, k, kc, vc, bt, plan, 0.0625, lse, torch.zeros(3, 1, 2560, device=cuda), head_dim=256))
+    want = call(own)
+    for qsl, seqs in (([0, 1901, 1901, 1901], [1901, 0, 0]), ([0, 40, 1900, 1901], [2500, 1860, 1]), ([0, 1, 2, 1901], [1, 1, 2500])):
+        plan = ops.plan_weights(qsl, seqs, has_new=True, device=cuda)
+        plan.qsl.copy_(own.qsl)
+        plan.seqs.copy_(own.seqs)
+        got = call(plan)
+        assert ((got - want).abs() <= 2e-6 * want + 1e-12).all()
+
+
+@pytest.mark.gpu
 def test_rows_that_hold_infinities_and_nan(cuda):
     """A row with lse = -inf adds nothing, with lse = +inf zeros; NaN stays with its request."""
     from oscar_amd import ops
