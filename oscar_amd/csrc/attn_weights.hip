@@ -481,13 +481,21 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(WeightsParams P) {
   __shared__ float s_sum[8][32];
   const int64_t pitch = A.cache.num_kv_heads * A.weights_cols;
   const float* p = P.part + ((int64_t)req * P.chunks * A.cache.num_kv_heads + kvh) * A.weights_cols;
+  const int nrows = x.nq * (int)P.group.d, chunks = ((nrows + 31) / 32 + P.chunk_blocks - 1) / P.chunk_blocks;
+  const int end = chunks < P.chunks ? chunks : P.chunks;
   for (int t0 = blockIdx.x * 32; t0 < x.seq; t0 += gridDim.x * 32) {
     const int t = t0 + lane;
+    // the chunks with rows (rows_of), eight loads of a lane in flight
+    const int tb = t0 / kGroupKeys * kGroupKeys, first = rows_of(P, 0, tb, x.before, nrows).first / P.chunk_blocks;
+    const int begin = first < P.chunks ? first : P.chunks - 1;
     float sum = 0.f;
     if (t < x.seq)
-      for (int c = part; c < P.chunks; c += 8) {
-        const Rows r = rows_of(P, c, t / kGroupKeys * kGroupKeys, x.before, x.nq * (int)P.group.d);
-        sum += r.first < r.end ? p[c * pitch + t] : 0.f;
+      for (int c0 = begin + part; c0 < end; c0 += 64) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c0 + 8 * i < end ? p[(c0 + 8 * i) * pitch + t] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += v[i];
       }
     __syncthreads();
     s_sum[part][lane] = sum;
