@@ -106,7 +106,7 @@ typedef struct oscarop_weights_args_v1 {
   /* the longest length and the most queries of a request: they size the launch, and any
    * batch gives the same results */
   int64_t max_seq_len;          /* at most 2^30, as weights_cols */
-  int64_t max_query_len;
+  int64_t max_query_len;        /* at most 2^24 */
   const oscar_staging_v1* staging; /* NULL = no window; its v side is not read */
   float scale;
   const float* lse;             /* [num_tokens, num_q_heads] */

@@ -19,8 +19,8 @@
 //                        waves; where the keys alone do not fill the chip the rows are cut
 //                        into chunks, whose sums weights_sum_kernel adds in their order.  A
 //                        block of 32 rows against 256 keys takes 2.1 us a workgroup with two
-//                        of them on a compute unit.  2500 fresh tokens of 6 heads: 29 us and
-//                        5 us for the sums, of which the keys' way into registers is 6 us
+//                        of them on a compute unit.  2500 fresh tokens of 6 heads: 28 us and
+//                        4 us for the sums, of which the keys' way into registers is 6 us
 //                        (eight waves of one tile each, their rows reordered through LDS
 //                        instead of loaded one a lane, took as long in all)
 #include <type_traits>
@@ -43,6 +43,7 @@ constexpr int kFewRows = 32;                           // of a KV head, for weig
 constexpr int kKeyTiles = 2;                           // per wave of weights_many_kernel
 constexpr int kGroupKeys = kWaves * kKeyTiles * kTile;  // per workgroup
 constexpr int kTable = 128;
+constexpr int64_t kMostTokens = 1 << 24, kMostKeys = 1 << 30;
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct WeightsParams {
@@ -568,7 +569,8 @@ using namespace oscar;
 
 extern "C" int64_t oscarop_attn_weights_workspace_bytes_v1(const oscarop_weights_args_v1* args) {
   if (!args || args->num_reqs < 0 || args->max_seq_len < 0 || args->max_query_len < 0 || args->cache.num_kv_heads < 1 ||
-      args->num_q_heads < 1 || args->num_q_heads % args->cache.num_kv_heads || args->weights_cols < 1)
+      args->num_q_heads < 1 || args->num_q_heads % args->cache.num_kv_heads || args->weights_cols < 1 ||
+      args->max_query_len > kMostTokens || args->max_seq_len > kMostKeys || args->weights_cols > kMostKeys)
     return -22;
   const Chunks c = chunks_of(*args);
   return c.count > 1 ? args->num_reqs * c.count * args->cache.num_kv_heads * args->weights_cols * (int64_t)sizeof(float) : 0;
@@ -595,7 +597,7 @@ extern "C" int oscarop_attn_weights_v1(const oscarop_weights_args_v1* args, cons
   if (a.num_reqs > 0xffff || a.cache.num_kv_heads > 0xffff || a.num_tokens * a.num_q_heads >= (1ll << 31))
     return fail(-22, "%s: too many requests or rows for one call", name);
   // (distances are counted in fp32, lengths in int)
-  if (a.num_tokens > (1 << 24) || a.max_seq_len > (1 << 30) || a.weights_cols > (1 << 30))
+  if (a.num_tokens > kMostTokens || a.max_query_len > kMostTokens || a.max_seq_len > kMostKeys || a.weights_cols > kMostKeys)
     return fail(-22, "%s: too many tokens for one call", name);
   if (a.block_table_rows < a.num_reqs || a.block_table_cols < 1 || a.block_table_stride < a.block_table_cols)
     return fail(-22, "%s: Missing request block-table rows", name);

@@ -67,6 +67,7 @@ def args(**changes):
     (dict(num_reqs=70000, block_table_rows=70000), "too many"),
     (dict(num_tokens=(1 << 24) + 1), "too many"),
     (dict(max_seq_len=(1 << 30) + 1), "too many"),
+    (dict(max_query_len=(1 << 24) + 1), "too many"),
     (dict(weights_cols=(1 << 30) + 1, weights_stride_head=1 << 31, weights_stride_request=1 << 31), "too many"),
     (dict(block_table_rows=1), "block-table rows"),
     (dict(block_table_cols=0), "block-table rows"),
@@ -96,6 +97,21 @@ def test_refused_arena_and_cap_and_empty_calls():
     assert lib.oscarop_attn_weights_v1(None, None, None) == -22
     assert lib.oscarop_attn_weights_workspace_bytes_v1(None) == -22
     assert lib.oscarop_attn_weights_workspace_bytes_v1(C.byref(args())) >= 0
+
+
+@pytest.mark.parametrize("seq,nq,hq,hk", [(2500, 2500, 6, 1), (8700, 700, 6, 1), (6000, 6000, 6, 1), (100000, 100000, 6, 1), (50, 700, 6, 1),
+                                          (600, 600, 16, 2), (33, 33, 8, 8), (1, 1, 64, 1), (1 << 30, 1 << 24, 6, 1)])
+def test_the_workspace_holds_whole_chunks_within_its_limit(seq, nq, hq, hk):
+    """A workspace is the sums of two or more row chunks, 256 MB at most, and no batch that fills
+    the chip by its keys alone has one."""
+    lib = _lib.load()
+    a = args(num_reqs=1, num_q_heads=hq, max_seq_len=seq, max_query_len=nq, weights_cols=seq, cache_num_kv_heads=hk)
+    need = lib.oscarop_attn_weights_workspace_bytes_v1(C.byref(a))
+    chunks, rest = divmod(need, 4 * hk * seq)
+    assert rest == 0 and chunks != 1 and 0 <= need <= 256 << 20
+    assert chunks <= max(1, -(-nq * (hq // hk) // 32))
+    if -(-seq // 256) * hk >= 512 or nq * (hq // hk) <= 32:
+        assert need == 0
 
 
 def test_plan_refusals():
