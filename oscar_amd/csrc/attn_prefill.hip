@@ -29,12 +29,15 @@ constexpr int kKeys = 32;
 constexpr int kRows = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-// SC: how far above the first maximum known the softmax reference of a row starts (log2).  A
-// larger score moves it, and O with it, only from kMargin + kLazy above that maximum on, and
-// the largest probability, 2^-kMargin, still has eight binary orders of normal fp16 below it.
-// 1600 tokens over 8000, capped, us: margin 0 184, 4 172, 6 169.
-constexpr float kMargin = 6.f;
 constexpr int kLazy = 10;     // log2 of the largest row sum of a tile's probabilities before O is rescaled
+// SC: the softmax reference of a row starts this far above the first maximum known (log2), and
+// a larger score moves it, and O with it, only from kMargin + kLazyScored above that maximum
+// on; probabilities stay below fp16's 2^16.  The drift of 16 binary orders lies above the
+// reference and not below it, since a row's many small probabilities need fp16's lower end (a
+// long tail of keys at 2^-19 of the largest one was off by 30% with a margin of 6).  1600
+// tokens over 8000, capped, by the drift in us: 10 184, 14 172, 16 169.
+constexpr float kMargin = 1.f;
+constexpr int kLazyScored = 15;
 // workgroups per CU the register budget of prefill_kernel<D> is set for
 constexpr int prefill_wgs(int D) { return D == 256 ? 1 : 2; }
 // PV runs on v_mfma_f32_32x32x16_f16 with P and V in fp16 for both query dtypes.  bf16
@@ -492,7 +495,7 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
   // starts at the unit's first keys would move, and all of O with it, in every tile of a
   // steep head.  It starts at the score of the row's own key instead, which it sees in any
   // case: what is so far below that its probability rounds to nothing in fp16 is below 2^-24
-  // of the row's sum.  (2047 fresh tokens, slopes from 0.4 down: 66 us before, 58 us so.)
+  // of the row's sum.  (2047 fresh tokens, slopes from 0.4 down: 66 us before, 53 us so.)
   float m_own[NB];
   const bool own_first = SC != 0 && P.sc.slopes != nullptr;
 #pragma unroll
@@ -821,7 +824,7 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
     vr = v1;
     bool moved = SC == 2 && masked;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) moved = moved || lsum[nb] > (float)(1 << kLazy) || m_run[nb] == -INFINITY;
+    for (int nb = 0; nb < NB; ++nb) moved = moved || lsum[nb] > (float)(1 << (SC ? kLazyScored : kLazy)) || m_run[nb] == -INFINITY;
     if (__builtin_expect(__any(moved), 0)) {
       asm volatile("s_nop 15\n\ts_nop 15");  // the PV MFMAs' results
 #pragma unroll

@@ -249,6 +249,30 @@ def test_prefill(cuda, hist, n, hq, hk, d, dtype, split, cap, steep):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("cap,steep", [(50.0, 0.0), (50.0, 1e-6), (0.0, 1e-6)])
+def test_many_keys_far_below_the_largest(cuda, cap, steep, split):
+    """One key takes nearly all of a row and thousands share the rest, each 2^-19 of it.  Their
+    probabilities are subnormal in fp16: each is off by half a step, 2^-25, where the row's
+    largest is 2^-1 or more (the reference lies at most one binary order above it): 2^-24 of
+    the row's sum a key."""
+    from oscar_amd import ops
+
+    n, hq, rows = 6000, 6, 64
+    q, k, v = torch.zeros(n, hq, 256), torch.zeros(n, 1, 256), torch.ones(n, 1, 256)
+    q[..., 0], k[:, 0, 0], k[0, 0, 0] = 16.0, 2.03125, 16.0 if cap else 15.5
+    v[0] = 0.0
+    q, k, v = q.bfloat16(), k.bfloat16(), v.bfloat16()
+    slopes = slopes_of(hq, steep) if steep else None
+    out = ops.attention_prefill(q.to(cuda), k.to(cuda), v.to(cuda), 0.0625, head_dim=256, split=split, soft_cap=cap,
+                                alibi_slopes=None if slopes is None else slopes.to(cuda))[-rows:].double().cpu()
+    want, _, size = reference(q[-rows:].float(), k.float(), v.float(), n - rows, 0.0625, cap, slopes, n - rows + 1)
+    assert 0.004 < want.min() and want.max() < 0.05
+    excess = (out - want).abs() - (REL_TOL * size + 2.0 ** -8 * want.abs() + ABS_TOL + n * 2.0 ** -24)
+    assert excess.max() <= 0, ((out - want) / want).abs().max()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("cap", [0.0, 20.0])
 def test_overflowing_products_and_later_tokens(cuda, cap):
     """A score that overflows is capped like any other; what a later token holds does not
