@@ -87,6 +87,36 @@ def test_a_fresh_prompt_and_its_weights(cuda, n, dtype, cap, steep):
 
 
 @pytest.mark.gpu
+def test_pages_past_four_gigabytes(cuda):
+    """The same pages at the front of a small cache and at the end of one of 4.3 GB a side: the
+    same bits from attention, weights and eviction."""
+    from oscar_amd import ops
+
+    c = cases.make_case([1500, 700], [3, 1], window=False)
+    q, k, v = (torch.from_numpy(c[x]).bfloat16().to(cuda) for x in "qkv")
+    small = [torch.from_numpy(c[x]).view(torch.int8).to(cuda) for x in ("k8", "v8")]
+    bt = torch.from_numpy(c["bt"]).to(cuda)
+    pages, blocks = small[0].shape[0], (1 << 32) // small[0][0].numel() + 1000
+    shift = blocks - pages
+    large = [torch.empty(blocks, *x.shape[1:], dtype=torch.int8, device=cuda) for x in small]
+    assert shift * large[0][0].numel() > 1 << 32
+    for a, b in zip(large, small):
+        a[shift:] = b
+    plan = ops.plan_decode(c["qsl"], c["seqs"], has_new=True, num_kv_heads=1, group=6, head_dim=256, device=cuda)
+    drop = ops.plan_evict([1500, 700], [6, 2], block_size=128, sink_tokens=7, device=cuda)
+
+    def run(caches, table):
+        out, lse = ops.attention_decode(q, k, v, *caches, table, plan, c["scale"], head_dim=256, soft_cap=20.0)
+        w = ops.accumulate_weights(q, k, *caches, table, plan, c["scale"], lse, torch.zeros(2, 1, 1503, device=cuda), head_dim=256,
+                                   soft_cap=20.0)
+        return out, lse, w, ops.evict(drop, w, *caches, table, head_dim=256)
+
+    want, got = run(small, bt), run(large, bt + shift)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    assert all(torch.equal(a[shift:], b) for a, b in zip(large, small))
+
+
+@pytest.mark.gpu
 def test_a_serving_loop(cuda):
     """Two requests: prompts, decode steps whose weights add up, an eviction, and a step over
     what is left.  Each attention is checked against a 64-bit evaluation of the cache as it
