@@ -323,7 +323,7 @@ __device__ __forceinline__ void hold_acc(f32x16 (&o)[N]) {
 // other launches: 1880 us before (four waves of 32 rows, tiles through registers, one phase
 // after the other), 1155 to 1200 us now, 0.98 PFLOP/s; a large library bf16 product reaches
 // 1.2 to 1.36 on this card.
-// SC: the score function (score.h); its work per score, three times the plain product's,
+// SC: the score function (score.h); a capped score's work, three times the plain product's,
 // takes the room beside the PV MFMAs that the second row block would need.
 template <int D, int QT, int NB, int SC>
 __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(PrefillParams P) {
@@ -980,7 +980,9 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams P) {
 // on 2, 1500 (288) 53 / 53, 1800 (398) 68 / 57; 8000 + 1600 (500) 144 / 121; 15360 + 9256
 // 1.60 / 1.23 ms.  At head dim 128 two unpaired workgroups fit a CU and overlap each other
 // (8000 + 4000 tokens, 16 heads on 2: 374 us against 380 us paired), so there are no pairs
-// there.
+// there.  Nor for scored calls, whose registers do not all fit then: a bias alone 8000 + 400
+// 89 / 94, 6000 228 / 247, 15360 + 9256 1336 / 1136; capped 8000 + 1600 166 / 177, 15360 + 9256
+// 1491 / 1652.
 constexpr int64_t kPairUnits = kSplitCUs + kSplitCUs / 8;
 template <int D, int QT>
 void launch_prefill(const PrefillParams& p, int sc, dim3 grid, bool pairs, hipStream_t s) {
