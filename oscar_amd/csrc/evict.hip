@@ -464,7 +464,9 @@ extern "C" int oscarop_evict_v1(const oscarop_evict_args_v1* args, void* stream)
   const dim3 lists((unsigned)hk, (unsigned)a.num_reqs);
   hipLaunchKernelGGL(evict_select_kernel, lists, dim3(kSelect), 0, s, p);
   OSCAR_CHECK_LAUNCH("evict_select_kernel");
-  const int64_t per = kMove / (D / 16), wgs = (a.max_drop + per - 1) / per;
+  // (moves, and the weights behind the new end: a few pages out of many columns)
+  const int64_t per = kMove / (D / 16), moves = (a.max_drop + per - 1) / per, copies = (a.weights_cols + 4 * kMove - 1) / (4 * kMove);
+  const int64_t wgs = moves > copies ? moves : copies;
   const int64_t most = (kMoveWorkgroups + hk * a.num_reqs - 1) / (hk * a.num_reqs);
   const dim3 grid((unsigned)(wgs < 1 ? 1 : wgs < most ? wgs : most), (unsigned)hk, (unsigned)a.num_reqs);
   if (D == 256) hipLaunchKernelGGL(evict_move_kernel<256>, grid, dim3(kMove), 0, s, p);
