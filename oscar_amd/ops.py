@@ -135,7 +135,8 @@ def upload(parts, device) -> list:
 class DeviceScratch:
     """Scratch of one (device, stream): last-writer claim tables, the claim epoch, the
     small store's arrival counters and the growable workspaces of the store, the decode,
-    the prefill and the native step.  Work enqueued on different streams gets different
+    the prefill and the native step (captured decodes and prefills have their own, see
+    _call_workspace).  Work enqueued on different streams gets different
     scratch, so concurrent calls never share these buffers (each is allocated while its
     stream is current, so torch's allocator orders its reuse on that stream)."""
 
@@ -205,6 +206,23 @@ class DeviceScratch:
         if self.step_ws.numel() < max(nbytes, 1):  # never hand out an empty buffer
             self.step_ws = torch.empty(max(nbytes, 4 << 20), dtype=torch.uint8, device=self.device)
         return self.step_ws
+
+
+# whether the current device's current stream captures a graph
+_is_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
+
+
+def _call_workspace(device: torch.device, kind: str, nbytes: int) -> torch.Tensor:
+    """The workspace of one attention call (kind: the DeviceScratch method): the stream's
+    shared one, or, while the stream captures a graph, one of the call's own out of the
+    graph's memory pool.  The graph keeps the address: the shared buffer may be replaced by a
+    larger one, and be in use by its stream while the graph is replayed on another."""
+    if device.index != _get_device():
+        with torch.cuda.device(device):
+            return _call_workspace(device, kind, nbytes)
+    if _is_capturing():
+        return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
+    return getattr(DeviceScratch.get(device), kind)(nbytes)
 
 
 class DeviceContext:
@@ -635,15 +653,13 @@ def attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, plan: Decod
         raise ValueError("the decode plan has not been uploaded")
     _check_table(table, plan, k_cache.shape[1])
     st = staging_struct(stage, k_cache, head_dim)
-    ws, ws_bytes = None, 0
-    if not static_scratch:
-        ws = DeviceScratch.get(dev).attn_workspace(plan.partial_bytes)
-        ws, ws_bytes = ws.data_ptr(), ws.numel()
+    ws = None if static_scratch else _call_workspace(dev, "attn_workspace", plan.partial_bytes)
     has_new = k_new is not None
     a = _lib.AttnArgs(q.data_ptr(), n, hq, q.stride(0), _ptr(k_new), _ptr(v_new), k_new.stride(0) if has_new else 0,
                       cache_struct(k_cache, v_cache, head_dim), table.data_ptr(), table.stride(0), plan.qsl.data_ptr(),
                       plan.seqs.data_ptr(), plan.seqs.numel(), None if st is None else C.pointer(st), scale,
-                      plan.items.data_ptr(), plan.num_items, plan.groups.data_ptr(), plan.num_groups, ws, ws_bytes,
+                      plan.items.data_ptr(), plan.num_items, plan.groups.data_ptr(), plan.num_groups, _ptr(ws),
+                      0 if ws is None else ws.numel(),
                       plan.max_group_items, out_rot.data_ptr(), lse.data_ptr(), phases, _DTYPES[q.dtype], *table.shape)
     lib, stream = _lib.load(), _stream(dev)
     if score is not None:
@@ -712,7 +728,7 @@ def attention_prefill(q, k, v, scale, *, head_dim, history=0, k_cache=None, v_ca
     if need > 0:
         # the size asked for, not the shared buffer's (which an earlier call may have
         # grown past v1's size: the call would then split)
-        ws = DeviceScratch.get(q.device).prefill_workspace(need)
+        ws = _call_workspace(q.device, "prefill_workspace", need)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
     if score is not None:
         _launch("oscarop_attn_prefill_v1", q.get_device(), C.byref(a), C.byref(score))

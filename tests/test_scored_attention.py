@@ -408,3 +408,59 @@ def test_captured_with_eager_calls_between(cuda):
         torch.cuda.synchronize()
         for a, b in zip((out, lse, fresh), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap,steep", [(0.0, 0.0), (9.0, 1.0)])
+def test_captured_calls_keep_their_workspaces(cuda, cap, steep):
+    """A captured decode and a captured split prefill: calls that need larger workspaces run
+    on the capture stream afterwards, memory is allocated and filled, and the graph is replayed
+    on another stream beside such calls."""
+    from oscar_amd import ops
+
+    score = dict(soft_cap=cap, alibi_slopes=slopes_of(6, steep).to(cuda) if steep else None)
+    gen = torch.Generator(device=cuda).manual_seed(4)
+
+    def calls(histories, chunks, tokens):
+        # (items of one tile each, whose sums have one order)
+        c = cases.make_case(histories, chunks)
+        plan = ops.plan_decode(c["qsl"], c["seqs"], has_new=True, num_kv_heads=1, group=6, head_dim=256, device=cuda,
+                               target_items=400)
+        kc, vc = (torch.from_numpy(c[x]).view(torch.int8).to(cuda) for x in ("k8", "v8"))
+        q, k, v = (torch.from_numpy(c[x]).bfloat16().to(cuda) for x in "qkv")
+        rows = [torch.randn(tokens, h, 256, generator=gen, device=cuda).bfloat16() for h in (6, 1, 1)]
+        bt, n = torch.from_numpy(c["bt"]).to(cuda), sum(chunks)
+        outs = (torch.zeros(n, 6, 256, device=cuda), torch.zeros(n, 6, device=cuda),
+                torch.zeros(tokens, 6, 256, device=cuda, dtype=torch.bfloat16))
+
+        def run():
+            ops.attention_decode(q, k, v, kc, vc, bt, plan, c["scale"], head_dim=256, out_rot=outs[0], lse=outs[1], **score)
+            ops.attention_prefill(*rows, c["scale"], head_dim=256, out=outs[2], **score)
+        return run, outs, plan.partial_bytes
+
+    small, outs, few = calls([700, 33], [3, 1], 900)
+    large, others, many = calls([5000], [4], 4000)
+    assert many > max(few, 1 << 20)  # (a shared workspace has a megabyte at least)
+    small()
+    large()
+    want, beside = [x.clone() for x in outs], [x.clone() for x in others]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        small()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            small()
+    for step in range(3):
+        for x in (*outs, *others):
+            x.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            large()
+            fillers = [torch.full((1 << 20,), 7.0, device=cuda) for _ in range(8)]
+            large()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((*outs, *others), (*want, *beside))), step
+        assert all((x == 7.0).all() for x in fillers)
