@@ -158,6 +158,8 @@ typedef struct oscarop_evict_args_v1 {
   int64_t workspace_bytes;
 } oscarop_evict_args_v1;
 
+/* -22 for sizes that the call would refuse: num_reqs or num_kv_heads past 65535, 2^30 or
+ * more tokens to drop, more bytes than an int64_t counts */
 int64_t oscarop_evict_workspace_bytes_v1(int64_t num_reqs, int64_t num_kv_heads, int64_t max_drop);
 int oscarop_evict_v1(const oscarop_evict_args_v1* args, void* stream);
 

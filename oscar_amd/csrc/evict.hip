@@ -42,6 +42,8 @@ constexpr int kFirst = 10;             // bits of the first: sign, exponent and 
 constexpr int kCopies = 4;             // of its bins: most weights share a few exponents, and atomics of one bin take turns
 constexpr int kBins = kCopies << kFirst;
 constexpr int kMove = 256;
+constexpr int64_t kMostLists = 0xffff;       // requests, and KV heads: an axis of the grid each
+constexpr int64_t kMostTokens = 1ll << 30;   // of a list, below: places are offsets of 32 bits
 // workgroups of evict_move_kernel: about one per 32 moves of a large call, since fewer than
 // max_drop tokens move (128000 moves in 8192 / 4096 / 2048 workgroups: 14.9 / 13.6 / 14.5 us)
 constexpr int64_t kMoveWorkgroups = 4096;
@@ -415,8 +417,10 @@ __global__ __launch_bounds__(kMove) void evict_move_kernel(EvictParams P) {
 using namespace oscar;
 
 extern "C" int64_t oscarop_evict_workspace_bytes_v1(int64_t num_reqs, int64_t num_kv_heads, int64_t max_drop) {
-  if (num_reqs < 0 || num_kv_heads < 1 || max_drop < 0) return -22;
-  return num_reqs * num_kv_heads * (2 * max_drop + 1) * (int64_t)sizeof(int32_t);
+  if (num_reqs < 0 || num_kv_heads < 1 || max_drop < 0 || num_reqs > kMostLists || num_kv_heads > kMostLists || max_drop >= kMostTokens)
+    return -22;
+  int64_t bytes;
+  return __builtin_mul_overflow(num_reqs * num_kv_heads, (2 * max_drop + 1) * (int64_t)sizeof(int32_t), &bytes) ? -22 : bytes;
 }
 
 extern "C" int oscarop_evict_v1(const oscarop_evict_args_v1* args, void* stream) {
@@ -429,7 +433,7 @@ extern "C" int oscarop_evict_v1(const oscarop_evict_args_v1* args, void* stream)
   if (a.num_reqs == 0) return 0;
   if (!a.weights || !a.weights_out || !a.block_table || !a.requests || !a.cache.k || !a.cache.v)
     return fail(-22, "%s: missing pointer", name);
-  if (hk < 1 || hk > 0xffff || a.num_reqs > 0xffff || a.weights_cols < 1 || a.weights_cols >= (1ll << 30))
+  if (hk < 1 || hk > kMostLists || a.num_reqs > kMostLists || a.weights_cols < 1 || a.weights_cols >= kMostTokens || a.max_drop >= kMostTokens)
     return fail(-22, "%s: sizes out of range", name);
   if (bs < 1 || bs > (1 << 20) || a.max_drop % bs) return fail(-22, "%s: max_drop must be whole pages", name);
   if (a.block_table_rows < a.num_reqs || a.block_table_cols < 1 || a.block_table_stride < a.block_table_cols)
@@ -450,6 +454,7 @@ extern "C" int oscarop_evict_v1(const oscarop_evict_args_v1* args, void* stream)
     return fail(-22, "%s: weights_out overlaps weights", name);
   if (a.staging && (a.staging->rows < 1 || !a.staging->owner)) return fail(-22, "%s: staging arena rows out of range", name);
   const int64_t need = oscarop_evict_workspace_bytes_v1(a.num_reqs, hk, a.max_drop);
+  if (need < 0) return fail(-22, "%s: sizes out of range", name);
   if (!a.workspace || a.workspace_bytes < need || (((uintptr_t)a.workspace) & 15))
     return fail(-22, "%s: 16-byte aligned workspace of %lld bytes required", name, (long long)need);
   EvictParams p{};

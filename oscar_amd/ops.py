@@ -933,7 +933,7 @@ def evict(plan: EvictPlan, weights, k_cache, v_cache, block_table, *, head_dim, 
         table = table.contiguous()
     st = staging_struct(stage, k_cache, head_dim)
     need = _lib.load().oscarop_evict_workspace_bytes_v1(reqs, hk, plan.max_drop)
-    ws = torch.empty(need, dtype=torch.uint8, device=weights.device)  # a captured call keeps its own
+    ws = torch.empty(max(need, 0), dtype=torch.uint8, device=weights.device)  # a captured call keeps its own
     a = _lib.EvictArgs(weights.data_ptr(), request, head, weights.shape[2], weights_out.data_ptr(), out_request, out_head,
                        cache, table.data_ptr(), table.stride(0), *table.shape, plan.requests.data_ptr(), reqs, 0,
                        plan.max_drop, None if st is None else C.pointer(st), ws.data_ptr(), ws.numel())

@@ -65,6 +65,26 @@ def test_workspace_and_empty_calls():
     assert lib.oscarop_evict_v1(C.byref(args(staging=C.pointer(stage))), None) == -22
 
 
+@pytest.mark.parametrize("sizes", [(1, 1, 1 << 61), (1, 1, 1 << 62), (1, 1, 1 << 30), (0xffff, 0xffff, 1 << 29), (1 << 40, 1, 128),
+                                   (1, 1 << 40, 128)])
+def test_sizes_that_overflow_are_refused(sizes):
+    """2 max_drop + 1 entries a list wrapped around to a few bytes, which a workspace then had."""
+    lib = _lib.load()
+    assert lib.oscarop_evict_workspace_bytes_v1(*sizes) == -22
+    reqs, heads, drop = sizes
+    if reqs < 1 << 31:
+        a = args(num_reqs=reqs, cache_num_kv_heads=heads, max_drop=drop, block_table_rows=reqs, workspace_bytes=1 << 62,
+                 weights_stride_head=1 << 9, weights_stride_request=1 << 26, out_stride_head=1 << 9, out_stride_request=1 << 26,
+                 weights_out=1 << 56)
+        assert lib.oscarop_evict_v1(C.byref(a), None) == -22
+        assert "sizes out of range" in lib.oscar_last_error().decode()
+
+
+def test_the_largest_sizes_have_a_workspace():
+    drop = (1 << 30) - 128
+    assert _lib.load().oscarop_evict_workspace_bytes_v1(1, 8, drop) == 8 * 4 * (2 * drop + 1)
+
+
 def plan_on_the_cpu(monkeypatch, *a, **kw):
     from oscar_amd import ops
 
