@@ -44,6 +44,8 @@ constexpr int kKeyTiles = 2;                           // per wave of weights_ma
 constexpr int kGroupKeys = kWaves * kKeyTiles * kTile;  // per workgroup
 constexpr int kTable = 128;
 constexpr int64_t kMostTokens = 1 << 24, kMostKeys = 1 << 30;
+constexpr int64_t kMostLists = 0xffff;  // requests, and KV heads: an axis of the grid each
+constexpr int64_t kMostHeads = 1 << 20;
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct WeightsParams {
@@ -570,6 +572,7 @@ using namespace oscar;
 extern "C" int64_t oscarop_attn_weights_workspace_bytes_v1(const oscarop_weights_args_v1* args) {
   if (!args || args->num_reqs < 0 || args->max_seq_len < 0 || args->max_query_len < 0 || args->cache.num_kv_heads < 1 ||
       args->num_q_heads < 1 || args->num_q_heads % args->cache.num_kv_heads || args->weights_cols < 1 ||
+      args->num_reqs > kMostLists || args->cache.num_kv_heads > kMostLists || args->num_q_heads > kMostHeads ||
       args->max_query_len > kMostTokens || args->max_seq_len > kMostKeys || args->weights_cols > kMostKeys)
     return -22;
   const Chunks c = chunks_of(*args);
@@ -594,9 +597,10 @@ extern "C" int oscarop_attn_weights_v1(const oscarop_weights_args_v1* args, cons
   if (a.num_reqs == 0 || a.num_tokens == 0 || a.max_seq_len == 0) return 0;
   if (!a.q || !a.lse || !a.weights || !a.query_start_loc || !a.seq_lens || !a.block_table || !a.cache.k)
     return fail(-22, "%s: missing pointer", name);
-  if (a.num_reqs > 0xffff || a.cache.num_kv_heads > 0xffff || a.num_tokens * a.num_q_heads >= (1ll << 31))
+  // (distances are counted in fp32, lengths and rows in int)
+  if (a.num_reqs > kMostLists || a.cache.num_kv_heads > kMostLists || a.num_q_heads > kMostHeads ||
+      a.num_tokens >= (1ll << 31) || a.num_tokens * a.num_q_heads >= (1ll << 31))
     return fail(-22, "%s: too many requests or rows for one call", name);
-  // (distances are counted in fp32, lengths in int)
   if (a.num_tokens > kMostTokens || a.max_query_len > kMostTokens || a.max_seq_len > kMostKeys || a.weights_cols > kMostKeys)
     return fail(-22, "%s: too many tokens for one call", name);
   if (a.block_table_rows < a.num_reqs || a.block_table_cols < 1 || a.block_table_stride < a.block_table_cols)

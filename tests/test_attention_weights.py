@@ -114,6 +114,21 @@ def test_the_workspace_holds_whole_chunks_within_its_limit(seq, nq, hq, hk):
         assert need == 0
 
 
+@pytest.mark.parametrize("changes", [dict(num_reqs=1 << 16), dict(cache_num_kv_heads=1 << 16, num_q_heads=1 << 16),
+                                     dict(num_reqs=4, cache_num_kv_heads=(1 << 62) + 1, num_q_heads=(1 << 62) + 1),
+                                     dict(num_q_heads=1 << 44, max_query_len=1 << 24)])
+def test_sizes_that_the_call_refuses_have_no_workspace(changes):
+    assert _lib.load().oscarop_attn_weights_workspace_bytes_v1(C.byref(args(**changes))) == -22
+
+
+@pytest.mark.parametrize("changes", [dict(num_tokens=1 << 20, num_q_heads=1 << 44), dict(num_tokens=1 << 60, num_q_heads=16),
+                                     dict(num_q_heads=(1 << 20) + 1), dict(cache_num_kv_heads=1 << 16, num_q_heads=1 << 16)])
+def test_sizes_whose_product_wraps_around_are_refused(changes):
+    lib = _lib.load()
+    assert lib.oscarop_attn_weights_v1(C.byref(args(**changes)), None, None) == -22
+    assert "too many" in lib.oscar_last_error().decode()
+
+
 def test_plan_refusals():
     from oscar_amd import ops
 
