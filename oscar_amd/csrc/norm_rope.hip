@@ -185,9 +185,11 @@ extern "C" int oscarop_norm_rope_v1(const oscarop_norm_rope_args_v1* args, void*
   if (!(a.eps >= 0.f)) return fail(-22, "%s: eps must not be negative", name);
   if (a.rotary_dim < 16 || a.rotary_dim > D || a.rotary_dim % 16)
     return fail(-22, "%s: rotary_dim %lld must be a multiple of 16 up to head_dim", name, (long long)a.rotary_dim);
-  const int64_t heads = a.num_q_heads + a.num_kv_heads;
+  constexpr int64_t kMostHeads = 1 << 20, kMostRows = 1ll << 31;  // below
+  const bool many = a.num_q_heads >= kMostHeads || a.num_kv_heads >= kMostHeads;
+  const int64_t heads = many ? kMostHeads : a.num_q_heads + a.num_kv_heads;
   if (a.num_tokens == 0 || heads == 0) return 0;
-  if (heads >= (1 << 20) || a.num_tokens * heads >= (1ll << 31))
+  if (heads >= kMostHeads || a.num_tokens >= kMostRows || a.num_tokens * heads >= kMostRows)
     return fail(-22, "%s: too many rows for one call", name);
   if (!a.positions || !a.cos_sin || a.cos_sin_rows < 1 || (a.num_q_heads && (!a.q || !a.q_out)) ||
       (a.num_kv_heads && (!a.k || !a.k_out)))

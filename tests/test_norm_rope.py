@@ -86,6 +86,14 @@ def test_refusals(changes, message):
     assert message in lib.oscar_last_error().decode()
 
 
+@pytest.mark.parametrize("changes", [dict(num_tokens=1 << 45, num_q_heads=1 << 18, num_kv_heads=1 << 18), dict(num_tokens=1 << 61, num_q_heads=7),
+                                     dict(num_q_heads=1 << 62, num_kv_heads=1 << 62), dict(num_q_heads=(1 << 63) - 1)])
+def test_sizes_whose_product_wraps_around_are_refused(changes):
+    lib = _lib.load()
+    assert lib.oscarop_norm_rope_v1(C.byref(args(**changes)), None) == -22
+    assert "too many rows" in lib.oscar_last_error().decode()
+
+
 def test_empty_calls_succeed_without_a_launch():
     lib = _lib.load()
     assert lib.oscarop_norm_rope_v1(C.byref(args(num_tokens=0, q=None, positions=None)), None) == 0
