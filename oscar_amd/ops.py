@@ -79,11 +79,19 @@ _CACHE = struct.Struct("=QQ10q").pack  # _lib.Cache's fields
 
 
 def cache_struct(k_cache: torch.Tensor, v_cache: torch.Tensor, head_dim: int) -> _lib.Cache:
-    """Byte view of a packed cache pair [num_blocks, block_size, Hk, D] (int8 or bf16)."""
+    """Byte view of a packed cache pair [num_blocks, block_size, Hk, D] (int8 or bf16).  The
+    kernels take the blocks, tokens and heads of K for both, so the two must have the same,
+    and their slots room for the constants (K's first 32 bytes) and the codes."""
     if k_cache.ndim != 4 or v_cache.ndim != 4 or not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise ValueError("OSCAR requires contiguous [blocks, tokens, heads, bytes] caches")
     blocks, tokens, heads, width = k_cache.shape
     k2, v2 = width * k_cache.element_size(), v_cache.shape[3] * v_cache.element_size()
+    if v_cache.shape[:3] != k_cache.shape[:3]:
+        raise ValueError(f"OSCAR requires K and V caches of the same blocks, tokens and heads, got "
+                         f"{list(k_cache.shape[:3])} and {list(v_cache.shape[:3])}")
+    if k2 < 32 + head_dim // 4 or v2 < head_dim // 4:
+        raise ValueError(f"OSCAR slots of head_dim {head_dim} take {32 + head_dim // 4} bytes of K and {head_dim // 4} of V, "
+                         f"the caches have {k2} and {v2}")
     return _lib.Cache.from_buffer_copy(_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), blocks, tokens, heads, head_dim,
                                               tokens * heads * k2, heads * k2, k2, tokens * heads * v2, heads * v2, v2))
 

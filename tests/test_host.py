@@ -252,6 +252,24 @@ def test_staging_struct_checks_the_arena_against_the_cache():
         staging_struct((good[0].half(), good[1], good[2]), kc, 64)
 
 
+def test_cache_struct_refuses_pairs_that_do_not_match():
+    """The kernels bound page ids by K's blocks and lay V out by K's tokens and heads."""
+    from oscar_amd import ops
+
+    k = torch.zeros(4, 128, 2, 160, dtype=torch.int8)
+    for shape in ((3, 128, 2, 160), (5, 128, 2, 160), (4, 64, 2, 160), (4, 128, 1, 160), (4, 128, 4, 80)):
+        with pytest.raises(ValueError, match="same blocks, tokens and heads"):
+            ops.cache_struct(k, torch.zeros(shape, dtype=torch.int8), 256)
+    for kw, vw in ((95, 64), (96, 63), (80, 256)):
+        with pytest.raises(ValueError, match="slots of head_dim 256"):
+            ops.cache_struct(k[..., :kw].contiguous(), torch.zeros(4, 128, 2, vw, dtype=torch.int8), 256)
+    for kw, vw, d in ((96, 64, 256), (64, 32, 128), (48, 16, 64)):
+        c = ops.cache_struct(k[..., :kw].contiguous(), torch.zeros(4, 128, 2, vw, dtype=torch.int8), d)
+        assert list(c.k_stride) == [256 * kw, 2 * kw, kw] and list(c.v_stride) == [256 * vw, 2 * vw, vw]
+    legacy = torch.zeros(4, 128, 2, 48, dtype=torch.bfloat16)
+    assert ops.cache_struct(legacy, legacy, 256).k_stride[2] == 96
+
+
 def test_mixed_batch_routes_slice_consecutive_decodes_and_gather_otherwise():
     """A batch with a continuation chunk or a fresh prefill sends its short requests to the
     split-K decode: as a slice of the batch's rows and block-table rows when they (and empty
