@@ -580,16 +580,19 @@ def cu_count(device) -> int:
 
 def _plan_sizes(plan, block_size: int) -> tuple:
     """Of a plan's requests with queries: (pages of the longest history, longest length, most
-    queries), worked out once for a plan and page size."""
-    sizes = getattr(plan, "_sizes", None)
-    if sizes is None or sizes[0] != block_size:
-        pages = longest = most = 0
-        for a, b, seq in zip(plan.host_qsl, plan.host_qsl[1:], plan.host_seqs):
-            if b > a:
-                pages = max(pages, -(-(seq - (b - a) if plan.has_new else seq) // block_size))
-                longest, most = max(longest, seq), max(most, b - a)
-        sizes = plan._sizes = (block_size, pages, longest, most)
-    return sizes[1:]
+    queries), worked out again only when the plan's lists or the page size are others."""
+    key = (block_size, plan.has_new, plan.host_qsl, plan.host_seqs)
+    known = getattr(plan, "_sizes", None)
+    if known is not None and known[0] == key:
+        return known[1]
+    pages = longest = most = 0
+    for a, b, seq in zip(plan.host_qsl, plan.host_qsl[1:], plan.host_seqs):
+        if b > a:
+            pages = max(pages, -(-(seq - (b - a) if plan.has_new else seq) // block_size))
+            longest, most = max(longest, seq), max(most, b - a)
+    sizes = pages, longest, most
+    plan._sizes = (block_size, plan.has_new, list(plan.host_qsl), list(plan.host_seqs)), sizes
+    return sizes
 
 
 def _covers(plan: DecodePlan, n: int) -> bool:

@@ -138,6 +138,27 @@ def test_plan_refusals():
             ops.plan_weights(qsl, seqs, has_new=new, device="cuda")
 
 
+def test_the_sizes_of_a_plan_follow_its_lists():
+    """A caller may change a plan's host lists between calls, as it does the device's."""
+    from oscar_amd import ops
+
+    plan = ops.WeightsPlan([0, 2, 2, 5], [300, 900, 40], True, None, None)
+    assert ops._plan_sizes(plan, 128) == (3, 300, 3)  # (a request without queries reads nothing)
+    assert ops._plan_sizes(plan, 32) == (10, 300, 3)
+    plan.host_seqs[0] = 1000
+    assert ops._plan_sizes(plan, 32) == (32, 1000, 3)
+    plan.host_qsl = [0, 2, 4, 5]
+    assert ops._plan_sizes(plan, 32) == (32, 1000, 2) and ops._plan_sizes(plan, 128) == (8, 1000, 2)
+    plan.has_new = False
+    plan.host_seqs[0] = 898
+    assert ops._plan_sizes(plan, 32) == (29, 900, 2)
+    table = torch.zeros(3, 28, dtype=torch.int32)
+    with pytest.raises(ValueError, match="cannot cover"):
+        ops._check_table(table, plan, 32)
+    plan.host_seqs[:] = [896, 896, 896]
+    ops._check_table(table, plan, 32)
+
+
 # ------------------------------------------------------------------ values
 BATCHES = [
     ("mtp_window", [129, 1025, 3, 300], [4, 3, 1, 2], {}),
