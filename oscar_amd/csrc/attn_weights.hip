@@ -442,7 +442,9 @@ __global__ __launch_bounds__(kThreads, 2) void weights_many_kernel(WeightsParams
         kop[i][2 * c + 1] = b;
       });
     }
-    float acc[kKeyTiles] = {};
+    // (64 bits: a prompt of 131072 tokens adds 24576 blocks' sums here, of which as many fp32
+    // additions lose 2e-4)
+    double acc[kKeyTiles] = {};
     for (int rb = rows.first; rb < rows.end; ++rb) {
       const int buf = (rb - rows.first) & 1;
       put_queries<D, SC>(P, q, s_q[buf], s_row[buf]);
@@ -466,7 +468,7 @@ __global__ __launch_bounds__(kThreads, 2) void weights_many_kernel(WeightsParams
 #pragma unroll
     for (int i = 0; i < kKeyTiles; ++i) {
       const int t = wave_t0 + i * kTile + m;
-      if (lane < 32 && t < x.seq) out[t] = P.chunks > 1 ? acc[i] : out[t] + acc[i];
+      if (lane < 32 && t < x.seq) out[t] = (float)(P.chunks > 1 ? acc[i] : out[t] + acc[i]);
     }
     __syncthreads();  // the next key group's first block goes over a buffer still being read
   }

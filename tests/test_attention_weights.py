@@ -411,3 +411,67 @@ def test_captured_with_lengths_that_grow(cuda):
         call(want)
         torch.cuda.synchronize()
         assert torch.equal(weights, want) and weights[0, 0, 700 + extra] > 0
+
+
+@pytest.mark.gpu
+def test_values_of_many_requests(cuda):
+    """As many key groups as the chip holds workgroups: rows are not cut into chunks, and sums go
+    straight to the weights."""
+    test_values(cuda, "", [260] * 127 + [200], [40] * 128, {"d": 128, "hk": 2, "group": 4}, 30.0, 1.0, torch.bfloat16)
+    test_values(cuda, "", [240] * 127 + [3000], [40] * 128, {"hk": 2, "group": 2, "window": False}, 0.0, 0.0, torch.float16)
+
+
+@pytest.mark.gpu
+def test_a_misfit_among_many_requests(cuda):
+    from oscar_amd import ops
+
+    c = cases.make_case([260] * 128, [40] * 128, d=128, hk=2, group=4)
+    q, k = (torch.from_numpy(c[x]).bfloat16().to(cuda) for x in "qk")
+    kc, vc = (torch.from_numpy(c[x]).view(torch.int8).to(cuda) for x in ("k8", "v8"))
+    bt, lse = torch.from_numpy(c["bt"]).to(cuda), torch.full((5120, 8), 3.0, device=cuda)
+    plan = ops.plan_weights(c["qsl"], c["seqs"], has_new=True, device=cuda)
+    call = (lambda: ops.accumulate_weights(q, k, kc, vc, bt, plan, 0.0625, lse, torch.zeros(128, 2, 320, device=cuda), head_dim=128))
+    want = call()
+    assert want.isfinite().all()
+    plan.seqs[5], plan.seqs[9], plan.seqs[127] = 321, 39, 2000000000
+    got = call()
+    bad = torch.tensor([5, 9, 127])
+    assert got[5].isnan().all() and got[9, :, :39].isnan().all() and (got[9, :, 39:] == 0).all() and got[127].isnan().all()
+    rest = [r for r in range(128) if r not in bad]
+    assert torch.equal(got[rest], want[rest])
+
+
+@pytest.mark.gpu
+def test_a_long_prompt_sums_many_rows(cuda):
+    """131072 tokens of 6 heads: key 0 gets 786432 equal weights.  An fp32 sum of the 24576 row
+    blocks one after the other is off by 2.3e-4.  Here an exp2 errs by 2^-22, its factor by
+    2^-24, the sum of a block's 32 rows by 17 2^-24, the result by 2^-24: below 2^-19."""
+    from oscar_amd import ops
+
+    n = 131072
+    q, k = torch.zeros(n, 6, 128, dtype=torch.bfloat16, device=cuda), torch.ones(n, 1, 128, dtype=torch.bfloat16, device=cuda)
+    kc = torch.zeros(1, 128, 1, 128, dtype=torch.int8, device=cuda)
+    plan = ops.plan_weights([0, n], [n], has_new=True, device=cuda)
+    got = ops.accumulate_weights(q, k, kc, kc, torch.zeros(1, 1, dtype=torch.int32, device=cuda).expand(1, 1024).contiguous(), plan, 0.0625,
+                                 torch.full((n, 6), 3.0, device=cuda), torch.zeros(1, 1, n, device=cuda), head_dim=128)
+    want = 6 * math.exp(-3.0) * torch.arange(n, 0, -1, dtype=torch.float64)
+    assert ((got[0, 0].double().cpu() - want).abs() <= 2.0 ** -19 * want).all()
+
+
+@pytest.mark.gpu
+def test_lengths_far_past_the_sizes_of_a_small_call(cuda):
+    """Few rows, sized for 40 tokens: each wave then goes through more than 64 tiles, whose pages
+    it looks up 64 at a time.  A key's sum does not depend on the grid."""
+    from oscar_amd import ops
+
+    c = cases.make_case([20000, 33], [3, 2], window=False)
+    q, k = (torch.from_numpy(c[x]).bfloat16().to(cuda) for x in "qk")
+    kc, vc = (torch.from_numpy(c[x]).view(torch.int8).to(cuda) for x in ("k8", "v8"))
+    bt, lse = torch.from_numpy(c["bt"]).to(cuda), torch.full((5, 6), 5.0, device=cuda)
+    own = ops.plan_weights(c["qsl"], c["seqs"], has_new=True, device=cuda)
+    call = (lambda plan: ops.accumulate_weights(q, k, kc, vc, bt, plan, 0.0625, lse, torch.zeros(2, 1, 20100, device=cuda), head_dim=256))
+    want = call(own)
+    assert (want[0, 0, :20001] > 0).all() and (want[0, 0, 20003:] == 0).all()
+    small = ops.plan_weights(c["qsl"], [40, 35], has_new=True, device=cuda)
+    small.seqs.copy_(own.seqs)
+    assert torch.equal(call(small), want)
