@@ -30,14 +30,18 @@ constexpr int kRows = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kLazy = 10;     // log2 of the largest row sum of a tile's probabilities before O is rescaled
-// SC: the softmax reference of a row starts this far above the first maximum known (log2), and
+// SC: the softmax reference of a row starts kMargin above the first maximum known (log2), and
 // a larger score moves it, and O with it, only from kMargin + kLazyScored above that maximum
 // on; probabilities stay below fp16's 2^16.  The drift of 16 binary orders lies above the
 // reference and not below it, since a row's many small probabilities need fp16's lower end (a
-// long tail of keys at 2^-19 of the largest one was off by 30% with a margin of 6).  1600
-// tokens over 8000, capped, by the drift in us: 10 184, 14 172, 16 169.
+// long tail of keys at 2^-19 of the largest one was off by 30% with a margin of 6): such a
+// probability is off by 2^-25 of the reference, 2^-24 of the largest key, and for that to stay
+// below 2^-12 of the row, a probability's own rounding, over all keys of a unit the reference
+// starts one binary order lower for every doubling of its key tiles past 128.  1600 tokens over
+// 8000, capped, by the drift in us: 10 184, 14 172, 16 169.
 constexpr float kMargin = 1.f;
 constexpr int kLazyScored = 15;
+constexpr float kFar = 12.f;
 // workgroups per CU the register budget of prefill_kernel<D> is set for
 constexpr int prefill_wgs(int D) { return D == 256 ? 1 : 2; }
 // PV runs on v_mfma_f32_32x32x16_f16 with P and V in fp16 for both query dtypes.  bf16
@@ -130,6 +134,7 @@ struct PrefillParams {
                        // chunks, as the MFMA results lie (32 rows x 32 columns per 4 x 64 x 4)
   float* part_lse;     // [slot][Hk][kRows] log2-domain LSE of each partial
   Score sc;            // SC != 0
+  float nothing;       // the merge leaves out a chunk whose log2 LSE lies this far below a row's largest
 };
 
 // key tiles seen by the last query of a tile ending at chunk token q1
@@ -493,47 +498,57 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
   const float c = A.scale * kLog2e;
   // With a distance bias a row's maximum lies near its own position, and a reference that
   // starts at the unit's first keys would move, and all of O with it, in every tile of a
-  // steep head.  It starts at the score of the row's own key instead, which it sees in any
-  // case: what is so far below that its probability rounds to nothing in fp16 is below 2^-24
-  // of the row's sum.  (2047 fresh tokens, slopes from 0.4 down: 66 us before, 53 us so.)
-  float m_own[NB];
-  const bool own_first = SC != 0 && P.sc.slopes != nullptr;
+  // steep head.  It starts at the larger of two scores that are known before:
+  //  - that of the last key of the unit that the row sees, plus the margin;
+  //  - kFar below that of the row's own key, which it sees in some unit: a probability's
+  //    rounding to fp16 (2^-25 where it is a subnormal or nothing) is then 2^-(25 + kFar) of the
+  //    row's sum, and most units of a steep head need no look at their keys' differences.
+  // (The row's own key plus a margin for every unit: 131072 keys 24.1 binary orders below it
+  // hold 0.7% of the row, and all were lost.  2047 fresh tokens, slopes from 0.4 down: 66 us
+  // with the first keys' reference.)
+  const float margin = SC ? kMargin - (float)max(25 - __builtin_clz(ke - kb), 0) : 0.f;
+  float m_last[NB], slope2[NB] = {}, row_pos[NB] = {}, bias0[NB] = {};
+  const bool last_first = SC != 0 && P.sc.slopes != nullptr;
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) m_own[nb] = -INFINITY;
-  if (own_first) {
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const Row r = row_of(nb);
-      const uint16_t* krow = (const uint16_t*)cur_k + (r.ok ? r.qi : 0) * A.kv_stride_token;
-      u32x4 kw[D / 16];
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j) kw[j] = *(const u32x4*)(krow + 16 * j + 8 * g);
-      __builtin_amdgcn_sched_barrier(0);  // all of them in flight at once
-      float dots[4] = {};
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
-        float qf[8], kf[8];
-        load8<QT>(&kw[j], 0, kf);
-        const u32x4 qw = __builtin_bit_cast(u32x4, qreg[nb][j]);
-        load8<QT>(&qw, 0, qf);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dots[e & 3] = fmaf(qf[e], kf[e], dots[e & 3]);
-      }
-      float dot = (dots[0] + dots[1]) + (dots[2] + dots[3]);
-      auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(dot), __float_as_uint(dot), false, false);
-      dot = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-      m_own[nb] = (SC == 2 ? capped2(P.sc, dot) : dot * P.sc.scale2) + kMargin;
-    }
-  }
-
-  // SC: the rows' slopes (log2 units) and positions, and the bias of a tile's first key
-  float slope2[NB] = {}, row_pos[NB] = {}, bias0[NB] = {};
+  for (int nb = 0; nb < NB; ++nb) m_last[nb] = -INFINITY;
+  // the rows' slopes (log2 units) and positions, and the bias of a tile's first key
   if constexpr (SC != 0) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const Row r = row_of(nb);
       slope2[nb] = slope2_of(P.sc, r.head);
       row_pos[nb] = (float)(hist + r.qi);
+    }
+  }
+  if (last_first) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const Row r = row_of(nb);
+      const int own = (int)(hist + (r.ok ? r.qi : 0)), last = own < ke * kKeys ? own : ke * kKeys - 1;
+      auto score_of_key = [&](int p) __attribute__((always_inline)) {  // without its bias
+        const bool in_hist = p < ihist;
+        const uint64_t krow = (in_hist ? hist_k : cur_k) + (uint64_t)(unsigned)(in_hist ? p : p - ihist) * (unsigned)(in_hist ? hrow : crow);
+        u32x4 kw[D / 16];
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) kw[j] = *(const u32x4*)((const uint16_t*)krow + 16 * j + 8 * g);
+        __builtin_amdgcn_sched_barrier(0);  // all of them in flight at once
+        float dots[4] = {};
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+          float qf[8], kf[8];
+          load8<QT>(&kw[j], 0, kf);
+          const u32x4 qw = __builtin_bit_cast(u32x4, qreg[nb][j]);
+          load8<QT>(&qw, 0, qf);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dots[e & 3] = fmaf(qf[e], kf[e], dots[e & 3]);
+        }
+        float dot = (dots[0] + dots[1]) + (dots[2] + dots[3]);
+        auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(dot), __float_as_uint(dot), false, false);
+        dot = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+        return SC == 2 ? capped2(P.sc, dot) : dot * P.sc.scale2;
+      };
+      m_last[nb] = fmaf(slope2[nb], (float)(last - own), score_of_key(last)) + margin;
+      if (ke * kKeys <= (int)(hist + q0)) m_last[nb] = fmaxf(m_last[nb], score_of_key(own) - kFar);  // a unit without any own key
     }
   }
   auto at_tile = [&](int kt) __attribute__((always_inline)) {
@@ -788,7 +803,7 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
   mask(kb);
   at_tile(kb);
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) m_run[nb] = SC ? fmaxf(row_max(nb) + (own_first ? 0.f : kMargin), m_own[nb]) : row_max(nb);
+  for (int nb = 0; nb < NB; ++nb) m_run[nb] = SC ? fmaxf(row_max(nb) + (last_first ? 0.f : margin), m_last[nb]) : row_max(nb);
   softmax();
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) l_run[nb] = lsum[nb];
@@ -889,7 +904,7 @@ __global__ __launch_bounds__(kThreads, prefill_wgs(D)) void prefill_kernel(Prefi
     const int rg = (int)(fresh(ulane) >> 5);
     if (!row.ok) continue;
     // O back from the PV scale of bf16 V values (a power of two: exact)
-    // (a chunk far from the row's own key, which the reference may be: below 2^-64 of the row
+    // (a chunk far from the row's own key, which the reference may be near: below 2^-64 of that
     // it counts as empty, its reciprocal could overflow)
     const bool some = l_tot > (SC ? 0x1p-64f : 0.f);
     const float inv = some ? (QT == OSCAR_F16 ? 1.f : (float)(1 << kVShift)) / l_tot : 0.f;
@@ -952,7 +967,7 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams P) {
   if (M != -INFINITY) {
     for (int c = 0; c < nch; ++c) {
       const float lc = P.part_lse[slot(c) * kRows + n];
-      if (lc != -INFINITY) {
+      if (lc != -INFINITY && !(lc <= M - P.nothing)) {
         const f32x4* po = (const f32x4*)(P.part_o + (slot(c) * (kRows / 32) + rb) * 32 * D) + 4 * b * 64 + lane;
         const float w = exp2f(lc - M);
         L += w;
@@ -1074,6 +1089,8 @@ static int prefill_launch(const oscar_prefill_args_v1* args, const oscarop_score
   PrefillParams p{};
   const int sc = score_of(score, a.scale, &p.sc);
   if (sc < 0) return fail(-22, kBadCap, name);
+  // (a bias leaves most of a steep head's chunks far below: their partials need not be read)
+  p.nothing = p.sc.slopes != nullptr ? 64.f : INFINITY;
   p.a = a;
   p.has_stage = a.staging != nullptr;
   if (a.staging) p.st = *a.staging;

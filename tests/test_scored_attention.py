@@ -273,6 +273,47 @@ def test_many_keys_far_below_the_largest(cuda, cap, steep, split):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("below", [16.703125, 15.25])
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("cap", [0.0, 512.0])
+@pytest.mark.parametrize("n", [1, 3])
+def test_a_long_history_far_below_the_own_key(cuda, n, cap, split, below):
+    """131072 cached keys, each `below` nats under the row's own key (24.1 and 22 binary orders): in
+    fp16 against that key every one would be nothing, or a subnormal of one or two bits.  A key's
+    probability is off by 2^-25 of the reference, which lies a binary order above the largest key
+    of a unit at most, and a unit has 2^12 keys, or a reference that is lower by the excess: 2^-12
+    of the row's sum."""
+    from oscar_amd import ops
+
+    hist, d, hq, bs = 131072, 256, 6, 128
+    kc, vc = (torch.zeros(1, bs, 1, d, dtype=torch.int8, device=cuda) for _ in range(2))
+    own = 16.0
+    kc.view(torch.float16)[..., 1] = own - below  # K: every code is the zero point; V: 1
+    kc.view(torch.float16)[..., 3] = 1.0
+    q, k, v = torch.zeros(n, hq, d), torch.zeros(n, 1, d), torch.zeros(n, 1, d)
+    q[..., 0] = 16.0
+    k[:, 0, 0] = own
+    q, k, v = q.bfloat16(), k.bfloat16(), v.bfloat16()
+    slopes, lse = slopes_of(hq, 1e-6), torch.empty(n, hq, device=cuda)
+    out = ops.attention_prefill(q.to(cuda), k.to(cuda), v.to(cuda), 0.0625, head_dim=d, history=hist, k_cache=kc, v_cache=vc,
+                                block_table_row=torch.zeros(hist // bs, dtype=torch.int32, device=cuda), lse=lse, split=split,
+                                soft_cap=cap, alibi_slopes=slopes.to(cuda))
+    assert torch.tensor(own - below).half().bfloat16() == own - below
+    s_own, s_far = own, own - below
+    if cap:
+        s_own, s_far = (cap * math.tanh(x / cap) for x in (s_own, s_far))
+    pos = torch.arange(hist, dtype=torch.float64)
+    for i in range(n):
+        for h in range(hq):
+            far = torch.exp(s_far - s_own + slopes[h].double() * (pos - (hist + i))).sum()
+            near = torch.exp(slopes[h].double() * -torch.arange(i + 1, dtype=torch.float64)).sum()
+            want = (far / (far + near)).item()
+            assert 0.001 < want < 0.1
+            assert (out[i, h].double().cpu() - want).abs().max() <= REL_TOL * want + ABS_TOL + 2.0 ** -12, (i, h, want, out[i, h, 0])
+            assert abs(lse[i, h].item() - s_own - math.log((far + near).item())) <= LSE_TOL
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("cap", [0.0, 20.0])
 def test_overflowing_products_and_later_tokens(cuda, cap):
     """A score that overflows is capped like any other; what a later token holds does not
