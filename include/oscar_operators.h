@@ -36,7 +36,8 @@ int oscarop_decode_step_v1(oscar_context_v1* ctx, oscar_step_args_v1* args, cons
 
 /* ---- RMS norm of every query and key head with the position rotation ----------------
  * For each row x of head_dim values (a token's head):
- *   y = x / sqrt(mean(x^2) + eps) * (w + weight_offset)          (w = 1 where NULL)
+ *   y = x / sqrt(mean(x^2) + eps) * (w + weight_offset)     (a NULL weight: no gain, and no
+ *                                                            offset either)
  * then, over its first rotary_dim values, pairs (a, b) turn by the token's angles:
  *   (a, b) -> (a cos - b sin, b cos + a sin),
  * a pair being (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when interleaved.  fp32
@@ -51,10 +52,10 @@ typedef struct oscarop_norm_rope_args_v1 {
   int64_t num_tokens;
   int64_t head_dim;             /* 128 or 256 */
   int32_t dtype;                /* enum oscar_dtype of q, k and the outputs */
-  const void* q_weight;         /* [head_dim], or NULL */
+  const void* q_weight;         /* [head_dim], or NULL: no gain */
   const void* k_weight;
   int32_t weight_dtype;
-  float weight_offset;          /* 1 for weights stored around zero */
+  float weight_offset;          /* added to the weights: 1 for those stored around zero */
   float eps;
   const void* positions;        /* [num_tokens] device */
   int32_t positions_int64;      /* 0: int32 */

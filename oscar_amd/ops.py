@@ -432,7 +432,7 @@ def norm_rope(q, k, positions, cos_sin, *, q_weight=None, k_weight=None, eps=1e-
     [P, R]: row p holds the R / 2 cosines of position p, then its sines (R a multiple of
     16, at most D; values past R are only normed).  Per row of D values
     y = x / sqrt(mean(x^2) + eps) * (weight + weight_offset), weights [D] or None (no
-    gain); pairs (i, i + R / 2), or (2 i, 2 i + 1) if interleaved, turn by the angles.
+    gain, whatever the offset); pairs (i, i + R / 2), or (2 i, 2 i + 1) if interleaved, turn by the angles.
     fp32 throughout, rounded once.  A position outside the table gives NaN rows.
 
     Returns (q_out, k_out): new tensors, or the ones given; q_out=q and k_out=k work in

@@ -181,6 +181,23 @@ def test_edges(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 9001])
+@pytest.mark.parametrize("gain", ["neither", "q", "k"])
+def test_a_missing_gain_takes_no_offset(cuda, n, gain):
+    """Norms without a gain beside ones whose weights are stored around zero (offset 1)."""
+    from oscar_amd import ops
+
+    gen = torch.Generator(device=cuda).manual_seed(n)
+    q, k = (torch.randn(n, h, 128, generator=gen, device=cuda) for h in (5, 3))
+    w = torch.randn(128, generator=gen, device=cuda)
+    qw, kw = (w if gain == side else None for side in "qk")
+    cs, positions = table(50, 64, device=cuda), torch.randint(0, 50, (n,), generator=gen, device=cuda)
+    got = ops.norm_rope(q, k, positions, cs, q_weight=qw, k_weight=kw, eps=1e-5, weight_offset=1.0)
+    for x, y, weight in zip(got, (q, k), (qw, kw)):
+        check(x, *reference(y, weight, positions, cs, 1e-5, 1.0, False))
+
+
+@pytest.mark.gpu
 def test_wrapper_refusals_on_the_device(cuda):
     from oscar_amd import ops
 
