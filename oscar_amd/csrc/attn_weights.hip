@@ -609,8 +609,8 @@ extern "C" int oscarop_attn_weights_v1(const oscarop_weights_args_v1* args, cons
     return fail(-22, "%s: Missing request block-table rows", name);
   if (a.cache.block_size < kTile || a.cache.block_size % kTile || a.cache.block_size > (1 << 20))
     return fail(-22, "%s: block_size %lld must be a multiple of %d (<= 2^20)", name, (long long)a.cache.block_size, kTile);
-  if (a.weights_cols < 1 || a.weights_stride_head < a.weights_cols ||
-      (a.num_reqs > 1 && a.weights_stride_request < a.weights_stride_head * a.cache.num_kv_heads))
+  const Rows2 lists{{a.num_reqs, a.cache.num_kv_heads}, {a.weights_stride_request, a.weights_stride_head}, a.weights_cols};
+  if (a.weights_cols < 1 || a.weights_stride_head < a.weights_cols || lists.overlap())
     return fail(-22, "%s: weights of two heads or requests overlap", name);
   if ((a.cache.k_stride[0] & 15) || (a.cache.k_stride[1] & 15) || (a.cache.k_stride[2] & 15) || (((uintptr_t)a.cache.k) & 15))
     return fail(-22, "%s: cache slots must be 16-byte aligned", name);

@@ -29,6 +29,39 @@ int fail(int code, const char* fmt, ...);
                                                hipGetErrorString(e_));            \
   } while (0)
 
+// ---------------------------------------------------------------- strided rows on the host
+// [outer][inner] rows of `cols` elements, either axis the outer one
+struct Rows2 {
+  int64_t n[2], stride[2], cols;
+  // whether two rows share an element
+  bool overlap() const {
+    auto within = [&](int in) {
+      const int out = 1 - in;
+      return (n[in] <= 1 || stride[in] >= cols) &&
+             (n[out] <= 1 || (__int128)stride[out] >= (__int128)(n[in] - 1) * (n[in] > 1 ? stride[in] : 0) + cols);
+    };
+    return !within(0) && !within(1);
+  }
+  __int128 extent() const {
+    return (__int128)(n[0] - 1) * (n[0] > 1 ? stride[0] : 0) + (__int128)(n[1] - 1) * (n[1] > 1 ? stride[1] : 0) + cols;
+  }
+  // whether rows at `by` elements from these share an element with them, `other` being the
+  // others' layout (of other strides: whether the extents do)
+  bool meets(const Rows2& other, int64_t by) const {
+    if (by >= extent() || -(__int128)by >= other.extent()) return false;
+    for (int a = 0; a < 2; ++a)
+      if (n[a] != other.n[a] || (n[a] > 1 && stride[a] != other.stride[a])) return true;
+    for (int64_t i = 1 - n[1]; i < n[1]; ++i) {
+      const __int128 x = by - (__int128)i * (n[1] > 1 ? stride[1] : 0);
+      const int64_t s = n[0] > 1 ? stride[0] : 0;
+      const __int128 j = s > 0 ? x / s : 0;  // x - k s is smallest at one of these
+      for (__int128 k = j - 1; k <= j + 1; ++k)
+        if (k > -n[0] && k < n[0] && x - k * s < cols && k * s - x < cols) return true;
+    }
+    return false;
+  }
+};
+
 // ---------------------------------------------------------------- conversions
 __device__ __forceinline__ float bf16_bits_to_f32(unsigned short b) {
   return __uint_as_float(((unsigned)b) << 16);

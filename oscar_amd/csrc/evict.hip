@@ -441,16 +441,10 @@ extern "C" int oscarop_evict_v1(const oscarop_evict_args_v1* args, void* stream)
   if ((a.cache.k_stride[0] & 15) || (a.cache.k_stride[1] & 15) || (a.cache.k_stride[2] & 15) || (((uintptr_t)a.cache.k) & 15) ||
       (a.cache.v_stride[0] & 15) || (a.cache.v_stride[1] & 15) || (a.cache.v_stride[2] & 15) || (((uintptr_t)a.cache.v) & 15))
     return fail(-22, "%s: cache slots must be 16-byte aligned", name);
-  auto overlap = [&](int64_t head, int64_t request) {
-    return (hk > 1 && head < a.weights_cols) || (a.num_reqs > 1 && request < (hk - 1) * head + a.weights_cols);
-  };
-  if (overlap(a.weights_stride_head, a.weights_stride_request) || overlap(a.out_stride_head, a.out_stride_request))
-    return fail(-22, "%s: weights of two heads or requests overlap", name);
-  auto end_of = [&](const float* p, int64_t head, int64_t request) {
-    return p + (a.num_reqs - 1) * request + (hk - 1) * head + a.weights_cols;
-  };
-  if (a.weights_out < end_of(a.weights, a.weights_stride_head, a.weights_stride_request) &&
-      a.weights < end_of(a.weights_out, a.out_stride_head, a.out_stride_request))
+  const Rows2 in{{a.num_reqs, hk}, {a.weights_stride_request, a.weights_stride_head}, a.weights_cols};
+  const Rows2 out{{a.num_reqs, hk}, {a.out_stride_request, a.out_stride_head}, a.weights_cols};
+  if (in.overlap() || out.overlap()) return fail(-22, "%s: weights of two heads or requests overlap", name);
+  if (in.meets(out, ((intptr_t)a.weights_out - (intptr_t)a.weights) / (intptr_t)sizeof(float)))
     return fail(-22, "%s: weights_out overlaps weights", name);
   if (a.staging && (a.staging->rows < 1 || !a.staging->owner)) return fail(-22, "%s: staging arena rows out of range", name);
   const int64_t need = oscarop_evict_workspace_bytes_v1(a.num_reqs, hk, a.max_drop);

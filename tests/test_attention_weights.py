@@ -475,3 +475,21 @@ def test_lengths_far_past_the_sizes_of_a_small_call(cuda):
     small = ops.plan_weights(c["qsl"], [40, 35], has_new=True, device=cuda)
     small.seqs.copy_(own.seqs)
     assert torch.equal(call(small), want)
+
+
+@pytest.mark.gpu
+def test_weights_with_the_heads_outermost(cuda):
+    """A model may keep [KV heads, requests, columns]: its view by request is taken as it lies."""
+    from oscar_amd import ops
+
+    for prefixes, lengths in (([700, 129, 40], [4, 2, 1]), ([0, 300, 40], [700, 90, 1])):
+        c = cases.make_case(prefixes, lengths, d=128, hk=2, group=4)
+        q, k = (torch.from_numpy(c[x]).bfloat16().to(cuda) for x in "qk")
+        kc, vc = (torch.from_numpy(c[x]).view(torch.int8).to(cuda) for x in ("k8", "v8"))
+        bt, lse = torch.from_numpy(c["bt"]).to(cuda), torch.full((sum(lengths), 8), 3.0, device=cuda)
+        plan = ops.plan_weights(c["qsl"], c["seqs"], has_new=True, device=cuda)
+        call = (lambda w: ops.accumulate_weights(q, k, kc, vc, bt, plan, 0.0625, lse, w, head_dim=128))
+        want = call(torch.zeros(3, 2, 720, device=cuda))
+        got = torch.zeros(2, 3, 720, device=cuda)
+        call(got.transpose(0, 1))
+        assert torch.equal(got, want.transpose(0, 1))

@@ -65,6 +65,41 @@ def test_workspace_and_empty_calls():
     assert lib.oscarop_evict_v1(C.byref(args(staging=C.pointer(stage))), None) == -22
 
 
+@pytest.mark.parametrize("seed", range(20))
+def test_overlaps_are_told_from_strides(seed):
+    """Small layouts against an enumeration of their elements: rows that share one are refused,
+    rows of either axis within the other are not, and two lists of the same such layout overlap
+    where they share one and nowhere else (the call then stops at the missing workspace)."""
+    g, lib, said = np.random.default_rng(seed), _lib.load(), {"heads or requests overlap": 0, "weights_out overlaps": 0, "workspace": 0}
+    for _ in range(200):
+        cols, reqs, hk = (int(g.integers(1, n)) for n in (6, 4, 4))
+        request, head = (int(x) for x in g.integers(0, 24, 2))
+        if g.random() < 0.8:  # one axis within the other
+            inner = cols + int(g.integers(0, 9))
+            count, outermost = (hk, "request") if g.random() < 0.5 else (reqs, "head")
+            outer = (count - 1) * inner + cols + int(g.integers(0, 9))
+            request, head = (outer, inner) if outermost == "request" else (inner, outer)
+            nested = True
+        else:
+            nested = False
+        by = int(g.integers(-60, 60))
+        elements = [r * request + h * head + c for r in range(reqs) for h in range(hk) for c in range(cols)]
+        x = args(weights=1 << 12, weights_out=(1 << 12) + 4 * by, weights_stride_request=request, weights_stride_head=head,
+                 out_stride_request=request, out_stride_head=head, weights_cols=cols, num_reqs=reqs, cache_num_kv_heads=hk,
+                 block_table_rows=reqs, workspace=None)
+        assert lib.oscarop_evict_v1(C.byref(x), None) == -22
+        got = [m for m in said if m in lib.oscar_last_error().decode()]
+        if len(set(elements)) < len(elements):
+            want = "heads or requests overlap"
+        elif {e + by for e in elements} & set(elements):
+            want = "weights_out overlaps"
+        else:
+            want = "workspace"
+        assert got == [want] or not nested and got == ["heads or requests overlap"], (cols, reqs, hk, request, head, by, got, want)
+        said[got[0]] += 1
+    assert min(said.values()) > 0, said
+
+
 @pytest.mark.parametrize("sizes", [(1, 1, 1 << 61), (1, 1, 1 << 62), (1, 1, 1 << 30), (0xffff, 0xffff, 1 << 29), (1 << 40, 1, 128),
                                    (1, 1 << 40, 128)])
 def test_sizes_that_overflow_are_refused(sizes):
@@ -238,6 +273,30 @@ def test_strided_weights_no_window_and_new_output(cuda):
     got = ops.evict(plan, big[1:4, :, 32:-32], dev["k"].view(torch.int8), dev["v"].view(torch.int8), dev["table"].long(), head_dim=128)
     assert np.array_equal(got[:2].cpu().numpy(), w[:2]) and np.array_equal(dev["k"].cpu().numpy(), k)
     assert np.array_equal(dev["v"].cpu().numpy(), v)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["heads outermost", "columns beside each other", "requests beside each other"])
+def test_weights_of_other_layouts(cuda, layout):
+    """[KV heads, requests, columns], and lists whose old and new weights share a buffer."""
+    from oscar_amd import ops
+
+    lengths, pages = [700, 1300], [2, 5]
+    x = make(lengths, 2, 128, 128, 3, "plain")
+    k, v, w, _ = reference(x, lengths, pages, 64, 70, 128)
+    reqs, hk, cols = x["w"].shape
+    if layout == "heads outermost":
+        old, new = torch.zeros(2, hk, reqs, cols, device=cuda).transpose(1, 2)
+    elif layout == "columns beside each other":
+        old, new = torch.zeros(reqs, hk, 2 * cols, device=cuda).split(cols, -1)
+    else:
+        old, new = torch.zeros(reqs, 2, hk, cols, device=cuda).unbind(1)
+    old.copy_(torch.from_numpy(x["w"]))
+    kc, vc = (torch.from_numpy(x[n].copy()).to(cuda) for n in "kv")
+    plan = ops.plan_evict(lengths, pages, block_size=128, sink_tokens=64, recent_tokens=70, device=cuda)
+    got = ops.evict(plan, old, kc.view(torch.int8), vc.view(torch.int8), torch.from_numpy(x["table"]).to(cuda), head_dim=128, weights_out=new)
+    assert got is new and np.array_equal(got[:2].cpu().numpy(), w[:2]) and np.array_equal(old.cpu().numpy(), x["w"])
+    assert np.array_equal(kc.cpu().numpy(), k) and np.array_equal(vc.cpu().numpy(), v)
 
 
 @pytest.mark.gpu
