@@ -609,6 +609,16 @@ def _check_table(table: torch.Tensor, plan: DecodePlan, block_size: int) -> None
         raise ValueError("Block table cannot cover the history")
 
 
+def _rows_apart(table: torch.Tensor) -> torch.Tensor:
+    """A block table as the entry points take it: int32, columns next to each other, rows not
+    on top of each other (one row broadcast to all requests, a single row out of a column)."""
+    if table.dtype != torch.int32:
+        table = table.to(torch.int32)
+    if table.ndim == 2 and (table.stride(1) != 1 or table.stride(0) < table.shape[1]):
+        table = table.clone(memory_format=torch.contiguous_format)
+    return table
+
+
 def attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, plan: DecodePlan, scale,
                      stage=None, *, head_dim, out_rot=None, lse=None, phases=0, static_scratch=False,
                      store=None, soft_cap=0.0, alibi_slopes=None):
@@ -654,10 +664,9 @@ def attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, plan: Decod
             raise ValueError("Current K/V must match the query dtype")
         k_new, v_new = k_new.contiguous(), v_new.contiguous()
     table = block_table
-    if table.dtype != torch.int32 or table.get_device() != q.get_device():
+    if table.get_device() != q.get_device():
         table = table.to(device=dev, dtype=torch.int32)
-    if table.stride(-1) != 1:
-        table = table.contiguous()
+    table = _rows_apart(table)
     if plan.has_new != (k_new is not None):
         raise ValueError("plan and call disagree on the presence of current K/V")
     if plan.items is None:
@@ -815,9 +824,7 @@ def accumulate_weights(q, k_new, k_cache, v_cache, block_table, plan, scale, lse
     head_stride, request_stride = _weight_strides("weights", weights, reqs, hk, longest)
     if reqs == 0 or n == 0 or longest == 0:
         return weights
-    table = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
-    if table.stride(-1) != 1:
-        table = table.contiguous()
+    table = _rows_apart(block_table)
     _check_table(table, plan, bs)
     if q.stride(2) != 1 or q.stride(1) != head_dim:
         q = q.contiguous()
@@ -935,13 +942,11 @@ def evict(plan: EvictPlan, weights, k_cache, v_cache, block_table, *, head_dim, 
         weights_out[reqs:].copy_(weights[reqs:])
     if reqs == 0 or weights.shape[2] == 0:
         return weights_out
-    table = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
+    table = _rows_apart(block_table)
     if table.ndim != 2 or table.shape[0] < reqs:
         raise ValueError("Missing request block-table rows")
     if -(-longest // bs) > table.shape[1]:
         raise ValueError("Block table cannot cover the history")
-    if table.stride(1) != 1:
-        table = table.contiguous()
     st = staging_struct(stage, k_cache, head_dim)
     need = _lib.load().oscarop_evict_workspace_bytes_v1(reqs, hk, plan.max_drop)
     ws = torch.empty(max(need, 0), dtype=torch.uint8, device=weights.device)  # a captured call keeps its own

@@ -159,6 +159,18 @@ def test_the_sizes_of_a_plan_follow_its_lists():
     ops._check_table(table, plan, 32)
 
 
+def test_block_tables_are_laid_out_by_rows():
+    from oscar_amd import ops
+
+    t = torch.arange(24, dtype=torch.int32).view(4, 6)
+    for same in (t, t[1:3], t[:, 1:4]):
+        assert ops._rows_apart(same).data_ptr() == same.data_ptr()
+    for other in (t.t(), t[:, ::2], t[:1].expand(3, 6), t[:, :1].t(), t[:, 2:3].expand(4, 5), t.long(), t[:, :1].long().t(),
+                  t[:, 0::7], torch.arange(5, dtype=torch.int32)[:, None].t()):
+        got = ops._rows_apart(other)
+        assert torch.equal(got, other.int()) and got.stride(1) == 1 and got.stride(0) >= got.shape[1]
+
+
 # ------------------------------------------------------------------ values
 BATCHES = [
     ("mtp_window", [129, 1025, 3, 300], [4, 3, 1, 2], {}),
@@ -493,3 +505,31 @@ def test_weights_with_the_heads_outermost(cuda):
         got = torch.zeros(2, 3, 720, device=cuda)
         call(got.transpose(0, 1))
         assert torch.equal(got, want.transpose(0, 1))
+
+
+@pytest.mark.gpu
+def test_one_table_row_for_all_requests_and_a_row_out_of_a_column(cuda):
+    """Requests that share a prefix's pages read them through one broadcast row."""
+    from oscar_amd import ops
+
+    c = cases.make_case([500], [6], window=False)
+    q, k, v = (torch.from_numpy(c[x]).bfloat16().to(cuda) for x in "qkv")
+    kc, vc = (torch.from_numpy(c[x]).view(torch.int8).to(cuda) for x in ("k8", "v8"))
+    bt, lse = torch.from_numpy(c["bt"]).to(cuda), torch.full((6, 6), 5.0, device=cuda)
+
+    def call(table, qsl, seqs):
+        plan = ops.plan_decode(qsl, seqs, has_new=True, num_kv_heads=1, group=6, head_dim=256, device=cuda)
+        out, _ = ops.attention_decode(q, k, v, kc, vc, table, plan, 0.0625, head_dim=256, soft_cap=20.0)
+        return out, ops.accumulate_weights(q, k, kc, vc, table, plan, 0.0625, lse, torch.zeros(len(seqs), 1, 512, device=cuda), head_dim=256)
+
+    for table, full, qsl, seqs in ((bt.expand(2, -1), bt.repeat(2, 1), [0, 2, 6], [502, 504]),
+                                   (bt[0][:, None].t(), bt, [0, 6], [506])):
+        assert table.stride(0) < table.shape[1]
+        for a, b in zip(call(table, qsl, seqs), call(full, qsl, seqs)):
+            assert torch.equal(a, b)
+    column = bt[0][:, None].contiguous().t()
+    plan = ops.plan_evict([500], [1], block_size=128, device=cuda)
+    w = torch.rand(1, 1, 512, device=cuda)
+    caches = [(kc.clone(), vc.clone()) for _ in range(2)]
+    a, b = (ops.evict(plan, w, *pair, table, head_dim=256) for pair, table in zip(caches, (column, bt)))
+    assert torch.equal(a, b) and torch.equal(caches[0][0], caches[1][0]) and torch.equal(caches[0][1], caches[1][1])
