@@ -219,14 +219,20 @@ class OscarAttentionBackendImpl(BaseAttentionImpl):  # type: ignore[misc,valid-t
     def _score_args(self, device) -> dict:
         """The cap and the distance bias that the model gives this layer (the impl's own
         logits_soft_cap and alibi_slopes; empty for the plain product).  The slopes move to
-        the device as fp32 once."""
-        cap = getattr(self, "logits_soft_cap", None) or 0.0
+        the device as fp32 once.
+
+        Models write 0, a negative number or infinity for no cap.  One below the least that
+        the kernels take leaves every score within that of zero, as the least itself does;
+        one above the largest stays unapplied: a score s differs from the capped one by less
+        than |s|^3 / (3 cap^2), 2^-10 for |s| up to 14."""
+        cap = float(getattr(self, "logits_soft_cap", None) or 0.0)
         slopes = getattr(self, "alibi_slopes", None)
+        cap = max(cap, ops.LEAST_CAP) if 0.0 < cap <= ops.MOST_CAP else 0.0
         if not cap and slopes is None:
             return {}
         if slopes is not None:
             slopes = self.alibi_slopes = torch.as_tensor(slopes, dtype=torch.float32, device=device).contiguous()
-        return dict(soft_cap=float(cap), alibi_slopes=slopes)
+        return dict(soft_cap=cap, alibi_slopes=slopes)
 
     # ------------------------------------------------------------------ geometry
     def _set_caches(self, kv_cache) -> None:

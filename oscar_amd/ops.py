@@ -257,6 +257,9 @@ class DeviceContext:
         return ctx
 
 
+LEAST_CAP, MOST_CAP = 2.0 ** -20, 1024.0  # the caps that the library takes
+
+
 def score_struct(soft_cap, alibi_slopes, num_q_heads: int, device) -> _lib.Score | None:
     """The score function of an attention call as a C struct; None for the plain product."""
     if alibi_slopes is not None:
@@ -265,7 +268,7 @@ def score_struct(soft_cap, alibi_slopes, num_q_heads: int, device) -> _lib.Score
             raise ValueError(f"alibi_slopes must be a contiguous fp32 [{num_q_heads}] tensor")
         if alibi_slopes.device != device:
             raise ValueError(f"alibi_slopes are on {alibi_slopes.device}, the queries on {device}")
-    if soft_cap != 0 and not 2.0 ** -20 <= soft_cap <= 1024:
+    if soft_cap != 0 and not LEAST_CAP <= soft_cap <= MOST_CAP:
         raise ValueError(f"soft_cap must lie in [2^-20, 1024], 0 for none, got {soft_cap}")
     if soft_cap == 0 and alibi_slopes is None:
         return None

@@ -118,6 +118,28 @@ def test_score_struct_refusals():
             ops.score_struct(cap, None, 6, cpu)
 
 
+@pytest.mark.parametrize("cap,want", [(None, 0), (0, 0), (0.0, 0), (-1.0, 0), (math.inf, 0), (30, 30), (2.0 ** -20, 2.0 ** -20), (1e-9, 2.0 ** -20),
+                                      (1024.0, 1024), (1025, 0), (1e30, 0), (np.float32(50), 50)])
+def test_a_layer_runs_with_any_cap(cap, want):
+    """What models write for no cap, and caps beside the kernels' range, ran before the kernels
+    took caps at all."""
+    from oscar_amd import ops
+
+    cpu = torch.device("cpu")
+    for slopes in (None, slopes_of(6).tolist()):
+        score = impl_of(cap, slopes)._score_args(cpu)
+        if slopes is None and not want:
+            assert score == {}
+            continue
+        assert score["soft_cap"] == want and (score["alibi_slopes"] is None) == (slopes is None)
+        struct = ops.score_struct(score["soft_cap"], score["alibi_slopes"], 6, cpu)
+        assert struct.soft_cap == want
+    # what is left out of a score that is not capped, and what the least cap adds to a smaller one
+    if cap and cap > 1024 and cap < 1e20:
+        s = torch.linspace(-14, 14, 999, dtype=torch.float64)
+        assert (s - cap * torch.tanh(s / cap)).abs().max() < 2.0 ** -10
+
+
 # ------------------------------------------------------------------ decode
 DECODE = [
     ("mtp_window", [129, 1025, 3, 300], [4, 3, 1, 2], {}),
