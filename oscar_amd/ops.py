@@ -85,8 +85,9 @@ def cache_struct(k_cache: torch.Tensor, v_cache: torch.Tensor, head_dim: int) ->
     if k_cache.ndim != 4 or v_cache.ndim != 4 or not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise ValueError("OSCAR requires contiguous [blocks, tokens, heads, bytes] caches")
     blocks, tokens, heads, width = k_cache.shape
-    k2, v2 = width * k_cache.element_size(), v_cache.shape[3] * v_cache.element_size()
-    if v_cache.shape[:3] != k_cache.shape[:3]:
+    v_blocks, v_tokens, v_heads, v_width = v_cache.shape
+    k2, v2 = width * k_cache.element_size(), v_width * v_cache.element_size()
+    if v_blocks != blocks or v_tokens != tokens or v_heads != heads:
         raise ValueError(f"OSCAR requires K and V caches of the same blocks, tokens and heads, got "
                          f"{list(k_cache.shape[:3])} and {list(v_cache.shape[:3])}")
     if k2 < 32 + head_dim // 4 or v2 < head_dim // 4:
@@ -220,17 +221,20 @@ class DeviceScratch:
 _is_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
 
 
-def _call_workspace(device: torch.device, kind: str, nbytes: int) -> torch.Tensor:
-    """The workspace of one attention call (kind: the DeviceScratch method): the stream's
-    shared one, or, while the stream captures a graph, one of the call's own out of the
-    graph's memory pool.  The graph keeps the address: the shared buffer may be replaced by a
-    larger one, and be in use by its stream while the graph is replayed on another."""
-    if device.index != _get_device():
-        with torch.cuda.device(device):
-            return _call_workspace(device, kind, nbytes)
+def _call_workspace(index: int, kind: str, nbytes: int) -> torch.Tensor:
+    """The workspace of one attention call on device `index` (kind: the DeviceScratch method):
+    the stream's shared one, or, while the stream captures a graph, one of the call's own out of
+    the graph's memory pool.  The graph keeps the address: the shared buffer may be replaced by
+    a larger one, and be in use by its stream while the graph is replayed on another."""
+    if index != _get_device():
+        with torch.cuda.device(index):
+            return _call_workspace(index, kind, nbytes)
     if _is_capturing():
-        return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
-    return getattr(DeviceScratch.get(device), kind)(nbytes)
+        return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=torch.device("cuda", index))
+    scratch = DeviceScratch._by_device.get((index, _raw_stream(index)))
+    if scratch is None:
+        scratch = DeviceScratch.get(torch.device("cuda", index))
+    return getattr(scratch, kind)(nbytes)
 
 
 class DeviceContext:
@@ -617,8 +621,10 @@ def _rows_apart(table: torch.Tensor) -> torch.Tensor:
     on top of each other (one row broadcast to all requests, a single row out of a column)."""
     if table.dtype != torch.int32:
         table = table.to(torch.int32)
-    if table.ndim == 2 and (table.stride(1) != 1 or table.stride(0) < table.shape[1]):
-        table = table.clone(memory_format=torch.contiguous_format)
+    if table.ndim == 2:
+        row, column = table.stride()
+        if column != 1 or row < table.shape[1]:
+            table = table.clone(memory_format=torch.contiguous_format)
     return table
 
 
@@ -676,7 +682,7 @@ def attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, plan: Decod
         raise ValueError("the decode plan has not been uploaded")
     _check_table(table, plan, k_cache.shape[1])
     st = staging_struct(stage, k_cache, head_dim)
-    ws = None if static_scratch else _call_workspace(dev, "attn_workspace", plan.partial_bytes)
+    ws = None if static_scratch else _call_workspace(q.get_device(), "attn_workspace", plan.partial_bytes)
     has_new = k_new is not None
     a = _lib.AttnArgs(q.data_ptr(), n, hq, q.stride(0), _ptr(k_new), _ptr(v_new), k_new.stride(0) if has_new else 0,
                       cache_struct(k_cache, v_cache, head_dim), table.data_ptr(), table.stride(0), plan.qsl.data_ptr(),
@@ -751,7 +757,7 @@ def attention_prefill(q, k, v, scale, *, head_dim, history=0, k_cache=None, v_ca
     if need > 0:
         # the size asked for, not the shared buffer's (which an earlier call may have
         # grown past v1's size: the call would then split)
-        ws = _call_workspace(q.device, "prefill_workspace", need)
+        ws = _call_workspace(q.get_device(), "prefill_workspace", need)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
     if score is not None:
         _launch("oscarop_attn_prefill_v1", q.get_device(), C.byref(a), C.byref(score))
