@@ -5,7 +5,8 @@
  * launches are asynchronous on `stream`; nothing is allocated; 0 or a negative errno-style
  * status is returned, with the message in oscar_last_error().
  *
- * All entry points but oscarop_decode_step_v1 may be captured into a HIP graph.
+ * All entry points but oscarop_decode_step_v1 may be captured into a HIP graph, with a
+ * workspace that nothing else uses while the graph may be replayed.
  */
 #ifndef OSCAR_OPERATORS_H
 #define OSCAR_OPERATORS_H
@@ -29,7 +30,12 @@ typedef struct oscarop_score_v1 {
 
 /* oscar_attn_decode_v1, oscar_attn_prefill_v1 and oscar_decode_step_v1 with these scores
  * (score == NULL, or no cap and no slopes: the plain calls).  out, lse and every rule of
- * the plain calls are the same otherwise. */
+ * the plain calls are the same otherwise, their roundings included: history values are
+ * q_dtype(fp16(x)), but V is unrounded in the decode's tiles without window copies or current
+ * keys; there the probabilities times V's scale are rounded to fp16, in its other tiles the
+ * probabilities to two parts in the queries' type, in the prefill to fp16; sums and the softmax
+ * are fp32.  A capped score keeps soft_cap 2^-22.  The decode's waves take an item's tiles as they get to them, so
+ * that its last bits may differ from run to run where an item has several tiles. */
 int oscarop_attn_decode_v1(const oscar_attn_args_v1* args, const oscarop_score_v1* score, void* stream);
 int oscarop_attn_prefill_v1(const oscar_prefill_args_v1* args, const oscarop_score_v1* score, void* stream);
 int oscarop_decode_step_v1(oscar_context_v1* ctx, oscar_step_args_v1* args, const oscarop_score_v1* score, void* stream);
@@ -85,7 +91,9 @@ int oscarop_norm_rope_v1(const oscarop_norm_rope_args_v1* args, void* stream);
  * queries are rows [query_start_loc[r], query_start_loc[r + 1]) of q, its length
  * seq_lens[r] includes the current chunk when k_new is given, and query i of n_q sees keys
  * [0, seq - n_q + i + 1).  With history 0 and k_new the rows may be unrotated ones.  No
- * rounding below fp32; the order of the sums is fixed.  A request that does not fit
+ * rounding below fp32.  The order of the sums follows from the call's sizes alone (num_reqs,
+ * heads, max_seq_len, max_query_len, weights_cols): the same call gives the same bits, a
+ * request in a call of other sizes may differ by fp32 roundings.  A request that does not fit
  * (queries past num_tokens, a length past weights_cols, a history past the block table)
  * reads nothing and its weights become NaN. */
 typedef struct oscarop_weights_args_v1 {
@@ -104,8 +112,8 @@ typedef struct oscarop_weights_args_v1 {
   const int32_t* seq_lens;        /* device [num_reqs] */
   int32_t num_reqs;
   int32_t q_dtype;              /* OSCAR_BF16 or OSCAR_F16 */
-  /* the longest length and the most queries of a request: they size the launch, and any
-   * batch gives the same results */
+  /* the longest length and the most queries of a request: they size the launch; requests past
+   * them are served as well */
   int64_t max_seq_len;          /* at most 2^30, as weights_cols */
   int64_t max_query_len;        /* at most 2^24 */
   const oscar_staging_v1* staging; /* NULL = no window; its v side is not read */

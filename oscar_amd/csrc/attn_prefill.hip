@@ -41,6 +41,9 @@ constexpr int kLazy = 10;     // log2 of the largest row sum of a tile's probabi
 // 8000, capped, by the drift in us: 10 184, 14 172, 16 169.
 constexpr float kMargin = 1.f;
 constexpr int kLazyScored = 15;
+// A unit's reference is at least this far below the score of the row's own key (see prefill_kernel).
+// 8000 + 400 tokens of 6 heads with a bias, us: 91.2 at 12, 91.4 at 20, 92.9 at 32, 94.4 without
+// the own key's score, 87.5 with that alone as every unit's reference.
 constexpr float kFar = 12.f;
 // workgroups per CU the register budget of prefill_kernel<D> is set for
 constexpr int prefill_wgs(int D) { return D == 256 ? 1 : 2; }
@@ -134,7 +137,6 @@ struct PrefillParams {
                        // chunks, as the MFMA results lie (32 rows x 32 columns per 4 x 64 x 4)
   float* part_lse;     // [slot][Hk][kRows] log2-domain LSE of each partial
   Score sc;            // SC != 0
-  float nothing;       // the merge leaves out a chunk whose log2 LSE lies this far below a row's largest
 };
 
 // key tiles seen by the last query of a tile ending at chunk token q1
@@ -967,7 +969,7 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams P) {
   if (M != -INFINITY) {
     for (int c = 0; c < nch; ++c) {
       const float lc = P.part_lse[slot(c) * kRows + n];
-      if (lc != -INFINITY && !(lc <= M - P.nothing)) {
+      if (lc != -INFINITY) {
         const f32x4* po = (const f32x4*)(P.part_o + (slot(c) * (kRows / 32) + rb) * 32 * D) + 4 * b * 64 + lane;
         const float w = exp2f(lc - M);
         L += w;
@@ -995,9 +997,9 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillParams P) {
 // on 2, 1500 (288) 53 / 53, 1800 (398) 68 / 57; 8000 + 1600 (500) 144 / 121; 15360 + 9256
 // 1.60 / 1.23 ms.  At head dim 128 two unpaired workgroups fit a CU and overlap each other
 // (8000 + 4000 tokens, 16 heads on 2: 374 us against 380 us paired), so there are no pairs
-// there.  Nor for scored calls, whose registers do not all fit then: a bias alone 8000 + 400
-// 89 / 94, 6000 228 / 247, 15360 + 9256 1336 / 1136; capped 8000 + 1600 166 / 177, 15360 + 9256
-// 1491 / 1652.
+// there.  Nor for scored calls, whose registers do not all fit then (measured with the row's own
+// key as every unit's reference): a bias alone 8000 + 400 89 / 94, 6000 228 / 247, 15360 + 9256
+// 1336 / 1136; capped 8000 + 1600 166 / 177, 15360 + 9256 1491 / 1652.
 constexpr int64_t kPairUnits = kSplitCUs + kSplitCUs / 8;
 template <int D, int QT>
 void launch_prefill(const PrefillParams& p, int sc, dim3 grid, bool pairs, hipStream_t s) {
@@ -1089,8 +1091,6 @@ static int prefill_launch(const oscar_prefill_args_v1* args, const oscarop_score
   PrefillParams p{};
   const int sc = score_of(score, a.scale, &p.sc);
   if (sc < 0) return fail(-22, kBadCap, name);
-  // (a bias leaves most of a steep head's chunks far below: their partials need not be read)
-  p.nothing = p.sc.slopes != nullptr ? 64.f : INFINITY;
   p.a = a;
   p.has_stage = a.staging != nullptr;
   if (a.staging) p.st = *a.staging;

@@ -7,7 +7,8 @@
 // S = Q K^T of 32 rows and 32 keys leaves a key's scores in one lane pair (lane % 32: the key;
 // registers: the rows), so that the sum over the rows is a sum over registers and crosses
 // lanes once.  Every number has one owner, so nothing is atomic and results do not depend on
-// the order of workgroups.
+// the order of workgroups; which kernel runs and where rows are cut depends on the call's sizes,
+// and the last bits with them.
 //
 //   weights_few_kernel   a batch of at most 32 rows per KV head (decode, verification): the
 //                        queries stay in LDS and every wave streams key tiles past them, the
@@ -19,10 +20,11 @@
 //                        waves; where the keys alone do not fill the chip the rows are cut
 //                        into chunks, whose sums weights_sum_kernel adds in their order.  A
 //                        block of 32 rows against 256 keys takes 2.1 us a workgroup with two
-//                        of them on a compute unit.  2500 fresh tokens of 6 heads: 28 us and
-//                        4 us for the sums, of which the keys' way into registers is 6 us
-//                        (eight waves of one tile each, their rows reordered through LDS
-//                        instead of loaded one a lane, took as long in all)
+//                        of them on a compute unit.  2500 fresh tokens of 6 heads: 28.6 us a
+//                        call (27 and 4 us by the profiler, which adds about a microsecond to
+//                        each), of which the keys' way into registers is 6 us (eight waves of
+//                        one tile each, their rows reordered through LDS instead of loaded one
+//                        a lane, took as long in all)
 #include <type_traits>
 
 #include "common.h"

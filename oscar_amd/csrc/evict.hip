@@ -18,8 +18,8 @@
 // all, not by the 4 bytes per token it reads (31000 tokens 23 us, a third of it the reading
 // with the first digit and a third the lists): the weights lie in LDS as ordered numbers and
 // every thread takes a run of consecutive tokens, so that marks and lists are counted without
-// talk between lanes and only a thread's totals are scanned.  (Further compute units a list
-// would have to meet between the digits: four launches more, at 3 to 5 us each.)
+// talk between lanes and only a thread's totals are scanned.  (More compute units a list would
+// have to meet after the first digit and before the lists are written; not built.)
 #include <type_traits>
 
 #include "common.h"
@@ -370,9 +370,10 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(EvictParams P) {
 }
 
 // A group of D / 16 lanes per move: 8 bytes of constants and the codes of K and V, 16 bytes a
-// lane (five lanes of eight at head dim 128, nine of sixteen at 256).  Bound by the lines that
-// the scattered slots touch, two read and two written for each move: 128000 moves at head dim
-// 128 14 us, 43 MB between the L2 and memory.  (Four moves of a group in flight: 17 us.)
+// lane (five lanes of eight at head dim 128, nine of sixteen at 256).  128000 moves at head dim
+// 128 14 us: the lines that the scattered slots touch, two read and two written for each move,
+// are 43 MB between the L2 and memory, 8.4 us at a large copy's rate.  A group's loads follow on
+// each other, list, page, slot; four moves of a group in flight took 17 us.
 template <int D>
 __global__ __launch_bounds__(kMove) void evict_move_kernel(EvictParams P) {
   constexpr int L = D / 16, W = D / 64;  // lanes of a move; 16-byte parts of a side's codes

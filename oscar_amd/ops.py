@@ -640,7 +640,8 @@ def attention_decode(q, k_new, v_new, k_cache, v_cache, block_table, plan: Decod
     and the decode (a small store's quantization then rides in the merge launch).
     soft_cap, alibi_slopes [Hq] fp32: a score s (scaled) of key t for a query at position p
     becomes soft_cap tanh(s / soft_cap) + alibi_slopes[h] (t - p); 0 and None leave it, a cap
-    lies in [2^-20, 1024] (a score keeps 2^-22 of it).  The position is that in the cache, so tokens that were evicted do not count."""
+    lies in [2^-20, 1024] (a score keeps 2^-22 of it).  Positions are places in the cache: after
+    an eviction a token that moved counts from the place it moved into."""
     _require_cuda(q, k_cache, v_cache, block_table)
     if store is not None and static_scratch:
         raise ValueError("store= goes with the workspace decode only")
@@ -805,8 +806,9 @@ def accumulate_weights(q, k_new, k_cache, v_cache, block_table, plan, scale, lse
     attention_decode took them for this batch, lse [n, Hq] (fp32) as it returned it (a row
     with -inf adds nothing).  After a fresh prompt's attention_prefill(lse=...), history 0:
     its unrotated q and k.  plan: plan_weights(...) or the batch's plan_decode(...).  Request
-    r is row r of block_table and of weights; weights is updated in place and returned, the
-    same bits whatever runs beside it.
+    r is row r of block_table and of weights; weights is updated in place and returned: the
+    same bits for calls of the same sizes (requests, heads, longest length, most queries,
+    columns), equal to fp32 roundings for others.
     """
     if plan.qsl is None:
         raise ValueError("the plan has not been uploaded")
@@ -930,8 +932,9 @@ def evict(plan: EvictPlan, weights, k_cache, v_cache, block_table, *, head_dim, 
     plan: plan_evict(...) of the batch.  Per request and KV head the plan's tokens of least
     weight between the first and the last ones go (equal weights: the later token first; NaN
     counts as the largest); the kept tokens of the last pages before the recent ones move
-    into their places (keys of attention have no order; with alibi_slopes they have one, and
-    distances then count what is left).  A place that is written loses its FP32 window copy.
+    into their places (keys of attention have no order; with alibi_slopes they have one: a
+    token that moved then counts from its new place, those before the new end are nearer by
+    the dropped tokens).  A place that is written loses its FP32 window copy.
     The caches and the owner tags of `stage` change in place, block_table does not: after the
     last layer plan.table(block_table) is the new one, plan.seq_lens the new lengths.  The
     pages between must be the request's own.
