@@ -588,7 +588,7 @@ def cu_count(device) -> int:
 def _plan_sizes(plan, block_size: int) -> tuple:
     """Of a plan's requests with queries: (pages of the longest history, longest length, most
     queries), worked out again only when the plan's lists or the page size are others."""
-    key = (block_size, plan.has_new, plan.host_qsl, plan.host_seqs)
+    key = (block_size, plan.has_new, tuple(plan.host_qsl), tuple(plan.host_seqs))
     known = getattr(plan, "_sizes", None)
     if known is not None and known[0] == key:
         return known[1]
@@ -598,7 +598,7 @@ def _plan_sizes(plan, block_size: int) -> tuple:
             pages = max(pages, -(-(seq - (b - a) if plan.has_new else seq) // block_size))
             longest, most = max(longest, seq), max(most, b - a)
     sizes = pages, longest, most
-    plan._sizes = (block_size, plan.has_new, list(plan.host_qsl), list(plan.host_seqs)), sizes
+    plan._sizes = key, sizes
     return sizes
 
 

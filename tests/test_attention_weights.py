@@ -159,6 +159,17 @@ def test_the_sizes_of_a_plan_follow_its_lists():
     ops._check_table(table, plan, 32)
 
 
+@pytest.mark.parametrize("kind", [list, tuple, np.array, torch.tensor])
+def test_a_plan_may_hold_its_lists_as_arrays(kind):
+    from oscar_amd import ops
+
+    plan = ops.WeightsPlan(kind([0, 2, 2, 5]), kind([300, 900, 40]), True, None, None)
+    for _ in range(2):
+        assert ops._plan_sizes(plan, 128) == (3, 300, 3)
+    plan.host_seqs = kind([600, 900, 40])
+    assert ops._plan_sizes(plan, 128) == (5, 600, 3)
+
+
 def test_block_tables_are_laid_out_by_rows():
     from oscar_amd import ops
 
