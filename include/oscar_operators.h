@@ -172,6 +172,170 @@ typedef struct oscarop_evict_args_v1 {
 int64_t oscarop_evict_workspace_bytes_v1(int64_t num_reqs, int64_t num_kv_heads, int64_t max_drop);
 int oscarop_evict_v1(const oscarop_evict_args_v1* args, void* stream);
 
+/* ---- pages and slots of a step's tokens -------------------------------------------------
+ * Request r has lengths[r] tokens in the cache and counts[r] (below 1: none) rows of the
+ * step, next to the rows of the request before it.  All of its rows, or those with a mark in
+ * `keep`, take the places lengths[r], lengths[r] + 1, ... in their order.  Pages that the table does
+ * not have yet come off the top of the pool, requests in their order: a request gets all of its
+ * pages if it needs none, or if they and those of the requests before it are in the pool
+ * (refused requests' pages count as well), and none otherwise.
+ *   query_start_loc[r]  its first row       slots[i]      page * block_size + offset of the row's
+ *   seq_lens[r]         its length after           place; -1 without a mark, for a request
+ *   granted[r]          whether it has             that was refused, behind the last request,
+ *                       its pages                  and where the table holds a negative page
+ *   positions[i]        lengths[r] + the row's number in its request; 0 behind the last one
+ * and the new pages are in block_table, their number off *pool_count.  A request that does not
+ * fit (a negative length, rows past num_tokens, an end past the table or 2^31) is refused as
+ * well, without counting.  Query starts stay within num_tokens.  No overlap of any two
+ * arrays. */
+typedef struct oscarop_map_args_v1 {
+  const int32_t* lengths;       /* [num_reqs] device, as all arrays */
+  const int32_t* counts;        /* [num_reqs] */
+  const uint8_t* keep;          /* [num_tokens], nonzero: a mark; or NULL */
+  int32_t num_reqs;             /* at most 65536 */
+  int32_t block_size;           /* tokens per page */
+  int64_t num_tokens;           /* rows of the step, at most 2^30 (65536 with keep) */
+  int32_t* block_table;         /* [block_table_rows, block_table_cols] */
+  int64_t block_table_stride;
+  int64_t block_table_rows;     /* at least num_reqs */
+  int64_t block_table_cols;
+  const int32_t* pool_pages;    /* [pool_size]: the first *pool_count are free */
+  int32_t* pool_count;
+  int64_t pool_size;
+  int32_t* query_start_loc;     /* [num_reqs + 1] */
+  int32_t* seq_lens;            /* [num_reqs] */
+  int64_t* slots;               /* [num_tokens] */
+  int64_t* positions;           /* [num_tokens] */
+  uint8_t* granted;             /* [num_reqs] */
+  void* workspace;              /* >= oscarop_map_workspace_bytes_v1(...), 4-byte aligned */
+  int64_t workspace_bytes;
+} oscarop_map_args_v1;
+
+/* -22 for sizes that the call would refuse */
+int64_t oscarop_map_workspace_bytes_v1(int64_t num_reqs, int64_t num_tokens, int32_t keep);
+int oscarop_map_v1(const oscarop_map_args_v1* args, void* stream);
+
+/* The pages of request r behind new_lengths[r], ceil(new / block_size) up to
+ * ceil(lengths[r] / block_size), go back on top of the pool, requests in their order (what
+ * oscarop_map_v1 took last comes to lie as it lay).  The table keeps them.  A request with a
+ * new length below 0 or above its length, or with pages past the table, gives none, nor do the
+ * first one that the pool has no room for and those with pages behind it. */
+typedef struct oscarop_release_args_v1 {
+  const int32_t* lengths;       /* [num_reqs] device, as all arrays */
+  const int32_t* new_lengths;   /* [num_reqs] */
+  int32_t num_reqs;             /* at most 65536 */
+  int32_t block_size;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  int64_t block_table_rows;
+  int64_t block_table_cols;
+  int32_t* pool_pages;          /* [pool_size] */
+  int32_t* pool_count;
+  int64_t pool_size;
+} oscarop_release_args_v1;
+
+int oscarop_release_v1(const oscarop_release_args_v1* args, void* stream);
+
+/* ---- ancestor masks of drafted trees ----------------------------------------------------
+ * Node i of request r is row query_start_loc[r] + i; parents holds each node's parent as a
+ * node of its request (-1: a root), which comes before it.  Bit j mod 64 of word j / 64 of a
+ * row of mask: node j is the row's node or one of its ancestors; depths: the number of
+ * these.  A node whose parent is no earlier one (nor -1), and all below it, has no bit and
+ * depth -1, as have the nodes of a request of more than max_nodes, and rows of no request. */
+typedef struct oscarop_tree_args_v1 {
+  const int32_t* parents;         /* [num_tokens] device, as all arrays */
+  const int32_t* query_start_loc; /* [num_reqs + 1] */
+  int32_t num_reqs;               /* at most 65535 */
+  int32_t max_nodes;              /* of a request, at most 1024 */
+  int64_t num_tokens;             /* at most 2^30 */
+  int64_t* mask;                  /* [num_tokens][mask_words] */
+  int64_t mask_words;             /* ceil(max_nodes / 64) */
+  int32_t* depths;                /* [num_tokens] */
+} oscarop_tree_args_v1;
+
+int oscarop_tree_mask_v1(const oscarop_tree_args_v1* args, void* stream);
+
+/* oscarop_attn_decode_v1 for a chunk whose rows see each other by a mask: query i of n_q sees
+ * all of the history, and chunk row j <= i if bit j of its row of mask is set (rows past the
+ * mask's words are not seen).  A row that sees no key gets zeros and lse -inf.  No
+ * alibi_slopes (a node's distance is its depth, not its row). */
+int oscarop_attn_tree_v1(const oscar_attn_args_v1* args, const oscarop_score_v1* score, const int64_t* mask,
+                         int64_t mask_words, void* stream);
+
+/* ---- bounds of the keys of each page ----------------------------------------------------
+ * bounds[page][h][0 / 1][d]: the least / largest of the page's keys fp16(code * scale + zero)
+ * over the tokens that it holds (NaN if one of them is), for the pages of request r's columns
+ * [lengths[r] / block_size, ceil(seq_lens[r] / block_size)) where seq_lens[r] > lengths[r]; all
+ * others stay.  Keys of the FP32 window count as their slots hold them.  A request with a
+ * negative length or columns past the table, and pages outside the cache, are left alone.
+ * No page may come twice. */
+typedef struct oscarop_bounds_args_v1 {
+  oscar_cache_v1 cache;           /* the v side is not read */
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  int64_t block_table_rows;
+  int64_t block_table_cols;
+  const int32_t* lengths;         /* [num_reqs] device: tokens before */
+  const int32_t* seq_lens;        /* [num_reqs] device: and after */
+  int32_t num_reqs;               /* at most 65535, as KV heads */
+  int32_t reserved;
+  int64_t max_new;                /* the most new tokens of a request: sizes the launch */
+  void* bounds;                   /* fp16 [num_blocks][Hk][2][D], 16-byte aligned */
+} oscarop_bounds_args_v1;
+
+int oscarop_page_bounds_v1(const oscarop_bounds_args_v1* args, void* stream);
+
+/* ---- pages that promise the largest scores ----------------------------------------------
+ * Request r has n_q queries and a history of h tokens (seq_lens[r], less n_q with has_new)
+ * in P = ceil(h / block_size) pages.  With P <= budget all of them are chosen, otherwise the first
+ * first_pages, the last last_pages and of the others those of the largest score (equal
+ * scores: the earlier page first; a NaN score counts as the largest), budget in all, for each
+ * KV head its own.  A page's score: the largest, over the request's queries and the query
+ * heads of the KV head, of the sum over the channels of max(q low, q high), summed in 64
+ * bits.  table[r][h] holds the chosen pages in ascending order of their columns and
+ * pages[r][h] these columns, -1 behind them.  A request that does not fit (queries past
+ * num_tokens, a negative history, columns past the table) gets -1 throughout. */
+typedef struct oscarop_select_args_v1 {
+  const void* q;                  /* [num_tokens, num_q_heads, D] in q_dtype */
+  int64_t num_tokens;
+  int64_t num_q_heads;
+  int64_t q_stride_token;         /* elements, a multiple of 8; rows 16-byte aligned */
+  int32_t q_dtype;                /* OSCAR_BF16 or OSCAR_F16 */
+  int32_t has_new;
+  const void* bounds;             /* as oscarop_page_bounds_v1 leaves them */
+  int64_t num_blocks;
+  int64_t num_kv_heads;           /* at most 65535 */
+  int64_t head_dim;               /* 128 or 256 */
+  int64_t block_size;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  int64_t block_table_rows;
+  int64_t block_table_cols;
+  const int32_t* query_start_loc; /* [num_reqs + 1] device */
+  const int32_t* seq_lens;        /* [num_reqs] device */
+  int32_t num_reqs;               /* at most 65535 */
+  int32_t max_pages;              /* the most pages of a history: sizes the launch */
+  int32_t budget;                 /* at least first_pages + last_pages + 1 */
+  int32_t first_pages;            /* >= 0 */
+  int32_t last_pages;             /* >= 1 */
+  int32_t reserved;
+  int32_t* table;                 /* [num_reqs][Hk][budget] */
+  int32_t* pages;                 /* [num_reqs][Hk][budget], or NULL */
+  void* workspace;                /* >= oscarop_select_workspace_bytes_v1(args), 16-byte aligned */
+  int64_t workspace_bytes;
+} oscarop_select_args_v1;
+
+/* reads the sizes of *args alone; -22 for sizes that the call would refuse */
+int64_t oscarop_select_workspace_bytes_v1(const oscarop_select_args_v1* args);
+int oscarop_select_v1(const oscarop_select_args_v1* args, void* stream);
+
+/* oscarop_attn_decode_v1 with a block table for each KV head: head h of request r reads row
+ * r of block_table shifted by h * table_stride_head, as oscarop_select_v1 writes it.  The
+ * lengths and the plan are those of the chosen tokens.  No alibi_slopes (the chosen pages' distances are
+ * not the table's). */
+int oscarop_attn_selected_v1(const oscar_attn_args_v1* args, const oscarop_score_v1* score, int64_t table_stride_head,
+                             void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -138,6 +138,48 @@ class EvictArgs(C.Structure):
     ]
 
 
+class MapArgs(C.Structure):
+    _fields_ = [
+        ("lengths", vp), ("counts", vp), ("keep", vp), ("num_reqs", i32), ("block_size", i32), ("num_tokens", i64),
+        ("block_table", vp), ("block_table_stride", i64), ("block_table_rows", i64), ("block_table_cols", i64),
+        ("pool_pages", vp), ("pool_count", vp), ("pool_size", i64),
+        ("query_start_loc", vp), ("seq_lens", vp), ("slots", vp), ("positions", vp), ("granted", vp),
+        ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+class ReleaseArgs(C.Structure):
+    _fields_ = [
+        ("lengths", vp), ("new_lengths", vp), ("num_reqs", i32), ("block_size", i32),
+        ("block_table", vp), ("block_table_stride", i64), ("block_table_rows", i64), ("block_table_cols", i64),
+        ("pool_pages", vp), ("pool_count", vp), ("pool_size", i64),
+    ]
+
+
+class TreeArgs(C.Structure):
+    _fields_ = [("parents", vp), ("query_start_loc", vp), ("num_reqs", i32), ("max_nodes", i32), ("num_tokens", i64),
+                ("mask", vp), ("mask_words", i64), ("depths", vp)]
+
+
+class BoundsArgs(C.Structure):
+    _fields_ = [
+        ("cache", Cache), ("block_table", vp), ("block_table_stride", i64), ("block_table_rows", i64),
+        ("block_table_cols", i64), ("lengths", vp), ("seq_lens", vp), ("num_reqs", i32), ("reserved", i32),
+        ("max_new", i64), ("bounds", vp),
+    ]
+
+
+class SelectArgs(C.Structure):
+    _fields_ = [
+        ("q", vp), ("num_tokens", i64), ("num_q_heads", i64), ("q_stride_token", i64), ("q_dtype", i32), ("has_new", i32),
+        ("bounds", vp), ("num_blocks", i64), ("num_kv_heads", i64), ("head_dim", i64), ("block_size", i64),
+        ("block_table", vp), ("block_table_stride", i64), ("block_table_rows", i64), ("block_table_cols", i64),
+        ("query_start_loc", vp), ("seq_lens", vp), ("num_reqs", i32), ("max_pages", i32), ("budget", i32),
+        ("first_pages", i32), ("last_pages", i32), ("reserved", i32), ("table", vp), ("pages", vp),
+        ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
 STEP_NOT_DECODE = 1
 
 # name -> (restype, argtypes); every symbol declared in include/oscar_amd.h
@@ -173,6 +215,15 @@ OPERATOR_SIGNATURES = {
     "oscarop_evict_workspace_bytes_v1": (i64, [i64, i64, i64]),
     "oscarop_evict_v1": (C.c_int, [C.POINTER(EvictArgs), vp]),
     "oscarop_norm_rope_v1": (C.c_int, [C.POINTER(NormRopeArgs), vp]),
+    "oscarop_map_workspace_bytes_v1": (i64, [i64, i64, i32]),
+    "oscarop_map_v1": (C.c_int, [C.POINTER(MapArgs), vp]),
+    "oscarop_release_v1": (C.c_int, [C.POINTER(ReleaseArgs), vp]),
+    "oscarop_tree_mask_v1": (C.c_int, [C.POINTER(TreeArgs), vp]),
+    "oscarop_attn_tree_v1": (C.c_int, [C.POINTER(AttnArgs), C.POINTER(Score), vp, i64, vp]),
+    "oscarop_page_bounds_v1": (C.c_int, [C.POINTER(BoundsArgs), vp]),
+    "oscarop_select_workspace_bytes_v1": (i64, [C.POINTER(SelectArgs)]),
+    "oscarop_select_v1": (C.c_int, [C.POINTER(SelectArgs), vp]),
+    "oscarop_attn_selected_v1": (C.c_int, [C.POINTER(AttnArgs), C.POINTER(Score), i64, vp]),
 }
 
 _LIB = None

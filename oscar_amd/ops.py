@@ -967,3 +967,356 @@ def evict(plan: EvictPlan, weights, k_cache, v_cache, block_table, *, head_dim, 
                        plan.max_drop, None if st is None else C.pointer(st), ws.data_ptr(), ws.numel())
     _launch("oscarop_evict_v1", index, C.byref(a))
     return weights_out
+
+
+# ------------------------------------------------------------------------ pages and slots
+@dataclass
+class PagePool:
+    """The free pages of a cache, on the device: pages[:count] (int32), the next one last."""
+    pages: torch.Tensor  # int32 [size]
+    count: torch.Tensor  # int32 [1]
+
+    @classmethod
+    def of(cls, num_blocks: int, device) -> "PagePool":
+        """The pool of an empty cache; page 0 is handed out first."""
+        pages = torch.arange(num_blocks - 1, -1, -1, dtype=torch.int32, device=device)
+        return cls(pages, torch.full((1,), num_blocks, dtype=torch.int32, device=device))
+
+
+@dataclass
+class SlotMap:
+    """What map_slots makes of a step: query starts [requests + 1] and lengths [requests]
+    (int32), a slot and a position for each row (int64), and which requests got their pages."""
+    qsl: torch.Tensor
+    seq_lens: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    granted: torch.Tensor  # bool [requests]
+
+
+def _int32_list(name: str, x: torch.Tensor, n: int) -> torch.Tensor:
+    if x.dtype != torch.int32 or x.shape != (n,):
+        raise ValueError(f"{name} must be int32 [{n}]")
+    return x.contiguous()
+
+
+def _check_pool(pool: PagePool) -> None:
+    if pool.pages.dtype != torch.int32 or pool.pages.ndim != 1 or not pool.pages.is_contiguous():
+        raise ValueError("the pool's pages must be a contiguous int32 list")
+    if pool.count.dtype != torch.int32 or pool.count.numel() != 1:
+        raise ValueError("the pool's count must be one int32")
+
+
+def _own_rows(table: torch.Tensor, reqs: int) -> int:
+    """The row stride of a block table that is written in place."""
+    if table.dtype != torch.int32 or table.ndim != 2 or table.shape[0] < reqs:
+        raise ValueError("Missing request block-table rows")
+    if table.shape[1] > 1 and table.stride(1) != 1 or reqs > 1 and table.stride(0) < table.shape[1]:
+        raise ValueError("the block table's rows must not overlap, its columns lie next to each other")
+    return table.stride(0) if reqs > 1 else max(table.shape[1], 1)
+
+
+def map_slots(pool: PagePool, block_table, lengths, counts, *, tokens: int, block_size: int, keep=None) -> SlotMap:
+    """Pages, slots and positions of a step, without a look at the lengths from the host.
+
+    Request r has lengths[r] tokens in the cache and counts[r] rows in the step (int32 on the
+    device), its rows after those of the request before it; the step has `tokens` rows, the
+    ones behind the last request are padding.  All of a request's rows, or those marked in
+    keep [tokens] (bool: a drafted tree's accepted nodes; up to 65536 rows), take the places
+    lengths[r], lengths[r] + 1, ...; the pages that they need come off the top of the pool and
+    into block_table [requests, columns] (int32, in place, as the pool's count).  Requests are
+    served in their order: one that the pool has too few pages left for gets none, nor does a
+    later one that needs any, nor one that does not fit (an end past the table, rows past
+    `tokens`); its length stays, its rows get no slot.
+
+    Slots are as ops.store takes them, -1 for rows without one; positions lengths[r] + the
+    row's number in its request, 0 in the padding.  May be captured; up to 65536 requests."""
+    index = _device_index(pool.pages, pool.count, block_table, lengths, counts, keep)
+    _check_pool(pool)
+    reqs, dev = lengths.shape[0] if lengths.ndim == 1 else -1, block_table.device
+    lengths, counts = _int32_list("lengths", lengths, reqs), _int32_list("counts", counts, reqs)
+    stride = _own_rows(block_table, reqs)
+    if tokens < 0 or block_size < 1:
+        raise ValueError("tokens must not be negative, block_size at least 1")
+    if keep is not None:
+        if keep.dtype != torch.bool or keep.shape != (tokens,):
+            raise ValueError(f"keep must be bool [{tokens}]")
+        keep = keep.contiguous()
+    need = _lib.load().oscarop_map_workspace_bytes_v1(reqs, tokens, keep is not None)
+    # one piece of memory: slots and positions, then starts, lengths and the workspace, then grants
+    words = 4 * tokens + 2 * reqs + 1 + max(need, 0) // 4
+    buf = torch.empty(4 * words + reqs, dtype=torch.uint8, device=dev)
+    wide, narrow = buf[:16 * tokens].view(torch.int64), buf[16 * tokens:4 * words].view(torch.int32)
+    out = SlotMap(narrow[:reqs + 1], narrow[reqs + 1:2 * reqs + 1], wide[:tokens], wide[tokens:],
+                  buf[4 * words:].view(torch.bool))
+    base = buf.data_ptr()
+    at = base + 16 * tokens
+    a = _lib.MapArgs(lengths.data_ptr(), counts.data_ptr(), _ptr(keep), reqs, block_size, tokens, block_table.data_ptr(),
+                     stride, *block_table.shape, pool.pages.data_ptr(), pool.count.data_ptr(), pool.pages.shape[0], at,
+                     at + 4 * (reqs + 1), base, base + 8 * tokens, base + 4 * words, at + 4 * (2 * reqs + 1), max(need, 0))
+    _launch("oscarop_map_v1", index, C.byref(a))
+    return out
+
+
+def release_pages(pool: PagePool, block_table, lengths, new_lengths, *, block_size: int) -> None:
+    """Give back the pages behind new_lengths[r] of requests of lengths[r] tokens (int32 on the
+    device): those of a request that ended (0), of a step's rejected tokens, of an eviction
+    (plan.lengths and plan.seq_lens, with plan.table(...)).  The pool grows in place, requests
+    in their order, their pages ascending, so that what map_slots took last lies as it lay;
+    the table keeps its entries.  A new length below 0 or above the old one gives nothing back,
+    nor does a request whose pages the pool has no room for, nor those with pages behind it."""
+    index = _device_index(pool.pages, pool.count, block_table, lengths, new_lengths)
+    _check_pool(pool)
+    reqs = lengths.shape[0] if lengths.ndim == 1 else -1
+    lengths, new_lengths = _int32_list("lengths", lengths, reqs), _int32_list("new_lengths", new_lengths, reqs)
+    if block_size < 1:
+        raise ValueError("block_size must be at least 1")
+    stride = _own_rows(block_table, reqs)
+    a = _lib.ReleaseArgs(lengths.data_ptr(), new_lengths.data_ptr(), reqs, block_size, block_table.data_ptr(), stride,
+                         *block_table.shape, pool.pages.data_ptr(), pool.count.data_ptr(), pool.pages.shape[0])
+    _launch("oscarop_release_v1", index, C.byref(a))
+
+
+# ------------------------------------------------------------------------ drafted trees
+MOST_NODES = 1024  # of a request's tree
+
+
+def tree_mask(parents, qsl, *, max_nodes: int) -> tuple:
+    """Ancestor masks of drafted trees: (mask int64 [N, words], depths int32 [N]).
+
+    parents [N] int32: row qsl[r] + i is node i of request r's tree, its parent a node before it
+    (-1: a root).  qsl [requests + 1] int32 on the device; max_nodes: the most nodes of a
+    request (1 to 1024), ceil(max_nodes / 64) words.  Bit j mod 64 of word j / 64: node j is the
+    row's node or an ancestor; depths: their number, a root's 0 (its position is the history's
+    length plus that).  Nodes without a proper parent, those below them, nodes of a larger
+    request and rows of none have no bit and depth -1."""
+    index = _device_index(parents, qsl)
+    n = parents.shape[0] if parents.ndim == 1 else -1
+    parents = _int32_list("parents", parents, n)
+    if qsl.ndim != 1 or qsl.shape[0] < 1:
+        raise ValueError("qsl must be int32 [requests + 1]")
+    qsl = _int32_list("qsl", qsl, qsl.shape[0])
+    if not 1 <= max_nodes <= MOST_NODES:
+        raise ValueError(f"max_nodes must lie in [1, {MOST_NODES}]")
+    words = -(-max_nodes // 64)
+    mask = torch.empty(n, words, dtype=torch.int64, device=parents.device)
+    depths = torch.empty(n, dtype=torch.int32, device=parents.device)
+    a = _lib.TreeArgs(parents.data_ptr(), qsl.data_ptr(), qsl.shape[0] - 1, max_nodes, n, mask.data_ptr(), words,
+                      depths.data_ptr())
+    _launch("oscarop_tree_mask_v1", index, C.byref(a))
+    return mask, depths
+
+
+def plan_tree(qsl, seqs, *, num_kv_heads: int, group: int, head_dim: int, device, window: tuple = (0, 0)) -> DecodePlan:
+    """Plan of attention_tree over a batch: request r's rows [qsl[r], qsl[r + 1]) are the nodes of
+    its tree, seqs[r] its length with them (host lists); sizes and window as plan_decode."""
+    qsl, seqs = _request_lists(qsl, seqs, True)
+    return plan_decode(qsl, seqs, has_new=True, num_kv_heads=num_kv_heads, group=group, head_dim=head_dim, device=device,
+                       window=window)
+
+
+def _attention_over(entry, q, k_new, v_new, k_cache, v_cache, table, rows_of_table, plan, scale, stage, head_dim, soft_cap,
+                    out_rot, lse, others, extra):
+    """The entry points beside attention_decode, which take its arguments and `extra` ones.
+    table: [requests, columns] as the kernels address it; others: more tensors of the call."""
+    index = _device_index(q, k_new, v_new, k_cache, v_cache, table, out_rot, lse, *others, *(stage or ()))
+    score = score_struct(soft_cap, None, q.shape[1], q.device)
+    code = _DTYPES.get(q.dtype)
+    if code is None or code == OSCAR_F32:
+        raise ValueError("OSCAR HIP attention requires bf16 or fp16 queries")
+    if q.ndim != 3 or q.shape[2] != head_dim:
+        raise ValueError("q must be [tokens, heads, head_dim]")
+    n, hq, _ = q.shape
+    hk = k_cache.shape[2]
+    if hq % hk:
+        raise ValueError("Hq must be a multiple of Hk")
+    if plan.has_new != (k_new is not None) or (k_new is None) != (v_new is None):
+        raise ValueError("plan and call disagree on the presence of current K/V")
+    if plan.items is None:
+        raise ValueError("the plan has not been uploaded")
+    if plan.host_qsl[-1] > n:
+        raise ValueError("the plan has more queries than the call")
+    if k_new is not None:
+        for x in (k_new, v_new):
+            if x.dtype != q.dtype or x.shape != (n, hk, head_dim):
+                raise ValueError("Current K/V must match the queries' type and tokens and the cache's heads")
+        k_new, v_new = _aligned(k_new), _aligned(v_new)
+    if q.stride(2) != 1 or q.stride(1) != head_dim or q.stride(0) % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    all_rows = plan.num_items > 0 and _covers(plan, n)
+    if out_rot is None:
+        # rows of no request stay zero (lse -inf); the merge writes every row of a request
+        out_rot = (torch.empty if all_rows else torch.zeros)(n, hq, head_dim, dtype=torch.float32, device=q.device)
+    elif out_rot.dtype != torch.float32 or out_rot.shape != q.shape or not out_rot.is_contiguous():
+        raise ValueError("out_rot must be contiguous fp32 [tokens, heads, head_dim]")
+    if lse is None:
+        lse = torch.empty(n, hq, dtype=torch.float32, device=q.device)
+        if not all_rows:
+            lse.fill_(-math.inf)
+    elif lse.dtype != torch.float32 or lse.shape != (n, hq) or not lse.is_contiguous():
+        raise ValueError("lse must be contiguous fp32 [tokens, heads]")
+    if plan.num_items == 0 or n == 0:
+        return out_rot, lse
+    if table.shape[0] < len(plan.host_seqs):
+        raise ValueError("Missing request block-table rows")
+    if _plan_sizes(plan, k_cache.shape[1])[0] > rows_of_table:
+        raise ValueError("Block table cannot cover the history")
+    st = staging_struct(stage, k_cache, head_dim)
+    ws = _call_workspace(index, "attn_workspace", plan.partial_bytes)
+    a = _lib.AttnArgs(q.data_ptr(), n, hq, q.stride(0), _ptr(k_new), _ptr(v_new), 0 if k_new is None else k_new.stride(0),
+                      cache_struct(k_cache, v_cache, head_dim), table.data_ptr(), table.stride(0), plan.qsl.data_ptr(),
+                      plan.seqs.data_ptr(), plan.seqs.numel(), None if st is None else C.pointer(st), scale,
+                      plan.items.data_ptr(), plan.num_items, plan.groups.data_ptr(), plan.num_groups, ws.data_ptr(),
+                      ws.numel(), plan.max_group_items, out_rot.data_ptr(), lse.data_ptr(), 0, code, table.shape[0],
+                      rows_of_table)
+    _launch(entry, index, C.byref(a), None if score is None else C.byref(score), *extra)
+    return out_rot, lse
+
+
+def attention_tree(q, k_new, v_new, k_cache, v_cache, block_table, plan: DecodePlan, mask, scale, stage=None, *, head_dim,
+                   soft_cap=0.0, out_rot=None, lse=None):
+    """Attention of drafted trees over the INT2 history: (out_rot fp32, lse fp32), rotated, as
+    attention_decode's, whose arguments these are.
+
+    Row i of a request sees all of its history and the request's rows j <= i whose bit is set in
+    the row's mask (tree_mask; int64 [N, words], bit j mod 64 of word j / 64: at least a word
+    for each 64 rows of the longest chunk).  A row that sees no key gets zeros and -inf.
+    plan: plan_tree(...).  The nodes' keys and values are k_new and v_new: accepted ones are
+    written afterwards, by ops.store with the slots of map_slots(keep=...)."""
+    if mask.dtype != torch.int64 or mask.ndim != 2 or mask.shape[0] != q.shape[0]:
+        raise ValueError("mask must be int64 [tokens, words]")
+    most = _plan_sizes(plan, k_cache.shape[1])[2]
+    if most > 64 * mask.shape[1]:
+        raise ValueError(f"a mask of {mask.shape[1]} words for {most} rows of a request")
+    if k_new is None:
+        raise ValueError("a tree's attention needs its nodes' K and V")
+    mask, table = mask.contiguous(), _rows_apart(block_table)
+    if table.ndim != 2:
+        raise ValueError("Missing request block-table rows")
+    return _attention_over("oscarop_attn_tree_v1", q, k_new, v_new, k_cache, v_cache, table, table.shape[1], plan, scale,
+                           stage, head_dim, soft_cap, out_rot, lse, (mask, plan.items), (mask.data_ptr(), mask.shape[1]))
+
+
+# ------------------------------------------------------------------------ chosen pages
+def page_bounds(k_cache, bounds, block_table, lengths, seq_lens, *, max_new: int, head_dim: int):
+    """Bring the bounds of the pages that a step touched up to date, in place; returns bounds.
+
+    bounds [blocks, Hk, 2, D] fp16: the least and the largest key that a page holds, for each
+    KV head and channel, of the keys as their slots hold them.  Request r had lengths[r] tokens
+    in the cache and has seq_lens[r] now (int32 on the device): its pages from the one of token
+    lengths[r] on are looked at again, those of a request that did not grow are not.  max_new:
+    the most new tokens of a request.  Call it after the step's store; after an eviction with
+    lengths 0 (kept tokens have moved)."""
+    index = _device_index(k_cache, bounds, block_table, lengths, seq_lens)
+    cache = cache_struct(k_cache, k_cache, head_dim)
+    reqs = lengths.shape[0] if lengths.ndim == 1 else -1
+    lengths, seq_lens = _int32_list("lengths", lengths, reqs), _int32_list("seq_lens", seq_lens, reqs)
+    if bounds.dtype != torch.float16 or bounds.shape != (cache.num_blocks, cache.num_kv_heads, 2, head_dim) \
+            or not bounds.is_contiguous():
+        raise ValueError("bounds must be contiguous fp16 [blocks, KV heads, 2, head_dim]")
+    if max_new < 0:
+        raise ValueError("max_new must not be negative")
+    table = _rows_apart(block_table)
+    if table.ndim != 2 or table.shape[0] < reqs:
+        raise ValueError("Missing request block-table rows")
+    a = _lib.BoundsArgs(cache, table.data_ptr(), table.stride(0), *table.shape, lengths.data_ptr(), seq_lens.data_ptr(), reqs, 0,
+                        max_new, bounds.data_ptr())
+    _launch("oscarop_page_bounds_v1", index, C.byref(a))
+    return bounds
+
+
+@dataclass
+class SelectPlan:
+    """A batch whose requests read `budget` pages of their history at most (plan_selected)."""
+    decode: DecodePlan   # of the chosen tokens
+    host_qsl: list
+    host_seqs: list
+    has_new: bool
+    block_size: int
+    budget: int
+    first_pages: int
+    last_pages: int
+    max_pages: int       # of the longest history
+    num_kv_heads: int
+    head_dim: int
+    qsl: torch.Tensor    # device int32
+    seqs: torch.Tensor
+
+
+def plan_selected(qsl, seqs, *, has_new: bool, block_size: int, budget: int, first_pages: int = 1, last_pages: int = 1,
+                  num_kv_heads: int, group: int, head_dim: int, device, window: tuple = (0, 0)) -> SelectPlan:
+    """Plan of select_pages and attention_selected (host lists, as plan_decode): of each history
+    at most `budget` pages are read, among them the first first_pages and the last last_pages (at
+    least 1; enough for the FP32 window, ceil(recent / block_size) + 1, if its tokens are to be
+    seen), for all queries of a request the same."""
+    qsl, seqs = _request_lists(qsl, seqs, has_new)
+    if block_size < 1 or first_pages < 0 or last_pages < 1 or budget <= first_pages + last_pages:
+        raise ValueError("the budget must exceed first_pages + last_pages, last_pages be 1 at least")
+    fewer, most = [], 0
+    for a, b, seq in zip(qsl, qsl[1:], seqs):
+        pages = -(-(seq - (b - a) if has_new else seq) // block_size)
+        most = max(most, pages)
+        fewer.append(seq - max(pages - budget, 0) * block_size)
+    plan = plan_decode(qsl, fewer, has_new=has_new, num_kv_heads=num_kv_heads, group=group, head_dim=head_dim,
+                       device=device, window=window, upload_now=False)
+    parts = upload(plan.host_parts() + [np.asarray(seqs or [0], np.int32)], device)
+    plan.adopt(parts[:4])
+    return SelectPlan(plan, qsl, seqs, bool(has_new), block_size, budget, first_pages, last_pages, most, num_kv_heads,
+                      head_dim, plan.qsl, parts[4])
+
+
+def select_pages(q, bounds, block_table, plan: SelectPlan) -> tuple:
+    """The pages of each history that promise the largest scores: (table, pages), int32
+    [requests, Hk, budget]: the chosen pages, and their columns in block_table, ascending; -1
+    behind them.
+
+    q [N, Hq, D] bf16 or fp16, rotated as the cache; bounds: page_bounds(...).  A page's
+    score is the largest, over the request's queries and the KV head's query heads, of
+    sum_d max(q_d low_d, q_d high_d), which no key of the page exceeds; summed in 64 bits.  Equal
+    scores: the earlier page; NaN counts as the largest.  A history of at most budget pages is
+    chosen whole."""
+    index = _device_index(q, bounds, block_table, plan.qsl)
+    code = _DTYPES.get(q.dtype)
+    if code is None or code == OSCAR_F32:
+        raise ValueError("OSCAR HIP attention requires bf16 or fp16 queries")
+    d, hk, reqs = plan.head_dim, plan.num_kv_heads, len(plan.host_seqs)
+    if q.ndim != 3 or q.shape[2] != d or q.shape[1] % hk:
+        raise ValueError("q must be [tokens, heads, head_dim], its heads a multiple of the KV heads")
+    if plan.host_qsl[-1] > q.shape[0]:
+        raise ValueError("the plan has more queries than the call")
+    if bounds.dtype != torch.float16 or bounds.ndim != 4 or bounds.shape[1:] != (hk, 2, d) or not bounds.is_contiguous():
+        raise ValueError("bounds must be contiguous fp16 [blocks, KV heads, 2, head_dim]")
+    table = _rows_apart(block_table)
+    if table.ndim != 2 or table.shape[0] < reqs:
+        raise ValueError("Missing request block-table rows")
+    if plan.max_pages > table.shape[1]:
+        raise ValueError("Block table cannot cover the history")
+    if q.stride(2) != 1 or q.stride(1) != d or q.stride(0) % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    out = torch.empty(2, reqs, hk, plan.budget, dtype=torch.int32, device=q.device)
+    a = _lib.SelectArgs(q.data_ptr(), q.shape[0], q.shape[1], q.stride(0), code, plan.has_new, bounds.data_ptr(),
+                        bounds.shape[0], hk, d, plan.block_size, table.data_ptr(), table.stride(0), *table.shape,
+                        plan.qsl.data_ptr(), plan.seqs.data_ptr(), reqs, plan.max_pages, plan.budget, plan.first_pages,
+                        plan.last_pages, 0, out.data_ptr(), out.data_ptr() + 4 * reqs * hk * plan.budget, None, 0)
+    need = _lib.load().oscarop_select_workspace_bytes_v1(C.byref(a))
+    if need > 0:
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)  # a captured call keeps its own
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    _launch("oscarop_select_v1", index, C.byref(a))
+    return out[0], out[1]
+
+
+def attention_selected(q, k_new, v_new, k_cache, v_cache, table, plan: SelectPlan, scale, stage=None, *, head_dim,
+                       soft_cap=0.0, out_rot=None, lse=None):
+    """Attention over the pages that select_pages chose, and the current chunk: (out_rot fp32,
+    lse fp32), rotated, as attention_decode's, whose other arguments these are.  table
+    [requests, Hk, budget]: each KV head's pages, ascending."""
+    hk = k_cache.shape[2]
+    if table.dtype != torch.int32 or table.ndim != 3 or table.shape[1:] != (hk, plan.budget):
+        raise ValueError("table must be int32 [requests, KV heads, budget]")
+    if plan.block_size != k_cache.shape[1] or plan.num_kv_heads != hk:
+        raise ValueError(f"the plan is for {plan.num_kv_heads} KV heads and pages of {plan.block_size} tokens")
+    table = table.contiguous()
+    flat = table.view(table.shape[0], hk * plan.budget)
+    return _attention_over("oscarop_attn_selected_v1", q, k_new, v_new, k_cache, v_cache, flat, plan.budget, plan.decode,
+                           scale, stage, head_dim, soft_cap, out_rot, lse, (plan.qsl,), (plan.budget,))
