@@ -255,12 +255,39 @@ typedef struct oscarop_tree_args_v1 {
 
 int oscarop_tree_mask_v1(const oscarop_tree_args_v1* args, void* stream);
 
-/* oscarop_attn_decode_v1 for a chunk whose rows see each other by a mask: query i of n_q sees
+/* ---- attention of drafted trees over the INT2 history -----------------------------------
+ * oscarop_attn_decode_v1 for chunks whose rows see each other by a mask: query i of n_q sees
  * all of the history, and chunk row j <= i if bit j of its row of mask is set (rows past the
  * mask's words are not seen).  A row that sees no key gets zeros and lse -inf.  No
- * alibi_slopes (a node's distance is its depth, not its row). */
-int oscarop_attn_tree_v1(const oscar_attn_args_v1* args, const oscarop_score_v1* score, const int64_t* mask,
-                         int64_t mask_words, void* stream);
+ * alibi_slopes (a node's distance is its depth, not its row).  History keys are
+ * q_dtype(fp16(x)), history values fp16(x), the chunk's as they are; probabilities are rounded to
+ * fp16 for the history, to two bf16 parts for a bf16 chunk; sums and the softmax are fp32.  The
+ * same plan gives the same bits. */
+#define OSCAROP_TREE_ITEM_INTS 12
+
+typedef struct oscarop_tree_sizes_v1 {
+  int32_t num_items;
+  int32_t num_groups;
+  int64_t partial_rows;
+  int64_t partial_bytes;        /* workspace of the call */
+} oscarop_tree_sizes_v1;
+
+/* Host plan, as oscar_attn_plan_v1: query starts [num_reqs + 1] and lengths (with the chunk);
+ * items [OSCAROP_TREE_ITEM_INTS] and groups [OSCAR_GROUP_INTS] each, which the caller copies to
+ * the device.  Returns the number of items, -28 with the sizes in *plan if the buffers are too
+ * small; items or groups NULL: only the sizes. */
+int oscarop_tree_plan_v1(const int32_t* qsl, const int32_t* seqs, int32_t num_reqs, int32_t num_kv_heads, int32_t group,
+                         int32_t head_dim, int32_t target_items, int32_t* items, int32_t max_items, int32_t* groups,
+                         int32_t max_groups, oscarop_tree_sizes_v1* plan);
+
+typedef struct oscarop_tree_attn_args_v1 {
+  oscar_attn_args_v1 attn;      /* as the decode's; items and groups are the tree plan's, phases 0 */
+  const int64_t* mask;          /* [num_tokens][mask_words] */
+  int64_t mask_words;
+  int64_t partial_rows;         /* the plan's */
+} oscarop_tree_attn_args_v1;
+
+int oscarop_attn_tree_v1(const oscarop_tree_attn_args_v1* args, const oscarop_score_v1* score, void* stream);
 
 /* ---- bounds of the keys of each page ----------------------------------------------------
  * bounds[page][h][0 / 1][d]: the least / largest of the page's keys fp16(code * scale + zero)

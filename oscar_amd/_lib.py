@@ -14,6 +14,7 @@ LIB_PATH = Path(__file__).resolve().parent / "liboscar_amd.so"
 OSCAR_F32, OSCAR_F16, OSCAR_BF16 = 0, 1, 2
 STAGE_NONE, STAGE_INVALIDATE, STAGE_WRITE = 0, 1, 2
 WORK_INTS = 8
+TREE_ITEM_INTS = 12
 GROUP_INTS = 8
 ABI_VERSION = 3
 DECODE_STATIC_MAX_ITEMS = 512
@@ -161,6 +162,14 @@ class TreeArgs(C.Structure):
                 ("mask", vp), ("mask_words", i64), ("depths", vp)]
 
 
+class TreeSizes(C.Structure):
+    _fields_ = [("num_items", i32), ("num_groups", i32), ("partial_rows", i64), ("partial_bytes", i64)]
+
+
+class TreeAttnArgs(C.Structure):
+    _fields_ = [("attn", AttnArgs), ("mask", vp), ("mask_words", i64), ("partial_rows", i64)]
+
+
 class BoundsArgs(C.Structure):
     _fields_ = [
         ("cache", Cache), ("block_table", vp), ("block_table_stride", i64), ("block_table_rows", i64),
@@ -219,7 +228,9 @@ OPERATOR_SIGNATURES = {
     "oscarop_map_v1": (C.c_int, [C.POINTER(MapArgs), vp]),
     "oscarop_release_v1": (C.c_int, [C.POINTER(ReleaseArgs), vp]),
     "oscarop_tree_mask_v1": (C.c_int, [C.POINTER(TreeArgs), vp]),
-    "oscarop_attn_tree_v1": (C.c_int, [C.POINTER(AttnArgs), C.POINTER(Score), vp, i64, vp]),
+    "oscarop_tree_plan_v1": (C.c_int, [C.POINTER(i32), C.POINTER(i32), i32, i32, i32, i32, i32, C.POINTER(i32), i32,
+                                       C.POINTER(i32), i32, C.POINTER(TreeSizes)]),
+    "oscarop_attn_tree_v1": (C.c_int, [C.POINTER(TreeAttnArgs), C.POINTER(Score), vp]),
     "oscarop_page_bounds_v1": (C.c_int, [C.POINTER(BoundsArgs), vp]),
     "oscarop_select_workspace_bytes_v1": (i64, [C.POINTER(SelectArgs)]),
     "oscarop_select_v1": (C.c_int, [C.POINTER(SelectArgs), vp]),

@@ -19,7 +19,8 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
 SOURCES = ["capi.cpp", "step.cpp", "store.hip", "rotate.hip", "attn_decode.hip", "attn_prefill.hip",
-           "norm_rope.hip", "attn_weights.hip", "evict.hip", "pages.hip", "tree_mask.hip", "page_select.hip"]
+           "norm_rope.hip", "attn_weights.hip", "evict.hip", "pages.hip", "tree_mask.hip",
+           "attn_tree.hip", "page_select.hip"]
 FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -1299,11 +1299,9 @@ extern "C" int oscar_attn_plan_v1(const int32_t* qsl, const int32_t* seqs, int32
   return (int)nitems;
 }
 
-namespace {
-
 // Argument checks of a non-empty plan that do not depend on where the item partials
 // go; `name` prefixes the messages.
-int check_args(const oscar_attn_args_v1& a, const char* name) {
+int oscar::attn_check_args(const oscar_attn_args_v1& a, const char* name) {
   const int64_t D = a.cache.head_dim;
   if (D != 128 && D != 256) return fail(-22, "%s: head_dim %lld unsupported", name, (long long)D);
   if (!a.q || !a.items || !a.groups || !a.out_rot || !a.lse || !a.block_table || !a.query_start_loc ||
@@ -1339,6 +1337,8 @@ int check_args(const oscar_attn_args_v1& a, const char* name) {
   return 0;
 }
 
+namespace {
+
 // what the tree and the selected entry points see of the cache and the chunk (AttnParams)
 struct View {
   int64_t table_head = 0;
@@ -1365,7 +1365,7 @@ int launch_checked(const oscar_attn_args_v1& a, const char* name, void* partials
     StoreParams sp{};
     return store != nullptr ? store_launch(store, s, false, name, &sp) : 0;
   }
-  if (const int rc = check_args(a, name)) return rc;
+  if (const int rc = attn_check_args(a, name)) return rc;
   if (!partials) return fail(-22, "%s: missing workspace", name);
   const int64_t need = (int64_t)a.num_items * 32 * (D + 1) * (int64_t)sizeof(float);
   if (partial_bytes < need)
@@ -1435,14 +1435,16 @@ extern "C" int oscarop_attn_decode_v1(const oscar_attn_args_v1* args, const osca
                         score);
 }
 
-extern "C" int oscarop_attn_tree_v1(const oscar_attn_args_v1* args, const oscarop_score_v1* score, const int64_t* mask,
+extern "C" int oscarop_attn_masked_v1(const oscar_attn_args_v1* args, const oscarop_score_v1* score, const int64_t* mask,
+                                    int64_t mask_words, void* stream);
+extern "C" int oscarop_attn_masked_v1(const oscar_attn_args_v1* args, const oscarop_score_v1* score, const int64_t* mask,
                                     int64_t mask_words, void* stream) {
-  if (!args) return fail(-22, "oscarop_attn_tree_v1: null args");
-  if (score && score->alibi_slopes) return fail(-22, "oscarop_attn_tree_v1: no alibi_slopes with a mask");
+  if (!args) return fail(-22, "oscarop_attn_masked_v1: null args");
+  if (score && score->alibi_slopes) return fail(-22, "oscarop_attn_masked_v1: no alibi_slopes with a mask");
   if (args->num_items > 0 && (!mask || ((uintptr_t)mask & 7) || mask_words < 1 || mask_words > 1 << 20))
-    return fail(-22, "oscarop_attn_tree_v1: a mask of at least one word a row, 8-byte aligned");
-  if (args->num_items > 0 && !args->k_new) return fail(-22, "oscarop_attn_tree_v1: a mask needs the chunk's keys");
-  return launch_checked(*args, "oscarop_attn_tree_v1", args->workspace, args->workspace_bytes, (hipStream_t)stream, score,
+    return fail(-22, "oscarop_attn_masked_v1: a mask of at least one word a row, 8-byte aligned");
+  if (args->num_items > 0 && !args->k_new) return fail(-22, "oscarop_attn_masked_v1: a mask needs the chunk's keys");
+  return launch_checked(*args, "oscarop_attn_masked_v1", args->workspace, args->workspace_bytes, (hipStream_t)stream, score,
                         nullptr, nullptr, View{0, (const uint64_t*)mask, mask_words});
 }
 
@@ -1477,7 +1479,7 @@ extern "C" int oscar_attn_decode_static_v1(const oscar_attn_args_v1* args, void*
     return fail(-22, "oscar_attn_decode_static_v1: %d items exceed the static scratch (at most %d)",
                 args->num_items, OSCAR_DECODE_STATIC_MAX_ITEMS);
   if (args->num_items <= 0 || args->num_groups <= 0) return 0;
-  if (const int rc = check_args(*args, "oscar_attn_decode_static_v1")) return rc;
+  if (const int rc = attn_check_args(*args, "oscar_attn_decode_static_v1")) return rc;
   void* partials = nullptr;
   const int rc = static_partials((hipStream_t)stream, &partials);
   if (rc != 0) return rc;

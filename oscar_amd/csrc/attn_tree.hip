@@ -1,0 +1,615 @@
+// Attention of drafted trees over the packed INT2 history (gfx950).
+//
+// A request of n nodes has M = n G rows per KV head (G query heads each), which all see its
+// history; among each other nodes see by a mask.  The split-K decode (attn_decode.hip) takes 32 rows
+// a wave and unpacks the codes for each of them anew, which its vector unit pays for: two
+// thirds of a tile's time.  Here a workgroup of four waves holds up to 256 rows, and unpacks a tile of
+// keys once for all of them, into LDS.
+//
+// Work: the plan (oscarop_tree_plan_v1) cuts M into blocks of 64 RT rows, RT <= 4, and
+// deals each block's tiles of KT keys (history tiles, then chunk tiles) round-robin to items,
+// one workgroup each.  Wave w holds rows [16 RT w, 16 RT (w + 1)) of the block: their queries (B
+// operands) and O^T in registers.  For a tile t, with 16x16x32 MFMA,
+//   S^T(t) = K(t) Q^T,   P(t) = exp2(scale S - m),   O^T += V(t)^T P(t)^T;
+// S^T's layout (lane: a row, four keys) is already that of the B operand of P.
+//
+// The loop is two phases that give the matrix unit and the vector unit something to do at
+// the same time: S(t) with the softmax of S(t - 1), then O += V(t - 1) P(t - 1) with the
+// unpacking of tile t + 1; the codes of tile t + 2 are on their way.  So K has two buffers in
+// LDS and V three, and one barrier a tile does.
+//
+// LDS: K in operand order, 16 bytes a lane.  V one row per key, 32 elements of padding, its
+// 16-byte units exchanged by the key's bits 2 and 3: rows then spread over all banks, for the
+// stores of a key per lane as for the transposing reads of a column per lane.
+//
+// Values: K is the reference's bf16 or fp16 of fp16(code * scale + zero), V fp16(...)
+// unrounded, the window's FP32 copies likewise; P fp16, up to 2^15, the reference m 2^7 below the
+// largest score at its last move, so that keys of 2^-21 of the largest still keep 11 bits.  The chunk's
+// V in bf16 have a wider range than fp16: chunk tiles multiply it by P in two bf16 parts.
+#include <vector>
+
+#include "common.h"
+#include "int2_tile.h"
+#include "score.h"
+
+namespace oscar {
+
+namespace {
+
+constexpr int kWaves = 8;        // two a SIMD
+constexpr int kThreads = 64 * kWaves;
+constexpr int kMostRows = 32 * kWaves;  // of a workgroup
+constexpr int kMostTiles = 512;  // of an item
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kBelow = 7.f;    // the reference below the maximum where it moves to,
+constexpr float kMost = 15.f;    // and how far above it a score may come (log2 units)
+typedef short __attribute__((ext_vector_type(4))) i16x4;
+
+template <int D>
+struct Cfg {
+  static constexpr int KT = 8192 / D;        // keys of a tile: two dwords of codes a thread
+  static constexpr int KSTEPS = D / 16;      // QK contraction steps
+  static constexpr int KSUB = KT / 32;       // 32-key parts of a tile
+  static constexpr int VSTEPS = KT / 16;     // PV contraction steps
+  static constexpr int NB = D / 32;          // 32-wide parts of O^T
+  static constexpr int VROW = D + 32;        // elements of a row of V in LDS
+  static constexpr int KBYTES = KT * D * 2;
+  static constexpr int VBYTES = KT * VROW * 2;
+};
+
+struct TreeParams {
+  oscarop_tree_attn_args_v1 a;
+  oscar_staging_v1 st;
+  int has_stage;
+  int group;
+  float* part_o;    // [partial rows][D], columns in LDS order
+  float* part_lse;  // [partial rows], log2 units
+  Score sc;
+};
+
+// elements (e0, e4) (e1, e5) (e2, e6) (e3, e7) of eight: the order in which codes are looked up
+__device__ __forceinline__ u32x4 kpairs8(const u32x4& x) {
+  return u32x4{__builtin_amdgcn_perm(x[2], x[0], 0x05040100u), __builtin_amdgcn_perm(x[2], x[0], 0x07060302u),
+               __builtin_amdgcn_perm(x[3], x[1], 0x05040100u), __builtin_amdgcn_perm(x[3], x[1], 0x07060302u)};
+}
+
+struct Item {
+  int req, kvh, qa, n, hist, row0, rows, first, stride, count, part;
+};
+
+// where 32 tokens lie: their page, the offset of the first in it, and its seat in the window
+struct Place {
+  int page, off, seat, pad;
+};
+
+template <int D, int QT, int SC>
+__global__ __launch_bounds__(kThreads, 2) void tree_main_kernel(TreeParams P) {
+  using C = Cfg<D>;
+  const oscarop_tree_attn_args_v1& T = P.a;
+  const oscar_attn_args_v1& A = T.attn;
+  const int32_t* it = A.items + (int64_t)blockIdx.x * OSCAROP_TREE_ITEM_INTS;
+  const Item I{it[0], it[1], it[2], it[3], it[4], it[5], it[6], it[7], it[8], it[9], it[10]};
+  const int bs = (int)A.cache.block_size, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = P.group;
+  const int htiles = (int)(((int64_t)I.hist + C::KT - 1) / C::KT);
+  const int64_t tiles = htiles + ((int64_t)I.n + C::KT - 1) / C::KT;
+  // an item that breaks the plan's rules reads nothing; its rows become NaN where they lie in
+  // the partials at all
+  if (I.rows < 1 || I.rows > kMostRows || I.part < 0 || (int64_t)I.part + I.rows > T.partial_rows) return;
+  if (I.req < 0 || I.req >= A.num_reqs || I.kvh < 0 || I.kvh >= A.cache.num_kv_heads || I.n < 1 || I.hist < 0 || I.qa < 0 ||
+      (int64_t)I.qa + I.n > A.num_tokens || I.row0 < 0 || (int64_t)I.row0 + I.rows > (int64_t)I.n * G || I.first < 0 ||
+      I.stride < 1 || I.count < 1 || I.count > kMostTiles || I.first + (int64_t)I.stride * (I.count - 1) >= tiles ||
+      (I.hist > 0 && (I.hist - 1) / bs >= A.block_table_cols)) {
+    for (int i = tid; i < I.rows; i += kThreads) P.part_lse[I.part + i] = NAN;
+    return;
+  }
+  __shared__ __attribute__((aligned(16))) uint8_t s_k[2 * C::KBYTES];
+  __shared__ __attribute__((aligned(16))) uint8_t s_v[2 * C::VBYTES];
+  __shared__ Place s_place[kMostTiles * C::KSUB];
+  for (int i = tid; i < I.count * C::KSUB; i += kThreads) {
+    const int64_t key = (int64_t)(I.first + I.stride * (i / C::KSUB)) * C::KT + 32 * (i % C::KSUB);
+    Place x{0, 0, 0, 0};
+    if (key < I.hist) {
+      x.page = A.block_table[(int64_t)I.req * A.block_table_stride + key / bs];
+      x.page = x.page < 0 || x.page >= A.cache.num_blocks ? 0 : x.page;
+      x.off = (int)(key % bs);
+      if (P.has_stage) x.seat = (int)((unsigned)x.page % (unsigned)P.st.rows) * bs + x.off;
+    }
+    s_place[i] = x;
+  }
+
+  // ---- this lane's row and its queries: half g of a step holds 8 of its 16 elements
+  const int m = lane & 31, g = lane >> 5;
+  const int row = 32 * wave + m;
+  const bool active = 32 * wave < I.rows;  // the wave has rows
+  int node = -1;
+  u32x4 q[C::KSTEPS];
+  {
+    const bool ok = row < I.rows;
+    const int mm = I.row0 + (ok ? row : 0);
+    if (ok) node = mm / G;
+    const uint16_t* src = (const uint16_t*)A.q + (int64_t)(I.qa + mm / G) * A.q_stride_token + (int64_t)(I.kvh * G + mm % G) * D;
+#pragma unroll
+    for (int ks = 0; ks < C::KSTEPS; ++ks) {
+      q[ks] = kpairs8(*(const u32x4*)(src + 16 * ks + 8 * g));
+      if (!ok) q[ks] = u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+
+  // ---- filling: waves 0 to 3 the keys, 4 to 7 the values; thread (token, 32 codes)
+  const bool vside = wave >= 4;
+  const int idx = tid & 255;
+  const int tok = idx % C::KT, vec = idx / C::KT, sub = tok >> 5, in32 = tok & 31;
+  const uint8_t* kbase = A.cache.k + (int64_t)I.kvh * A.cache.k_stride[2];
+  const uint8_t* cbase = vside ? A.cache.v + (int64_t)I.kvh * A.cache.v_stride[2] : kbase + 32;
+  const int64_t ks0 = A.cache.k_stride[0], ks1 = A.cache.k_stride[1];
+  const int64_t cs0 = vside ? A.cache.v_stride[0] : ks0, cs1 = vside ? A.cache.v_stride[1] : ks1;
+  u32x2 codes = {0u, 0u};
+  unsigned meta = 0;
+  int tag = -1, page = 0, seat = 0;
+  auto load_at = [&](const Place& x, int off) {
+    page = x.page;
+    seat = x.seat + off - x.off;
+    codes = *(const u32x2*)(cbase + (int64_t)page * cs0 + (int64_t)off * cs1 + 8 * vec);
+    meta = *(const unsigned*)(kbase + (int64_t)page * ks0 + (int64_t)off * ks1 + (vside ? 4 : 0));
+    tag = P.has_stage ? ((const int32_t*)P.st.owner)[2 * (int64_t)seat] : -1;
+  };
+  // the item's first `fast` tiles are full ones of the history
+  const int full = I.hist / C::KT;
+  int fast = full > I.first ? (full - I.first + I.stride - 1) / I.stride : 0;
+  fast = fast < I.count ? fast : I.count;
+  auto load = [&](int j) {
+    const Place x = s_place[(j < fast ? j : fast - 1) * C::KSUB + sub];
+    load_at(x, x.off + in32);
+  };
+  // where piece i (8 elements) of the thread's four goes
+  const int piece = vside ? 16 : 512, step = vside ? 32 : C::KSUB * 1024;
+  const int to = vside ? tok * (C::VROW * 2) + 64 * vec : (2 * vec * C::KSUB + sub) * 1024 + in32 * 16;
+  auto dest = [&](int i, int buf) -> u32x4* {
+    uint8_t* base = vside ? s_v + buf * C::VBYTES : s_k + buf * C::KBYTES;
+    return (u32x4*)(base + to + (i >> 1) * step + (i & 1) * piece);
+  };
+  auto fill_codes = [&](bool some, int buf) {
+    // both sides' tables, without a branch between the matrix instructions
+    unsigned t_lo, t_hi;
+    byte_tables<OSCAR_F16>(meta, t_lo, t_hi);
+    if constexpr (QT == OSCAR_BF16) {
+      unsigned k_lo, k_hi;
+      byte_tables<OSCAR_BF16>(meta, k_lo, k_hi);
+      t_lo = vside ? t_lo : k_lo;
+      t_hi = vside ? t_hi : k_hi;
+    }
+    if (!some) t_lo = t_hi = 0;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      unsigned o[8];
+      lut16(codes[c], t_lo, t_hi, o);
+      *dest(2 * c, buf) = u32x4{o[0], o[1], o[2], o[3]};
+      *dest(2 * c + 1, buf) = u32x4{o[4], o[5], o[6], o[7]};
+    }
+  };
+  // the window's copy of a token
+  auto fill_staged = [&](int buf) {
+    const f32x4* src = (const f32x4*)((vside ? P.st.stage_v : P.st.stage_k) + ((int64_t)seat * A.cache.num_kv_heads + I.kvh) * D + 32 * vec);
+#pragma unroll 2
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 a = src[2 * i], b = src[2 * i + 1];
+      u32x4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = vside ? hist_pair<OSCAR_F16>(a[e], b[e]) : hist_pair<QT>(a[e], b[e]);
+      *dest(i, buf) = o;
+    }
+  };
+  // tile t at once: the history's ragged end (unseen keys zero), or one of the chunk's
+  auto fill_slow = [&](int t, int j) {
+    const bool chunk = t >= htiles;
+    const int key = (chunk ? t - htiles : t) * C::KT + tok;
+    if (!chunk) {
+      const bool in = key < I.hist;
+      const Place x = s_place[j * C::KSUB + (in ? sub : 0)];
+      load_at(x, in ? x.off + in32 : x.off);
+      fill_codes(in, 0);
+      if (in && tag == page) fill_staged(0);
+      return;
+    }
+    const u32x4* src = (const u32x4*)((const uint16_t*)(vside ? A.v_new : A.k_new) + (int64_t)(I.qa + (key < I.n ? key : 0)) * A.kv_new_stride_token +
+                                      (int64_t)I.kvh * D + 32 * vec);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *dest(i, 0) = key < I.n ? kpairs8(src[i]) : u32x4{0u, 0u, 0u, 0u};
+  };
+
+  // ---- running state of this lane's row
+  float m_run = -INFINITY, l_run = 0.f;
+  f32x16 O[C::NB];
+#pragma unroll
+  for (int b = 0; b < C::NB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) O[b][r] = 0.f;
+  const float c_score = A.scale * kLog2e;
+  constexpr bool kScaled = SC == 2;  // the scores carry the scale already
+  f32x16 S[C::KSUB];
+  u32x4 ph[C::VSTEPS];
+
+  auto qk = [&](int buf) {
+    const u32x4* src = (const u32x4*)(s_k + buf * C::KBYTES) + lane;
+#pragma unroll
+    for (int a = 0; a < C::KSUB; ++a)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[a][r] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < C::KSTEPS; ++ks)
+#pragma unroll
+      for (int a = 0; a < C::KSUB; ++a) S[a] = mma16<QT>(src[(ks * C::KSUB + a) * 64], q[ks], S[a]);
+    if constexpr (SC == 2) {
+#pragma unroll
+      for (int a = 0; a < C::KSUB; ++a)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[a][r] = capped2(P.sc, S[a][r]);
+    }
+  };
+  // unseen keys of a slow tile
+  auto mask = [&](int t) {
+    const int j0 = (t - htiles) * C::KT;  // a multiple of 32
+    const int left = I.hist - t * C::KT;  // keys of a history tile
+    uint64_t see = left >= 64 ? ~0ull : (1ull << (left > 0 ? left : 0)) - 1;
+    if (t >= htiles) {
+      see = 0;
+      if (node >= j0 && (j0 >> 6) < T.mask_words) {
+        see = (uint64_t)T.mask[(int64_t)(I.qa + node) * T.mask_words + (j0 >> 6)] >> (j0 & 63);
+        const int last = node - j0;  // no node after its own
+        if (last < 63) see &= (2ull << last) - 1;
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < C::KSUB; ++a)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (!((see >> (32 * a + out_tok(r, g))) & 1)) S[a][r] = -INFINITY;
+  };
+  // p = exp2(score - reference); the reference moves, and O with it, where a score comes 2^15 above it
+  auto softmax = [&]() {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int a = 0; a < C::KSUB; ++a)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[a][r]);
+    if (!kScaled) mx *= c_score;
+    mx = fmaxf(mx, swap_halves(mx));
+    const bool up = mx > m_run + kMost;
+    if (__builtin_expect_with_probability(__any(up) != 0, 0, 0.999)) {
+      const float to = up ? mx - kBelow : m_run;
+      const float f = !up ? 1.f : (m_run == -INFINITY ? 0.f : exp2f(m_run - to));
+      l_run *= f;
+      m_run = to;
+#pragma unroll
+      for (int b = 0; b < C::NB; ++b) {
+        O[b] *= f;
+        __builtin_amdgcn_sched_barrier(0);  // (not all of O in vector registers at a time)
+      }
+    }
+    const float nm = m_run == -INFINITY ? 0.f : -m_run;
+    float sum = 0.f;
+#pragma unroll
+    for (int a = 0; a < C::KSUB; ++a)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = __builtin_amdgcn_exp2f(kScaled ? S[a][r] + nm : fmaf(S[a][r], c_score, nm));
+        S[a][r] = p;
+        sum += p;
+      }
+    l_run += sum;
+  };
+  auto half = [&]() {
+#pragma unroll
+    for (int s = 0; s < C::VSTEPS; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ph[s][e] = q_pair<OSCAR_F16>(S[s >> 1][8 * (s & 1) + 2 * e], S[s >> 1][8 * (s & 1) + 2 * e + 1]);
+  };
+  // the A operand of O^T's part b in step s: eight keys of column lane % 32
+  const int i16 = lane & 15, g16 = lane >> 4;
+  const int vat = (4 * (g16 >> 1) + (i16 >> 2)) * (C::VROW * 2) + 32 * (g16 & 1) + 8 * (i16 & 3);
+  auto vop = [&](int buf, int s, int b) {
+    u32x4 v;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const u32x2 t = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(
+                                                    s_v + buf * C::VBYTES + vat + (16 * s + 8 * h) * (C::VROW * 2) + 64 * b)));
+      v[2 * h] = t[0];
+      v[2 * h + 1] = t[1];
+    }
+    return v;
+  };
+  auto pv = [&](int buf) {
+#pragma unroll
+    for (int b = 0; b < C::NB; ++b)
+#pragma unroll
+      for (int s = 0; s < C::VSTEPS; ++s) O[b] = mma16<OSCAR_F16>(vop(buf, s, b), ph[s], O[b]);
+  };
+  // a chunk tile of bf16 values: P = hi + lo, both bf16
+  auto pv_chunk = [&](int buf) {
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+#pragma unroll
+      for (int s = 0; s < C::VSTEPS; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p0 = S[s >> 1][8 * (s & 1) + 2 * e], p1 = S[s >> 1][8 * (s & 1) + 2 * e + 1];
+          const unsigned hb = q_pair<OSCAR_BF16>(p0, p1);
+          ph[s][e] = hb;
+          S[s >> 1][8 * (s & 1) + 2 * e] = p0 - q_half<OSCAR_BF16>(hb, 0);
+          S[s >> 1][8 * (s & 1) + 2 * e + 1] = p1 - q_half<OSCAR_BF16>(hb, 1);
+        }
+#pragma unroll
+      for (int b = 0; b < C::NB; ++b)
+#pragma unroll
+        for (int s = 0; s < C::VSTEPS; ++s) O[b] = mma16<OSCAR_BF16>(vop(buf, s, b), ph[s], O[b]);
+    }
+  };
+
+  __syncthreads();  // s_place
+  // ---- full history tiles
+  if (fast > 0) {
+    load(0);
+    fill_codes(true, 0);
+    if (__builtin_expect(tag == page, 0)) fill_staged(0);
+    load(1);
+#pragma unroll 1
+    for (int j = 0; j < fast; ++j) {
+      __syncthreads();  // tile j is there, and tile j - 1 has been read
+      if (active) qk(j & 1);
+      fill_codes(true, (j + 1) & 1);
+      if (__builtin_expect(tag == page, 0)) fill_staged((j + 1) & 1);
+      load(j + 2);
+      if (active) {
+        softmax();
+        half();
+        pv(j & 1);
+      }
+    }
+  }
+  // ---- the others, one after the other
+  auto slow = [&](int j) {
+    const int t = I.first + I.stride * j;
+    __syncthreads();  // the buffers have been read
+    fill_slow(t, j);
+    __syncthreads();
+    qk(0);
+    mask(t);
+    softmax();
+  };
+  int j = fast;
+  if (j < I.count && I.first + I.stride * j < htiles) {  // the history's ragged end
+    slow(j++);
+    half();
+    pv(0);
+  }
+#pragma unroll 1
+  for (; j < I.count; ++j) {
+    slow(j);
+    if constexpr (QT == OSCAR_BF16) {
+      pv_chunk(0);
+    } else {
+      half();
+      pv(0);
+    }
+  }
+
+  // ---- the item's partial: O / l and the log-sum-exp
+  const float l = l_run + swap_halves(l_run);
+  if (row >= I.rows) return;
+  const float f = l > 0.f ? 1.f / l : (l != l ? NAN : 0.f);
+  float* out = P.part_o + (int64_t)(I.part + row) * D + 4 * g;
+#pragma unroll
+  for (int b = 0; b < C::NB; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      *(f32x4*)(out + 32 * b + 8 * e) = f32x4{O[b][4 * e], O[b][4 * e + 1], O[b][4 * e + 2], O[b][4 * e + 3]} * f;
+  if (g == 0) P.part_lse[I.part + row] = l != l ? NAN : (l > 0.f ? m_run + log2f(l) : -INFINITY);
+}
+
+// The items of a block of rows, merged by their log-sum-exps.  One row a 64-lane (D 256) or
+// 32-lane (D 128) group, four columns a lane.
+constexpr int kBatch = 8;
+constexpr int kMergeThreads = 256;
+
+template <int D>
+__global__ __launch_bounds__(kMergeThreads) void tree_merge_kernel(TreeParams P) {
+  const oscarop_tree_attn_args_v1& T = P.a;
+  const oscar_attn_args_v1& A = T.attn;
+  const int32_t* gr = A.groups + (int64_t)blockIdx.x * OSCAR_GROUP_INTS;
+  const int kvh = gr[0], qa = gr[1], row0 = gr[2], rows = gr[3], part = gr[4], many = gr[5], step = gr[6];
+  const int lanes = D / 4;
+  const int col = threadIdx.x % lanes, G = P.group;
+  const int row = blockIdx.y * (kMergeThreads / lanes) + threadIdx.x / lanes;
+  if (row >= rows) return;
+  const int m = row0 + row;
+  const int64_t token = (int64_t)qa + m / G;
+  if (row0 < 0 || kvh < 0 || kvh >= A.cache.num_kv_heads || qa < 0 || token >= A.num_tokens) return;
+  bool nan = part < 0 || many < 0 || step < rows || (int64_t)part + (int64_t)step * (many - 1) + rows > T.partial_rows;
+  const int n = nan ? 0 : many;
+  const float* lse = P.part_lse + part + row;
+  const f32x4* po = (const f32x4*)(P.part_o + (int64_t)(nan ? 0 : part + row) * D) + col;
+  float M = -INFINITY, L = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < n; i += kBatch) {
+    float l[kBatch];
+    f32x4 x[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const bool in = i + u < n;
+      l[u] = in ? lse[(int64_t)(i + u) * step] : -INFINITY;
+      x[u] = in ? po[(int64_t)(i + u) * step * (D / 4)] : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    float top = M;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      nan |= l[u] != l[u];
+      top = fmaxf(top, l[u]);
+    }
+    if (top == -INFINITY) continue;
+    const float f = M == -INFINITY ? 0.f : exp2f(M - top);
+    acc *= f;
+    L *= f;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const float w = l[u] == -INFINITY ? 0.f : exp2f(l[u] - top);
+      L += w;
+      acc += w > 0.f ? x[u] * w : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    M = top;
+  }
+  const bool some = M != -INFINITY && L > 0.f;
+  acc = nan ? f32x4{NAN, NAN, NAN, NAN} : (some ? acc * (1.f / L) : f32x4{0.f, 0.f, 0.f, 0.f});
+  const int head = kvh * G + m % G;
+  // columns 4 i .. 4 i + 3 of a part in LDS order are elements e, e + 4, e + 1, e + 5
+  const int e = 16 * (col / 4) + 8 * ((col & 3) >> 1) + 2 * (col & 1);
+  float* out = A.out_rot + (token * A.num_q_heads + head) * D + e;
+  *(float2*)out = make_float2(acc[0], acc[2]);
+  *(float2*)(out + 4) = make_float2(acc[1], acc[3]);
+  if (col == 0) A.lse[token * A.num_q_heads + head] = nan ? NAN : (some ? (M + log2f(L)) * kLn2 : -INFINITY);
+}
+
+template <int D>
+int launch_tree(const TreeParams& p, int sc, hipStream_t s) {
+  const oscar_attn_args_v1& a = p.a.attn;
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.num_items), dim3(kThreads), 0, s, p); };
+  const bool f16 = a.q_dtype == OSCAR_F16;
+  if (sc == 0) f16 ? launch(tree_main_kernel<D, OSCAR_F16, 0>) : launch(tree_main_kernel<D, OSCAR_BF16, 0>);
+  else f16 ? launch(tree_main_kernel<D, OSCAR_F16, 2>) : launch(tree_main_kernel<D, OSCAR_BF16, 2>);
+  OSCAR_CHECK_LAUNCH("tree_main_kernel");
+  constexpr int kRows = kMergeThreads / (D / 4);
+  hipLaunchKernelGGL(tree_merge_kernel<D>, dim3(a.num_groups, kMostRows / kRows), dim3(kMergeThreads), 0, s, p);
+  OSCAR_CHECK_LAUNCH("tree_merge_kernel");
+  return 0;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+struct Block {
+  int req, kvh, qa, n, hist, row0, rows, waves;
+  int64_t tiles;
+};
+
+}  // namespace
+
+}  // namespace oscar
+
+using namespace oscar;
+
+extern "C" int oscarop_tree_plan_v1(const int32_t* qsl, const int32_t* seqs, int32_t num_reqs, int32_t num_kv_heads, int32_t group,
+                                    int32_t head_dim, int32_t target_items, int32_t* items, int32_t max_items, int32_t* groups,
+                                    int32_t max_groups, oscarop_tree_sizes_v1* plan) try {
+  if (!qsl || !seqs || !plan || num_reqs < 0 || num_kv_heads < 1 || num_kv_heads > 0xffff || group < 1 || group > 1 << 16)
+    return fail(-22, "oscarop_tree_plan_v1: invalid arguments");
+  if (head_dim != 128 && head_dim != 256) return fail(-22, "oscarop_tree_plan_v1: head_dim %d unsupported (128/256)", head_dim);
+  const int kt = 8192 / head_dim;
+  if (target_items < 1) target_items = 1;
+  std::vector<Block> blocks;
+  for (int r = 0; r < num_reqs; ++r) {
+    const int64_t n = (int64_t)qsl[r + 1] - qsl[r];
+    if (n <= 0) continue;
+    if (qsl[r] < 0 || seqs[r] < n) return fail(-22, "oscarop_tree_plan_v1: sequence length must cover its query chunk");
+    const int64_t rows = n * group;
+    if (rows > 1 << 24) return fail(-22, "oscarop_tree_plan_v1: query chunk of request %d too long", r);
+    // as few blocks of at most kMostRows rows as there can be, alike
+    const int64_t count = ceil_div(rows, kMostRows), each = ceil_div(rows, count);
+    if ((int64_t)blocks.size() + count * num_kv_heads > 1 << 20)
+      return fail(-22, "oscarop_tree_plan_v1: too many request x kv-head groups");
+    for (int64_t a = 0; a < rows; a += each) {
+      const int64_t b = a + each < rows ? a + each : rows;
+      const int hist = seqs[r] - (int)n;
+      // the block's last node sees no later one
+      const int64_t tiles = ceil_div(hist, kt) + ceil_div((b - 1) / group + 1, kt);
+      for (int h = 0; h < num_kv_heads; ++h)
+        blocks.push_back({r, h, qsl[r], (int)n, hist, (int)a, (int)(b - a), (int)ceil_div(b - a, 32), tiles});
+    }
+  }
+  // an item costs its tiles, and a tile its rows and its unpacking; the smallest bound that keeps to
+  // target_items (one for each block at least)
+  auto split = [&](const Block& b, int64_t most) {
+    const int64_t cap = most / (b.waves + 2) < 1 ? 1 : (most / (b.waves + 2) > kMostTiles ? kMostTiles : most / (b.waves + 2));
+    return ceil_div(b.tiles, cap);
+  };
+  int64_t lo = 1, hi = (int64_t)(kWaves + 2) * kMostTiles;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) / 2;
+    int64_t total = 0;
+    for (const Block& b : blocks) total += split(b, mid);
+    if (total <= target_items) hi = mid;
+    else lo = mid + 1;
+  }
+  int64_t num = 0, part = 0, longest = 0;
+  for (const Block& b : blocks) {
+    const int64_t k = split(b, lo);
+    num += k;
+    part += k * b.rows;
+    longest = k > longest ? k : longest;
+  }
+  if (num > 1 << 24 || part > INT32_MAX) return fail(-22, "oscarop_tree_plan_v1: too many work items");
+  plan->num_items = (int32_t)num;
+  plan->num_groups = (int32_t)blocks.size();
+  plan->partial_rows = part;
+  plan->partial_bytes = part * (head_dim + 1) * (int64_t)sizeof(float);
+  if (items == nullptr || groups == nullptr) return (int)num;  // size query
+  if (num > max_items || (int64_t)blocks.size() > max_groups) return fail(-28, "oscarop_tree_plan_v1: buffers too small");
+  int64_t at = 0;
+  std::vector<int64_t> first(blocks.size());
+  for (size_t g = 0; g < blocks.size(); ++g) {
+    const Block& b = blocks[g];
+    first[g] = at;
+    int32_t* gr = groups + g * OSCAR_GROUP_INTS;
+    const int64_t k = split(b, lo);
+    const int32_t record[OSCAR_GROUP_INTS] = {b.kvh, b.qa, b.row0, b.rows, (int32_t)at, (int32_t)k, b.rows, 0};
+    for (int i = 0; i < OSCAR_GROUP_INTS; ++i) gr[i] = record[i];
+    at += k * b.rows;
+  }
+  // item p of every block, then p + 1: blocks progress together
+  int64_t out = 0;
+  for (int64_t p = 0; p < longest; ++p)
+    for (size_t g = 0; g < blocks.size(); ++g) {
+      const Block& b = blocks[g];
+      const int64_t k = split(b, lo);
+      if (p >= k) continue;
+      int32_t* it = items + out++ * OSCAROP_TREE_ITEM_INTS;
+      const int32_t record[OSCAROP_TREE_ITEM_INTS] = {b.req, b.kvh, b.qa, b.n, b.hist, b.row0, b.rows, (int32_t)p,
+                                                      (int32_t)k, (int32_t)ceil_div(b.tiles - p, k),
+                                                      (int32_t)(first[g] + p * b.rows), 0};
+      for (int i = 0; i < OSCAROP_TREE_ITEM_INTS; ++i) it[i] = record[i];
+    }
+  return (int)num;
+} catch (const std::bad_alloc&) {
+  return fail(-12, "oscarop_tree_plan_v1: out of memory");
+}
+
+extern "C" int oscarop_attn_tree_v1(const oscarop_tree_attn_args_v1* args, const oscarop_score_v1* score, void* stream) {
+  const char* name = "oscarop_attn_tree_v1";
+  if (!args) return fail(-22, "%s: null args", name);
+  const oscar_attn_args_v1& a = args->attn;
+  TreeParams p{};
+  const int sc = score_of(score, a.scale, &p.sc);
+  if (sc < 0) return fail(-22, kBadCap, name);
+  if (p.sc.slopes != nullptr) return fail(-22, "%s: no alibi_slopes with a mask", name);
+  const int64_t d = a.cache.head_dim;
+  if (d != 128 && d != 256) return fail(-22, "%s: head_dim %lld unsupported", name, (long long)d);
+  if (a.num_items <= 0 || a.num_groups <= 0) return 0;
+  if (const int rc = attn_check_args(a, name)) return rc;
+  if (a.phases != 0) return fail(-22, "%s: phases must be 0", name);
+  if (!a.k_new) return fail(-22, "%s: a tree's attention needs its nodes' K and V", name);
+  if (!args->mask || ((uintptr_t)args->mask & 7) || args->mask_words < 1)
+    return fail(-22, "%s: a mask of at least one word a row, 8-byte aligned", name);
+  if (a.num_q_heads / a.cache.num_kv_heads > 1 << 16 || a.cache.num_kv_heads > 0xffff || a.num_groups > 1 << 20)
+    return fail(-22, "%s: too many heads or groups", name);
+  const int64_t need = args->partial_rows * (d + 1) * (int64_t)sizeof(float);
+  if (args->partial_rows < 1 || args->partial_rows > INT32_MAX || !a.workspace || ((uintptr_t)a.workspace & 15) ||
+      a.workspace_bytes < need)
+    return fail(-22, "%s: workspace of %lld bytes < %lld", name, (long long)a.workspace_bytes, (long long)need);
+  p.a = *args;
+  p.has_stage = a.staging != nullptr;
+  if (a.staging) p.st = *a.staging;
+  p.group = (int)(a.num_q_heads / a.cache.num_kv_heads);
+  p.part_o = (float*)a.workspace;
+  p.part_lse = p.part_o + args->partial_rows * d;
+  return d == 256 ? launch_tree<256>(p, sc, (hipStream_t)stream) : launch_tree<128>(p, sc, (hipStream_t)stream);
+}

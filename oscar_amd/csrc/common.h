@@ -29,6 +29,9 @@ int fail(int code, const char* fmt, ...);
                                                hipGetErrorString(e_));            \
   } while (0)
 
+// the argument checks that the attention entry points over the cache share (attn_decode.hip)
+int attn_check_args(const oscar_attn_args_v1& a, const char* name);
+
 // ---------------------------------------------------------------- strided rows on the host
 // [outer][inner] rows of `cols` elements, either axis the outer one
 struct Rows2 {

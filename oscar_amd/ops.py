@@ -1107,16 +1107,49 @@ def tree_mask(parents, qsl, *, max_nodes: int) -> tuple:
     return mask, depths
 
 
-def plan_tree(qsl, seqs, *, num_kv_heads: int, group: int, head_dim: int, device, window: tuple = (0, 0)) -> DecodePlan:
+@dataclass
+class TreePlan:
+    """A plan of attention_tree: the requests of a batch, host lists and device records."""
+    host_qsl: list
+    host_seqs: list
+    num_items: int
+    num_groups: int
+    partial_rows: int
+    partial_bytes: int
+    items: torch.Tensor     # device int32, as all of these
+    groups: torch.Tensor
+    qsl: torch.Tensor
+    seqs: torch.Tensor
+    has_new = True
+    max_group_items = 0
+
+
+def plan_tree(qsl, seqs, *, num_kv_heads: int, group: int, head_dim: int, device, window: tuple = (0, 0)) -> TreePlan:
     """Plan of attention_tree over a batch: request r's rows [qsl[r], qsl[r + 1]) are the nodes of
     its tree, seqs[r] its length with them (host lists); sizes and window as plan_decode."""
     qsl, seqs = _request_lists(qsl, seqs, True)
-    return plan_decode(qsl, seqs, has_new=True, num_kv_heads=num_kv_heads, group=group, head_dim=head_dim, device=device,
-                       window=window)
+    lib, sizes, target = _lib.load(), _lib.TreeSizes(), cu_count(device)
+    qa, sa = (C.c_int32 * len(qsl))(*qsl), (C.c_int32 * max(len(seqs), 1))(*seqs)
+
+    def plan(items, groups):
+        i32p = C.POINTER(C.c_int32)
+        n = lib.oscarop_tree_plan_v1(qa, sa, len(seqs), num_kv_heads, group, head_dim, target,
+                                     None if items is None else items.ctypes.data_as(i32p), 0 if items is None else items.shape[0],
+                                     None if groups is None else groups.ctypes.data_as(i32p),
+                                     0 if groups is None else groups.shape[0], C.byref(sizes))
+        if n < 0:
+            _lib.check(n, "oscarop_tree_plan_v1")
+
+    plan(None, None)
+    items = np.zeros((max(sizes.num_items, 1), _lib.TREE_ITEM_INTS), np.int32)
+    groups = np.zeros((max(sizes.num_groups, 1), GROUP_INTS), np.int32)
+    plan(items, groups)
+    parts = upload([items.reshape(-1), groups.reshape(-1), np.asarray(qsl, np.int32), np.asarray(seqs or [0], np.int32)], device)
+    return TreePlan(qsl, seqs, sizes.num_items, sizes.num_groups, sizes.partial_rows, sizes.partial_bytes, *parts)
 
 
 def _attention_over(entry, q, k_new, v_new, k_cache, v_cache, table, rows_of_table, plan, scale, stage, head_dim, soft_cap,
-                    out_rot, lse, others, extra):
+                    out_rot, lse, others, extra=(), mask=None):
     """The entry points beside attention_decode, which take its arguments and `extra` ones.
     table: [requests, columns] as the kernels address it; others: more tensors of the call."""
     index = _device_index(q, k_new, v_new, k_cache, v_cache, table, out_rot, lse, *others, *(stage or ()))
@@ -1169,11 +1202,13 @@ def _attention_over(entry, q, k_new, v_new, k_cache, v_cache, table, rows_of_tab
                       plan.items.data_ptr(), plan.num_items, plan.groups.data_ptr(), plan.num_groups, ws.data_ptr(),
                       ws.numel(), plan.max_group_items, out_rot.data_ptr(), lse.data_ptr(), 0, code, table.shape[0],
                       rows_of_table)
+    if mask is not None:
+        a = _lib.TreeAttnArgs(a, mask.data_ptr(), mask.shape[1], plan.partial_rows)
     _launch(entry, index, C.byref(a), None if score is None else C.byref(score), *extra)
     return out_rot, lse
 
 
-def attention_tree(q, k_new, v_new, k_cache, v_cache, block_table, plan: DecodePlan, mask, scale, stage=None, *, head_dim,
+def attention_tree(q, k_new, v_new, k_cache, v_cache, block_table, plan: TreePlan, mask, scale, stage=None, *, head_dim,
                    soft_cap=0.0, out_rot=None, lse=None):
     """Attention of drafted trees over the INT2 history: (out_rot fp32, lse fp32), rotated, as
     attention_decode's, whose arguments these are.
@@ -1194,7 +1229,7 @@ def attention_tree(q, k_new, v_new, k_cache, v_cache, block_table, plan: DecodeP
     if table.ndim != 2:
         raise ValueError("Missing request block-table rows")
     return _attention_over("oscarop_attn_tree_v1", q, k_new, v_new, k_cache, v_cache, table, table.shape[1], plan, scale,
-                           stage, head_dim, soft_cap, out_rot, lse, (mask, plan.items), (mask.data_ptr(), mask.shape[1]))
+                           stage, head_dim, soft_cap, out_rot, lse, (mask, plan.items), mask=mask)
 
 
 # ------------------------------------------------------------------------ chosen pages
