@@ -40,6 +40,8 @@ constexpr int kWaves = 8;        // two a SIMD
 constexpr int kThreads = 64 * kWaves;
 constexpr int kMostRows = 32 * kWaves;  // of a workgroup
 constexpr int kMostTiles = 512;  // of an item
+constexpr int kAhead = 3, kAheadV = 3;  // operands of products read ahead
+constexpr int kSlowCost = 3;      // a slow tile's time in full ones
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kBelow = 7.f;    // the reference below the maximum where it moves to,
@@ -83,42 +85,17 @@ struct Place {
   int page, off, seat, pad;
 };
 
-template <int D, int QT, int SC>
-__global__ __launch_bounds__(kThreads, 2) void tree_main_kernel(TreeParams P) {
+// The tiles of one item: full ones of the history, or (SLOW) its ragged end and the chunk's.  Apart, since
+// what the latter need does not fit beside O and the queries in the others' loop.
+template <int D, int QT, int SC, bool SLOW>
+__device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uint8_t* s_k, uint8_t* s_v, const Place* s_place) {
   using C = Cfg<D>;
   const oscarop_tree_attn_args_v1& T = P.a;
   const oscar_attn_args_v1& A = T.attn;
-  const int32_t* it = A.items + (int64_t)blockIdx.x * OSCAROP_TREE_ITEM_INTS;
-  const Item I{it[0], it[1], it[2], it[3], it[4], it[5], it[6], it[7], it[8], it[9], it[10]};
-  const int bs = (int)A.cache.block_size, tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = P.group;
   const int htiles = (int)(((int64_t)I.hist + C::KT - 1) / C::KT);
-  const int64_t tiles = htiles + ((int64_t)I.n + C::KT - 1) / C::KT;
-  // an item that breaks the plan's rules reads nothing; its rows become NaN where they lie in
-  // the partials at all
-  if (I.rows < 1 || I.rows > kMostRows || I.part < 0 || (int64_t)I.part + I.rows > T.partial_rows) return;
-  if (I.req < 0 || I.req >= A.num_reqs || I.kvh < 0 || I.kvh >= A.cache.num_kv_heads || I.n < 1 || I.hist < 0 || I.qa < 0 ||
-      (int64_t)I.qa + I.n > A.num_tokens || I.row0 < 0 || (int64_t)I.row0 + I.rows > (int64_t)I.n * G || I.first < 0 ||
-      I.stride < 1 || I.count < 1 || I.count > kMostTiles || I.first + (int64_t)I.stride * (I.count - 1) >= tiles ||
-      (I.hist > 0 && (I.hist - 1) / bs >= A.block_table_cols)) {
-    for (int i = tid; i < I.rows; i += kThreads) P.part_lse[I.part + i] = NAN;
-    return;
-  }
-  __shared__ __attribute__((aligned(16))) uint8_t s_k[2 * C::KBYTES];
-  __shared__ __attribute__((aligned(16))) uint8_t s_v[2 * C::VBYTES];
-  __shared__ Place s_place[kMostTiles * C::KSUB];
-  for (int i = tid; i < I.count * C::KSUB; i += kThreads) {
-    const int64_t key = (int64_t)(I.first + I.stride * (i / C::KSUB)) * C::KT + 32 * (i % C::KSUB);
-    Place x{0, 0, 0, 0};
-    if (key < I.hist) {
-      x.page = A.block_table[(int64_t)I.req * A.block_table_stride + key / bs];
-      x.page = x.page < 0 || x.page >= A.cache.num_blocks ? 0 : x.page;
-      x.off = (int)(key % bs);
-      if (P.has_stage) x.seat = (int)((unsigned)x.page % (unsigned)P.st.rows) * bs + x.off;
-    }
-    s_place[i] = x;
-  }
 
   // ---- this lane's row and its queries: half g of a step holds 8 of its 16 elements
   const int m = lane & 31, g = lane >> 5;
@@ -156,31 +133,22 @@ __global__ __launch_bounds__(kThreads, 2) void tree_main_kernel(TreeParams P) {
     meta = *(const unsigned*)(kbase + (int64_t)page * ks0 + (int64_t)off * ks1 + (vside ? 4 : 0));
     tag = P.has_stage ? ((const int32_t*)P.st.owner)[2 * (int64_t)seat] : -1;
   };
-  // the item's first `fast` tiles are full ones of the history
-  const int full = I.hist / C::KT;
-  int fast = full > I.first ? (full - I.first + I.stride - 1) / I.stride : 0;
-  fast = fast < I.count ? fast : I.count;
   auto load = [&](int j) {
-    const Place x = s_place[(j < fast ? j : fast - 1) * C::KSUB + sub];
+    const Place x = s_place[(j < I.count ? j : I.count - 1) * C::KSUB + sub];
     load_at(x, x.off + in32);
   };
   // where piece i (8 elements) of the thread's four goes
-  const int piece = vside ? 16 : 512, step = vside ? 32 : C::KSUB * 1024;
+  // (a row of values has its 16-byte units exchanged, within four, by the key's bits 2 and 3)
   const int to = vside ? tok * (C::VROW * 2) + 64 * vec : (2 * vec * C::KSUB + sub) * 1024 + in32 * 16;
+  const int turn = (tok >> 2) & 3;
   auto dest = [&](int i, int buf) -> u32x4* {
-    uint8_t* base = vside ? s_v + buf * C::VBYTES : s_k + buf * C::KBYTES;
-    return (u32x4*)(base + to + (i >> 1) * step + (i & 1) * piece);
+    if (vside) return (u32x4*)(s_v + buf * C::VBYTES + to + 16 * (i ^ turn));
+    return (u32x4*)(s_k + buf * C::KBYTES + to + (i >> 1) * (C::KSUB * 1024) + (i & 1) * 512);
   };
   auto fill_codes = [&](bool some, int buf) {
-    // both sides' tables, without a branch between the matrix instructions
     unsigned t_lo, t_hi;
-    byte_tables<OSCAR_F16>(meta, t_lo, t_hi);
-    if constexpr (QT == OSCAR_BF16) {
-      unsigned k_lo, k_hi;
-      byte_tables<OSCAR_BF16>(meta, k_lo, k_hi);
-      t_lo = vside ? t_lo : k_lo;
-      t_hi = vside ? t_hi : k_hi;
-    }
+    if (QT == OSCAR_F16 || vside) byte_tables<OSCAR_F16>(meta, t_lo, t_hi);
+    else byte_tables<OSCAR_BF16>(meta, t_lo, t_hi);
     if (!some) t_lo = t_hi = 0;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -242,6 +210,13 @@ __global__ __launch_bounds__(kThreads, 2) void tree_main_kernel(TreeParams P) {
     for (int ks = 0; ks < C::KSTEPS; ++ks)
 #pragma unroll
       for (int a = 0; a < C::KSUB; ++a) S[a] = mma16<QT>(src[(ks * C::KSUB + a) * 64], q[ks], S[a]);
+    // operands three products ahead: all of them at once do not fit beside O and the queries
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < C::KSTEPS * C::KSUB; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
     if constexpr (SC == 2) {
 #pragma unroll
       for (int a = 0; a < C::KSUB; ++a)
@@ -309,13 +284,14 @@ __global__ __launch_bounds__(kThreads, 2) void tree_main_kernel(TreeParams P) {
   };
   // the A operand of O^T's part b in step s: eight keys of column lane % 32
   const int i16 = lane & 15, g16 = lane >> 4;
-  const int vat = (4 * (g16 >> 1) + (i16 >> 2)) * (C::VROW * 2) + 32 * (g16 & 1) + 8 * (i16 & 3);
+  const int vrow = (4 * (g16 >> 1) + (i16 >> 2)) * (C::VROW * 2) + 8 * (i16 & 1), unit = 2 * (g16 & 1) + ((i16 & 3) >> 1);
+  const int vat0 = vrow + 16 * (unit ^ (g16 >> 1)), vat1 = vrow + 16 * (unit ^ (2 + (g16 >> 1)));
   auto vop = [&](int buf, int s, int b) {
     u32x4 v;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const u32x2 t = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(
-                                                    s_v + buf * C::VBYTES + vat + (16 * s + 8 * h) * (C::VROW * 2) + 64 * b)));
+                                                    s_v + buf * C::VBYTES + (h ? vat1 : vat0) + (16 * s + 8 * h) * (C::VROW * 2) + 64 * b)));
       v[2 * h] = t[0];
       v[2 * h + 1] = t[1];
     }
@@ -326,6 +302,12 @@ __global__ __launch_bounds__(kThreads, 2) void tree_main_kernel(TreeParams P) {
     for (int b = 0; b < C::NB; ++b)
 #pragma unroll
       for (int s = 0; s < C::VSTEPS; ++s) O[b] = mma16<OSCAR_F16>(vop(buf, s, b), ph[s], O[b]);
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAheadV, 1);
+#pragma unroll
+    for (int i = 0; i < C::NB * C::VSTEPS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+    }
   };
   // a chunk tile of bf16 values: P = hi + lo, both bf16
   auto pv_chunk = [&](int buf) {
@@ -349,50 +331,58 @@ __global__ __launch_bounds__(kThreads, 2) void tree_main_kernel(TreeParams P) {
   };
 
   __syncthreads();  // s_place
-  // ---- full history tiles
-  if (fast > 0) {
+  if constexpr (!SLOW) {
     load(0);
     fill_codes(true, 0);
     if (__builtin_expect(tag == page, 0)) fill_staged(0);
     load(1);
 #pragma unroll 1
-    for (int j = 0; j < fast; ++j) {
+    for (int j = 0; j < I.count; ++j) {
       __syncthreads();  // tile j is there, and tile j - 1 has been read
-      if (active) qk(j & 1);
-      fill_codes(true, (j + 1) & 1);
-      if (__builtin_expect(tag == page, 0)) fill_staged((j + 1) & 1);
-      load(j + 2);
+      auto next = [&]() {
+        fill_codes(true, (j + 1) & 1);
+        if (__builtin_expect(tag == page, 0)) fill_staged((j + 1) & 1);
+        load(j + 2);
+        __builtin_amdgcn_sched_barrier(0);  // the scores and what unpacking takes share registers
+      };
+      // The two waves of a SIMD out of step: one unpacks before its products, the other after
+      if (!vside) next();
       if (active) {
+        qk(j & 1);
+        __builtin_amdgcn_sched_barrier(0);
         softmax();
         half();
+        __builtin_amdgcn_sched_barrier(0);
         pv(j & 1);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      if (vside) next();
     }
-  }
-  // ---- the others, one after the other
-  auto slow = [&](int j) {
-    const int t = I.first + I.stride * j;
-    __syncthreads();  // the buffers have been read
-    fill_slow(t, j);
-    __syncthreads();
-    qk(0);
-    mask(t);
-    softmax();
-  };
-  int j = fast;
-  if (j < I.count && I.first + I.stride * j < htiles) {  // the history's ragged end
-    slow(j++);
-    half();
-    pv(0);
-  }
-#pragma unroll 1
-  for (; j < I.count; ++j) {
-    slow(j);
-    if constexpr (QT == OSCAR_BF16) {
-      pv_chunk(0);
-    } else {
+  } else {
+    auto scores = [&](int j) {
+      const int t = I.first + I.stride * j;
+      if (j > 0) __syncthreads();  // the buffers have been read
+      fill_slow(t, j);
+      __syncthreads();
+      qk(0);
+      mask(t);
+      softmax();
+    };
+    int j = 0;
+    if (I.first < htiles) {  // the ragged end
+      scores(j++);
       half();
       pv(0);
+    }
+#pragma unroll 1
+    for (; j < I.count; ++j) {
+      scores(j);
+      if constexpr (QT == OSCAR_BF16) {
+        pv_chunk(0);
+      } else {
+        half();
+        pv(0);
+      }
     }
   }
 
@@ -407,6 +397,48 @@ __global__ __launch_bounds__(kThreads, 2) void tree_main_kernel(TreeParams P) {
     for (int e = 0; e < 4; ++e)
       *(f32x4*)(out + 32 * b + 8 * e) = f32x4{O[b][4 * e], O[b][4 * e + 1], O[b][4 * e + 2], O[b][4 * e + 3]} * f;
   if (g == 0) P.part_lse[I.part + row] = l != l ? NAN : (l > 0.f ? m_run + log2f(l) : -INFINITY);
+}
+
+template <int D, int QT, int SC>
+__global__ __launch_bounds__(kThreads, 2) void tree_main_kernel(TreeParams P) {
+  using C = Cfg<D>;
+  const oscarop_tree_attn_args_v1& T = P.a;
+  const oscar_attn_args_v1& A = T.attn;
+  const int32_t* it = A.items + (int64_t)blockIdx.x * OSCAROP_TREE_ITEM_INTS;
+  const Item I{it[0], it[1], it[2], it[3], it[4], it[5], it[6], it[7], it[8], it[9], it[10]};
+  const int bs = (int)A.cache.block_size, tid = threadIdx.x;
+  const int G = P.group;
+  const int htiles = (int)(((int64_t)I.hist + C::KT - 1) / C::KT);
+  const int64_t tiles = htiles + ((int64_t)I.n + C::KT - 1) / C::KT;
+  // an item that breaks the plan's rules reads nothing; its rows become NaN where they lie in
+  // the partials at all
+  if (I.rows < 1 || I.rows > kMostRows || I.part < 0 || (int64_t)I.part + I.rows > T.partial_rows) return;
+  if (I.req < 0 || I.req >= A.num_reqs || I.kvh < 0 || I.kvh >= A.cache.num_kv_heads || I.n < 1 || I.hist < 0 || I.qa < 0 ||
+      (int64_t)I.qa + I.n > A.num_tokens || I.row0 < 0 || (int64_t)I.row0 + I.rows > (int64_t)I.n * G || I.first < 0 ||
+      I.stride < 1 || I.count < 1 || I.count > kMostTiles || I.first + (int64_t)I.stride * (I.count - 1) >= tiles ||
+      (I.first < I.hist / C::KT && I.first + (int64_t)I.stride * (I.count - 1) >= I.hist / C::KT) ||
+      (I.hist > 0 && (I.hist - 1) / bs >= A.block_table_cols)) {
+    for (int i = tid; i < I.rows; i += kThreads) P.part_lse[I.part + i] = NAN;
+    return;
+  }
+  __shared__ __attribute__((aligned(16))) uint8_t s_k[2 * C::KBYTES];
+  __shared__ __attribute__((aligned(16))) uint8_t s_v[2 * C::VBYTES];
+  __shared__ Place s_place[kMostTiles * C::KSUB];
+  const int full = I.hist / C::KT;  // full tiles of the history
+  for (int i = tid; i < I.count * C::KSUB; i += kThreads) {
+    const int64_t key = (int64_t)(I.first + I.stride * (i / C::KSUB)) * C::KT + 32 * (i % C::KSUB);
+    Place x{0, 0, 0, 0};
+    if (key < I.hist) {
+      x.page = A.block_table[(int64_t)I.req * A.block_table_stride + key / bs];
+      x.page = x.page < 0 || x.page >= A.cache.num_blocks ? 0 : x.page;
+      x.off = (int)(key % bs);
+      if (P.has_stage) x.seat = (int)((unsigned)x.page % (unsigned)P.st.rows) * bs + x.off;
+    }
+    s_place[i] = x;
+  }
+
+  if (I.first >= full) run_item<D, QT, SC, true>(P, I, s_k, s_v, s_place);
+  else run_item<D, QT, SC, false>(P, I, s_k, s_v, s_place);
 }
 
 // The items of a block of rows, merged by their log-sum-exps.  One row a 64-lane (D 256) or
@@ -489,7 +521,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct Block {
   int req, kvh, qa, n, hist, row0, rows, waves;
-  int64_t tiles;
+  int64_t full, slow;  // tiles: full ones of the history; its ragged end and the chunk's
 };
 
 }  // namespace
@@ -521,18 +553,20 @@ extern "C" int oscarop_tree_plan_v1(const int32_t* qsl, const int32_t* seqs, int
       const int64_t b = a + each < rows ? a + each : rows;
       const int hist = seqs[r] - (int)n;
       // the block's last node sees no later one
-      const int64_t tiles = ceil_div(hist, kt) + ceil_div((b - 1) / group + 1, kt);
+      const int64_t slow = (hist % kt != 0) + ceil_div((b - 1) / group + 1, kt);
       for (int h = 0; h < num_kv_heads; ++h)
-        blocks.push_back({r, h, qsl[r], (int)n, hist, (int)a, (int)(b - a), (int)ceil_div(b - a, 32), tiles});
+        blocks.push_back({r, h, qsl[r], (int)n, hist, (int)a, (int)(b - a), (int)ceil_div(b - a, 32), hist / kt, slow});
     }
   }
-  // an item costs its tiles, and a tile its rows and its unpacking; the smallest bound that keeps to
-  // target_items (one for each block at least)
-  auto split = [&](const Block& b, int64_t most) {
-    const int64_t cap = most / (b.waves + 2) < 1 ? 1 : (most / (b.waves + 2) > kMostTiles ? kMostTiles : most / (b.waves + 2));
-    return ceil_div(b.tiles, cap);
+  // an item costs its tiles, and a tile its rows and its unpacking, a slow one more; the smallest bound
+  // that keeps to target_items (one for each block's kind of tiles at least)
+  auto items_of = [&](int64_t tiles, int64_t cost, int64_t most) {
+    const int64_t cap = most / cost < 1 ? 1 : (most / cost > kMostTiles ? kMostTiles : most / cost);
+    return ceil_div(tiles, cap);
   };
-  int64_t lo = 1, hi = (int64_t)(kWaves + 2) * kMostTiles;
+  auto fast_items = [&](const Block& b, int64_t most) { return items_of(b.full, b.waves + 2, most); };
+  auto split = [&](const Block& b, int64_t most) { return fast_items(b, most) + items_of(b.slow, kSlowCost * (b.waves + 2), most); };
+  int64_t lo = 1, hi = (int64_t)kSlowCost * (kWaves + 2) * kMostTiles;
   while (lo < hi) {
     const int64_t mid = (lo + hi) / 2;
     int64_t total = 0;
@@ -570,11 +604,14 @@ extern "C" int oscarop_tree_plan_v1(const int32_t* qsl, const int32_t* seqs, int
   for (int64_t p = 0; p < longest; ++p)
     for (size_t g = 0; g < blocks.size(); ++g) {
       const Block& b = blocks[g];
-      const int64_t k = split(b, lo);
+      const int64_t kf = fast_items(b, lo), k = split(b, lo);
       if (p >= k) continue;
+      // the slow items first: theirs are the longest
+      const int64_t ks = k - kf, x = p < ks ? p : p - ks, of = p < ks ? ks : kf;
+      const int64_t begin = p < ks ? b.full + x : x, tiles = p < ks ? b.slow : b.full;
       int32_t* it = items + out++ * OSCAROP_TREE_ITEM_INTS;
-      const int32_t record[OSCAROP_TREE_ITEM_INTS] = {b.req, b.kvh, b.qa, b.n, b.hist, b.row0, b.rows, (int32_t)p,
-                                                      (int32_t)k, (int32_t)ceil_div(b.tiles - p, k),
+      const int32_t record[OSCAROP_TREE_ITEM_INTS] = {b.req, b.kvh, b.qa, b.n, b.hist, b.row0, b.rows, (int32_t)begin,
+                                                      (int32_t)of, (int32_t)ceil_div(tiles - x, of),
                                                       (int32_t)(first[g] + p * b.rows), 0};
       for (int i = 0; i < OSCAROP_TREE_ITEM_INTS; ++i) it[i] = record[i];
     }
