@@ -350,6 +350,9 @@ typedef struct oscarop_select_args_v1 {
   int32_t* pages;                 /* [num_reqs][Hk][budget], or NULL */
   void* workspace;                /* >= oscarop_select_workspace_bytes_v1(args), 16-byte aligned */
   int64_t workspace_bytes;
+  /* [num_reqs * Hk], zero before the first call; each call leaves them zero.  As the workspace,
+   * nothing else uses them while a call runs.  Not read if no history exceeds the budget. */
+  int32_t* arrivals;
 } oscarop_select_args_v1;
 
 /* reads the sizes of *args alone; -22 for sizes that the call would refuse */

@@ -185,7 +185,7 @@ class SelectArgs(C.Structure):
         ("block_table", vp), ("block_table_stride", i64), ("block_table_rows", i64), ("block_table_cols", i64),
         ("query_start_loc", vp), ("seq_lens", vp), ("num_reqs", i32), ("max_pages", i32), ("budget", i32),
         ("first_pages", i32), ("last_pages", i32), ("reserved", i32), ("table", vp), ("pages", vp),
-        ("workspace", vp), ("workspace_bytes", i64),
+        ("workspace", vp), ("workspace_bytes", i64), ("arrivals", vp),
     ]
 
 

@@ -94,9 +94,7 @@ struct AttnParams {
   float* part_o;   // [num_items][32 * D] in MFMA register order
   float* part_lse; // [num_items][32]
   Score sc;        // SC != 0
-  int64_t table_head;     // VIEW 1: elements from one KV head's block table to the next
-  const uint64_t* mask;   // VIEW 2: [num_tokens][mask_words]
-  int64_t mask_words;
+  int64_t table_head;  // OWN: elements from one KV head's block table to the next
 };
 
 __device__ __forceinline__ f16x8 as_f16x8(u32x4 v) { return __builtin_bit_cast(f16x8, v); }
@@ -159,9 +157,8 @@ struct TileRegs {
 // SC: the score function (score.h).  Distance-biased scores grow towards the query, so the
 // scored variants walk an item's tiles from its last to its first: the reference maximum
 // of a row settles on the near tiles instead of moving (and O with it) tile by tile.
-// VIEW 0: the plain call; 1: each KV head reads a block table of its own; 2: the chunk's rows
-// see each other by a mask (in the slow tiles, where the chunk is).
-template <int D, int QT, int SC, int VIEW>
+// OWN: each KV head reads a block table of its own, the pages chosen for it (oscarop_attn_selected_v1).
+template <int D, int QT, int SC, bool OWN>
 __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   using C = Cfg<D>;
   using QV = typename QVec<QT>::type;  // one MFMA operand in the query dtype
@@ -241,7 +238,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   int wblk = 0, wseat = 0;
   if (lane < my) {
     const int t0 = tile_t0(wave + kWaves * lane);
-    if (t0 < hist) wblk = A.block_table[(int64_t)req * A.block_table_stride + (VIEW == 1 ? kvh * P.table_head : 0) + t0 / bs];
+    if (t0 < hist) wblk = A.block_table[(int64_t)req * A.block_table_stride + (OWN ? kvh * P.table_head : 0) + t0 / bs];
   }
   const int n = m;
   const bool row_ok = n < nrows;
@@ -439,9 +436,6 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   // while the runner wave computes the current one.
   f32x4 sx[NU][4];
   u32x2 smeta = {0u, 0u};
-  // VIEW 2: the keys of the tile that row tid < 32 sees, one bit each (history all)
-  __shared__ uint32_t s_see[VIEW == 2 ? 32 : 1];
-  uint32_t see = 0;
   auto slow_flags = [&](int j, bool& b_staged, bool& b_codes, bool& b_cur) {
     const int bp = tile_t0(j) + bt;
     b_staged = (s_tmask[j] >> bt) & 1u;
@@ -460,22 +454,6 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
     const int64_t cur_off = (int64_t)(cur0 + (b_cur ? bp - hist : 0)) * A.kv_new_stride_token + (int64_t)kvh * D;
     const int64_t seat_row = ((int64_t)seat0 + off0 + bt) * hk + kvh;  // staged row of the token
     smeta = b_codes ? *(const u32x2*)ks : u32x2{0u, 0u};
-    if constexpr (VIEW == 2) {
-      const int j0 = t0 - hist;  // the tile's first key as a row of the chunk
-      if (tid < nrows && j0 > -kTile) {
-        const uint64_t* words = P.mask + (int64_t)(qa + tid / G) * P.mask_words;
-        const int w = j0 < 0 ? 0 : j0 >> 6, sh = j0 & 63;
-        const uint64_t x0 = w < P.mask_words ? words[w] : 0;
-        if (j0 < 0) {
-          see = (uint32_t)(x0 << -j0) | ((1u << -j0) - 1u);
-        } else {
-          const uint64_t x1 = sh > 32 && w + 1 < P.mask_words ? words[w + 1] : 0;
-          see = (uint32_t)(x0 >> sh) | (sh > 32 ? (uint32_t)(x1 << (64 - sh)) : 0u);
-        }
-      } else {
-        see = ~0u;
-      }
-    }
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int uid = bpart + 16 * u, kv = uid / (2 * C::NCH), hg = (uid / C::NCH) & 1, c = uid % C::NCH;
@@ -497,7 +475,6 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   auto build_slow = [&](int j) {
     bool b_staged, b_codes, b_cur;
     slow_flags(j, b_staged, b_codes, b_cur);
-    if (VIEW == 2 && tid < 32) s_see[tid] = see;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int uid = bpart + 16 * u, kv = uid / (2 * C::NCH), hg = (uid / C::NCH) & 1, c = uid % C::NCH;
@@ -569,12 +546,10 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
         float xs[16];
         float mx = -INFINITY;
         const int limit = seq - nq + (row_ok ? n / G : 0) + 1;
-        const uint32_t sees = VIEW == 2 ? s_see[m] : 0;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int tp = t0 + out_tok(r, g);
-          bool vis = row_ok && tp < limit;  // limit <= seq
-          if constexpr (VIEW == 2) vis = vis && ((sees >> out_tok(r, g)) & 1u);
+          const bool vis = row_ok && tp < limit;  // limit <= seq
           if constexpr (SC == 0) xs[r] = vis ? S[r] * c_score : -INFINITY;
           else xs[r] = vis ? score2<SC>(P.sc, S[r], slope2, (float)(near + t0) + out_tok(r, 0)) : -INFINITY;
           mx = fmaxf(mx, xs[r]);
@@ -679,7 +654,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
     update_max(mx);
     const float nm = -m_run;
     u32x4 pb[2];
-    float lsum = 0.f, zsum = 0.f;
+    float lsum = 0.f, zsum = 0.f, rest = 0.f;
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4) {
       const f32x4 sv = *(const f32x4*)&s_cst[wave][0][8 * q4 + 4 * g];
@@ -693,11 +668,16 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
         lsum += p0 + p1;
         zsum = fmaf(p0, zv[i], fmaf(p1, zv[i + 1], zsum));
         const f16x2 h = {(_Float16)(p0 * sv[i]), (_Float16)(p1 * sv[i + 1])};
+        // OWN: what the rounding of P' leaves out, at the codes' middle: the error of P' meets c - 1.5
+        // then, not c, of a value c s + z whose two parts are larger than itself (fp16 outputs of 12
+        // ragged requests 2.8e-4 -> 2.5e-4 off, their last rounding alone 2.1e-4)
+        if constexpr (OWN) rest += fmaf(p0, sv[i], -(float)h[0]) + fmaf(p1, sv[i + 1], -(float)h[1]);
         pb[r0 >> 3][(r0 & 7) >> 1] = __builtin_bit_cast(unsigned, h);
       }
     }
     l_run += lsum;
     z_run += zsum;
+    if constexpr (OWN) z_run = fmaf(rest, 1.5f / v_fac, z_run);
     const int G16 = lane >> 4, i16 = lane & 15;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -1008,15 +988,12 @@ int launch_decode(const AttnParams& p, int sc, hipStream_t s, const StoreParams&
   if (p.a.phases != 2) {
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(p.a.num_items), dim3(kThreads), 0, s, p); };
     const bool f16 = p.a.q_dtype == OSCAR_F16;
-    if (p.mask != nullptr) {
-      if (sc == 0) f16 ? launch(attn_main_kernel<D, OSCAR_F16, 0, 2>) : launch(attn_main_kernel<D, OSCAR_BF16, 0, 2>);
-      else f16 ? launch(attn_main_kernel<D, OSCAR_F16, 2, 2>) : launch(attn_main_kernel<D, OSCAR_BF16, 2, 2>);
-    } else if (p.table_head != 0) {
-      if (sc == 0) f16 ? launch(attn_main_kernel<D, OSCAR_F16, 0, 1>) : launch(attn_main_kernel<D, OSCAR_BF16, 0, 1>);
-      else f16 ? launch(attn_main_kernel<D, OSCAR_F16, 2, 1>) : launch(attn_main_kernel<D, OSCAR_BF16, 2, 1>);
-    } else if (sc == 0) f16 ? launch(attn_main_kernel<D, OSCAR_F16, 0, 0>) : launch(attn_main_kernel<D, OSCAR_BF16, 0, 0>);
-    else if (sc == 1) f16 ? launch(attn_main_kernel<D, OSCAR_F16, 1, 0>) : launch(attn_main_kernel<D, OSCAR_BF16, 1, 0>);
-    else f16 ? launch(attn_main_kernel<D, OSCAR_F16, 2, 0>) : launch(attn_main_kernel<D, OSCAR_BF16, 2, 0>);
+    if (p.table_head != 0) {
+      if (sc == 0) f16 ? launch(attn_main_kernel<D, OSCAR_F16, 0, true>) : launch(attn_main_kernel<D, OSCAR_BF16, 0, true>);
+      else f16 ? launch(attn_main_kernel<D, OSCAR_F16, 2, true>) : launch(attn_main_kernel<D, OSCAR_BF16, 2, true>);
+    } else if (sc == 0) f16 ? launch(attn_main_kernel<D, OSCAR_F16, 0, false>) : launch(attn_main_kernel<D, OSCAR_BF16, 0, false>);
+    else if (sc == 1) f16 ? launch(attn_main_kernel<D, OSCAR_F16, 1, false>) : launch(attn_main_kernel<D, OSCAR_BF16, 1, false>);
+    else f16 ? launch(attn_main_kernel<D, OSCAR_F16, 2, false>) : launch(attn_main_kernel<D, OSCAR_BF16, 2, false>);
     OSCAR_CHECK_LAUNCH("attn_main_kernel");
   }
   if (p.a.phases != 1) {
@@ -1339,25 +1316,16 @@ int oscar::attn_check_args(const oscar_attn_args_v1& a, const char* name) {
 
 namespace {
 
-// what the tree and the selected entry points see of the cache and the chunk (AttnParams)
-struct View {
-  int64_t table_head = 0;
-  const uint64_t* mask = nullptr;
-  int64_t mask_words = 0;
-};
-
 // The decode entry points after their own checks.  `partials` / `partial_bytes`: where
 // the item partials go and how much room there is.  `store` (oscar_decode_write_v1): the
 // store enqueued once the decode's arguments have passed, deferred (its quantization in
-// the merge launch) when it is a small call.
+// the merge launch) when it is a small call.  table_head: 0, or AttnParams'.
 int launch_checked(const oscar_attn_args_v1& a, const char* name, void* partials, int64_t partial_bytes,
                    hipStream_t s, const oscarop_score_v1* score = nullptr, const oscar_store_args_v1* store = nullptr,
-                   const MetaCopy* meta = nullptr, const View& view = {}) {
+                   const MetaCopy* meta = nullptr, int64_t table_head = 0) {
   const int64_t D = a.cache.head_dim;
   AttnParams p{};
-  p.table_head = view.table_head;
-  p.mask = view.mask;
-  p.mask_words = view.mask_words;
+  p.table_head = table_head;
   const int sc = score_of(score, a.scale, &p.sc);
   if (sc < 0) return fail(-22, kBadCap, name);
   if (D != 128 && D != 256) return fail(-22, "%s: head_dim %lld unsupported", name, (long long)D);
@@ -1435,19 +1403,6 @@ extern "C" int oscarop_attn_decode_v1(const oscar_attn_args_v1* args, const osca
                         score);
 }
 
-extern "C" int oscarop_attn_masked_v1(const oscar_attn_args_v1* args, const oscarop_score_v1* score, const int64_t* mask,
-                                    int64_t mask_words, void* stream);
-extern "C" int oscarop_attn_masked_v1(const oscar_attn_args_v1* args, const oscarop_score_v1* score, const int64_t* mask,
-                                    int64_t mask_words, void* stream) {
-  if (!args) return fail(-22, "oscarop_attn_masked_v1: null args");
-  if (score && score->alibi_slopes) return fail(-22, "oscarop_attn_masked_v1: no alibi_slopes with a mask");
-  if (args->num_items > 0 && (!mask || ((uintptr_t)mask & 7) || mask_words < 1 || mask_words > 1 << 20))
-    return fail(-22, "oscarop_attn_masked_v1: a mask of at least one word a row, 8-byte aligned");
-  if (args->num_items > 0 && !args->k_new) return fail(-22, "oscarop_attn_masked_v1: a mask needs the chunk's keys");
-  return launch_checked(*args, "oscarop_attn_masked_v1", args->workspace, args->workspace_bytes, (hipStream_t)stream, score,
-                        nullptr, nullptr, View{0, (const uint64_t*)mask, mask_words});
-}
-
 extern "C" int oscarop_attn_selected_v1(const oscar_attn_args_v1* args, const oscarop_score_v1* score,
                                         int64_t table_stride_head, void* stream) {
   if (!args) return fail(-22, "oscarop_attn_selected_v1: null args");
@@ -1457,7 +1412,7 @@ extern "C" int oscarop_attn_selected_v1(const oscar_attn_args_v1* args, const os
                               table_stride_head > args->block_table_stride / hk))
     return fail(-22, "oscarop_attn_selected_v1: a request's row holds a table for each KV head");
   return launch_checked(*args, "oscarop_attn_selected_v1", args->workspace, args->workspace_bytes, (hipStream_t)stream,
-                        score, nullptr, nullptr, View{table_stride_head, nullptr, 0});
+                        score, nullptr, nullptr, table_stride_head);
 }
 
 int oscar::decode_write_launch(const oscar_store_args_v1& store, const oscar_attn_args_v1& attn,

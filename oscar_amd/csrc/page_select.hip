@@ -9,9 +9,11 @@
 //
 //   bounds_kernel   one workgroup per page: the codes of its tokens, each token's four values from a
 //                   table, packed minimum and maximum
-//   score_kernel    eight lanes a page, the bounds in registers, the queries from LDS
-//   select_kernel   one workgroup per (request, KV head): the budget-th largest score by radix
-//                   selection, then the chosen columns in their order
+//   select_kernel   eight lanes a page, the bounds in registers; the last workgroup of a (request,
+//                   KV head) finds the budget-th largest score by radix selection and writes
+//                   the chosen columns in their order
+#include <type_traits>
+
 #include "common.h"
 #include "int2_tile.h"
 
@@ -51,18 +53,28 @@ __global__ __launch_bounds__(kThreads) void bounds_kernel(oscarop_bounds_args_v1
   f16x2 low[8], high[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) low[k] = as_f16x2(0x7c007c00u), high[k] = as_f16x2(0xfc00fc00u);
-  for (int t = group; t < held; t += GROUPS) {
-    const uint8_t* slot = base + t * ks1;
-    const unsigned consts = *(const unsigned*)slot, w = *(const unsigned*)(slot + 32 + 4 * c);
-    unsigned lo, hi;
-    value_table<OSCAR_F16>(consts, lo, hi);
+  constexpr int BATCH = 128 / GROUPS;  // slots of a thread in flight: a page of 128 tokens at once
+  for (int t0 = group; t0 < held; t0 += BATCH * GROUPS) {
+    unsigned consts[BATCH], w[BATCH];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      // channels k and k + 8 of the chunk
-      const unsigned y = (w >> (2 * k)) & 0x00030003u;
-      const f16x2 v = as_f16x2(__builtin_amdgcn_perm(hi, lo, y * 0x202u + 0x01000100u));
-      low[k] = pk_min(low[k], v);
-      high[k] = pk_max(high[k], v);
+    for (int u = 0; u < BATCH; ++u) {
+      // (behind the page's tokens: the thread's first one again)
+      const uint8_t* slot = base + (t0 + u * GROUPS < held ? t0 + u * GROUPS : t0) * ks1;
+      consts[u] = *(const unsigned*)slot;
+      w[u] = *(const unsigned*)(slot + 32 + 4 * c);
+    }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      unsigned lo, hi;
+      value_table<OSCAR_F16>(consts[u], lo, hi);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        // channels k and k + 8 of the chunk
+        const unsigned y = (w[u] >> (2 * k)) & 0x00030003u;
+        const f16x2 v = as_f16x2(__builtin_amdgcn_perm(hi, lo, y * 0x202u + 0x01000100u));
+        low[k] = pk_min(low[k], v);
+        high[k] = pk_max(high[k], v);
+      }
     }
   }
   __shared__ unsigned s_part[GROUPS][CH][17];
@@ -86,10 +98,15 @@ __global__ __launch_bounds__(kThreads) void bounds_kernel(oscarop_bounds_args_v1
   }
 }
 
-// ------------------------------------------------------------------------ scores
-constexpr int kLanes = 8;                               // lanes of a page
-constexpr int kPages = kThreads / kLanes;               // pages of a workgroup at a time
-constexpr int kRowsHeld = 32;                           // queries in LDS at a time
+// ------------------------------------------------------------------------ scores and selection
+constexpr int kLanes = 8;                // lanes of a page
+constexpr int kPages = 64 / kLanes;      // pages of a workgroup at a time
+constexpr int kHeld = 4096;              // scores in LDS; more are read again in each pass
+constexpr int kFew = 64;                 // candidates that one wave ranks
+constexpr int kBatch = 4;                // scores of a thread in flight
+constexpr int kRowsHeld = 16;            // queries in LDS at a time, in 64 bits: a conversion costs four products
+// workgroups up to which the waves of one share their pages: what the card holds at a time
+constexpr int64_t kByRows = 512;
 
 struct SelectParams {
   oscarop_select_args_v1 a;
@@ -123,147 +140,93 @@ __device__ __forceinline__ double dpp_row64(double x) {
   return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
 }
 
-template <int D, int QT>
-__global__ __launch_bounds__(kThreads) void score_kernel(SelectParams P) {
-  constexpr int STEPS = D / (8 * kLanes);  // 16-byte pieces of a lane
-  const oscarop_select_args_v1& A = P.a;
-  const int tid = threadIdx.x, h = blockIdx.y, r = blockIdx.z;
-  const History x = history_of(A, r);
-  if (x.pages <= A.budget) return;
-  const int group = (int)(A.num_q_heads / A.num_kv_heads);
-  const int first = A.first_pages, end = (int)x.pages - A.last_pages;
-  const int j = tid % kLanes;
-  __shared__ __attribute__((aligned(16))) float s_q[kRowsHeld][D];
-  const int64_t rows = (int64_t)x.nq * group;
-  for (int p0 = first + blockIdx.x * kPages; p0 < end; p0 += gridDim.x * kPages) {
-    const int p = p0 + tid / kLanes;
-    const bool in = p < end;
-    int page = A.block_table[r * A.block_table_stride + (in ? p : first)];
-    page = page < 0 || page >= A.num_blocks ? 0 : page;
-    const uint16_t* b = (const uint16_t*)A.bounds + ((int64_t)page * A.num_kv_heads + h) * 2 * D + 8 * j;
-    u32x4 lo[STEPS], hi[STEPS];
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      lo[s] = *(const u32x4*)(b + 8 * kLanes * s);
-      hi[s] = *(const u32x4*)(b + D + 8 * kLanes * s);
-    }
-    double best = -INFINITY;
-    bool nan = false;
-    for (int64_t row0 = 0; row0 < rows; row0 += kRowsHeld) {
-      const int held = rows - row0 < kRowsHeld ? (int)(rows - row0) : kRowsHeld;
-      __syncthreads();  // the rows before have been read
-      for (int i = tid; i < held * (D / 8); i += kThreads) {
-        const int64_t row = row0 + i / (D / 8);
-        const int e = i % (D / 8) * 8;
-        float v[8];
-        load8<QT>(A.q, (x.q0 + row / group) * A.q_stride_token + (h * group + row % group) * (int64_t)D + e, v);
-        *(f32x4*)&s_q[i / (D / 8)][e] = f32x4{v[0], v[1], v[2], v[3]};
-        *(f32x4*)&s_q[i / (D / 8)][e + 4] = f32x4{v[4], v[5], v[6], v[7]};
-      }
-      __syncthreads();
-      double m[STEPS][8], w[STEPS][8];
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const double l = f16_bits_to_f32((lo[s][e / 2] >> (16 * (e & 1))) & 0xffff);
-          const double u = f16_bits_to_f32((hi[s][e / 2] >> (16 * (e & 1))) & 0xffff);
-          m[s][e] = 0.5 * (u + l);
-          w[s][e] = 0.5 * (u - l);
-        }
-      for (int i = 0; i < held; ++i) {
-        double sum = 0.0;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const double q = s_q[i][8 * kLanes * s + 8 * j + e];
-            sum = fma(q, m[s][e], sum);
-            sum = fma(fabs(q), w[s][e], sum);
-          }
-        sum += dpp_row64<kDppXor1>(sum);
-        sum += dpp_row64<kDppXor2>(sum);
-        sum += dpp_row64<kDppHalfMirror>(sum);
-        nan |= sum != sum;
-        best = sum > best ? sum : best;
-      }
-    }
-    if (in && j == 0) P.keys[((int64_t)r * A.num_kv_heads + h) * A.max_pages + p] = nan ? ~0ull : order_of(best);
-  }
+// what a wave's lanes give, combined into its last lane: within rows of 16 lanes, then the
+// rows' last lanes into the rows behind them (0: what lanes without a neighbour take)
+template <class Op>
+__device__ __forceinline__ unsigned wave_prefix(unsigned v, Op op) {
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+  return op(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
 }
 
-// ------------------------------------------------------------------------ selection
-constexpr int kHeld = 4096;  // scores in LDS; more are read again in each pass
-
-// exclusive prefix sum over the workgroup of one number per thread; *total gets the sum
-__device__ __forceinline__ unsigned scan(unsigned x, unsigned* total, unsigned* s_part) {
+// exclusive prefix sum over the workgroup of one number per thread
+__device__ __forceinline__ unsigned scan(unsigned x, unsigned* s_part) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  unsigned v = x;
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  const unsigned v = wave_prefix(x, [](unsigned a, unsigned b) { return a + b; });
   __syncthreads();  // s_part of the call before has been read
   if (lane == 63) s_part[wave] = v;
   __syncthreads();
-  unsigned before = 0, sum = 0;
+  unsigned before = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    before += w < wave ? s_part[w] : 0;
-    sum += s_part[w];
-  }
-  *total = sum;
+  for (int w = 0; w < kWaves; ++w) before += w < wave ? s_part[w] : 0;
   return before + v - x;
 }
 
-__global__ __launch_bounds__(kThreads) void select_kernel(SelectParams P) {
+// One list's choice: the want-th largest key of `first` to `end`, then the chosen columns in
+// their order.  The keys agree in their upper bits, so digits begin at the highest one in which two
+// differ; the few candidates that are left in the digit's bin are ranked against each other.
+__device__ void choose(const SelectParams& P, int many, int64_t list, const int32_t* row) {
   const oscarop_select_args_v1& A = P.a;
-  const int tid = threadIdx.x, h = blockIdx.x, r = blockIdx.y;
-  const History x = history_of(A, r);
-  const int64_t list = (int64_t)r * A.num_kv_heads + h;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int32_t* table = A.table + list * A.budget;
   int32_t* pages = A.pages == nullptr ? nullptr : A.pages + list * A.budget;
-  const int32_t* row = A.block_table + (int64_t)r * A.block_table_stride;
   auto put = [&](int at, int col) {
     table[at] = row[col];
     if (pages != nullptr) pages[at] = col;
   };
-  const int many = (int)x.pages;
-  if (many <= A.budget) {
-    for (int i = tid; i < A.budget; i += kThreads) {
-      if (i < many) put(i, i);
-      else {
-        table[i] = -1;
-        if (pages != nullptr) pages[i] = -1;
-      }
-    }
-    return;
-  }
   const int first = A.first_pages, n = many - first - A.last_pages, want = A.budget - first - A.last_pages;
   const uint64_t* keys = P.keys + list * A.max_pages + first;
   __shared__ uint64_t s_key[kHeld];
   __shared__ int s_bin[256];
   __shared__ unsigned s_part[kWaves];
-  __shared__ int s_found[3];  // digit, rest to take, size of its bin
+  __shared__ unsigned s_diff[kWaves][2];
+  __shared__ uint64_t s_few[kFew];
+  __shared__ int s_place[kFew];
+  __shared__ int s_found[3];       // digit, rest to take, size of its bin
+  __shared__ uint64_t s_limit;
   const bool held = n <= kHeld;
-  if (held)
-    for (int i = tid; i < n; i += kThreads) s_key[i] = keys[i];
-  auto key = [&](int i) { return held ? s_key[i] : keys[i]; };
-  uint64_t prefix = 0, mask = 0;
-  unsigned rest = want, total;
-  for (int shift = 56; shift >= 0; shift -= 8) {
-    s_bin[tid] = 0;
-    __syncthreads();
+  auto load = [&](int i) { return __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  const uint64_t some = load(0);
+  uint64_t diff = 0;
+  for (int i = tid; i < n; i += kBatch * kThreads) {
+    uint64_t k[kBatch];  // all on their way before the first is used
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) k[u] = load(min(i + u * kThreads, n - 1));
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (held && i + u * kThreads < n) s_key[i + u * kThreads] = k[u];
+      diff |= k[u] ^ some;
+    }
+  }
+  auto key = [&](int i) { return held ? s_key[i] : load(i); };
+  auto both = [](unsigned a, unsigned b) { return a | b; };
+  const unsigned low = wave_prefix((unsigned)diff, both), high = wave_prefix((unsigned)(diff >> 32), both);
+  if (lane == 63) {
+    s_diff[wave][0] = low;
+    s_diff[wave][1] = high;
+  }
+  s_bin[tid] = 0;
+  if (tid == 0) s_found[2] = 0;
+  __syncthreads();
+  diff = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) diff |= (uint64_t)s_diff[w][1] << 32 | s_diff[w][0];
+  // keys are told apart by `mask`; those with `prefix` there are still to be told apart
+  int left = diff == 0 ? 0 : 64 - __clzll((long long)diff);
+  uint64_t mask = left >= 64 ? 0 : ~0ull << left, prefix = some & mask;
+  unsigned rest = want;
+  while (left > 0) {
+    const int shift = left > 8 ? left - 8 : 0, digits = (1 << (left - shift)) - 1;
     for (int i = tid; i < n; i += kThreads) {
       const uint64_t k = key(i);
-      if ((k & mask) == prefix) atomicAdd(&s_bin[(int)(k >> shift) & 255], 1);
+      if ((k & mask) == prefix) atomicAdd(&s_bin[(int)(k >> shift) & digits], 1);
     }
     __syncthreads();
     // thread t: the t-th largest digit
-    const int mine = s_bin[255 - tid];
-    const unsigned above = scan(mine, &total, s_part);
+    const unsigned mine = s_bin[255 - tid], above = scan(mine, s_part);
     if (above < rest && above + mine >= rest) {
       s_found[0] = 255 - tid;
       s_found[1] = rest - above;
@@ -271,12 +234,49 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectParams P) {
     }
     __syncthreads();
     prefix |= (uint64_t)s_found[0] << shift;
-    mask |= 255ull << shift;
+    mask |= (uint64_t)digits << shift;
     rest = s_found[1];
-    if ((unsigned)s_found[2] == rest) break;  // all of the bin
-    __syncthreads();  // s_found has been read
+    left = shift;
+    const unsigned size = s_found[2];
+    if (size == rest) break;  // all of the bin
+    s_bin[tid] = 0;
+    if (size <= kFew && left > 0) {
+      __syncthreads();  // s_found has been read
+      if (tid == 0) s_found[2] = 0;
+      __syncthreads();
+      for (int i = tid; i < n; i += kThreads) {
+        const uint64_t k = key(i);
+        if ((k & mask) == prefix) {
+          const int at = atomicAdd(&s_found[2], 1);
+          s_few[at] = k;
+          s_place[at] = i;
+        }
+      }
+      __syncthreads();
+      if (wave == 0) {
+        const bool in = lane < (int)size;
+        const uint64_t k = in ? s_few[lane] : 0;
+        const int at = in ? s_place[lane] : 0;
+        unsigned rank = 0, ahead = 0;  // those before this one, and those of a larger key
+        for (int i = 0; i < (int)size; ++i) {
+          const uint64_t o = s_few[i];
+          ahead += o > k;
+          rank += o > k || (o == k && s_place[i] < at);
+        }
+        if (in && rank == rest - 1) {
+          s_limit = k;
+          s_found[1] = rest - ahead;  // of the keys that equal the limit
+        }
+      }
+      __syncthreads();
+      prefix = s_limit;
+      mask = ~0ull;
+      rest = s_found[1];
+      break;
+    }
+    __syncthreads();  // s_found has been read, the bins are clear
   }
-  // scores above the prefix, and the first `rest` that equal it: thread t looks at the columns
+  // keys above the prefix, and the first `rest` that equal it: thread t looks at the columns
   // [t run, (t + 1) run)
   const int run = (n + kThreads - 1) / kThreads;
   const int a = min(tid * run, n), b = min(a + run, n);
@@ -286,9 +286,9 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectParams P) {
     same += k == prefix;
     over += k > prefix;
   }
-  unsigned ties = scan(same, &total, s_part);
+  unsigned ties = scan(same, s_part);
   const unsigned taken = ties < rest ? min(same, rest - ties) : 0;
-  unsigned at = first + scan(over + taken, &total, s_part);
+  unsigned at = first + scan(over + taken, s_part);
   for (int i = a; i < b; ++i) {
     const uint64_t k = key(i) & mask;
     const bool tie = k == prefix;
@@ -297,6 +297,119 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectParams P) {
   }
   for (int i = tid; i < first; i += kThreads) put(i, i);
   for (int i = tid; i < A.last_pages; i += kThreads) put(A.budget - A.last_pages + i, many - A.last_pages + i);
+}
+
+// A workgroup scores eight pages at a time, its waves a quarter of the rows each (ROWS), or 32
+// pages, eight a wave; the last one of a (request, KV head) to arrive makes the choice.
+template <int D, int QT, bool ROWS>
+__global__ __launch_bounds__(kThreads, 2) void select_kernel(SelectParams P) {
+  constexpr int STEPS = D / (8 * kLanes);  // 16-byte pieces of a lane
+  const oscarop_select_args_v1& A = P.a;
+  const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.y, r = blockIdx.z;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const History x = history_of(A, r);
+  const int64_t list = (int64_t)r * A.num_kv_heads + h;
+  const int32_t* table_row = A.block_table + (int64_t)r * A.block_table_stride;
+  if (x.pages <= A.budget) {
+    // all of them
+    if (blockIdx.x > 0) return;
+    for (int i = tid; i < A.budget; i += kThreads) {
+      A.table[list * A.budget + i] = i < x.pages ? table_row[i] : -1;
+      if (A.pages != nullptr) A.pages[list * A.budget + i] = i < x.pages ? i : -1;
+    }
+    return;
+  }
+  const int group = (int)(A.num_q_heads / A.num_kv_heads);
+  const int first = A.first_pages, end = (int)x.pages - A.last_pages;
+  const int j = lane % kLanes;
+  const int64_t rows = (int64_t)x.nq * group;
+  __shared__ double s_best[kWaves][kPages];
+  __shared__ __attribute__((aligned(16))) double s_q[kRowsHeld][D];
+  __shared__ int s_last;
+  constexpr int kAtOnce = ROWS ? kPages : kWaves * kPages;
+  const int p_first = first + blockIdx.x * kAtOnce;
+  for (int p0 = p_first; p0 < end; p0 += gridDim.x * kAtOnce) {
+    const int p = p0 + lane / kLanes + (ROWS ? 0 : kPages * wave);
+    int page = table_row[p < end ? p : first];
+    page = page < 0 || page >= A.num_blocks ? 0 : page;
+    const uint16_t* b = (const uint16_t*)A.bounds + ((int64_t)page * A.num_kv_heads + h) * 2 * D + 8 * j;
+    u32x4 lo[STEPS], hi[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      lo[s] = *(const u32x4*)(b + 8 * kLanes * s);
+      hi[s] = *(const u32x4*)(b + D + 8 * kLanes * s);
+    }
+    double m[STEPS][8], w[STEPS][8];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double l = f16_bits_to_f32((lo[s][e / 2] >> (16 * (e & 1))) & 0xffff);
+        const double u = f16_bits_to_f32((hi[s][e / 2] >> (16 * (e & 1))) & 0xffff);
+        m[s][e] = 0.5 * (u + l);
+        w[s][e] = 0.5 * (u - l);
+      }
+    double best = -INFINITY;
+    for (int64_t from = 0; from < rows; from += kRowsHeld) {
+      const int many = rows - from < kRowsHeld ? (int)(rows - from) : kRowsHeld;
+      if (p0 == p_first || rows > kRowsHeld) {
+        __syncthreads();  // the rows before have been read
+        for (int i = tid; i < many * (D / 8); i += kThreads) {
+          const int64_t row = from + i / (D / 8);
+          const int e0 = i % (D / 8) * 8;
+          float v[8];
+          load8<QT>(A.q, (x.q0 + row / group) * A.q_stride_token + (h * group + row % group) * (int64_t)D + e0, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s_q[i / (D / 8)][e0 + e] = v[e];
+        }
+        __syncthreads();
+      }
+      for (int row = ROWS ? wave : 0; row < many; row += ROWS ? kWaves : 1) {
+        double part[4] = {0.0, 0.0, 0.0, 0.0};  // four sums at a time: one alone waits for itself
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const double v = s_q[row][8 * kLanes * s + 8 * j + e];
+            part[e & 3] = fma(v, m[s][e], part[e & 3]);
+            part[e & 3] = fma(fabs(v), w[s][e], part[e & 3]);
+          }
+        double sum = (part[0] + part[1]) + (part[2] + part[3]);
+        sum += dpp_row64<kDppXor1>(sum);
+        sum += dpp_row64<kDppXor2>(sum);
+        sum += dpp_row64<kDppHalfMirror>(sum);
+        // (a NaN stays)
+        best = best != best || sum <= best ? best : sum;
+      }
+    }
+    auto put = [&](int at, uint64_t k) {
+      __hip_atomic_store(P.keys + list * A.max_pages + at, k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
+    if constexpr (ROWS) {
+      if (j == 0) s_best[wave][lane / kLanes] = best;
+      __syncthreads();
+      if (tid < kPages && p0 + tid < end) {
+        uint64_t k = 0;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+          const uint64_t o = order_of(s_best[i][tid]);
+          k = o > k ? o : k;
+        }
+        put(p0 + tid, k);
+      }
+      __syncthreads();  // s_best has been read
+    } else if (j == 0 && p < end) {
+      put(p, order_of(best));
+    }
+  }
+  // The keys go past this XCD's L2 and are read past the reader's (agent-scope atomics), so that
+  // the barrier, which waits for them, and the counter, which wraps to zero, order them; an agent-scope
+  // fence would write back the whole L2 instead, for every workgroup (16 lists of 1024 pages: 64 us)
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (tid == 0) s_last = atomicInc((unsigned*)&A.arrivals[list], gridDim.x - 1) == gridDim.x - 1;
+  __syncthreads();
+  if (s_last) choose(P, (int)x.pages, list, table_row);
 }
 
 // -22 for sizes that are refused
@@ -370,21 +483,29 @@ extern "C" int oscarop_select_v1(const oscarop_select_args_v1* args, void* strea
   p.a = a;
   p.keys = (uint64_t*)a.workspace;
   const hipStream_t s = (hipStream_t)stream;
+  dim3 grid(1, (unsigned)a.num_kv_heads, (unsigned)a.num_reqs);
+  bool by_rows = true;
   if (need > 0) {
     if (!a.q || !a.bounds || a.num_blocks < 1) return fail(-22, "oscarop_select_v1: missing pointer");
     if ((a.q_stride_token & 7) || ((uintptr_t)a.q & 15) || ((uintptr_t)a.bounds & 15))
       return fail(-22, "oscarop_select_v1: q rows and bounds must be 16-byte aligned");
     if (a.workspace_bytes < need || !a.workspace || ((uintptr_t)a.workspace & 15))
       return fail(-28, "oscarop_select_v1: workspace of %lld bytes < %lld", (long long)a.workspace_bytes, (long long)need);
+    if (!a.arrivals) return fail(-22, "oscarop_select_v1: missing pointer");
     const int64_t scored = a.max_pages - a.first_pages - a.last_pages;
-    const dim3 grid((unsigned)((scored + kPages - 1) / kPages), (unsigned)a.num_kv_heads, (unsigned)a.num_reqs);
-    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, p); };
-    const bool f16 = a.q_dtype == OSCAR_F16;
-    if (a.head_dim == 256) f16 ? launch(score_kernel<256, OSCAR_F16>) : launch(score_kernel<256, OSCAR_BF16>);
-    else f16 ? launch(score_kernel<128, OSCAR_F16>) : launch(score_kernel<128, OSCAR_BF16>);
-    OSCAR_CHECK_LAUNCH("score_kernel");
+    grid.x = (unsigned)((scored + kPages - 1) / kPages);
+    by_rows = (int64_t)grid.x * a.num_kv_heads * a.num_reqs <= kByRows;
+    if (!by_rows) grid.x = (unsigned)((scored + kWaves * kPages - 1) / (kWaves * kPages));
   }
-  hipLaunchKernelGGL(select_kernel, dim3((unsigned)a.num_kv_heads, (unsigned)a.num_reqs), dim3(kThreads), 0, s, p);
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, p); };
+  const bool f16 = a.q_dtype == OSCAR_F16;
+  auto launch_rows = [&](auto rows) {
+    constexpr bool R = decltype(rows)::value;
+    if (a.head_dim == 256) f16 ? launch(select_kernel<256, OSCAR_F16, R>) : launch(select_kernel<256, OSCAR_BF16, R>);
+    else f16 ? launch(select_kernel<128, OSCAR_F16, R>) : launch(select_kernel<128, OSCAR_BF16, R>);
+  };
+  if (by_rows) launch_rows(std::true_type{});
+  else launch_rows(std::false_type{});
   OSCAR_CHECK_LAUNCH("select_kernel");
   return 0;
 }

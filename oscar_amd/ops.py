@@ -78,8 +78,8 @@ def _launch(name: str, index: int, *args) -> None:
 _CACHE = struct.Struct("=QQ10q").pack  # _lib.Cache's fields
 
 
-def cache_struct(k_cache: torch.Tensor, v_cache: torch.Tensor, head_dim: int) -> _lib.Cache:
-    """Byte view of a packed cache pair [num_blocks, block_size, Hk, D] (int8 or bf16).  The
+def _cache_values(k_cache: torch.Tensor, v_cache: torch.Tensor, head_dim: int) -> tuple:
+    """_lib.Cache's fields for a packed cache pair [num_blocks, block_size, Hk, D] (int8 or bf16).  The
     kernels take the blocks, tokens and heads of K for both, so the two must have the same,
     and their slots room for the constants (K's first 32 bytes) and the codes."""
     if k_cache.ndim != 4 or v_cache.ndim != 4 or not k_cache.is_contiguous() or not v_cache.is_contiguous():
@@ -93,8 +93,13 @@ def cache_struct(k_cache: torch.Tensor, v_cache: torch.Tensor, head_dim: int) ->
     if k2 < 32 + head_dim // 4 or v2 < head_dim // 4:
         raise ValueError(f"OSCAR slots of head_dim {head_dim} take {32 + head_dim // 4} bytes of K and {head_dim // 4} of V, "
                          f"the caches have {k2} and {v2}")
-    return _lib.Cache.from_buffer_copy(_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), blocks, tokens, heads, head_dim,
-                                              tokens * heads * k2, heads * k2, k2, tokens * heads * v2, heads * v2, v2))
+    return (k_cache.data_ptr(), v_cache.data_ptr(), blocks, tokens, heads, head_dim,
+            tokens * heads * k2, heads * k2, k2, tokens * heads * v2, heads * v2, v2)
+
+
+def cache_struct(k_cache: torch.Tensor, v_cache: torch.Tensor, head_dim: int) -> _lib.Cache:
+    """Byte view of a packed cache pair, see _cache_values."""
+    return _lib.Cache.from_buffer_copy(_CACHE(*_cache_values(k_cache, v_cache, head_dim)))
 
 
 def staging_struct(stage, k_cache: torch.Tensor | None = None, head_dim: int | None = None) -> _lib.Staging | None:
@@ -160,6 +165,7 @@ class DeviceScratch:
         self.seat_claims = torch.zeros(0, dtype=torch.int64, device=device)
         self.store_ws = torch.empty(0, dtype=torch.uint8, device=device)
         self.arrivals = torch.zeros(0, dtype=torch.int32, device=device)
+        self.list_arrivals = torch.zeros(0, dtype=torch.int32, device=device)
         self.attn_ws = torch.empty(0, dtype=torch.uint8, device=device)
         self.prefill_ws = torch.empty(0, dtype=torch.uint8, device=device)
 
@@ -199,6 +205,13 @@ class DeviceScratch:
             self.arrivals = torch.zeros(need, dtype=torch.int32, device=self.device)
         return self.arrivals
 
+    def select_arrivals(self, lists: int) -> torch.Tensor:
+        """Arrival counters of select_pages, one for each request and KV head: zeroed once, and
+        every call leaves them zero."""
+        if self.list_arrivals.numel() < lists:
+            self.list_arrivals = torch.zeros(max(lists, 1024), dtype=torch.int32, device=self.device)
+        return self.list_arrivals
+
     def prefill_workspace(self, nbytes: int) -> torch.Tensor:
         if self.prefill_ws.numel() < nbytes:
             self.prefill_ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=self.device)
@@ -235,6 +248,17 @@ def _call_workspace(index: int, kind: str, nbytes: int) -> torch.Tensor:
     if scratch is None:
         scratch = DeviceScratch.get(torch.device("cuda", index))
     return getattr(scratch, kind)(nbytes)
+
+
+def _arrivals(index: int, lists: int) -> torch.Tensor:
+    """The arrival counters of a select_pages call on device `index`: the stream's, or, while the
+    stream captures a graph, the call's own, cleared within the graph."""
+    if index != _get_device():
+        with torch.cuda.device(index):
+            return _arrivals(index, lists)
+    if _is_capturing():
+        return torch.zeros(lists, dtype=torch.int32, device=torch.device("cuda", index))
+    return DeviceScratch.get(torch.device("cuda", index)).select_arrivals(lists)
 
 
 class DeviceContext:
@@ -994,6 +1018,14 @@ class SlotMap:
     granted: torch.Tensor  # bool [requests]
 
 
+_MAP = struct.Struct("@3P2iq P3q PPq 5P Pq").pack         # _lib.MapArgs's fields, as the others'
+_RELEASE = struct.Struct("@2P2i P3q PPq").pack
+_ATTN = struct.Struct("@P3q PPq PP10q Pq PPi Pf Pi Pi Pq i PP ii qq").pack
+_TREE = struct.Struct("@Pqq").pack
+_SELECT = struct.Struct("@P3q2i P4q P3q PP6i PP PqP").pack
+_BOUNDS = struct.Struct("@PP10q P3q PP2i qP").pack
+
+
 def _int32_list(name: str, x: torch.Tensor, n: int) -> torch.Tensor:
     if x.dtype != torch.int32 or x.shape != (n,):
         raise ValueError(f"{name} must be int32 [{n}]")
@@ -1042,20 +1074,23 @@ def map_slots(pool: PagePool, block_table, lengths, counts, *, tokens: int, bloc
         if keep.dtype != torch.bool or keep.shape != (tokens,):
             raise ValueError(f"keep must be bool [{tokens}]")
         keep = keep.contiguous()
-    need = _lib.load().oscarop_map_workspace_bytes_v1(reqs, tokens, keep is not None)
-    # one piece of memory: slots and positions, then starts, lengths and the workspace, then grants
-    words = 4 * tokens + 2 * reqs + 1 + max(need, 0) // 4
-    buf = torch.empty(4 * words + reqs, dtype=torch.uint8, device=dev)
-    wide, narrow = buf[:16 * tokens].view(torch.int64), buf[16 * tokens:4 * words].view(torch.int32)
-    out = SlotMap(narrow[:reqs + 1], narrow[reqs + 1:2 * reqs + 1], wide[:tokens], wide[tokens:],
-                  buf[4 * words:].view(torch.bool))
-    base = buf.data_ptr()
-    at = base + 16 * tokens
-    a = _lib.MapArgs(lengths.data_ptr(), counts.data_ptr(), _ptr(keep), reqs, block_size, tokens, block_table.data_ptr(),
-                     stride, *block_table.shape, pool.pages.data_ptr(), pool.count.data_ptr(), pool.pages.shape[0], at,
-                     at + 4 * (reqs + 1), base, base + 8 * tokens, base + 4 * words, at + 4 * (2 * reqs + 1), max(need, 0))
+    wide = torch.empty(2, tokens, dtype=torch.int64, device=dev)
+    narrow = torch.empty(2 * reqs + 1, dtype=torch.int32, device=dev)
+    granted = torch.empty(reqs, dtype=torch.bool, device=dev)
+    slots, positions, at = wide.data_ptr(), wide.data_ptr() + 8 * tokens, narrow.data_ptr()
+    ws, need = None, 0
+    if keep is not None:
+        need = _lib.load().oscarop_map_workspace_bytes_v1(reqs, tokens, 1)
+        if need > 0:
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)  # a captured call keeps its own
+    rows, cols = block_table.shape
+    a = _lib.MapArgs.from_buffer_copy(_MAP(
+        lengths.data_ptr(), counts.data_ptr(), 0 if keep is None else keep.data_ptr(), reqs, block_size, tokens,
+        block_table.data_ptr(), stride, rows, cols, pool.pages.data_ptr(), pool.count.data_ptr(), pool.pages.shape[0], at,
+        at + 4 * (reqs + 1), slots, positions, granted.data_ptr(), 0 if ws is None else ws.data_ptr(), max(need, 0)))
     _launch("oscarop_map_v1", index, C.byref(a))
-    return out
+    starts, seq_lens = narrow.split_with_sizes([reqs + 1, reqs])
+    return SlotMap(starts, seq_lens, *wide.unbind(), granted)
 
 
 def release_pages(pool: PagePool, block_table, lengths, new_lengths, *, block_size: int) -> None:
@@ -1072,8 +1107,9 @@ def release_pages(pool: PagePool, block_table, lengths, new_lengths, *, block_si
     if block_size < 1:
         raise ValueError("block_size must be at least 1")
     stride = _own_rows(block_table, reqs)
-    a = _lib.ReleaseArgs(lengths.data_ptr(), new_lengths.data_ptr(), reqs, block_size, block_table.data_ptr(), stride,
-                         *block_table.shape, pool.pages.data_ptr(), pool.count.data_ptr(), pool.pages.shape[0])
+    a = _lib.ReleaseArgs.from_buffer_copy(_RELEASE(lengths.data_ptr(), new_lengths.data_ptr(), reqs, block_size,
+                                                   block_table.data_ptr(), stride, *block_table.shape, pool.pages.data_ptr(),
+                                                   pool.count.data_ptr(), pool.pages.shape[0]))
     _launch("oscarop_release_v1", index, C.byref(a))
 
 
@@ -1107,21 +1143,25 @@ def tree_mask(parents, qsl, *, max_nodes: int) -> tuple:
     return mask, depths
 
 
-@dataclass
+@dataclass(frozen=True)
 class TreePlan:
-    """A plan of attention_tree: the requests of a batch, host lists and device records."""
-    host_qsl: list
-    host_seqs: list
+    """A plan of attention_tree: the requests of a batch and the records of its launch."""
+    host_qsl: tuple
+    host_seqs: tuple
+    num_kv_heads: int
+    group: int
+    head_dim: int
     num_items: int
     num_groups: int
     partial_rows: int
     partial_bytes: int
+    max_history: int        # tokens
+    max_nodes: int
+    rows: int               # query rows that the requests tile, -1 if they leave some out
     items: torch.Tensor     # device int32, as all of these
     groups: torch.Tensor
     qsl: torch.Tensor
     seqs: torch.Tensor
-    has_new = True
-    max_group_items = 0
 
 
 def plan_tree(qsl, seqs, *, num_kv_heads: int, group: int, head_dim: int, device, window: tuple = (0, 0)) -> TreePlan:
@@ -1145,15 +1185,15 @@ def plan_tree(qsl, seqs, *, num_kv_heads: int, group: int, head_dim: int, device
     groups = np.zeros((max(sizes.num_groups, 1), GROUP_INTS), np.int32)
     plan(items, groups)
     parts = upload([items.reshape(-1), groups.reshape(-1), np.asarray(qsl, np.int32), np.asarray(seqs or [0], np.int32)], device)
-    return TreePlan(qsl, seqs, sizes.num_items, sizes.num_groups, sizes.partial_rows, sizes.partial_bytes, *parts)
+    nodes = [b - a for a, b in zip(qsl, qsl[1:])]
+    return TreePlan(tuple(qsl), tuple(seqs), num_kv_heads, group, head_dim, sizes.num_items, sizes.num_groups,
+                    sizes.partial_rows, sizes.partial_bytes, max((s - n for s, n in zip(seqs, nodes)), default=0),
+                    max(nodes, default=0), qsl[-1] if qsl[0] == 0 else -1, *parts)
 
 
-def _attention_over(entry, q, k_new, v_new, k_cache, v_cache, table, rows_of_table, plan, scale, stage, head_dim, soft_cap,
-                    out_rot, lse, others, extra=(), mask=None):
-    """The entry points beside attention_decode, which take its arguments and `extra` ones.
-    table: [requests, columns] as the kernels address it; others: more tensors of the call."""
-    index = _device_index(q, k_new, v_new, k_cache, v_cache, table, out_rot, lse, *others, *(stage or ()))
-    score = score_struct(soft_cap, None, q.shape[1], q.device)
+def _attention_rows(q, k_new, v_new, k_cache, rows: int, plan, head_dim: int, out_rot, lse) -> tuple:
+    """The checks that attention_tree and attention_selected share; their operands as the kernels
+    read them.  rows: the query rows that the plan's requests tile, -1 if they leave some out."""
     code = _DTYPES.get(q.dtype)
     if code is None or code == OSCAR_F32:
         raise ValueError("OSCAR HIP attention requires bf16 or fp16 queries")
@@ -1161,51 +1201,31 @@ def _attention_over(entry, q, k_new, v_new, k_cache, v_cache, table, rows_of_tab
         raise ValueError("q must be [tokens, heads, head_dim]")
     n, hq, _ = q.shape
     hk = k_cache.shape[2]
-    if hq % hk:
-        raise ValueError("Hq must be a multiple of Hk")
-    if plan.has_new != (k_new is not None) or (k_new is None) != (v_new is None):
-        raise ValueError("plan and call disagree on the presence of current K/V")
-    if plan.items is None:
-        raise ValueError("the plan has not been uploaded")
+    if hk != plan.num_kv_heads or hq != hk * plan.group or head_dim != plan.head_dim:
+        raise ValueError(f"the plan is for {plan.num_kv_heads} KV heads of {plan.head_dim} and {plan.group} query heads each")
     if plan.host_qsl[-1] > n:
         raise ValueError("the plan has more queries than the call")
     if k_new is not None:
-        for x in (k_new, v_new):
-            if x.dtype != q.dtype or x.shape != (n, hk, head_dim):
-                raise ValueError("Current K/V must match the queries' type and tokens and the cache's heads")
+        shape = (n, hk, head_dim)
+        if k_new.dtype != q.dtype or v_new.dtype != q.dtype or k_new.shape != shape or v_new.shape != shape:
+            raise ValueError("Current K/V must match the queries' type and tokens and the cache's heads")
         k_new, v_new = _aligned(k_new), _aligned(v_new)
-    if q.stride(2) != 1 or q.stride(1) != head_dim or q.stride(0) % 8 or q.data_ptr() % 16:
+    s0, s1, s2 = q.stride()
+    if s2 != 1 or s1 != head_dim or s0 % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
-    all_rows = plan.num_items > 0 and _covers(plan, n)
+        s0 = hq * head_dim
+    # rows of no request stay zero (lse -inf); the kernels write every row of a request
     if out_rot is None:
-        # rows of no request stay zero (lse -inf); the merge writes every row of a request
-        out_rot = (torch.empty if all_rows else torch.zeros)(n, hq, head_dim, dtype=torch.float32, device=q.device)
+        out_rot = (torch.empty if rows == n else torch.zeros)(n, hq, head_dim, dtype=torch.float32, device=q.device)
     elif out_rot.dtype != torch.float32 or out_rot.shape != q.shape or not out_rot.is_contiguous():
         raise ValueError("out_rot must be contiguous fp32 [tokens, heads, head_dim]")
     if lse is None:
         lse = torch.empty(n, hq, dtype=torch.float32, device=q.device)
-        if not all_rows:
+        if rows != n:
             lse.fill_(-math.inf)
     elif lse.dtype != torch.float32 or lse.shape != (n, hq) or not lse.is_contiguous():
         raise ValueError("lse must be contiguous fp32 [tokens, heads]")
-    if plan.num_items == 0 or n == 0:
-        return out_rot, lse
-    if table.shape[0] < len(plan.host_seqs):
-        raise ValueError("Missing request block-table rows")
-    if _plan_sizes(plan, k_cache.shape[1])[0] > rows_of_table:
-        raise ValueError("Block table cannot cover the history")
-    st = staging_struct(stage, k_cache, head_dim)
-    ws = _call_workspace(index, "attn_workspace", plan.partial_bytes)
-    a = _lib.AttnArgs(q.data_ptr(), n, hq, q.stride(0), _ptr(k_new), _ptr(v_new), 0 if k_new is None else k_new.stride(0),
-                      cache_struct(k_cache, v_cache, head_dim), table.data_ptr(), table.stride(0), plan.qsl.data_ptr(),
-                      plan.seqs.data_ptr(), plan.seqs.numel(), None if st is None else C.pointer(st), scale,
-                      plan.items.data_ptr(), plan.num_items, plan.groups.data_ptr(), plan.num_groups, ws.data_ptr(),
-                      ws.numel(), plan.max_group_items, out_rot.data_ptr(), lse.data_ptr(), 0, code, table.shape[0],
-                      rows_of_table)
-    if mask is not None:
-        a = _lib.TreeAttnArgs(a, mask.data_ptr(), mask.shape[1], plan.partial_rows)
-    _launch(entry, index, C.byref(a), None if score is None else C.byref(score), *extra)
-    return out_rot, lse
+    return q, s0, k_new, v_new, code, out_rot, lse
 
 
 def attention_tree(q, k_new, v_new, k_cache, v_cache, block_table, plan: TreePlan, mask, scale, stage=None, *, head_dim,
@@ -1218,18 +1238,35 @@ def attention_tree(q, k_new, v_new, k_cache, v_cache, block_table, plan: TreePla
     for each 64 rows of the longest chunk).  A row that sees no key gets zeros and -inf.
     plan: plan_tree(...).  The nodes' keys and values are k_new and v_new: accepted ones are
     written afterwards, by ops.store with the slots of map_slots(keep=...)."""
-    if mask.dtype != torch.int64 or mask.ndim != 2 or mask.shape[0] != q.shape[0]:
-        raise ValueError("mask must be int64 [tokens, words]")
-    most = _plan_sizes(plan, k_cache.shape[1])[2]
-    if most > 64 * mask.shape[1]:
-        raise ValueError(f"a mask of {mask.shape[1]} words for {most} rows of a request")
-    if k_new is None:
+    index = _device_index(q, k_new, v_new, k_cache, v_cache, block_table, mask, plan.items, out_rot, lse, *(stage or ()))
+    if k_new is None or v_new is None:
         raise ValueError("a tree's attention needs its nodes' K and V")
+    score = None if soft_cap == 0 else score_struct(soft_cap, None, q.shape[1], q.device)
+    q, stride, k_new, v_new, code, out_rot, lse = _attention_rows(q, k_new, v_new, k_cache, plan.rows, plan, head_dim, out_rot,
+                                                                  lse)
+    n, hq = lse.shape
+    if mask.dtype != torch.int64 or mask.ndim != 2 or mask.shape[0] != n:
+        raise ValueError("mask must be int64 [tokens, words]")
+    if plan.max_nodes > 64 * mask.shape[1]:
+        raise ValueError(f"a mask of {mask.shape[1]} words for {plan.max_nodes} rows of a request")
+    if plan.num_items == 0:
+        return out_rot, lse
     mask, table = mask.contiguous(), _rows_apart(block_table)
-    if table.ndim != 2:
+    if table.ndim != 2 or table.shape[0] < len(plan.host_seqs):
         raise ValueError("Missing request block-table rows")
-    return _attention_over("oscarop_attn_tree_v1", q, k_new, v_new, k_cache, v_cache, table, table.shape[1], plan, scale,
-                           stage, head_dim, soft_cap, out_rot, lse, (mask, plan.items), mask=mask)
+    cache = _cache_values(k_cache, v_cache, head_dim)
+    if -(-plan.max_history // cache[3]) > table.shape[1]:
+        raise ValueError("Block table cannot cover the history")
+    st = staging_struct(stage, k_cache, head_dim)
+    ws = _call_workspace(index, "attn_workspace", plan.partial_bytes)
+    a = _lib.TreeAttnArgs.from_buffer_copy(_ATTN(
+        q.data_ptr(), n, hq, stride, k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), *cache, table.data_ptr(),
+        table.stride(0), plan.qsl.data_ptr(), plan.seqs.data_ptr(), len(plan.host_seqs),
+        0 if st is None else C.addressof(st), scale, plan.items.data_ptr(), plan.num_items, plan.groups.data_ptr(),
+        plan.num_groups, ws.data_ptr(), ws.numel(), 0, out_rot.data_ptr(), lse.data_ptr(), 0, code, *table.shape)
+        + _TREE(mask.data_ptr(), mask.shape[1], plan.partial_rows))
+    _launch("oscarop_attn_tree_v1", index, C.byref(a), None if score is None else C.byref(score))
+    return out_rot, lse
 
 
 # ------------------------------------------------------------------------ chosen pages
@@ -1243,37 +1280,39 @@ def page_bounds(k_cache, bounds, block_table, lengths, seq_lens, *, max_new: int
     the most new tokens of a request.  Call it after the step's store; after an eviction with
     lengths 0 (kept tokens have moved)."""
     index = _device_index(k_cache, bounds, block_table, lengths, seq_lens)
-    cache = cache_struct(k_cache, k_cache, head_dim)
+    cache = _cache_values(k_cache, k_cache, head_dim)
     reqs = lengths.shape[0] if lengths.ndim == 1 else -1
     lengths, seq_lens = _int32_list("lengths", lengths, reqs), _int32_list("seq_lens", seq_lens, reqs)
-    if bounds.dtype != torch.float16 or bounds.shape != (cache.num_blocks, cache.num_kv_heads, 2, head_dim) \
-            or not bounds.is_contiguous():
+    if bounds.dtype != torch.float16 or bounds.shape != (cache[2], cache[4], 2, head_dim) or not bounds.is_contiguous():
         raise ValueError("bounds must be contiguous fp16 [blocks, KV heads, 2, head_dim]")
     if max_new < 0:
         raise ValueError("max_new must not be negative")
     table = _rows_apart(block_table)
     if table.ndim != 2 or table.shape[0] < reqs:
         raise ValueError("Missing request block-table rows")
-    a = _lib.BoundsArgs(cache, table.data_ptr(), table.stride(0), *table.shape, lengths.data_ptr(), seq_lens.data_ptr(), reqs, 0,
-                        max_new, bounds.data_ptr())
+    a = _lib.BoundsArgs.from_buffer_copy(_BOUNDS(*cache, table.data_ptr(), table.stride(0), *table.shape, lengths.data_ptr(),
+                                                 seq_lens.data_ptr(), reqs, 0, max_new, bounds.data_ptr()))
     _launch("oscarop_page_bounds_v1", index, C.byref(a))
     return bounds
 
 
-@dataclass
+@dataclass(frozen=True)
 class SelectPlan:
     """A batch whose requests read `budget` pages of their history at most (plan_selected)."""
     decode: DecodePlan   # of the chosen tokens
-    host_qsl: list
-    host_seqs: list
+    host_qsl: tuple
+    host_seqs: tuple
     has_new: bool
     block_size: int
     budget: int
     first_pages: int
     last_pages: int
-    max_pages: int       # of the longest history
     num_kv_heads: int
+    group: int
     head_dim: int
+    max_pages: int       # of the longest history
+    rows: int            # query rows that the requests tile, -1 if they leave some out
+    workspace_bytes: int # of select_pages
     qsl: torch.Tensor    # device int32
     seqs: torch.Tensor
 
@@ -1296,8 +1335,13 @@ def plan_selected(qsl, seqs, *, has_new: bool, block_size: int, budget: int, fir
                        device=device, window=window, upload_now=False)
     parts = upload(plan.host_parts() + [np.asarray(seqs or [0], np.int32)], device)
     plan.adopt(parts[:4])
-    return SelectPlan(plan, qsl, seqs, bool(has_new), block_size, budget, first_pages, last_pages, most, num_kv_heads,
-                      head_dim, plan.qsl, parts[4])
+    sizes = _lib.SelectArgs(num_kv_heads=num_kv_heads, num_reqs=len(seqs), max_pages=most, budget=budget)
+    need = _lib.load().oscarop_select_workspace_bytes_v1(C.byref(sizes))
+    if need < 0:
+        raise ValueError("plan_selected: requests, KV heads or pages out of range")
+    covered = qsl[-1] if qsl[0] == 0 and plan.num_items > 0 else -1
+    return SelectPlan(plan, tuple(qsl), tuple(seqs), bool(has_new), block_size, budget, first_pages, last_pages, num_kv_heads,
+                      group, head_dim, most, covered, need, plan.qsl, parts[4])
 
 
 def select_pages(q, bounds, block_table, plan: SelectPlan) -> tuple:
@@ -1326,19 +1370,22 @@ def select_pages(q, bounds, block_table, plan: SelectPlan) -> tuple:
         raise ValueError("Missing request block-table rows")
     if plan.max_pages > table.shape[1]:
         raise ValueError("Block table cannot cover the history")
-    if q.stride(2) != 1 or q.stride(1) != d or q.stride(0) % 8 or q.data_ptr() % 16:
+    s0, s1, s2 = q.stride()
+    if s2 != 1 or s1 != d or s0 % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
+        s0 = q.shape[1] * d
     out = torch.empty(2, reqs, hk, plan.budget, dtype=torch.int32, device=q.device)
-    a = _lib.SelectArgs(q.data_ptr(), q.shape[0], q.shape[1], q.stride(0), code, plan.has_new, bounds.data_ptr(),
-                        bounds.shape[0], hk, d, plan.block_size, table.data_ptr(), table.stride(0), *table.shape,
-                        plan.qsl.data_ptr(), plan.seqs.data_ptr(), reqs, plan.max_pages, plan.budget, plan.first_pages,
-                        plan.last_pages, 0, out.data_ptr(), out.data_ptr() + 4 * reqs * hk * plan.budget, None, 0)
-    need = _lib.load().oscarop_select_workspace_bytes_v1(C.byref(a))
+    at, need, ws, arrivals = out.data_ptr(), plan.workspace_bytes, None, None
     if need > 0:
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)  # a captured call keeps its own
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        arrivals = _arrivals(index, reqs * hk)
+    a = _lib.SelectArgs.from_buffer_copy(_SELECT(
+        q.data_ptr(), q.shape[0], q.shape[1], s0, code, plan.has_new, bounds.data_ptr(), bounds.shape[0], hk, d,
+        plan.block_size, table.data_ptr(), table.stride(0), *table.shape, plan.qsl.data_ptr(), plan.seqs.data_ptr(), reqs,
+        plan.max_pages, plan.budget, plan.first_pages, plan.last_pages, 0, at, at + 4 * reqs * hk * plan.budget,
+        0 if ws is None else ws.data_ptr(), need, 0 if arrivals is None else arrivals.data_ptr()))
     _launch("oscarop_select_v1", index, C.byref(a))
-    return out[0], out[1]
+    return out.unbind()
 
 
 def attention_selected(q, k_new, v_new, k_cache, v_cache, table, plan: SelectPlan, scale, stage=None, *, head_dim,
@@ -1346,12 +1393,32 @@ def attention_selected(q, k_new, v_new, k_cache, v_cache, table, plan: SelectPla
     """Attention over the pages that select_pages chose, and the current chunk: (out_rot fp32,
     lse fp32), rotated, as attention_decode's, whose other arguments these are.  table
     [requests, Hk, budget]: each KV head's pages, ascending."""
-    hk = k_cache.shape[2]
-    if table.dtype != torch.int32 or table.ndim != 3 or table.shape[1:] != (hk, plan.budget):
+    index = _device_index(q, k_new, v_new, k_cache, v_cache, table, plan.qsl, out_rot, lse, *(stage or ()))
+    if plan.has_new != (k_new is not None) or (k_new is None) != (v_new is None):
+        raise ValueError("plan and call disagree on the presence of current K/V")
+    score = None if soft_cap == 0 else score_struct(soft_cap, None, q.shape[1], q.device)
+    q, stride, k_new, v_new, code, out_rot, lse = _attention_rows(q, k_new, v_new, k_cache, plan.rows, plan, head_dim, out_rot,
+                                                                  lse)
+    n, hq = lse.shape
+    hk, budget, decode = plan.num_kv_heads, plan.budget, plan.decode
+    if table.dtype != torch.int32 or table.ndim != 3 or table.shape[1:] != (hk, budget):
         raise ValueError("table must be int32 [requests, KV heads, budget]")
-    if plan.block_size != k_cache.shape[1] or plan.num_kv_heads != hk:
-        raise ValueError(f"the plan is for {plan.num_kv_heads} KV heads and pages of {plan.block_size} tokens")
+    reqs = table.shape[0]
+    if reqs < len(plan.host_seqs):
+        raise ValueError("Missing request block-table rows")
+    cache = _cache_values(k_cache, v_cache, head_dim)
+    if plan.block_size != cache[3]:
+        raise ValueError(f"the plan is for pages of {plan.block_size} tokens, the cache has {cache[3]}")
+    if decode.num_items == 0:
+        return out_rot, lse
     table = table.contiguous()
-    flat = table.view(table.shape[0], hk * plan.budget)
-    return _attention_over("oscarop_attn_selected_v1", q, k_new, v_new, k_cache, v_cache, flat, plan.budget, plan.decode,
-                           scale, stage, head_dim, soft_cap, out_rot, lse, (plan.qsl,), (plan.budget,))
+    st = staging_struct(stage, k_cache, head_dim)
+    ws = _call_workspace(index, "attn_workspace", decode.partial_bytes)
+    a = _lib.AttnArgs.from_buffer_copy(_ATTN(
+        q.data_ptr(), n, hq, stride, *((0, 0, 0) if k_new is None else (k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0))),
+        *cache, table.data_ptr(), hk * budget, decode.qsl.data_ptr(), decode.seqs.data_ptr(), len(plan.host_seqs),
+        0 if st is None else C.addressof(st), scale, decode.items.data_ptr(), decode.num_items, decode.groups.data_ptr(),
+        decode.num_groups, ws.data_ptr(), ws.numel(), decode.max_group_items, out_rot.data_ptr(), lse.data_ptr(), 0, code,
+        reqs, budget))
+    _launch("oscarop_attn_selected_v1", index, C.byref(a), None if score is None else C.byref(score), budget)
+    return out_rot, lse
