@@ -25,7 +25,9 @@
 // Values: K is the reference's bf16 or fp16 of fp16(code * scale + zero), V fp16(...)
 // unrounded, the window's FP32 copies likewise; P fp16, up to 2^15, the reference m 2^7 below the
 // largest score at its last move, so that keys of 2^-21 of the largest still keep 11 bits.  The chunk's
-// V in bf16 have a wider range than fp16: chunk tiles multiply it by P in two bf16 parts.
+// V in bf16 have a wider range than fp16: chunk tiles multiply it by P in two bf16 parts.  A
+// value of the chunk that is not finite goes into LDS as zero and is added afterwards, to the
+// rows alone that see its node.
 #include <vector>
 
 #include "common.h"
@@ -76,6 +78,9 @@ __device__ __forceinline__ u32x4 kpairs8(const u32x4& x) {
                __builtin_amdgcn_perm(x[3], x[1], 0x05040100u), __builtin_amdgcn_perm(x[3], x[1], 0x07060302u)};
 }
 
+// element of a row in LDS order (kpairs8)
+__device__ __forceinline__ int column(int i) { return (i & ~7) + ((i & 7) >> 1) + 4 * (i & 1); }
+
 struct Item {
   int req, kvh, qa, n, hist, row0, rows, first, stride, count, part;
 };
@@ -88,7 +93,8 @@ struct Place {
 // The tiles of one item: full ones of the history, or (SLOW) its ragged end and the chunk's.  Apart, since
 // what the latter need does not fit beside O and the queries in the others' loop.
 template <int D, int QT, int SC, bool SLOW>
-__device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uint8_t* s_k, uint8_t* s_v, const Place* s_place) {
+__device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uint8_t* s_k, uint8_t* s_v, const Place* s_place,
+                                         uint32_t* s_odd) {
   using C = Cfg<D>;
   const oscarop_tree_attn_args_v1& T = P.a;
   const oscar_attn_args_v1& A = T.attn;
@@ -170,6 +176,7 @@ __device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uin
       *dest(i, buf) = o;
     }
   };
+  constexpr unsigned kInf = QT == OSCAR_BF16 ? 0x7f80u : 0x7c00u;  // the exponent of infinities and NaN
   // tile t at once: the history's ragged end (unseen keys zero), or one of the chunk's
   auto fill_slow = [&](int t, int j) {
     const bool chunk = t >= htiles;
@@ -184,8 +191,21 @@ __device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uin
     }
     const u32x4* src = (const u32x4*)((const uint16_t*)(vside ? A.v_new : A.k_new) + (int64_t)(I.qa + (key < I.n ? key : 0)) * A.kv_new_stride_token +
                                       (int64_t)I.kvh * D + 32 * vec);
+    bool odd = false;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *dest(i, 0) = key < I.n ? kpairs8(src[i]) : u32x4{0u, 0u, 0u, 0u};
+    for (int i = 0; i < 4; ++i) {
+      u32x4 x = key < I.n ? kpairs8(src[i]) : u32x4{0u, 0u, 0u, 0u};
+      if (vside) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned low = x[e] & kInf, high = (x[e] >> 16) & kInf;
+          odd |= low == kInf || high == kInf;
+          x[e] &= (low == kInf ? 0u : 0xffffu) | (high == kInf ? 0u : 0xffff0000u);
+        }
+      }
+      *dest(i, 0) = x;
+    }
+    if (odd) atomicOr(&s_odd[sub], 1u << in32);
   };
 
   // ---- running state of this lane's row
@@ -225,6 +245,7 @@ __device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uin
     }
   };
   // unseen keys of a slow tile
+  uint64_t sees = 0;  // the tile's keys that this lane's row sees
   auto mask = [&](int t) {
     const int j0 = (t - htiles) * C::KT;  // a multiple of 32
     const int left = I.hist - t * C::KT;  // keys of a history tile
@@ -237,11 +258,31 @@ __device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uin
         if (last < 63) see &= (2ull << last) - 1;
       }
     }
+    sees = see;
 #pragma unroll
     for (int a = 0; a < C::KSUB; ++a)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         if (!((see >> (32 * a + out_tok(r, g))) & 1)) S[a][r] = -INFINITY;
+  };
+  // O += p v for the values of key k of chunk tile t that are not finite, in the rows that see it;
+  // p comes from the lane of the row that holds the key
+  auto add_odd = [&](int t, int k) {
+    float mine = 0.f;
+#pragma unroll
+    for (int a = 0; a < C::KSUB; ++a)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mine = 32 * a + out_tok(r, g) == k ? S[a][r] : mine;
+    const float other = swap_halves(mine), p = ((k >> 2) & 1) == g ? mine : other;
+    const bool seen = (sees >> k) & 1;
+    const uint16_t* v = (const uint16_t*)A.v_new + (int64_t)(I.qa + (t - htiles) * C::KT + k) * A.kv_new_stride_token + (int64_t)I.kvh * D;
+#pragma unroll
+    for (int b = 0; b < C::NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const unsigned x = v[column(32 * b + out_tok(r, g))];
+        if (seen && (x & kInf) == kInf) O[b][r] = fmaf(p, QT == OSCAR_BF16 ? bf16_bits_to_f32(x) : f16_bits_to_f32(x), O[b][r]);
+      }
   };
   // p = exp2(score - reference); the reference moves, and O with it, where a score comes 2^15 above it
   auto softmax = [&]() {
@@ -361,7 +402,9 @@ __device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uin
   } else {
     auto scores = [&](int j) {
       const int t = I.first + I.stride * j;
-      if (j > 0) __syncthreads();  // the buffers have been read
+      __syncthreads();  // the buffers and s_odd have been read
+      if (tid < 2) s_odd[tid] = 0;
+      __syncthreads();
       fill_slow(t, j);
       __syncthreads();
       qk(0);
@@ -377,6 +420,10 @@ __device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uin
 #pragma unroll 1
     for (; j < I.count; ++j) {
       scores(j);
+#pragma unroll 1
+      for (int a = 0; a < C::KSUB; ++a)
+        for (uint32_t odd = __builtin_amdgcn_readfirstlane(s_odd[a]); odd != 0; odd &= odd - 1)
+          add_odd(I.first + I.stride * j, 32 * a + __builtin_ctz(odd));
       if constexpr (QT == OSCAR_BF16) {
         pv_chunk(0);
       } else {
@@ -424,6 +471,8 @@ __global__ __launch_bounds__(kThreads, 2) void tree_main_kernel(TreeParams P) {
   __shared__ __attribute__((aligned(16))) uint8_t s_k[2 * C::KBYTES];
   __shared__ __attribute__((aligned(16))) uint8_t s_v[2 * C::VBYTES];
   __shared__ Place s_place[kMostTiles * C::KSUB];
+  __shared__ uint32_t s_odd[2];  // a chunk tile's keys whose values are not all finite
+  if (tid < 2) s_odd[tid] = 0;
   const int full = I.hist / C::KT;  // full tiles of the history
   for (int i = tid; i < I.count * C::KSUB; i += kThreads) {
     const int64_t key = (int64_t)(I.first + I.stride * (i / C::KSUB)) * C::KT + 32 * (i % C::KSUB);
@@ -437,8 +486,8 @@ __global__ __launch_bounds__(kThreads, 2) void tree_main_kernel(TreeParams P) {
     s_place[i] = x;
   }
 
-  if (I.first >= full) run_item<D, QT, SC, true>(P, I, s_k, s_v, s_place);
-  else run_item<D, QT, SC, false>(P, I, s_k, s_v, s_place);
+  if (I.first >= full) run_item<D, QT, SC, true>(P, I, s_k, s_v, s_place, s_odd);
+  else run_item<D, QT, SC, false>(P, I, s_k, s_v, s_place, s_odd);
 }
 
 // The items of a block of rows, merged by their log-sum-exps.  One row a 64-lane (D 256) or

@@ -183,3 +183,102 @@ def evict(weights: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
 def _(weights, k_cache, v_cache, block_table, seq_lens, drop_pages, stage_k, stage_v, owner, head_dim, sink_tokens=0,
       recent_tokens=0):
     return weights.new_empty(weights.shape)
+
+
+# ------------------------------------------------------------------ pages and slots
+@torch.library.custom_op(f"{_LIB}::map_slots", mutates_args=("pool_count", "block_table"), device_types="cuda")
+def map_slots(pool_pages: torch.Tensor, pool_count: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+              counts: torch.Tensor, tokens: int, block_size: int,
+              keep: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    m = ops.map_slots(ops.PagePool(pool_pages, pool_count), block_table, lengths, counts, tokens=tokens, block_size=block_size,
+                      keep=keep)
+    # (outputs of an operator share no memory)
+    return m.qsl, m.seq_lens.clone(), m.slots, m.positions.clone(), m.granted
+
+
+@map_slots.register_fake
+def _(pool_pages, pool_count, block_table, lengths, counts, tokens, block_size, keep=None):
+    reqs = lengths.shape[0]
+    return (lengths.new_empty(reqs + 1), lengths.new_empty(reqs), lengths.new_empty(tokens, dtype=torch.int64),
+            lengths.new_empty(tokens, dtype=torch.int64), lengths.new_empty(reqs, dtype=torch.bool))
+
+
+@torch.library.custom_op(f"{_LIB}::release_pages", mutates_args=("pool_pages", "pool_count"), device_types="cuda")
+def release_pages(pool_pages: torch.Tensor, pool_count: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+                  new_lengths: torch.Tensor, block_size: int) -> None:
+    ops.release_pages(ops.PagePool(pool_pages, pool_count), block_table, lengths, new_lengths, block_size=block_size)
+
+
+@release_pages.register_fake
+def _(pool_pages, pool_count, block_table, lengths, new_lengths, block_size):
+    return None
+
+
+# ------------------------------------------------------------------ drafted trees
+@torch.library.custom_op(f"{_LIB}::tree_mask", mutates_args=(), device_types="cuda")
+def tree_mask(parents: torch.Tensor, query_start_loc: torch.Tensor, max_nodes: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return ops.tree_mask(parents, query_start_loc, max_nodes=max_nodes)
+
+
+@tree_mask.register_fake
+def _(parents, query_start_loc, max_nodes):
+    n = parents.shape[0]
+    return parents.new_empty((n, -(-max_nodes // 64)), dtype=torch.int64), parents.new_empty(n)
+
+
+@torch.library.custom_op(f"{_LIB}::attention_tree", mutates_args=(), device_types="cuda")
+def attention_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   block_table: torch.Tensor, query_start_loc: list[int], seq_lens: list[int], mask: torch.Tensor, scale: float,
+                   head_dim: int, stage_k: torch.Tensor | None = None, stage_v: torch.Tensor | None = None,
+                   owner: torch.Tensor | None = None, soft_cap: float = 0.0) -> tuple[torch.Tensor, torch.Tensor]:
+    hq, hk = q.shape[1], k_cache.shape[2]
+    plan = ops.plan_tree(query_start_loc, seq_lens, num_kv_heads=hk, group=hq // hk, head_dim=head_dim, device=q.device)
+    return ops.attention_tree(q, k_new, v_new, k_cache, v_cache, block_table, plan, mask, scale, _stage(stage_k, stage_v, owner),
+                              head_dim=head_dim, soft_cap=soft_cap)
+
+
+@attention_tree.register_fake
+def _(q, k_new, v_new, k_cache, v_cache, block_table, query_start_loc, seq_lens, mask, scale, head_dim, stage_k=None,
+      stage_v=None, owner=None, soft_cap=0.0):
+    n, hq = q.shape[0], q.shape[1]
+    return (q.new_empty((n, hq, head_dim), dtype=torch.float32), q.new_empty((n, hq), dtype=torch.float32))
+
+
+# ------------------------------------------------------------------ chosen pages
+@torch.library.custom_op(f"{_LIB}::page_bounds", mutates_args=("bounds",), device_types="cuda")
+def page_bounds(k_cache: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+                seq_lens: torch.Tensor, max_new: int, head_dim: int) -> None:
+    ops.page_bounds(k_cache, bounds, block_table, lengths, seq_lens, max_new=max_new, head_dim=head_dim)
+
+
+@page_bounds.register_fake
+def _(k_cache, bounds, block_table, lengths, seq_lens, max_new, head_dim):
+    return None
+
+
+@torch.library.custom_op(f"{_LIB}::attention_selected", mutates_args=(), device_types="cuda")
+def attention_selected(q: torch.Tensor, k_new: torch.Tensor | None, v_new: torch.Tensor | None, k_cache: torch.Tensor,
+                       v_cache: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, query_start_loc: list[int],
+                       seq_lens: list[int], budget: int, scale: float, head_dim: int, first_pages: int = 1,
+                       last_pages: int = 1, stage_k: torch.Tensor | None = None, stage_v: torch.Tensor | None = None,
+                       owner: torch.Tensor | None = None, sink_tokens_eff: int = 0, recent_tokens: int = 0,
+                       soft_cap: float = 0.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The choice and the attention in one: (out_rot, lse, chosen columns)."""
+    hq, hk = q.shape[1], k_cache.shape[2]
+    stage = _stage(stage_k, stage_v, owner)
+    window = (sink_tokens_eff, recent_tokens) if stage is not None else (0, 0)
+    plan = ops.plan_selected(query_start_loc, seq_lens, has_new=k_new is not None, block_size=k_cache.shape[1], budget=budget,
+                             first_pages=first_pages, last_pages=last_pages, num_kv_heads=hk, group=hq // hk,
+                             head_dim=head_dim, device=q.device, window=window)
+    table, pages = ops.select_pages(q, bounds, block_table, plan)
+    out, lse = ops.attention_selected(q, k_new, v_new, k_cache, v_cache, table, plan, scale, stage, head_dim=head_dim,
+                                      soft_cap=soft_cap)
+    return out, lse, pages
+
+
+@attention_selected.register_fake
+def _(q, k_new, v_new, k_cache, v_cache, bounds, block_table, query_start_loc, seq_lens, budget, scale, head_dim,
+      first_pages=1, last_pages=1, stage_k=None, stage_v=None, owner=None, sink_tokens_eff=0, recent_tokens=0, soft_cap=0.0):
+    n, hq = q.shape[0], q.shape[1]
+    return (q.new_empty((n, hq, head_dim), dtype=torch.float32), q.new_empty((n, hq), dtype=torch.float32),
+            block_table.new_empty((len(seq_lens), k_cache.shape[2], budget)))
