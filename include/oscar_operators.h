@@ -316,8 +316,8 @@ int oscarop_page_bounds_v1(const oscarop_bounds_args_v1* args, void* stream);
  * Request r has n_q queries and a history of h tokens (seq_lens[r], less n_q with has_new)
  * in P = ceil(h / block_size) pages.  With P <= budget all of them are chosen, otherwise the first
  * first_pages, the last last_pages and of the others those of the largest score (equal
- * scores: the earlier page first; a NaN score counts as the largest), budget in all, for each
- * KV head its own.  A page's score: the largest, over the request's queries and the query
+ * scores: the earlier page first; a score of a bound or a query that is not finite counts as the
+ * largest), budget in all, for each KV head its own.  A page's score: the largest, over the request's queries and the query
  * heads of the KV head, of the sum over the channels of max(q low, q high), summed in 64
  * bits.  table[r][h] holds the chosen pages in ascending order of their columns and
  * pages[r][h] these columns, -1 behind them.  A request that does not fit (queries past

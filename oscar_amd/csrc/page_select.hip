@@ -378,7 +378,9 @@ __global__ __launch_bounds__(kThreads, 2) void select_kernel(SelectParams P) {
         sum += dpp_row64<kDppXor1>(sum);
         sum += dpp_row64<kDppXor2>(sum);
         sum += dpp_row64<kDppHalfMirror>(sum);
-        // (a NaN stays)
+        // Finite bounds and queries have finite sums; m and w of an infinite bound give NaN or an
+        // infinity by the query's sign, and all of these count alike (a NaN stays)
+        sum = fabs(sum) < INFINITY ? sum : NAN;
         best = best != best || sum <= best ? best : sum;
       }
     }
