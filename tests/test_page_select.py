@@ -172,6 +172,33 @@ def test_bounds_of_odd_constants(cuda):
         ops.page_bounds(cache.to(cuda), got, table.to(cuda), x, x, max_new=1, head_dim=256)
 
 
+@pytest.mark.gpu
+def test_pages_past_four_gigabytes(cuda):
+    """Bounds and attention of pages at both ends of a cache of 5.2 GB: what the same pages give in a
+    small one."""
+    hk, d, blocks = 4, 256, 40000
+    g = torch.Generator().manual_seed(9)
+    small = [torch.randint(-128, 128, (8, 128, hk, d), generator=g, dtype=torch.int8) for _ in range(2)]
+    for c in small:
+        c[..., :8] = (torch.randn(8, 128, hk, 4, generator=g) * 0.5).half().view(torch.int8)
+    large = [torch.empty(blocks, 128, hk, d, dtype=torch.int8, device=cuda) for _ in range(2)]
+    where = torch.tensor([0, blocks - 1, 3, blocks - 2, 16383, 16384, 32768, blocks - 3])
+    q, k, v = (torch.randn(1, n * hk, d, generator=g).bfloat16().to(cuda) for n in (2, 1, 1))
+    ends = torch.tensor([1000], dtype=torch.int32, device=cuda)
+    got = []
+    for caches, at in (([c.to(cuda) for c in small], torch.arange(8)), (large, where)):
+        for c, s in zip(caches, small):
+            c[at.to(cuda)] = s.to(cuda)
+        table = at.to(torch.int32)[None].to(cuda)
+        bounds = torch.zeros(caches[0].shape[0], hk, 2, d, dtype=torch.float16, device=cuda)
+        ops.page_bounds(caches[0], bounds, table, ends * 0, ends, max_new=1000, head_dim=d)
+        plan = ops.plan_selected([0, 1], [1001], has_new=True, block_size=128, budget=5, num_kv_heads=hk, group=2, head_dim=d, device=cuda)
+        chosen, pages = ops.select_pages(q, bounds, table, plan)
+        got.append((bounds[at.to(cuda)], pages, *ops.attention_selected(q, k, v, *caches, chosen, plan, d ** -0.5, head_dim=d)))
+    assert all(torch.equal(a, b) for a, b in zip(got[0][:2], got[1][:2])) and got[0][0].any()
+    assert (got[0][2] - got[1][2]).abs().max() <= 1e-3 and (got[0][3] - got[1][3]).abs().max() <= 1e-5
+
+
 # ------------------------------------------------------------------ the choice
 def plain_choice(q, bounds, table, qsl, seqs, has_new, bs, budget, first, last, hk):
     """Scores in 64 bits from the definition, then the pages one by one."""
