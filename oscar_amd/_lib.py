@@ -264,6 +264,22 @@ def load() -> C.CDLL:
     return lib
 
 
+_PACKED: dict = {}
+
+
+def packed(name: str):
+    """The entry point `name`, its first argument not a struct but the bytes of one (struct.pack): a
+    handle of its own beside the typed one.  Building the struct and a pointer to it takes the host
+    twice as long as the bytes (1.8 against 0.9 us a call)."""
+    call = _PACKED.get(name)
+    if call is None:
+        call = load()[name]
+        call.restype, (_, *rest) = {**SIGNATURES, **OPERATOR_SIGNATURES}[name]
+        call.argtypes = [C.c_char_p, *rest]
+        _PACKED[name] = call
+    return call
+
+
 EINVAL = -22
 
 

@@ -2,21 +2,23 @@
 //
 // A request of n nodes has M = n G rows per KV head (G query heads each), which all see its
 // history; among each other nodes see by a mask.  The split-K decode (attn_decode.hip) takes 32 rows
-// a wave and unpacks the codes for each of them anew, which its vector unit pays for: two
-// thirds of a tile's time.  Here a workgroup of four waves holds up to 256 rows, and unpacks a tile of
+// a wave and unpacks the codes for each 32 anew, which its vector unit pays for: two thirds of a
+// tile's time.  Here a workgroup of eight waves holds up to 256 rows, 32 a wave, and unpacks a tile of
 // keys once for all of them, into LDS.
 //
-// Work: the plan (oscarop_tree_plan_v1) cuts M into blocks of 64 RT rows, RT <= 4, and
-// deals each block's tiles of KT keys (history tiles, then chunk tiles) round-robin to items,
-// one workgroup each.  Wave w holds rows [16 RT w, 16 RT (w + 1)) of the block: their queries (B
-// operands) and O^T in registers.  For a tile t, with 16x16x32 MFMA,
+// Work: the plan (oscarop_tree_plan_v1) cuts M into blocks of at most 256 rows and deals each
+// block's tiles of KT = 8192 / D keys round-robin to items, one workgroup each: full tiles of the
+// history to some, its ragged end and the chunk's tiles to others (SLOW), whose masks and second
+// parts of P do not fit in registers beside the full tiles' loop.  Wave w holds rows [32 w, 32 w + 32)
+// of the block: their queries (B operands) and O^T in registers.  For a tile t, with 32x32x16 MFMA,
 //   S^T(t) = K(t) Q^T,   P(t) = exp2(scale S - m),   O^T += V(t)^T P(t)^T;
-// S^T's layout (lane: a row, four keys) is already that of the B operand of P.
+// S^T's layout (lane: a row, keys in fours) is already that of the B operand of P.  The items' O / l
+// and log-sum-exps are merged by tree_merge_kernel.
 //
-// The loop is two phases that give the matrix unit and the vector unit something to do at
-// the same time: S(t) with the softmax of S(t - 1), then O += V(t - 1) P(t - 1) with the
-// unpacking of tile t + 1; the codes of tile t + 2 are on their way.  So K has two buffers in
-// LDS and V three, and one barrier a tile does.
+// The loop: K and V have two buffers each in LDS, so one barrier a tile does; the codes of tile
+// t + 2 are on their way while t is computed.  Waves 0 to 3 unpack keys before their products and
+// waves 4 to 7 values after theirs: the two waves of a SIMD are out of step, and give its matrix unit
+// and its vector unit something to do at the same time.
 //
 // LDS: K in operand order, 16 bytes a lane.  V one row per key, 32 elements of padding, its
 // 16-byte units exchanged by the key's bits 2 and 3: rows then spread over all banks, for the
@@ -28,6 +30,17 @@
 // V in bf16 have a wider range than fp16: chunk tiles multiply it by P in two bf16 parts.  A
 // value of the chunk that is not finite goes into LDS as zero and is added afterwards, to the
 // rows alone that see its node.
+//
+// What bounds it: 8 requests of 24576 tokens with 32 nodes (192 rows, D 256) take 66 to 70 us, 0.57
+// PFLOP/s in 39 GFLOP: 24 tiles a workgroup at 2.2 us and 12 us before and after them, of which
+// 50 MB of partials; their merge takes another 10 us.  A tile's products alone take 1.0 us at the 2.0 to
+// 2.1 GHz that the matrix units leave the clock, its softmax and unpacking (about 300 vector
+// instructions a wave) as long again, and the two overlap in part.  12 ragged requests of up to 64
+// nodes, D 128 with capped scores: 71 us, bound by the cap's exponentials and divides.  One request of 500
+// tokens and 16 nodes: 15 us, latency.  Measured against it, at 8 x 24576 tokens: four waves of 16 or
+// 64 rows with 16x16x32 products, 99 to 165 us; the softmax of tile t - 1 between the products
+// of tile t in one wave, 86 to 114; slow tiles in the same loop, 113 (registers spill); codes two
+// tiles ahead, two accumulators of S or a higher wave priority, no gain beyond the noise.
 #include <vector>
 
 #include "common.h"
@@ -491,7 +504,8 @@ __global__ __launch_bounds__(kThreads, 2) void tree_main_kernel(TreeParams P) {
 }
 
 // The items of a block of rows, merged by their log-sum-exps.  One row a 64-lane (D 256) or
-// 32-lane (D 128) group, four columns a lane.
+// 32-lane (D 128) group, four columns a lane.  Bound by memory: 50 MB of partials of
+// 8 x 24576 tokens with 32 nodes in 10 us, eight items' loads of a row in flight at a time.
 constexpr int kBatch = 8;
 constexpr int kMergeThreads = 256;
 

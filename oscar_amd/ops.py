@@ -64,8 +64,8 @@ def _device_index(*tensors) -> int:
 
 def _launch(name: str, index: int, *args) -> None:
     """Call the entry point `name` on the device's current stream, with the device made the
-    current one (the library launches there)."""
-    call = getattr(_lib.load(), name)
+    current one (the library launches there).  Its struct comes first: as a pointer or as bytes."""
+    call = _lib.packed(name) if type(args[0]) is bytes else getattr(_lib.load(), name)
     if index == _get_device():
         status = call(*args, _raw_stream(index))
     else:
@@ -76,6 +76,7 @@ def _launch(name: str, index: int, *args) -> None:
 
 
 _CACHE = struct.Struct("=QQ10q").pack  # _lib.Cache's fields
+_ROTATE = struct.Struct("@Pi2q Pi Pi2q").pack
 
 
 def _cache_values(k_cache: torch.Tensor, v_cache: torch.Tensor, head_dim: int) -> tuple:
@@ -418,17 +419,23 @@ def rotate(x: torch.Tensor, r: torch.Tensor, *, transpose=False, out_dtype=None,
     _require_cuda(x, r)
     d = x.shape[-1]
     rows = x.numel() // d
-    x2 = x.reshape(rows, d)
-    if x2.stride(1) != 1:
-        x2 = x2.contiguous()
+    x2, stride = x, d
+    if not x.is_contiguous():
+        x2 = x.reshape(rows, d)
+        if x2.stride(1) != 1:
+            x2 = x2.contiguous()
+        stride = x2.stride(0)
     out_dtype = out_dtype or x.dtype
     if out is None:
-        out = torch.empty(*x.shape[:-1], d, dtype=out_dtype, device=x.device)
-    o2 = out.reshape(rows, d)
+        out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+        o2, out_stride = out, d
+    else:
+        o2 = out.reshape(rows, d)
+        out_stride = o2.stride(0)
     r = r.contiguous()
-    a = _lib.RotateArgs(x2.data_ptr(), _DTYPES[x2.dtype], rows, x2.stride(0), r.data_ptr(), int(bool(transpose)),
-                        o2.data_ptr(), _DTYPES[out_dtype], o2.stride(0), d)
-    status = _lib.load().oscar_rotate_v1(C.byref(a), _stream(x.device))
+    a = _ROTATE(x2.data_ptr(), _DTYPES[x2.dtype], rows, stride, r.data_ptr(), bool(transpose), o2.data_ptr(),
+                _DTYPES[out_dtype], out_stride, d)
+    status = _lib.packed("oscar_rotate_v1")(a, _stream(x.device))
     if status:
         _lib.check(status, "oscar_rotate_v1")
     return out
@@ -1021,7 +1028,8 @@ class SlotMap:
 _MAP = struct.Struct("@3P2iq P3q PPq 5P Pq").pack         # _lib.MapArgs's fields, as the others'
 _RELEASE = struct.Struct("@2P2i P3q PPq").pack
 _ATTN = struct.Struct("@P3q PPq PP10q Pq PPi Pf Pi Pi Pq i PP ii qq").pack
-_TREE = struct.Struct("@Pqq").pack
+_TREE = struct.Struct("@Pqq").pack                        # what _lib.TreeAttnArgs has behind an AttnArgs
+_TREE_MASK = struct.Struct("@PP2iq PqP").pack
 _SELECT = struct.Struct("@P3q2i P4q P3q PP6i PP PqP").pack
 _BOUNDS = struct.Struct("@PP10q P3q PP2i qP").pack
 
@@ -1084,11 +1092,11 @@ def map_slots(pool: PagePool, block_table, lengths, counts, *, tokens: int, bloc
         if need > 0:
             ws = torch.empty(need, dtype=torch.uint8, device=dev)  # a captured call keeps its own
     rows, cols = block_table.shape
-    a = _lib.MapArgs.from_buffer_copy(_MAP(
+    a = _MAP(
         lengths.data_ptr(), counts.data_ptr(), 0 if keep is None else keep.data_ptr(), reqs, block_size, tokens,
         block_table.data_ptr(), stride, rows, cols, pool.pages.data_ptr(), pool.count.data_ptr(), pool.pages.shape[0], at,
-        at + 4 * (reqs + 1), slots, positions, granted.data_ptr(), 0 if ws is None else ws.data_ptr(), max(need, 0)))
-    _launch("oscarop_map_v1", index, C.byref(a))
+        at + 4 * (reqs + 1), slots, positions, granted.data_ptr(), 0 if ws is None else ws.data_ptr(), max(need, 0))
+    _launch("oscarop_map_v1", index, a)
     starts, seq_lens = narrow.split_with_sizes([reqs + 1, reqs])
     return SlotMap(starts, seq_lens, *wide.unbind(), granted)
 
@@ -1107,10 +1115,9 @@ def release_pages(pool: PagePool, block_table, lengths, new_lengths, *, block_si
     if block_size < 1:
         raise ValueError("block_size must be at least 1")
     stride = _own_rows(block_table, reqs)
-    a = _lib.ReleaseArgs.from_buffer_copy(_RELEASE(lengths.data_ptr(), new_lengths.data_ptr(), reqs, block_size,
-                                                   block_table.data_ptr(), stride, *block_table.shape, pool.pages.data_ptr(),
-                                                   pool.count.data_ptr(), pool.pages.shape[0]))
-    _launch("oscarop_release_v1", index, C.byref(a))
+    a = _RELEASE(lengths.data_ptr(), new_lengths.data_ptr(), reqs, block_size, block_table.data_ptr(), stride,
+                 *block_table.shape, pool.pages.data_ptr(), pool.count.data_ptr(), pool.pages.shape[0])
+    _launch("oscarop_release_v1", index, a)
 
 
 # ------------------------------------------------------------------------ drafted trees
@@ -1137,9 +1144,8 @@ def tree_mask(parents, qsl, *, max_nodes: int) -> tuple:
     words = -(-max_nodes // 64)
     mask = torch.empty(n, words, dtype=torch.int64, device=parents.device)
     depths = torch.empty(n, dtype=torch.int32, device=parents.device)
-    a = _lib.TreeArgs(parents.data_ptr(), qsl.data_ptr(), qsl.shape[0] - 1, max_nodes, n, mask.data_ptr(), words,
-                      depths.data_ptr())
-    _launch("oscarop_tree_mask_v1", index, C.byref(a))
+    a = _TREE_MASK(parents.data_ptr(), qsl.data_ptr(), qsl.shape[0] - 1, max_nodes, n, mask.data_ptr(), words, depths.data_ptr())
+    _launch("oscarop_tree_mask_v1", index, a)
     return mask, depths
 
 
@@ -1166,7 +1172,8 @@ class TreePlan:
 
 def plan_tree(qsl, seqs, *, num_kv_heads: int, group: int, head_dim: int, device, window: tuple = (0, 0)) -> TreePlan:
     """Plan of attention_tree over a batch: request r's rows [qsl[r], qsl[r + 1]) are the nodes of
-    its tree, seqs[r] its length with them (host lists); sizes and window as plan_decode."""
+    its tree, seqs[r] its length with them (host lists); sizes as plan_decode's.  window is taken for the
+    sake of calls alike: a token's copy in the FP32 window costs a tile too little to plan for."""
     qsl, seqs = _request_lists(qsl, seqs, True)
     lib, sizes, target = _lib.load(), _lib.TreeSizes(), cu_count(device)
     qa, sa = (C.c_int32 * len(qsl))(*qsl), (C.c_int32 * max(len(seqs), 1))(*seqs)
@@ -1259,13 +1266,13 @@ def attention_tree(q, k_new, v_new, k_cache, v_cache, block_table, plan: TreePla
         raise ValueError("Block table cannot cover the history")
     st = staging_struct(stage, k_cache, head_dim)
     ws = _call_workspace(index, "attn_workspace", plan.partial_bytes)
-    a = _lib.TreeAttnArgs.from_buffer_copy(_ATTN(
+    a = _ATTN(
         q.data_ptr(), n, hq, stride, k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), *cache, table.data_ptr(),
         table.stride(0), plan.qsl.data_ptr(), plan.seqs.data_ptr(), len(plan.host_seqs),
         0 if st is None else C.addressof(st), scale, plan.items.data_ptr(), plan.num_items, plan.groups.data_ptr(),
         plan.num_groups, ws.data_ptr(), ws.numel(), 0, out_rot.data_ptr(), lse.data_ptr(), 0, code, *table.shape)
-        + _TREE(mask.data_ptr(), mask.shape[1], plan.partial_rows))
-    _launch("oscarop_attn_tree_v1", index, C.byref(a), None if score is None else C.byref(score))
+    a += _TREE(mask.data_ptr(), mask.shape[1], plan.partial_rows)
+    _launch("oscarop_attn_tree_v1", index, a, None if score is None else C.byref(score))
     return out_rot, lse
 
 
@@ -1290,9 +1297,9 @@ def page_bounds(k_cache, bounds, block_table, lengths, seq_lens, *, max_new: int
     table = _rows_apart(block_table)
     if table.ndim != 2 or table.shape[0] < reqs:
         raise ValueError("Missing request block-table rows")
-    a = _lib.BoundsArgs.from_buffer_copy(_BOUNDS(*cache, table.data_ptr(), table.stride(0), *table.shape, lengths.data_ptr(),
-                                                 seq_lens.data_ptr(), reqs, 0, max_new, bounds.data_ptr()))
-    _launch("oscarop_page_bounds_v1", index, C.byref(a))
+    a = _BOUNDS(*cache, table.data_ptr(), table.stride(0), *table.shape, lengths.data_ptr(), seq_lens.data_ptr(), reqs, 0,
+                max_new, bounds.data_ptr())
+    _launch("oscarop_page_bounds_v1", index, a)
     return bounds
 
 
@@ -1377,14 +1384,14 @@ def select_pages(q, bounds, block_table, plan: SelectPlan) -> tuple:
     out = torch.empty(2, reqs, hk, plan.budget, dtype=torch.int32, device=q.device)
     at, need, ws, arrivals = out.data_ptr(), plan.workspace_bytes, None, None
     if need > 0:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)  # a captured call keeps its own
+        ws = _call_workspace(index, "attn_workspace", need)  # the attention that follows is ordered behind it
         arrivals = _arrivals(index, reqs * hk)
-    a = _lib.SelectArgs.from_buffer_copy(_SELECT(
+    a = _SELECT(
         q.data_ptr(), q.shape[0], q.shape[1], s0, code, plan.has_new, bounds.data_ptr(), bounds.shape[0], hk, d,
         plan.block_size, table.data_ptr(), table.stride(0), *table.shape, plan.qsl.data_ptr(), plan.seqs.data_ptr(), reqs,
         plan.max_pages, plan.budget, plan.first_pages, plan.last_pages, 0, at, at + 4 * reqs * hk * plan.budget,
-        0 if ws is None else ws.data_ptr(), need, 0 if arrivals is None else arrivals.data_ptr()))
-    _launch("oscarop_select_v1", index, C.byref(a))
+        0 if ws is None else ws.data_ptr(), need, 0 if arrivals is None else arrivals.data_ptr())
+    _launch("oscarop_select_v1", index, a)
     return out.unbind()
 
 
@@ -1414,11 +1421,11 @@ def attention_selected(q, k_new, v_new, k_cache, v_cache, table, plan: SelectPla
     table = table.contiguous()
     st = staging_struct(stage, k_cache, head_dim)
     ws = _call_workspace(index, "attn_workspace", decode.partial_bytes)
-    a = _lib.AttnArgs.from_buffer_copy(_ATTN(
+    a = _ATTN(
         q.data_ptr(), n, hq, stride, *((0, 0, 0) if k_new is None else (k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0))),
         *cache, table.data_ptr(), hk * budget, decode.qsl.data_ptr(), decode.seqs.data_ptr(), len(plan.host_seqs),
         0 if st is None else C.addressof(st), scale, decode.items.data_ptr(), decode.num_items, decode.groups.data_ptr(),
         decode.num_groups, ws.data_ptr(), ws.numel(), decode.max_group_items, out_rot.data_ptr(), lse.data_ptr(), 0, code,
-        reqs, budget))
-    _launch("oscarop_attn_selected_v1", index, C.byref(a), None if score is None else C.byref(score), budget)
+        reqs, budget)
+    _launch("oscarop_attn_selected_v1", index, a, None if score is None else C.byref(score), budget)
     return out_rot, lse

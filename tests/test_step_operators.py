@@ -39,6 +39,23 @@ def test_structs_match_c_layout(tmp_path):
             assert int(got[f"{name} {field}"]) == getattr(py, field).offset, (name, field)
 
 
+def test_packed_fields_are_the_structs():
+    """struct.pack of ascending numbers, read back through the structs."""
+    def flat(x):
+        for name, _ in x._fields_:
+            y = getattr(x, name)
+            if isinstance(y, C._Pointer):
+                y = C.cast(y, C.c_void_p).value
+            yield from flat(y) if isinstance(y, C.Structure) else y if isinstance(y, C.Array) else [y]
+
+    for pack, py in ((ops._MAP, _lib.MapArgs), (ops._RELEASE, _lib.ReleaseArgs), (ops._ATTN, _lib.AttnArgs), (ops._SELECT, _lib.SelectArgs),
+                     (ops._BOUNDS, _lib.BoundsArgs), (ops._TREE_MASK, _lib.TreeArgs), (ops._ROTATE, _lib.RotateArgs)):
+        many = len(list(flat(py())))
+        data = pack(*range(1, many + 1))
+        assert len(data) == C.sizeof(py) and list(flat(py.from_buffer_copy(data))) == list(range(1, many + 1)), py
+    assert C.sizeof(_lib.TreeAttnArgs) == C.sizeof(_lib.AttnArgs) + len(ops._TREE(1, 2, 3))
+
+
 def test_every_declared_operator_is_exported():
     text = re.sub(r"/\*.*?\*/", "", HEADER.with_name("oscar_operators.h").read_text(), flags=re.S)
     lib = _lib.load()
