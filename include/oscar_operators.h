@@ -322,6 +322,7 @@ int oscarop_page_bounds_v1(const oscarop_bounds_args_v1* args, void* stream);
  * bits.  table[r][h] holds the chosen pages in ascending order of their columns and
  * pages[r][h] these columns, -1 behind them.  A request that does not fit (queries past
  * num_tokens, a negative history, columns past the table) gets -1 throughout. */
+#define OSCAROP_SELECT_ARRIVAL 32 /* int32 of a list's arrival counter: a cache line of its own */
 typedef struct oscarop_select_args_v1 {
   const void* q;                  /* [num_tokens, num_q_heads, D] in q_dtype */
   int64_t num_tokens;
@@ -350,8 +351,9 @@ typedef struct oscarop_select_args_v1 {
   int32_t* pages;                 /* [num_reqs][Hk][budget], or NULL */
   void* workspace;                /* >= oscarop_select_workspace_bytes_v1(args), 16-byte aligned */
   int64_t workspace_bytes;
-  /* [num_reqs * Hk], zero before the first call; each call leaves them zero.  As the workspace,
-   * nothing else uses them while a call runs.  Not read if no history exceeds the budget. */
+  /* [num_reqs * Hk][OSCAROP_SELECT_ARRIVAL], of which the first is used, zero before the first
+   * call; each call leaves them zero.  As the workspace, nothing else uses them while a call runs.
+   * Not read if no history exceeds the budget. */
   int32_t* arrivals;
 } oscarop_select_args_v1;
 

@@ -14,6 +14,7 @@ LIB_PATH = Path(__file__).resolve().parent / "liboscar_amd.so"
 OSCAR_F32, OSCAR_F16, OSCAR_BF16 = 0, 1, 2
 STAGE_NONE, STAGE_INVALIDATE, STAGE_WRITE = 0, 1, 2
 WORK_INTS = 8
+SELECT_ARRIVAL = 32  # int32 of a list's arrival counter
 TREE_ITEM_INTS = 12
 GROUP_INTS = 8
 ABI_VERSION = 3

@@ -102,9 +102,9 @@ __global__ __launch_bounds__(kThreads) void bounds_kernel(oscarop_bounds_args_v1
 constexpr int kLanes = 8;                // lanes of a page
 constexpr int kPages = 64 / kLanes;      // pages of a workgroup at a time
 constexpr int kHeld = 4096;              // scores in LDS; more are read again in each pass
-constexpr int kFew = 64;                 // candidates that one wave ranks
+constexpr int kFew = 64;                 // candidates that are ranked against each other
 constexpr int kBatch = 4;                // scores of a thread in flight
-constexpr int kRowsHeld = 16;            // queries in LDS at a time, in 64 bits: a conversion costs four products
+constexpr int kRowsHeld = 32;            // queries in LDS at a time, in 64 bits: a conversion costs four products
 // workgroups up to which the waves of one share their pages: what the card holds at a time
 constexpr int64_t kByRows = 512;
 
@@ -168,27 +168,37 @@ __device__ __forceinline__ unsigned scan(unsigned x, unsigned* s_part) {
 // One list's choice: the want-th largest key of `first` to `end`, then the chosen columns in
 // their order.  The keys agree in their upper bits, so digits begin at the highest one in which two
 // differ; the few candidates that are left in the digit's bin are ranked against each other.
-__device__ void choose(const SelectParams& P, int many, int64_t list, const int32_t* row) {
+__device__ void choose(const SelectParams& P, int many, int64_t list, const int32_t* row, uint64_t* s_key) {
   const oscarop_select_args_v1& A = P.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int32_t* table = A.table + list * A.budget;
   int32_t* pages = A.pages == nullptr ? nullptr : A.pages + list * A.budget;
-  auto put = [&](int at, int col) {
-    table[at] = row[col];
+  auto put = [&](int at, int col, int page) {
+    table[at] = page;
     if (pages != nullptr) pages[at] = col;
   };
   const int first = A.first_pages, n = many - first - A.last_pages, want = A.budget - first - A.last_pages;
   const uint64_t* keys = P.keys + list * A.max_pages + first;
-  __shared__ uint64_t s_key[kHeld];
   __shared__ int s_bin[256];
   __shared__ unsigned s_part[kWaves];
   __shared__ unsigned s_diff[kWaves][2];
   __shared__ uint64_t s_few[kFew];
-  __shared__ int s_place[kFew];
+  __shared__ unsigned s_rank[kFew];
   __shared__ int s_found[3];       // digit, rest to take, size of its bin
   __shared__ uint64_t s_limit;
   const bool held = n <= kHeld;
   auto load = [&](int i) { return __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  // at the end thread t looks at the columns [t run, (t + 1) run): its first ones' pages early
+  const int run = (n + kThreads - 1) / kThreads;
+  const int a = min(tid * run, n), b = min(a + run, n);
+  int page[kBatch];
+  auto load_pages = [&](int i) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) page[u] = row[first + min(i + u, n - 1)];
+  };
+  load_pages(a);
+  for (int i = tid; i < first; i += kThreads) put(i, i, row[i]);
+  for (int i = tid; i < A.last_pages; i += kThreads) put(A.budget - A.last_pages + i, many - A.last_pages + i, row[many - A.last_pages + i]);
   const uint64_t some = load(0);
   uint64_t diff = 0;
   for (int i = tid; i < n; i += kBatch * kThreads) {
@@ -243,29 +253,30 @@ __device__ void choose(const SelectParams& P, int many, int64_t list, const int3
     if (size <= kFew && left > 0) {
       __syncthreads();  // s_found has been read
       if (tid == 0) s_found[2] = 0;
+      if (tid < kFew) s_rank[tid] = 0;
       __syncthreads();
       for (int i = tid; i < n; i += kThreads) {
         const uint64_t k = key(i);
-        if ((k & mask) == prefix) {
-          const int at = atomicAdd(&s_found[2], 1);
-          s_few[at] = k;
-          s_place[at] = i;
-        }
+        if ((k & mask) == prefix) s_few[atomicAdd(&s_found[2], 1)] = k;
       }
       __syncthreads();
+      // each wave's share of the candidates, against a lane's one: those above it, and those alike
+      const uint64_t own = s_few[lane < (int)size ? lane : 0];
+      unsigned above = 0, alike = 0;
+#pragma unroll
+      for (int u = 0; u < kFew / kWaves; ++u) {
+        const int at = wave * (kFew / kWaves) + u;
+        const uint64_t o = s_few[at < (int)size ? at : 0];
+        above += at < (int)size && o > own;
+        alike += at < (int)size && o == own;
+      }
+      atomicAdd(&s_rank[lane], above << 16 | alike);
+      __syncthreads();
       if (wave == 0) {
-        const bool in = lane < (int)size;
-        const uint64_t k = in ? s_few[lane] : 0;
-        const int at = in ? s_place[lane] : 0;
-        unsigned rank = 0, ahead = 0;  // those before this one, and those of a larger key
-        for (int i = 0; i < (int)size; ++i) {
-          const uint64_t o = s_few[i];
-          ahead += o > k;
-          rank += o > k || (o == k && s_place[i] < at);
-        }
-        if (in && rank == rest - 1) {
-          s_limit = k;
-          s_found[1] = rest - ahead;  // of the keys that equal the limit
+        const unsigned rank = s_rank[lane], over = rank >> 16;
+        if (lane < (int)size && over < rest && over + (rank & 0xffffu) >= rest) {
+          s_limit = own;
+          s_found[1] = rest - over;  // of the keys that equal the limit
         }
       }
       __syncthreads();
@@ -276,10 +287,7 @@ __device__ void choose(const SelectParams& P, int many, int64_t list, const int3
     }
     __syncthreads();  // s_found has been read, the bins are clear
   }
-  // keys above the prefix, and the first `rest` that equal it: thread t looks at the columns
-  // [t run, (t + 1) run)
-  const int run = (n + kThreads - 1) / kThreads;
-  const int a = min(tid * run, n), b = min(a + run, n);
+  // keys above the prefix, and the first `rest` that equal it
   unsigned same = 0, over = 0;
   for (int i = a; i < b; ++i) {
     const uint64_t k = key(i) & mask;
@@ -289,14 +297,17 @@ __device__ void choose(const SelectParams& P, int many, int64_t list, const int3
   unsigned ties = scan(same, s_part);
   const unsigned taken = ties < rest ? min(same, rest - ties) : 0;
   unsigned at = first + scan(over + taken, s_part);
-  for (int i = a; i < b; ++i) {
-    const uint64_t k = key(i) & mask;
-    const bool tie = k == prefix;
-    if (k > prefix || (tie && ties < rest)) put(at++, first + i);
-    ties += tie;
+  for (int i0 = a; i0 < b; i0 += kBatch) {
+    if (i0 > a) load_pages(i0);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (i0 + u >= b) break;
+      const uint64_t k = key(i0 + u) & mask;
+      const bool tie = k == prefix;
+      if (k > prefix || (tie && ties < rest)) put(at++, first + i0 + u, page[u]);
+      ties += tie;
+    }
   }
-  for (int i = tid; i < first; i += kThreads) put(i, i);
-  for (int i = tid; i < A.last_pages; i += kThreads) put(A.budget - A.last_pages + i, many - A.last_pages + i);
 }
 
 // A workgroup scores eight pages at a time, its waves a quarter of the rows each (ROWS), or 32
@@ -307,9 +318,16 @@ __global__ __launch_bounds__(kThreads, 2) void select_kernel(SelectParams P) {
   const oscarop_select_args_v1& A = P.a;
   const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.y, r = blockIdx.z;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const History x = history_of(A, r);
   const int64_t list = (int64_t)r * A.num_kv_heads + h;
   const int32_t* table_row = A.block_table + (int64_t)r * A.block_table_stride;
+  constexpr int kAtOnce = ROWS ? kPages : kWaves * kPages;
+  const int j = lane % kLanes;
+  const int64_t p0 = (int64_t)A.first_pages + (int64_t)blockIdx.x * kAtOnce, p = p0 + lane / kLanes + (ROWS ? 0 : kPages * wave);
+  // the page and its bounds are on their way while the request's lengths come (behind the
+  // last page: some page's)
+  int page = -1;
+  if (A.block_table_cols > 0) page = table_row[p < A.block_table_cols ? p : A.block_table_cols - 1];
+  const History x = history_of(A, r);
   if (x.pages <= A.budget) {
     // all of them
     if (blockIdx.x > 0) return;
@@ -320,17 +338,14 @@ __global__ __launch_bounds__(kThreads, 2) void select_kernel(SelectParams P) {
     return;
   }
   const int group = (int)(A.num_q_heads / A.num_kv_heads);
-  const int first = A.first_pages, end = (int)x.pages - A.last_pages;
-  const int j = lane % kLanes;
+  const int64_t end = x.pages - A.last_pages;
   const int64_t rows = (int64_t)x.nq * group;
   __shared__ double s_best[kWaves][kPages];
-  __shared__ __attribute__((aligned(16))) double s_q[kRowsHeld][D];
+  // the queries, and for the choice the scores
+  __shared__ __attribute__((aligned(16))) uint64_t s_mem[kRowsHeld * D > kHeld ? kRowsHeld * D : kHeld];
+  double(*s_q)[D] = (double(*)[D])s_mem;
   __shared__ int s_last;
-  constexpr int kAtOnce = ROWS ? kPages : kWaves * kPages;
-  const int p_first = first + blockIdx.x * kAtOnce;
-  for (int p0 = p_first; p0 < end; p0 += gridDim.x * kAtOnce) {
-    const int p = p0 + lane / kLanes + (ROWS ? 0 : kPages * wave);
-    int page = table_row[p < end ? p : first];
+  if (p0 < end) {
     page = page < 0 || page >= A.num_blocks ? 0 : page;
     const uint16_t* b = (const uint16_t*)A.bounds + ((int64_t)page * A.num_kv_heads + h) * 2 * D + 8 * j;
     u32x4 lo[STEPS], hi[STEPS];
@@ -339,6 +354,25 @@ __global__ __launch_bounds__(kThreads, 2) void select_kernel(SelectParams P) {
       lo[s] = *(const u32x4*)(b + 8 * kLanes * s);
       hi[s] = *(const u32x4*)(b + D + 8 * kLanes * s);
     }
+    auto rows_from = [&](int64_t from, int many) {
+      constexpr int PIECES = kRowsHeld * (D / 8) / kThreads;  // of eight elements, all on their way at once
+      float v[PIECES][8];
+#pragma unroll
+      for (int u = 0; u < PIECES; ++u) {
+        const int i = min(tid + u * kThreads, many * (D / 8) - 1);
+        const int64_t row = from + i / (D / 8);
+        load8<QT>(A.q, (x.q0 + row / group) * A.q_stride_token + (h * group + row % group) * (int64_t)D + i % (D / 8) * 8, v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < PIECES; ++u) {
+        const int i = tid + u * kThreads;
+        if (i >= many * (D / 8)) break;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s_q[i / (D / 8)][i % (D / 8) * 8 + e] = v[u][e];
+      }
+      __syncthreads();
+    };
+    if (rows > 0) rows_from(0, rows < kRowsHeld ? (int)rows : kRowsHeld);
     double m[STEPS][8], w[STEPS][8];
 #pragma unroll
     for (int s = 0; s < STEPS; ++s)
@@ -352,17 +386,9 @@ __global__ __launch_bounds__(kThreads, 2) void select_kernel(SelectParams P) {
     double best = -INFINITY;
     for (int64_t from = 0; from < rows; from += kRowsHeld) {
       const int many = rows - from < kRowsHeld ? (int)(rows - from) : kRowsHeld;
-      if (p0 == p_first || rows > kRowsHeld) {
+      if (from > 0) {
         __syncthreads();  // the rows before have been read
-        for (int i = tid; i < many * (D / 8); i += kThreads) {
-          const int64_t row = from + i / (D / 8);
-          const int e0 = i % (D / 8) * 8;
-          float v[8];
-          load8<QT>(A.q, (x.q0 + row / group) * A.q_stride_token + (h * group + row % group) * (int64_t)D + e0, v);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) s_q[i / (D / 8)][e0 + e] = v[e];
-        }
-        __syncthreads();
+        rows_from(from, many);
       }
       for (int row = ROWS ? wave : 0; row < many; row += ROWS ? kWaves : 1) {
         double part[4] = {0.0, 0.0, 0.0, 0.0};  // four sums at a time: one alone waits for itself
@@ -384,7 +410,7 @@ __global__ __launch_bounds__(kThreads, 2) void select_kernel(SelectParams P) {
         best = best != best || sum <= best ? best : sum;
       }
     }
-    auto put = [&](int at, uint64_t k) {
+    auto put = [&](int64_t at, uint64_t k) {
       __hip_atomic_store(P.keys + list * A.max_pages + at, k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     };
     if constexpr (ROWS) {
@@ -399,7 +425,6 @@ __global__ __launch_bounds__(kThreads, 2) void select_kernel(SelectParams P) {
         }
         put(p0 + tid, k);
       }
-      __syncthreads();  // s_best has been read
     } else if (j == 0 && p < end) {
       put(p, order_of(best));
     }
@@ -409,9 +434,9 @@ __global__ __launch_bounds__(kThreads, 2) void select_kernel(SelectParams P) {
   // fence would write back the whole L2 instead, for every workgroup (16 lists of 1024 pages: 64 us)
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  if (tid == 0) s_last = atomicInc((unsigned*)&A.arrivals[list], gridDim.x - 1) == gridDim.x - 1;
+  if (tid == 0) s_last = atomicInc((unsigned*)&A.arrivals[list * OSCAROP_SELECT_ARRIVAL], gridDim.x - 1) == gridDim.x - 1;
   __syncthreads();
-  if (s_last) choose(P, (int)x.pages, list, table_row);
+  if (s_last) choose(P, (int)x.pages, list, table_row, s_mem);
 }
 
 // -22 for sizes that are refused

@@ -209,8 +209,8 @@ class DeviceScratch:
     def select_arrivals(self, lists: int) -> torch.Tensor:
         """Arrival counters of select_pages, one for each request and KV head: zeroed once, and
         every call leaves them zero."""
-        if self.list_arrivals.numel() < lists:
-            self.list_arrivals = torch.zeros(max(lists, 1024), dtype=torch.int32, device=self.device)
+        if self.list_arrivals.numel() < lists * _lib.SELECT_ARRIVAL:
+            self.list_arrivals = torch.zeros(max(lists, 64) * _lib.SELECT_ARRIVAL, dtype=torch.int32, device=self.device)
         return self.list_arrivals
 
     def prefill_workspace(self, nbytes: int) -> torch.Tensor:
@@ -258,7 +258,7 @@ def _arrivals(index: int, lists: int) -> torch.Tensor:
         with torch.cuda.device(index):
             return _arrivals(index, lists)
     if _is_capturing():
-        return torch.zeros(lists, dtype=torch.int32, device=torch.device("cuda", index))
+        return torch.zeros(lists * _lib.SELECT_ARRIVAL, dtype=torch.int32, device=torch.device("cuda", index))
     return DeviceScratch.get(torch.device("cuda", index)).select_arrivals(lists)
 
 
