@@ -9,9 +9,23 @@
 //
 //   bounds_kernel   one workgroup per page: the codes of its tokens, each token's four values from a
 //                   table, packed minimum and maximum
-//   select_kernel   eight lanes a page, the bounds in registers; the last workgroup of a (request,
-//                   KV head) finds the budget-th largest score by radix selection and writes
-//                   the chosen columns in their order
+//   select_kernel   eight lanes a page, the bounds in registers, the queries in LDS in 64 bits; the
+//                   last workgroup of a (request, KV head) finds the budget-th largest score by
+//                   radix selection and writes the chosen columns in their order
+//
+// bounds_kernel is bound by latency: a page of 128 tokens is one round of loads.  4.1 us for 24 requests
+// of four new tokens, 7.1 for 938 full pages of D 256 (9.1 MB of slots' bytes in use, 2.6 times the
+// 1.9 us of a large copy).
+//
+// select_kernel: about 3.6 us of launch and the counters' line, 2 to 3 until the bounds are there, the
+// products, then 4 to 6 for the choice, whose chain is the keys' stores, the counter, the keys' loads, two
+// or three digits and the stores.  One list of 250 pages and 6 rows 9 us, 8 of 192 pages and 24 rows
+// 12.4, 16 of 1024 pages and 6 rows 16 (16.8 MB of bounds; scores 4, choice 6), 12 ragged of up to 470 pages, two
+// heads of D 128 and 16 rows 13.3.  A launch of its own for the choice costs the 4 to 5 us of a launch.
+// Products in 32 bits would take half the time of a third of the kernel, and could miss the order of
+// near scores.  What took the 16 lists from 19.9 us to 15.1 in a graph: counters a cache line apart (in one
+// line the 512 arrivals wait for each other, 3.7 us), the last digit's candidates ranked by all waves (a loop
+// over LDS in one took 1 to 2), 32 queries at a time.
 #include <type_traits>
 
 #include "common.h"
@@ -105,7 +119,9 @@ constexpr int kHeld = 4096;              // scores in LDS; more are read again i
 constexpr int kFew = 64;                 // candidates that are ranked against each other
 constexpr int kBatch = 4;                // scores of a thread in flight
 constexpr int kRowsHeld = 32;            // queries in LDS at a time, in 64 bits: a conversion costs four products
-// workgroups up to which the waves of one share their pages: what the card holds at a time
+// Workgroups up to which the waves of one share their pages, what the card holds at a time: 8 lists of
+// 192 pages and 24 rows 192 workgroups of 8 pages.  Beyond, 32 pages: 6 lists of 1500 pages and 6 rows
+// 16 us (8 pages: 22), 8 of 800 and 24 rows 19 (23), 8 of 700 with two heads of D 128 and 8 rows 13 (16).
 constexpr int64_t kByRows = 512;
 
 struct SelectParams {

@@ -13,8 +13,12 @@
 //   rows_kernel   slots and positions of a larger step's rows, one a lane
 //   release_kernel  one workgroup: pages behind the new lengths go back on the stack
 //
-// All of it is latency: a step of one token reads and writes 37 bytes, one of 256 requests
-// and 17000 rows 270 KB.  The sums saturate at 2^32 - 1, which keeps them associative, and a
+// All of it is latency, a chain of a few dependent accesses and barriers: a step of one token
+// reads and writes 37 bytes (map_kernel 4.5 us, release_kernel 2.3, an empty kernel 1.5 to 2), one of 256
+// requests and 16600 rows 270 KB (6.7 and 4.1 in rows_kernel, release 5.0), one of 48 requests and 1536
+// marked rows 27 KB (8.6, release 3.4).  One workgroup, since the sums go over all requests;
+// rows beyond kSmallStep have a launch of their own, where one workgroup would take 1024 of them a round.
+// The sums saturate at 2^32 - 1, which keeps them associative, and a
 // saturated one is more than any pool or step holds.
 #include "common.h"
 

@@ -1104,7 +1104,7 @@ def map_slots(pool: PagePool, block_table, lengths, counts, *, tokens: int, bloc
 def release_pages(pool: PagePool, block_table, lengths, new_lengths, *, block_size: int) -> None:
     """Give back the pages behind new_lengths[r] of requests of lengths[r] tokens (int32 on the
     device): those of a request that ended (0), of a step's rejected tokens, of an eviction
-    (plan.lengths and plan.seq_lens, with plan.table(...)).  The pool grows in place, requests
+    (its plan's lengths and seq_lens, with plan.table(...)).  The pool grows in place, requests
     in their order, their pages ascending, so that what map_slots took last lies as it lay;
     the table keeps its entries.  A new length below 0 or above the old one gives nothing back,
     nor does a request whose pages the pool has no room for, nor those with pages behind it."""
@@ -1398,7 +1398,7 @@ def select_pages(q, bounds, block_table, plan: SelectPlan) -> tuple:
 def attention_selected(q, k_new, v_new, k_cache, v_cache, table, plan: SelectPlan, scale, stage=None, *, head_dim,
                        soft_cap=0.0, out_rot=None, lse=None):
     """Attention over the pages that select_pages chose, and the current chunk: (out_rot fp32,
-    lse fp32), rotated, as attention_decode's, whose other arguments these are.  table
+    lse fp32), rotated, as attention_decode's, whose other arguments and rules these are.  table
     [requests, Hk, budget]: each KV head's pages, ascending."""
     index = _device_index(q, k_new, v_new, k_cache, v_cache, table, plan.qsl, out_rot, lse, *(stage or ()))
     if plan.has_new != (k_new is not None) or (k_new is None) != (v_new is None):

@@ -34,6 +34,23 @@ layer's FP32 window arena):
 * ``evict(weights, k_cache!, v_cache!, block_table, seq_lens, drop_pages, stage_k, stage_v,
   owner!, head_dim, sink_tokens, recent_tokens) -> weights``: drops the tokens of
   least weight, whole pages at a time (``oscarop_evict_v1``).
+* ``map_slots(pool_pages, pool_count!, block_table!, lengths, counts, tokens, block_size,
+  keep) -> (query_start_loc, seq_lens, slots, positions, granted)``: a step's pages, slots and
+  positions from lengths on the device (``oscarop_map_v1``); ``release_pages(pool_pages!,
+  pool_count!, block_table, lengths, new_lengths, block_size) -> ()``: pages behind the new
+  lengths back to the pool (``oscarop_release_v1``).
+* ``tree_mask(parents, query_start_loc, max_nodes) -> (mask, depths)``: ancestors of drafted
+  nodes (``oscarop_tree_mask_v1``); ``attention_tree(q, k_new, v_new, k_cache, v_cache,
+  block_table, query_start_loc, seq_lens, mask, scale, head_dim, stage_k, stage_v, owner,
+  soft_cap) -> (out_rot, lse)``: their attention (``oscarop_tree_plan_v1`` /
+  ``oscarop_attn_tree_v1``).
+* ``page_bounds(k_cache, bounds!, block_table, lengths, seq_lens, max_new, head_dim) -> ()``: the
+  least and the largest keys of the pages that a step touched (``oscarop_page_bounds_v1``);
+  ``attention_selected(q, k_new, v_new, k_cache, v_cache, bounds, block_table,
+  query_start_loc, seq_lens, budget, scale, head_dim, first_pages, last_pages, stage_k,
+  stage_v, owner, sink_tokens_eff, recent_tokens, soft_cap) -> (out_rot, lse, pages)``: the
+  choice of pages and the attention over them (``oscarop_select_v1`` /
+  ``oscarop_attn_selected_v1``).
 """
 from __future__ import annotations
 
