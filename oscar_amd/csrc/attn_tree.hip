@@ -41,6 +41,7 @@
 // 64 rows with 16x16x32 products, 99 to 165 us; the softmax of tile t - 1 between the products
 // of tile t in one wave, 86 to 114; slow tiles in the same loop, 113 (registers spill); codes two
 // tiles ahead, two accumulators of S or a higher wave priority, no gain beyond the noise.
+#include <type_traits>
 #include <vector>
 
 #include "common.h"
@@ -134,81 +135,99 @@ __device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uin
     }
   }
 
-  // ---- filling: waves 0 to 3 the keys, 4 to 7 the values; thread (token, 32 codes)
-  const bool vside = wave >= 4;
-  const int idx = tid & 255;
-  const int tok = idx % C::KT, vec = idx / C::KT, sub = tok >> 5, in32 = tok & 31;
+  // ---- filling, in eight units of 256 / 4 threads: 0 to 3 the keys, 4 to 7 the values; thread
+  // (token, 32 codes)
   const uint8_t* kbase = A.cache.k + (int64_t)I.kvh * A.cache.k_stride[2];
-  const uint8_t* cbase = vside ? A.cache.v + (int64_t)I.kvh * A.cache.v_stride[2] : kbase + 32;
+  const uint8_t* vbase = A.cache.v + (int64_t)I.kvh * A.cache.v_stride[2];
+  struct Unit {
+    bool v;                            // values
+    int tok, vec, sub, in32, to, turn;
+    u32x2 codes;
+    unsigned meta;
+    int tag, page, seat;
+  };
+  auto unit_of = [&](int which) {
+    Unit u;
+    const int idx = 64 * (which & 3) + lane;
+    u.v = which >= 4;
+    u.tok = idx % C::KT, u.vec = idx / C::KT, u.sub = u.tok >> 5, u.in32 = u.tok & 31;
+    // where piece i (8 elements) of the thread's four goes
+    // (a row of values has its 16-byte units exchanged, within four, by the key's bits 2 and 3)
+    u.to = u.v ? u.tok * (C::VROW * 2) + 64 * u.vec : (2 * u.vec * C::KSUB + u.sub) * 1024 + u.in32 * 16;
+    u.turn = (u.tok >> 2) & 3;
+    u.codes = u32x2{0u, 0u};
+    u.meta = 0;
+    u.tag = -1, u.page = 0, u.seat = 0;
+    return u;
+  };
   const int64_t ks0 = A.cache.k_stride[0], ks1 = A.cache.k_stride[1];
-  const int64_t cs0 = vside ? A.cache.v_stride[0] : ks0, cs1 = vside ? A.cache.v_stride[1] : ks1;
-  u32x2 codes = {0u, 0u};
-  unsigned meta = 0;
-  int tag = -1, page = 0, seat = 0;
-  auto load_at = [&](const Place& x, int off) {
-    page = x.page;
-    seat = x.seat + off - x.off;
-    codes = *(const u32x2*)(cbase + (int64_t)page * cs0 + (int64_t)off * cs1 + 8 * vec);
-    meta = *(const unsigned*)(kbase + (int64_t)page * ks0 + (int64_t)off * ks1 + (vside ? 4 : 0));
-    tag = P.has_stage ? ((const int32_t*)P.st.owner)[2 * (int64_t)seat] : -1;
+  const int64_t vs0 = A.cache.v_stride[0], vs1 = A.cache.v_stride[1];
+  auto load_at = [&](Unit& u, const Place& x, int off) {
+    u.page = x.page;
+    u.seat = x.seat + off - x.off;
+    const uint8_t* slot = u.v ? vbase + (int64_t)u.page * vs0 + (int64_t)off * vs1 : kbase + 32 + (int64_t)u.page * ks0 + (int64_t)off * ks1;
+    u.codes = *(const u32x2*)(slot + 8 * u.vec);
+    u.meta = *(const unsigned*)(kbase + (int64_t)u.page * ks0 + (int64_t)off * ks1 + (u.v ? 4 : 0));
+    u.tag = P.has_stage ? ((const int32_t*)P.st.owner)[2 * (int64_t)u.seat] : -1;
   };
-  auto load = [&](int j) {
-    const Place x = s_place[(j < I.count ? j : I.count - 1) * C::KSUB + sub];
-    load_at(x, x.off + in32);
+  auto load = [&](Unit& u, int j) {
+    const Place x = s_place[(j < I.count ? j : I.count - 1) * C::KSUB + u.sub];
+    load_at(u, x, x.off + u.in32);
   };
-  // where piece i (8 elements) of the thread's four goes
-  // (a row of values has its 16-byte units exchanged, within four, by the key's bits 2 and 3)
-  const int to = vside ? tok * (C::VROW * 2) + 64 * vec : (2 * vec * C::KSUB + sub) * 1024 + in32 * 16;
-  const int turn = (tok >> 2) & 3;
-  auto dest = [&](int i, int buf) -> u32x4* {
-    if (vside) return (u32x4*)(s_v + buf * C::VBYTES + to + 16 * (i ^ turn));
-    return (u32x4*)(s_k + buf * C::KBYTES + to + (i >> 1) * (C::KSUB * 1024) + (i & 1) * 512);
+  auto dest = [&](const Unit& u, int i, int buf) -> u32x4* {
+    if (u.v) return (u32x4*)(s_v + buf * C::VBYTES + u.to + 16 * (i ^ u.turn));
+    return (u32x4*)(s_k + buf * C::KBYTES + u.to + (i >> 1) * (C::KSUB * 1024) + (i & 1) * 512);
   };
-  auto fill_codes = [&](bool some, int buf) {
+  auto fill_codes = [&](const Unit& u, bool some, int buf) {
     unsigned t_lo, t_hi;
-    if (QT == OSCAR_F16 || vside) byte_tables<OSCAR_F16>(meta, t_lo, t_hi);
-    else byte_tables<OSCAR_BF16>(meta, t_lo, t_hi);
+    if (QT == OSCAR_F16 || u.v) byte_tables<OSCAR_F16>(u.meta, t_lo, t_hi);
+    else byte_tables<OSCAR_BF16>(u.meta, t_lo, t_hi);
     if (!some) t_lo = t_hi = 0;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       unsigned o[8];
-      lut16(codes[c], t_lo, t_hi, o);
-      *dest(2 * c, buf) = u32x4{o[0], o[1], o[2], o[3]};
-      *dest(2 * c + 1, buf) = u32x4{o[4], o[5], o[6], o[7]};
+      lut16(u.codes[c], t_lo, t_hi, o);
+      *dest(u, 2 * c, buf) = u32x4{o[0], o[1], o[2], o[3]};
+      *dest(u, 2 * c + 1, buf) = u32x4{o[4], o[5], o[6], o[7]};
     }
   };
   // the window's copy of a token
-  auto fill_staged = [&](int buf) {
-    const f32x4* src = (const f32x4*)((vside ? P.st.stage_v : P.st.stage_k) + ((int64_t)seat * A.cache.num_kv_heads + I.kvh) * D + 32 * vec);
+  auto fill_staged = [&](const Unit& u, int buf) {
+    const f32x4* src = (const f32x4*)((u.v ? P.st.stage_v : P.st.stage_k) + ((int64_t)u.seat * A.cache.num_kv_heads + I.kvh) * D + 32 * u.vec);
 #pragma unroll 2
     for (int i = 0; i < 4; ++i) {
       const f32x4 a = src[2 * i], b = src[2 * i + 1];
       u32x4 o;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = vside ? hist_pair<OSCAR_F16>(a[e], b[e]) : hist_pair<QT>(a[e], b[e]);
-      *dest(i, buf) = o;
+      for (int e = 0; e < 4; ++e) o[e] = u.v ? hist_pair<OSCAR_F16>(a[e], b[e]) : hist_pair<QT>(a[e], b[e]);
+      *dest(u, i, buf) = o;
     }
+  };
+  // tile j, loaded before, into its buffer
+  auto fill = [&](const Unit& u, int j) {
+    fill_codes(u, true, j & 1);
+    if (__builtin_expect(u.tag == u.page, 0)) fill_staged(u, j & 1);
   };
   constexpr unsigned kInf = QT == OSCAR_BF16 ? 0x7f80u : 0x7c00u;  // the exponent of infinities and NaN
   // tile t at once: the history's ragged end (unseen keys zero), or one of the chunk's
-  auto fill_slow = [&](int t, int j) {
+  auto fill_slow = [&](Unit& own, int t, int j) {
     const bool chunk = t >= htiles;
-    const int key = (chunk ? t - htiles : t) * C::KT + tok;
+    const int key = (chunk ? t - htiles : t) * C::KT + own.tok;
     if (!chunk) {
       const bool in = key < I.hist;
-      const Place x = s_place[j * C::KSUB + (in ? sub : 0)];
-      load_at(x, in ? x.off + in32 : x.off);
-      fill_codes(in, 0);
-      if (in && tag == page) fill_staged(0);
+      const Place x = s_place[j * C::KSUB + (in ? own.sub : 0)];
+      load_at(own, x, in ? x.off + own.in32 : x.off);
+      fill_codes(own, in, 0);
+      if (in && own.tag == own.page) fill_staged(own, 0);
       return;
     }
-    const u32x4* src = (const u32x4*)((const uint16_t*)(vside ? A.v_new : A.k_new) + (int64_t)(I.qa + (key < I.n ? key : 0)) * A.kv_new_stride_token +
-                                      (int64_t)I.kvh * D + 32 * vec);
+    const u32x4* src = (const u32x4*)((const uint16_t*)(own.v ? A.v_new : A.k_new) + (int64_t)(I.qa + (key < I.n ? key : 0)) * A.kv_new_stride_token +
+                                      (int64_t)I.kvh * D + 32 * own.vec);
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       u32x4 x = key < I.n ? kpairs8(src[i]) : u32x4{0u, 0u, 0u, 0u};
-      if (vside) {
+      if (own.v) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const unsigned low = x[e] & kInf, high = (x[e] >> 16) & kInf;
@@ -216,9 +235,9 @@ __device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uin
           x[e] &= (low == kInf ? 0u : 0xffffu) | (high == kInf ? 0u : 0xffff0000u);
         }
       }
-      *dest(i, 0) = x;
+      *dest(own, i, 0) = x;
     }
-    if (odd) atomicOr(&s_odd[sub], 1u << in32);
+    if (odd) atomicOr(&s_odd[own.sub], 1u << own.in32);
   };
 
   // ---- running state of this lane's row
@@ -386,39 +405,80 @@ __device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uin
 
   __syncthreads();  // s_place
   if constexpr (!SLOW) {
-    load(0);
-    fill_codes(true, 0);
-    if (__builtin_expect(tag == page, 0)) fill_staged(0);
-    load(1);
+    // Who unpacks: waves without rows where there are enough of them, since a SIMD that has two waves
+    // with rows has the most to do (wave w runs on SIMD w % 4)
+    const int busy = (I.rows + 31) / 32;
+    // a wave without rows: the units from, from + step and from + 2 step - 2
+    auto serve = [&](auto units, int from, int step) {
+      constexpr int N = decltype(units)::value;
+      Unit u[N > 0 ? N : 1];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        u[i] = unit_of(from + step * i - (i == 2 ? 2 : 0));
+        load(u[i], 0);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        fill(u[i], 0);
+        load(u[i], 1);
+      }
 #pragma unroll 1
-    for (int j = 0; j < I.count; ++j) {
-      __syncthreads();  // tile j is there, and tile j - 1 has been read
-      auto next = [&]() {
-        fill_codes(true, (j + 1) & 1);
-        if (__builtin_expect(tag == page, 0)) fill_staged((j + 1) & 1);
-        load(j + 2);
-        __builtin_amdgcn_sched_barrier(0);  // the scores and what unpacking takes share registers
-      };
-      // The two waves of a SIMD out of step: one unpacks before its products, the other after
-      if (!vside) next();
-      if (active) {
+      for (int j = 0; j < I.count; ++j) {
+        __syncthreads();  // tile j is there, and tile j - 1 has been read
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          fill(u[i], j + 1);
+          load(u[i], j + 2);
+        }
+      }
+    };
+    if (!active) {
+      if (wave < 4 || (wave == 5 && busy == 5)) serve(std::integral_constant<int, 0>{}, 0, 0);
+      else if (busy <= 4) serve(std::integral_constant<int, 2>{}, wave - 4, 4);
+      else if (busy <= 6) serve(std::integral_constant<int, 3>{}, wave - 6, 4);
+      else serve(std::integral_constant<int, 1>{}, wave, 0);
+      return;
+    }
+    // a wave with rows, and a unit of the keys (1), of the values (2) or none
+    auto compute = [&](auto kind) {
+      constexpr int K = decltype(kind)::value;
+      Unit u = unit_of(K == 2 ? 4 + (wave & 3) : wave & 3);
+      u.v = K == 2;
+      if (K) {
+        load(u, 0);
+        fill(u, 0);
+        load(u, 1);
+      }
+#pragma unroll 1
+      for (int j = 0; j < I.count; ++j) {
+        __syncthreads();  // tile j is there, and tile j - 1 has been read
+        auto next = [&]() {
+          fill(u, j + 1);
+          load(u, j + 2);
+          __builtin_amdgcn_sched_barrier(0);  // the scores and what unpacking takes share registers
+        };
+        // The two waves of a SIMD out of step: one unpacks before its products, the other after
+        if (K == 1) next();
         qk(j & 1);
         __builtin_amdgcn_sched_barrier(0);
         softmax();
         half();
         __builtin_amdgcn_sched_barrier(0);
         pv(j & 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if (K == 2) next();
       }
-      __builtin_amdgcn_sched_barrier(0);
-      if (vside) next();
-    }
+    };
+    if (busy > 6 || (busy > 4 && (wave & 6) == 2)) wave < 4 ? compute(std::integral_constant<int, 1>{}) : compute(std::integral_constant<int, 2>{});
+    else compute(std::integral_constant<int, 0>{});
   } else {
+    Unit own = unit_of(wave);
     auto scores = [&](int j) {
       const int t = I.first + I.stride * j;
       __syncthreads();  // the buffers and s_odd have been read
       if (tid < 2) s_odd[tid] = 0;
       __syncthreads();
-      fill_slow(t, j);
+      fill_slow(own, t, j);
       __syncthreads();
       qk(0);
       mask(t);
