@@ -16,9 +16,11 @@
 // and log-sum-exps are merged by tree_merge_kernel.
 //
 // The loop: K and V have two buffers each in LDS, so one barrier a tile does; the codes of tile
-// t + 2 are on their way while t is computed.  Waves 0 to 3 unpack keys before their products and
-// waves 4 to 7 values after theirs: the two waves of a SIMD are out of step, and give its matrix unit
-// and its vector unit something to do at the same time.
+// t + 2 are on their way while t is computed.  With more than 192 rows waves 0 to 3 unpack keys before
+// their products and waves 4 to 7 values after theirs: the two waves of a SIMD are out of step, and
+// give its matrix unit and its vector unit something to do at the same time.  With fewer, waves without
+// rows unpack for those with them (192 rows 79 -> 72 us with the merge).  Each kind of wave has a
+// loop of its own: with one for all, the queries did not stay in registers.
 //
 // LDS: K in operand order, 16 bytes a lane.  V one row per key, 32 elements of padding, its
 // 16-byte units exchanged by the key's bits 2 and 3: rows then spread over all banks, for the
@@ -31,16 +33,19 @@
 // value of the chunk that is not finite goes into LDS as zero and is added afterwards, to the
 // rows alone that see its node.
 //
-// What bounds it: 8 requests of 24576 tokens with 32 nodes (192 rows, D 256) take 66 to 70 us, 0.57
-// PFLOP/s in 39 GFLOP: 24 tiles a workgroup at 2.2 us and 12 us before and after them, of which
+// What bounds it: 8 requests of 24576 tokens with 32 nodes (192 rows, D 256) take 61 to 63 us, 0.62
+// PFLOP/s in 39 GFLOP: 24 tiles a workgroup at 2.0 us and 12 us before and after them, of which
 // 50 MB of partials; their merge takes another 10 us.  A tile's products alone take 1.0 us at the 2.0 to
-// 2.1 GHz that the matrix units leave the clock, its softmax and unpacking (about 300 vector
-// instructions a wave) as long again, and the two overlap in part.  12 ragged requests of up to 64
-// nodes, D 128 with capped scores: 71 us, bound by the cap's exponentials and divides.  One request of 500
-// tokens and 16 nodes: 15 us, latency.  Measured against it, at 8 x 24576 tokens: four waves of 16 or
-// 64 rows with 16x16x32 products, 99 to 165 us; the softmax of tile t - 1 between the products
-// of tile t in one wave, 86 to 114; slow tiles in the same loop, 113 (registers spill); codes two
-// tiles ahead, two accumulators of S or a higher wave priority, no gain beyond the noise.
+// 2.1 GHz that the matrix units leave the clock, its softmax and unpacking (about 255 vector
+// instructions a wave) as long again, and the two overlap in part (252 rows: the matrix unit busy for 36%
+// of the cycles, the waves waiting for a third).  12 ragged requests of up to 64 nodes, D 128 with capped
+// scores: 65 to 69 us, bound by the cap's exponentials and divides.  One request of 500 tokens and 16
+// nodes: 15 us, latency.  Measured against it, at 8 x 24576 tokens: four waves of 16 or 64 rows with
+// 16x16x32 products, 99 to 165 us; the softmax of tile t - 1 between the products of tile t in one
+// wave, 86 to 114; slow tiles in the same loop, 113 (registers spill); two tiles a barrier, 14 us more; the
+// products of values a tile late in the second wave of a SIMD, 4 us less with 252 rows, 2 more in
+// ragged calls; LDS operands read once instead of anew for each product, 1 us (they are not the
+// bound); two accumulators of S or a higher wave priority, no gain beyond the noise.
 #include <type_traits>
 #include <vector>
 
