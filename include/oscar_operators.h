@@ -259,7 +259,7 @@ int oscarop_tree_mask_v1(const oscarop_tree_args_v1* args, void* stream);
  * oscarop_attn_decode_v1 for chunks whose rows see each other by a mask: query i of n_q sees
  * all of the history, and chunk row j <= i if bit j of its row of mask is set (rows past the
  * mask's words are not seen).  A row that sees no key gets zeros and lse -inf.  No
- * alibi_slopes (a node's distance is its depth, not its row).  History keys are
+ * alibi_slopes (a node's distance is its depth, not its row); scale > 0.  History keys are
  * q_dtype(fp16(x)), history values fp16(x), the chunk's as they are; probabilities are rounded to
  * fp16 for the history, to two bf16 parts for a bf16 chunk; sums and the softmax are fp32.  The
  * same plan gives the same bits. */
@@ -364,7 +364,7 @@ int oscarop_select_v1(const oscarop_select_args_v1* args, void* stream);
 /* oscarop_attn_decode_v1 with a block table for each KV head: head h of request r reads row
  * r of block_table shifted by h * table_stride_head, as oscarop_select_v1 writes it.  The
  * lengths and the plan are those of the chosen tokens.  No alibi_slopes (the chosen pages' distances are
- * not the table's). */
+ * not the table's); scale > 0. */
 int oscarop_attn_selected_v1(const oscar_attn_args_v1* args, const oscarop_score_v1* score, int64_t table_stride_head,
                              void* stream);
 

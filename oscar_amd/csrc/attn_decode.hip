@@ -1413,6 +1413,8 @@ extern "C" int oscarop_attn_selected_v1(const oscar_attn_args_v1* args, const os
   if (args->num_items > 0 && (hk < 1 || table_stride_head < 1 || table_stride_head < args->block_table_cols ||
                               table_stride_head > args->block_table_stride / hk))
     return fail(-22, "oscarop_attn_selected_v1: a request's row holds a table for each KV head");
+  if (args->num_items > 0 && (!(args->scale > 0.f) || args->scale > 3e38f))
+    return fail(-22, "oscarop_attn_selected_v1: scale must be positive and finite");
   return launch_checked(*args, "oscarop_attn_selected_v1", args->workspace, args->workspace_bytes, (hipStream_t)stream,
                         score, nullptr, nullptr, table_stride_head);
 }

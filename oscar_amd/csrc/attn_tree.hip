@@ -782,6 +782,8 @@ extern "C" int oscarop_attn_tree_v1(const oscarop_tree_attn_args_v1* args, const
   if (args->partial_rows < 1 || args->partial_rows > INT32_MAX || !a.workspace || ((uintptr_t)a.workspace & 15) ||
       a.workspace_bytes < need)
     return fail(-22, "%s: workspace of %lld bytes < %lld", name, (long long)a.workspace_bytes, (long long)need);
+  // (the largest product is the largest score)
+  if (!(a.scale > 0.f) || a.scale > 3e38f) return fail(-22, "%s: scale must be positive and finite", name);
   p.a = *args;
   p.has_stage = a.staging != nullptr;
   if (a.staging) p.st = *a.staging;

@@ -1107,7 +1107,8 @@ def release_pages(pool: PagePool, block_table, lengths, new_lengths, *, block_si
     (its plan's lengths and seq_lens, with plan.table(...)).  The pool grows in place, requests
     in their order, their pages ascending, so that what map_slots took last lies as it lay;
     the table keeps its entries.  A new length below 0 or above the old one gives nothing back,
-    nor does a request whose pages the pool has no room for, nor those with pages behind it."""
+    nor does a request whose pages the pool has no room for, nor those with pages behind it.  The
+    pages must be the request's own: one that two requests name comes back twice."""
     index = _device_index(pool.pages, pool.count, block_table, lengths, new_lengths)
     _check_pool(pool)
     reqs = lengths.shape[0] if lengths.ndim == 1 else -1

@@ -15,7 +15,7 @@ from oracle.attention import read_history
 from oscar_amd import _lib, ops
 from test_capi import HEADER
 from test_page_select import plain_choice
-from test_tree_attention import bits, check, random_parents, reference
+from test_tree_attention import attn_args, bits, check, random_parents, reference
 
 D, HQ, HK, BS, SCALE = 256, 12, 2, 128, 256 ** -0.5
 
@@ -210,6 +210,53 @@ def test_drafts_and_sparse_steps_on_the_device(cuda):
         loop.check()
     ops.release_pages(loop.pool, loop.table, loop.lengths, loop.lengths * 0, block_size=BS)
     assert int(loop.pool.count) == 40 and sorted(loop.pool.pages.tolist()) == list(range(40))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, float("nan"), float("inf")])
+def test_scales_refused(scale):
+    lib = _lib.load()
+    a = attn_args(scale=scale)
+    assert lib.oscarop_attn_tree_v1(C.byref(a), None, None) == -22 and b"scale" in lib.oscar_last_error()
+    assert lib.oscarop_attn_selected_v1(C.byref(a.attn), None, 4, None) == -22 and b"scale" in lib.oscar_last_error()
+
+
+@pytest.mark.gpu
+def test_accepted_nodes_and_the_window(cuda):
+    """The store of a tree's accepted rows keeps their FP32 copies, as one of these rows alone does, and
+    the next tree reads them."""
+    loop = Loop(cuda, 2, 20, 8)
+    loop.write([300, 140], loop.rand(440, HK), loop.rand(440, HK))
+    stages = [tuple([torch.zeros(64, BS, HK, D, device=cuda), torch.zeros(64, BS, HK, D, device=cuda),
+                     torch.full((64, BS), -1, dtype=torch.int64, device=cuda)]) for _ in range(2)]
+    nodes, kept = [9, 6], [[0, 3, 4, 8], [1, 2]]
+    keep = torch.zeros(15, dtype=torch.bool)
+    keep[[0, 3, 4, 8, 10, 11]] = True
+    k, v = loop.rand(15, HK), loop.rand(15, HK)
+    m = ops.map_slots(loop.pool, loop.table, loop.lengths, torch.tensor(nodes, dtype=torch.int32, device=cuda), tokens=15, block_size=BS,
+                      keep=keep.to(cuda))
+    window = dict(head_dim=D, stage_mode=ops.STAGE_WRITE, num_reqs=2, recent_tokens=64)
+    caches = [[c.clone() for c in loop.caches] for _ in range(2)]
+    ops.store(k, v, *caches[0], m.slots, stage=stages[0], qsl_dev=m.qsl, seqs_dev=m.seq_lens, **window)
+    rows = keep.nonzero()[:, 0].to(cuda)
+    starts = torch.tensor([0, len(kept[0]), len(kept[0]) + len(kept[1])], dtype=torch.int32, device=cuda)
+    ops.store(k[rows], v[rows], *caches[1], m.slots[rows], stage=stages[1], qsl_dev=starts, seqs_dev=m.seq_lens, **window)
+    assert all(torch.equal(a, b) for a, b in zip((*caches[0], *stages[0]), (*caches[1], *stages[1])))
+    assert (stages[0][2] >= 0).sum() == 6
+    # all nodes of a chain see the copies: their products with the copies' own keys
+    q = loop.rand(2, HQ)
+    plan = ops.plan_tree([0, 1, 2], [305, 143], num_kv_heads=HK, group=HQ // HK, head_dim=D, device=cuda)
+    mask, _ = ops.tree_mask(torch.tensor([-1, -1], dtype=torch.int32, device=cuda), torch.tensor([0, 1, 2], dtype=torch.int32, device=cuda), max_nodes=1)
+    new = [loop.rand(2, HK) for _ in range(2)]
+    out, lse = ops.attention_tree(q, *new, *caches[0], loop.table, plan, mask, SCALE, stages[0], head_dim=D)
+    for r, h in enumerate([304, 142]):
+        table, st = loop.table[r].cpu().numpy(), tuple(x.cpu().numpy() for x in stages[0])
+        flat = [c.cpu().numpy().view(np.uint8) for c in caches[0]]
+        old = read_history(*flat, table, 0, h, HK, D, st, "bf16")[0], read_history(*flat, table, 0, h, HK, D, st, "f16")[1]
+        plain = read_history(*flat, table, 0, h, HK, D, None, "bf16")[0]
+        assert (np.abs(old[0] - plain).max((1, 2)) > 0).sum() == len(kept[r])
+        keys, values = (np.concatenate([x, y[r:r + 1].float().cpu().numpy()]) for x, y in zip(old, new))
+        want = reference(q[r:r + 1].float().cpu().numpy(), keys, values, np.ones((1, h + 1), bool), SCALE, 0.0)
+        check((out[r:r + 1], lse[r:r + 1]), (*want, (h + 1) * np.abs(values).max() * 2.0 ** -32))
 
 
 @pytest.mark.gpu
