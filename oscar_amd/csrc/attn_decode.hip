@@ -427,6 +427,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   __syncthreads();
   u32x4* s_kop = (u32x4*)s_u;                                 // [kTile][2][NCH][2]
   uint16_t* s_slowv = (uint16_t*)(s_u + kKopBytes);           // [kTile][VROW]
+  __shared__ uint32_t s_odd[2];  // OWN: tokens of a slow tile and of the next with values that are not finite
+  constexpr unsigned kInf = QT == OSCAR_BF16 ? 0x7f80u : 0x7c00u;  // the exponent of these
   // builder share: token bt of the tile, units uid = bpart + 16 u (u < NU) of the
   // 4 * NCH (K|V, half, 16-element chunk) units of the token
   constexpr int NU = C::NCH / 4;
@@ -474,7 +476,9 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   };
   // slow tile j (its inputs loaded by load_slow): every thread builds its units' K
   // operands and V values into LDS with the reference rounding
-  auto build_slow = [&](int j) {
+  // (OWN: values of the current chunk that are not finite go in as zeros, since a row that does not see
+  // them multiplies them by zero; *odd gets their tokens' bits)
+  auto build_slow = [&](int j, uint32_t* odd) {
     bool b_staged, b_codes, b_cur;
     slow_flags(j, b_staged, b_codes, b_cur);
 #pragma unroll
@@ -506,6 +510,16 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
         // V values as (e, e+8) pairs
         if (b_cur) {
           interleave8(__builtin_bit_cast(u32x4, sx[u][0]), __builtin_bit_cast(u32x4, sx[u][1]), o);
+          if constexpr (OWN) {
+            bool any = false;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              const bool low = (o[x] & kInf) == kInf, high = ((o[x] >> 16) & kInf) == kInf;
+              any |= low || high;
+              o[x] &= (low ? 0u : 0xffffu) | (high ? 0u : 0xffff0000u);
+            }
+            if (any) atomicOr(odd, 1u << bt);
+          }
         } else if (b_codes) {
           unsigned vlo, vhi;
           value_table<QT>(smeta[1], vlo, vhi);
@@ -529,7 +543,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
     }
   };
   // wave `runner` adds slow tile j (built in LDS) to its softmax state
-  auto compute_slow = [&](int j, int runner) {
+  auto compute_slow = [&](int j, int runner, const uint32_t* odd) {
       const int t0 = tile_t0(j);
       if (wave == runner) {
         f32x16 S = {};
@@ -566,6 +580,10 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
           const float p0 = (xs[r] == -INFINITY) ? 0.f : exp2f(xs[r] - m_run);
           const float p1 = (xs[r + 1] == -INFINITY) ? 0.f : exp2f(xs[r + 1] - m_run);
           lsum += p0 + p1;
+          if constexpr (OWN) {
+            xs[r] = p0;
+            xs[r + 1] = p1;
+          }
           const unsigned hb = q_pair<QT>(p0, p1);
           ph[r >> 3][(r & 7) >> 1] = hb;
           pl[r >> 3][(r & 7) >> 1] = q_pair<QT>(p0 - q_half<QT>(hb, 0), p1 - q_half<QT>(hb, 1));
@@ -588,6 +606,27 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
             }
             O[b] = mma16<QT>(va, ph[s], O[b]);
             O[b] = mma16<QT>(va, pl[s], O[b]);
+          }
+        }
+        if constexpr (OWN) {
+          // the values that went in as zeros, for the rows that see them; a key's p is in the
+          // lane of the row that holds the key
+#pragma unroll 1
+          for (uint32_t left = __builtin_amdgcn_readfirstlane(*odd); left != 0; left &= left - 1) {
+            const int key = __builtin_ctz(left), tp = t0 + key;
+            float mine = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mine = out_tok(r, g) == key ? xs[r] : mine;
+            const float other = swap_halves(mine), p = ((key >> 2) & 1) == g ? mine : other;
+            const bool seen = row_ok && tp < limit;
+            const uint16_t* v = (const uint16_t*)A.v_new + (int64_t)(cur0 + tp - hist) * A.kv_new_stride_token + (int64_t)kvh * D;
+#pragma unroll
+            for (int b = 0; b < C::MBLK; ++b)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const unsigned x = v[pv_d<D>(b, out_tok(r, g))];
+                if (seen && (x & kInf) == kInf) O[b][r] = fmaf(p, QT == OSCAR_BF16 ? bf16_bits_to_f32(x) : f16_bits_to_f32(x), O[b][r]);
+              }
           }
         }
       }
@@ -781,15 +820,17 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   // waits until all waves are past it (nslow is the same for the whole workgroup).
   if (nslow > 0) {
     load_slow(__builtin_amdgcn_readfirstlane(s_slow[0]));
+    if (OWN && tid < 2) s_odd[tid] = 0;
     __syncthreads();
   }
 #pragma unroll 1
   for (int k = 0; k < nslow; ++k) {
     const int j = __builtin_amdgcn_readfirstlane(s_slow[k]);
-    build_slow(j);
+    build_slow(j, &s_odd[k & 1]);
     __syncthreads();  // the tile's K operands and V values are in LDS
+    if (OWN && tid == 0) s_odd[(k + 1) & 1] = 0;
     if (k + 1 < nslow) load_slow(__builtin_amdgcn_readfirstlane(s_slow[k + 1]));
-    compute_slow(j, k % kWaves);
+    compute_slow(j, k % kWaves, &s_odd[k & 1]);
     __syncthreads();  // the LDS buffers are rewritten by the next tile
   }
 

@@ -1399,7 +1399,8 @@ def select_pages(q, bounds, block_table, plan: SelectPlan) -> tuple:
 def attention_selected(q, k_new, v_new, k_cache, v_cache, table, plan: SelectPlan, scale, stage=None, *, head_dim,
                        soft_cap=0.0, out_rot=None, lse=None):
     """Attention over the pages that select_pages chose, and the current chunk: (out_rot fp32,
-    lse fp32), rotated, as attention_decode's, whose other arguments and rules these are.  table
+    lse fp32), rotated, as attention_decode's, whose other arguments and rules these are, but
+    that a value of the chunk that is not finite reaches the queries that see it alone.  table
     [requests, Hk, budget]: each KV head's pages, ascending."""
     index = _device_index(q, k_new, v_new, k_cache, v_cache, table, plan.qsl, out_rot, lse, *(stage or ()))
     if plan.has_new != (k_new is not None) or (k_new is None) != (v_new is None):

@@ -446,3 +446,36 @@ def test_captured_streams_and_refusals(cuda):
                          (lambda: ops.attention_selected(q, k, v, k_cache[:, :64].contiguous(), v_cache[:, :64].contiguous(), t, plan, 0.1, head_dim=128), "pages of 128")):
         with pytest.raises(ValueError, match=message):
             bad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_values_that_are_not_finite(cuda, bad, shape, dtype):
+    """A value of the chunk that is not finite reaches the queries that see it, in its channel, and a
+    key the queries that see it: the others and the other channels stay what they were."""
+    hists, chunks = [1500, 40], [4, 3]
+    c, x, k_cache, v_cache, stage, table, bounds, plan = sparse_case(cuda, hists, chunks, dtype=dtype, budget=6, first=1, last=3, **shape)
+    q, k, v = (x[n].to(cuda) for n in "qkv")
+    got_table, _ = ops.select_pages(q, bounds, table.to(cuda), plan)
+    call = lambda k, v: ops.attention_selected(q, k, v, k_cache, v_cache, got_table, plan, c["scale"], stage, head_dim=shape["d"])[0].cpu()  # noqa: E731
+    clean = call(k, v)
+    for row, head, channel in ((2, 0, 5), (3, shape["hk"] - 1, shape["d"] - 1), (5, 0, 64)):
+        sees = torch.zeros(7, dtype=torch.bool)
+        sees[row:4 if row < 4 else 7] = True
+        heads = slice(head * shape["group"], (head + 1) * shape["group"])
+        hit = torch.zeros_like(clean, dtype=torch.bool)
+        hit[:, heads, channel] = sees[:, None]
+        worse = v.clone()
+        worse[row, head, channel] = bad
+        out = call(k, worse)
+        assert torch.equal(~out.isfinite(), hit)
+        assert math.isnan(bad) or (out[hit] == bad).all()
+        # (the decode's waves take tiles as they get to them: its last bits are not fixed)
+        assert (out - clean)[~hit].abs().max() <= 1e-3
+        worse = k.clone()
+        worse[row, head, channel] = math.nan
+        out = call(worse, v)
+        hit[:, heads] = sees[:, None, None]
+        assert torch.equal(~out.isfinite(), hit) and (out - clean)[~hit].abs().max() <= 1e-3
