@@ -321,7 +321,8 @@ int oscarop_page_bounds_v1(const oscarop_bounds_args_v1* args, void* stream);
  * heads of the KV head, of the sum over the channels of max(q low, q high), summed in 64
  * bits.  table[r][h] holds the chosen pages in ascending order of their columns and
  * pages[r][h] these columns, -1 behind them.  A request that does not fit (queries past
- * num_tokens, a negative history, columns past the table) gets -1 throughout. */
+ * num_tokens, a negative history, columns past the table) gets -1 throughout.  Without has_new
+ * the queries have to lie in the last last_pages pages for the attention to know what each sees. */
 #define OSCAROP_SELECT_ARRIVAL 32 /* int32 of a list's arrival counter: a cache line of its own */
 typedef struct oscarop_select_args_v1 {
   const void* q;                  /* [num_tokens, num_q_heads, D] in q_dtype */

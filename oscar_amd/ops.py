@@ -1330,7 +1330,9 @@ def plan_selected(qsl, seqs, *, has_new: bool, block_size: int, budget: int, fir
     """Plan of select_pages and attention_selected (host lists, as plan_decode): of each history
     at most `budget` pages are read, among them the first first_pages and the last last_pages (at
     least 1; enough for the FP32 window, ceil(recent / block_size) + 1, if its tokens are to be
-    seen), for all queries of a request the same."""
+    seen), for all queries of a request the same.  Queries whose keys are in the cache already
+    (has_new False) must lie in the last last_pages pages, where what each sees is told by
+    its place."""
     qsl, seqs = _request_lists(qsl, seqs, has_new)
     if block_size < 1 or first_pages < 0 or last_pages < 1 or budget <= first_pages + last_pages:
         raise ValueError("the budget must exceed first_pages + last_pages, last_pages be 1 at least")
@@ -1338,6 +1340,8 @@ def plan_selected(qsl, seqs, *, has_new: bool, block_size: int, budget: int, fir
     for a, b, seq in zip(qsl, qsl[1:], seqs):
         pages = -(-(seq - (b - a) if has_new else seq) // block_size)
         most = max(most, pages)
+        if not has_new and pages > budget and b - a > seq - (pages - last_pages) * block_size:
+            raise ValueError(f"{b - a} cached queries reach beyond the last {last_pages} pages")
         fewer.append(seq - max(pages - budget, 0) * block_size)
     plan = plan_decode(qsl, fewer, has_new=has_new, num_kv_heads=num_kv_heads, group=group, head_dim=head_dim,
                        device=device, window=window, upload_now=False)

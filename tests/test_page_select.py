@@ -103,6 +103,23 @@ def test_plan_refusals():
             plan(**bad)
 
 
+@pytest.mark.parametrize("seq,n,last,fits", [(1280, 128, 1, True), (1280, 129, 1, False), (1281, 1, 1, True), (1281, 2, 1, False),
+                                             (1281, 129, 2, True), (1281, 130, 2, False), (512, 500, 1, True)])
+def test_cached_queries_in_the_last_pages(monkeypatch, seq, n, last, fits):
+    """A query in a page that may be left out would not know what it sees (512 tokens: all pages are
+    read); new keys stand behind the chosen pages, and any number of queries is served."""
+    monkeypatch.setattr(ops, "cu_count", lambda device: 256)
+    sizes = dict(block_size=128, budget=4, last_pages=last, num_kv_heads=1, group=6, head_dim=256, device="cpu")
+    plan = lambda seq, has_new: ops.plan_selected([0, n], [seq], has_new=has_new, **sizes)  # noqa: E731
+    monkeypatch.setattr(ops, "upload", lambda parts, device: [torch.from_numpy(np.array(p)) for p in parts])
+    if fits:
+        assert plan(seq, False).max_pages == -(-seq // 128)
+    else:
+        with pytest.raises(ValueError, match="cached queries"):
+            plan(seq, False)
+    assert plan(seq + n, True).max_pages == -(-seq // 128)
+
+
 # ------------------------------------------------------------------ bounds
 def plain_keys(k8, d):
     """The keys of every slot, fp16 [blocks, bs, hk, d]: mul, then add, in fp32, as the cache's reader."""
@@ -348,7 +365,8 @@ def sparse_case(cuda, hists, chunks, *, hk, group, d, dtype, budget, first, last
 @pytest.mark.parametrize("cap", [0.0, 20.0])
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("shape", SHAPES, ids=str)
-@pytest.mark.parametrize("hists,chunks,has_new", [([6000], [1], True), ([2000, 130, 128 * 12, 0], [4, 2, 9, 3], True), ([3000, 500], [2, 3], False)])
+@pytest.mark.parametrize("hists,chunks,has_new", [([6000], [1], True), ([2000, 130, 128 * 12, 0], [4, 2, 9, 3], True), ([3000, 500], [2, 3], False),
+                                                  ([2700, 1500], [260, 300], False), ([1400], [200], True)])
 def test_attention(cuda, hists, chunks, has_new, shape, dtype, cap):
     """Chosen pages with their window copies and the current chunk, against the formula over those
     tokens alone; the pages that the kernel chose are the plain choice."""
