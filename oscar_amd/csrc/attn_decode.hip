@@ -160,6 +160,9 @@ struct TileRegs {
 // OWN: each KV head reads a block table of its own, the pages chosen for it (oscarop_attn_selected_v1).
 // 8 requests of 48 pages and 24 rows 16.0 us, 16 of 64 pages and 6 rows 23.7: the plain decode of as many
 // tokens, about 8 us of prologue, drain and merge with it, and 0.3 to 0.7 for values that are not finite.
+// Its slow tiles hold history values as fp16(x) for bf16 queries as well (the plain ones as the reference
+// rounds them, bf16(fp16(x))): 0 to 0.8 us of 36 to 49; one request of 5 pages 2.0e-3 -> 1.7e-3 off,
+// its outputs' last rounding alone.
 template <int D, int QT, int SC, bool OWN>
 __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   using C = Cfg<D>;
@@ -216,7 +219,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   // output blocks [kWaves][4][4][64] f32x4
   constexpr int kVcodeBytes = kWaves * kTile * C::NB;
   constexpr int kKopBytes = kTile * 2 * C::NCH * 8 * 4;
-  constexpr int kSlowBytes = kKopBytes + kTile * C::VROW * 2;
+  constexpr bool kParts = OWN && QT == OSCAR_BF16;  // V values in two parts, see build_slow
+  constexpr int kSlowBytes = kKopBytes + (kParts ? 2 : 1) * kTile * C::VROW * 2;
   constexpr int kMergeBytes = kWaves * 4 * 4 * 64 * 16;
   constexpr int kU0 = kVcodeBytes > kSlowBytes ? kVcodeBytes : kSlowBytes;
   __shared__ __attribute__((aligned(16))) uint8_t s_u[kU0 > kMergeBytes ? kU0 : kMergeBytes];
@@ -427,6 +431,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   __syncthreads();
   u32x4* s_kop = (u32x4*)s_u;                                 // [kTile][2][NCH][2]
   uint16_t* s_slowv = (uint16_t*)(s_u + kKopBytes);           // [kTile][VROW]
+  uint16_t* s_slowl = s_slowv + kTile * C::VROW;              // kParts: what bf16 leaves out, alike
   __shared__ uint32_t s_odd[2];  // OWN: tokens of a slow tile and of the next with values that are not finite
   constexpr unsigned kInf = QT == OSCAR_BF16 ? 0x7f80u : 0x7c00u;  // the exponent of these
   // builder share: token bt of the tile, units uid = bpart + 16 u (u < NU) of the
@@ -476,6 +481,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   };
   // slow tile j (its inputs loaded by load_slow): every thread builds its units' K
   // operands and V values into LDS with the reference rounding
+  // (kParts: history values stay fp16(x), as the fast tiles have them, beside bf16 ones of the chunk: as the
+  // sum of two bf16 parts, which hold its 11 bits)
   // (OWN: values of the current chunk that are not finite go in as zeros, since a row that does not see
   // them multiplies them by zero; *odd gets their tokens' bits)
   auto build_slow = [&](int j, uint32_t* odd) {
@@ -496,7 +503,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
           }
         } else {
 #pragma unroll
-          for (int x = 0; x < 8; ++x) o[x] = hist_pair<QT>(f[x >> 2][x & 3], f[2 + (x >> 2)][x & 3]);
+          for (int x = 0; x < 8; ++x) o[x] = hist_pair<kParts ? OSCAR_F16 : QT>(f[x >> 2][x & 3], f[2 + (x >> 2)][x & 3]);
         }
       } else if (kv == 0) {
         if (b_cur) {
@@ -522,7 +529,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
           }
         } else if (b_codes) {
           unsigned vlo, vhi;
-          value_table<QT>(smeta[1], vlo, vhi);
+          value_table<kParts ? OSCAR_F16 : QT>(smeta[1], vlo, vhi);
           table_pairs(__float_as_uint(sx[u][0][0]), vlo, vhi, o);
         }
       }
@@ -535,6 +542,20 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
         // reads column 32 b + i (d = pv_d(b, i))
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
+          if constexpr (kParts) {
+            unsigned low[2] = {0u, 0u};
+            if (!b_cur) {
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const float a = f16_bits_to_f32(o[q + 4 * x] & 0xffffu), b = f16_bits_to_f32(o[q + 4 * x] >> 16);
+                const unsigned hb = q_pair<OSCAR_BF16>(a, b);
+                low[x] = q_pair<OSCAR_BF16>(a - q_half<OSCAR_BF16>(hb, 0), b - q_half<OSCAR_BF16>(hb, 1));
+                o[q + 4 * x] = hb;
+              }
+            }
+            *(u32x2*)&s_slowl[bt * C::VROW + vbuf_col<D>(hg, q, c)] = u32x2{__builtin_amdgcn_perm(low[1], low[0], 0x05040100u),
+                                                                            __builtin_amdgcn_perm(low[1], low[0], 0x07060302u)};
+          }
           const u32x2 w = {__builtin_amdgcn_perm(o[q + 4], o[q], 0x05040100u),
                            __builtin_amdgcn_perm(o[q + 4], o[q], 0x07060302u)};
           *(u32x2*)&s_slowv[bt * C::VROW + vbuf_col<D>(hg, q, c)] = w;
@@ -590,22 +611,36 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
         }
         l_run += lsum;
         const int G16 = lane >> 4, i16 = lane & 15;
+        // the A operand of output block b, K-step s
+        auto operand = [&](const uint16_t* values, int b, int s) {
+          u32x4 va;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int key = 16 * s + 4 * (G16 >> 1) + 8 * h + (i16 >> 2);
+            const uint16_t* addr = &values[key * C::VROW + 32 * b + 16 * (G16 & 1) + 4 * (i16 & 3)];
+            const u32x2 t = __builtin_bit_cast(
+                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(addr)));
+            va[2 * h] = t[0];
+            va[2 * h + 1] = t[1];
+          }
+          return va;
+        };
 #pragma unroll
         for (int b = 0; b < C::MBLK; ++b) {
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            u32x4 va;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int key = 16 * s + 4 * (G16 >> 1) + 8 * h + (i16 >> 2);
-              const uint16_t* addr = &s_slowv[key * C::VROW + 32 * b + 16 * (G16 & 1) + 4 * (i16 & 3)];
-              const u32x2 t = __builtin_bit_cast(
-                  u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(addr)));
-              va[2 * h] = t[0];
-              va[2 * h + 1] = t[1];
-            }
+            const u32x4 va = operand(s_slowv, b, s);
             O[b] = mma16<QT>(va, ph[s], O[b]);
             O[b] = mma16<QT>(va, pl[s], O[b]);
+          }
+        }
+        if constexpr (kParts) {
+          // (the two low parts' product, 2^-18 of a value, is left out; a tile of the chunk alone has none)
+          if (t0 < hist) {
+#pragma unroll
+            for (int b = 0; b < C::MBLK; ++b)
+#pragma unroll
+              for (int s = 0; s < 2; ++s) O[b] = mma16<QT>(operand(s_slowl, b, s), ph[s], O[b]);
           }
         }
         if constexpr (OWN) {
