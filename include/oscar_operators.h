@@ -367,7 +367,7 @@ int oscarop_select_v1(const oscarop_select_args_v1* args, void* stream);
  * lengths and the plan are those of the chosen tokens.  History keys are q_dtype(fp16(x)), history
  * values fp16(x) (full tiles of codes: x itself), the chunk's as they are; probabilities are rounded to
  * fp16 times a value's scale in full tiles of codes, to two parts in q_dtype elsewhere; sums and the softmax
- * are fp32.  A value of the current chunk that is not finite reaches the queries that see it alone.  No alibi_slopes (the chosen pages' distances are
+ * are fp32.  A value that is not finite reaches no query that does not see its token.  No alibi_slopes (the chosen pages' distances are
  * not the table's); scale > 0. */
 int oscarop_attn_selected_v1(const oscar_attn_args_v1* args, const oscarop_score_v1* score, int64_t table_stride_head,
                              void* stream);

@@ -222,7 +222,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   constexpr bool kParts = OWN && QT == OSCAR_BF16;  // V values in two parts, see build_slow
   constexpr int kSlowBytes = kKopBytes + (kParts ? 2 : 1) * kTile * C::VROW * 2;
   constexpr int kMergeBytes = kWaves * 4 * 4 * 64 * 16;
-  constexpr int kU0 = kVcodeBytes > kSlowBytes ? kVcodeBytes : kSlowBytes;
+  constexpr int kOddBytes = OWN ? D * 4 : 0;
+  constexpr int kU0 = kVcodeBytes > kSlowBytes + kOddBytes ? kVcodeBytes : kSlowBytes + kOddBytes;
   __shared__ __attribute__((aligned(16))) uint8_t s_u[kU0 > kMergeBytes ? kU0 : kMergeBytes];
   uint8_t (*s_vcode)[kTile * C::NB] = (uint8_t (*)[kTile * C::NB])s_u;
   const unsigned st_rows = (unsigned)P.st.rows;
@@ -432,8 +433,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   u32x4* s_kop = (u32x4*)s_u;                                 // [kTile][2][NCH][2]
   uint16_t* s_slowv = (uint16_t*)(s_u + kKopBytes);           // [kTile][VROW]
   uint16_t* s_slowl = s_slowv + kTile * C::VROW;              // kParts: what bf16 leaves out, alike
+  float* s_oddv = (float*)(s_u + kSlowBytes);                 // OWN: a token's values that are not finite
   __shared__ uint32_t s_odd[2];  // OWN: tokens of a slow tile and of the next with values that are not finite
-  constexpr unsigned kInf = QT == OSCAR_BF16 ? 0x7f80u : 0x7c00u;  // the exponent of these
   // builder share: token bt of the tile, units uid = bpart + 16 u (u < NU) of the
   // 4 * NCH (K|V, half, 16-element chunk) units of the token
   constexpr int NU = C::NCH / 4;
@@ -483,8 +484,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
   // operands and V values into LDS with the reference rounding
   // (kParts: history values stay fp16(x), as the fast tiles have them, beside bf16 ones of the chunk: as the
   // sum of two bf16 parts, which hold its 11 bits)
-  // (OWN: values of the current chunk that are not finite go in as zeros, since a row that does not see
-  // them multiplies them by zero; *odd gets their tokens' bits)
+  // (OWN: values that are not finite go in as zeros, since a row that does not see them multiplies them
+  // by zero; *odd gets their tokens' bits)
   auto build_slow = [&](int j, uint32_t* odd) {
     bool b_staged, b_codes, b_cur;
     slow_flags(j, b_staged, b_codes, b_cur);
@@ -517,20 +518,23 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
         // V values as (e, e+8) pairs
         if (b_cur) {
           interleave8(__builtin_bit_cast(u32x4, sx[u][0]), __builtin_bit_cast(u32x4, sx[u][1]), o);
-          if constexpr (OWN) {
-            bool any = false;
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const bool low = (o[x] & kInf) == kInf, high = ((o[x] >> 16) & kInf) == kInf;
-              any |= low || high;
-              o[x] &= (low ? 0u : 0xffffu) | (high ? 0u : 0xffff0000u);
-            }
-            if (any) atomicOr(odd, 1u << bt);
-          }
         } else if (b_codes) {
           unsigned vlo, vhi;
           value_table<kParts ? OSCAR_F16 : QT>(smeta[1], vlo, vhi);
           table_pairs(__float_as_uint(sx[u][0][0]), vlo, vhi, o);
+        }
+      }
+      if constexpr (OWN) {
+        if (kv == 1) {
+          const unsigned inf = kParts && b_cur ? 0x7f80u : 0x7c00u;  // the exponent of infinities and NaN
+          bool any = false;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const bool low = (o[x] & inf) == inf, high = ((o[x] >> 16) & inf) == inf;
+            any |= low || high;
+            o[x] &= (low ? 0u : 0xffffu) | (high ? 0u : 0xffff0000u);
+          }
+          if (any) atomicOr(odd, 1u << bt);
         }
       }
       if (kv == 0) {
@@ -654,14 +658,37 @@ __global__ __launch_bounds__(kThreads, 1) void attn_main_kernel(AttnParams P) {
             for (int r = 0; r < 16; ++r) mine = out_tok(r, g) == key ? xs[r] : mine;
             const float other = swap_halves(mine), p = ((key >> 2) & 1) == g ? mine : other;
             const bool seen = row_ok && tp < limit;
-            const uint16_t* v = (const uint16_t*)A.v_new + (int64_t)(cur0 + tp - hist) * A.kv_new_stride_token + (int64_t)kvh * D;
+            // the token's values as they are held (the chunk's, a window copy or a code's), the finite ones zero
+            int blk, off0, seat0;
+            tile_page(j, t0, blk, off0, seat0);
+            const uint8_t* slot = vbase + (int64_t)blk * vs0 + (int64_t)(off0 + key) * vs1;
+            unsigned lo = 0u, hi = 0u;
+            if (tp < hist) value_table<OSCAR_F16>(*(const unsigned*)(kbase + (int64_t)blk * ks0 + (int64_t)(off0 + key) * ks1 + 4), lo, hi);
+#pragma unroll 1
+            for (int d = lane; d < D; d += 64) {
+              float x;
+              if (tp >= hist) {
+                x = q_half<QT>(((const uint16_t*)A.v_new)[(int64_t)(cur0 + tp - hist) * A.kv_new_stride_token + (int64_t)kvh * D + d], 0);
+              } else if ((s_tmask[j] >> key) & 1u) {
+                x = (float)(_Float16)P.st.stage_v[(((int64_t)seat0 + off0 + key) * hk + kvh) * D + d];
+              } else {
+                const unsigned c = slot[d >> 2] >> (2 * (d & 3));
+                x = q_half<OSCAR_F16>(c & 2u ? hi : lo, c & 1u);
+              }
+              s_oddv[d] = fabsf(x) < INFINITY ? 0.f : x;
+            }
+            wait_lds();
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int b = 0; b < C::MBLK; ++b)
+            for (int b = 0; b < C::MBLK; ++b) {
 #pragma unroll
               for (int r = 0; r < 16; ++r) {
-                const unsigned x = v[pv_d<D>(b, out_tok(r, g))];
-                if (seen && (x & kInf) == kInf) O[b][r] = fmaf(p, QT == OSCAR_BF16 ? bf16_bits_to_f32(x) : f16_bits_to_f32(x), O[b][r]);
+                const float x = s_oddv[pv_d<D>(b, out_tok(r, g))];
+                if (seen && x != 0.f) O[b][r] = fmaf(p, x, O[b][r]);
               }
+              __builtin_amdgcn_sched_barrier(0);  // (not all of them in registers at a time)
+            }
+            __builtin_amdgcn_wave_barrier();  // the values are rewritten for the next token
           }
         }
       }

@@ -1404,7 +1404,7 @@ def attention_selected(q, k_new, v_new, k_cache, v_cache, table, plan: SelectPla
                        soft_cap=0.0, out_rot=None, lse=None):
     """Attention over the pages that select_pages chose, and the current chunk: (out_rot fp32,
     lse fp32), rotated, as attention_decode's, whose other arguments and rules these are, but
-    that a value of the chunk that is not finite reaches the queries that see it alone.  table
+    that a value that is not finite reaches no query that does not see its token.  table
     [requests, Hk, budget]: each KV head's pages, ascending."""
     index = _device_index(q, k_new, v_new, k_cache, v_cache, table, plan.qsl, out_rot, lse, *(stage or ()))
     if plan.has_new != (k_new is not None) or (k_new is None) != (v_new is None):

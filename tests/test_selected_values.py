@@ -86,6 +86,42 @@ def test_means_of_window_copies(cuda, hists, chunks, has_new, shape, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 1e6])
+def test_cached_values_that_are_not_finite(cuda, bad, shape, dtype):
+    """Cached queries: a later token's value reaches none of the earlier queries, whether its copy in the
+    FP32 window is not finite (or past fp16, 1e6) in a channel or its slot's constants are in all of them."""
+    hk, group, d = shape["hk"], shape["group"], shape["d"]
+    c, x, k_cache, v_cache, stage, table, bounds, plan = sparse_case(cuda, [1500, 40], [4, 5], dtype=dtype, budget=6, first=1, last=3, has_new=False, **shape)
+    call = lambda stage: attend(cuda, c, x, (k_cache, v_cache), stage, table, bounds, plan, d, False)[0]  # noqa: E731
+    clean, packed = call(stage), call(None)
+    for r, at, sees in ((0, 1498, [2, 3]), (0, 1499, [3]), (1, 38, [7, 8])):
+        page, off, head = int(table[r, at // 128]), at % 128, (at + r) % hk
+        heads = slice(head * group, (head + 1) * group)
+        seat = (page % stage[0].shape[0], off, head)
+        assert stage[2][seat[0], off] == page
+        hit = torch.zeros_like(clean, dtype=torch.bool)
+        hit[sees, heads, 7] = True
+        was = stage[1][seat].clone()
+        stage[1][seat][7] = bad
+        out = call(stage)
+        assert torch.equal(~out.isfinite(), hit) and (math.isnan(bad) or (out[hit] == math.copysign(math.inf, bad)).all())
+        assert (out - clean)[~hit].abs().max() <= 1e-3
+        stage[1][seat] = was
+        if abs(bad) == 1e6:
+            continue
+        hit[sees, heads] = True
+        constants = k_cache[page, off, head, 6:8].view(torch.float16)
+        was = constants.clone()
+        constants[0] = bad  # the values' zero
+        out = call(None)
+        assert torch.equal(~out.isfinite(), hit) and (math.isnan(bad) or (out[hit] == bad).all())
+        assert (out - packed)[~hit].abs().max() <= 1e-3
+        constants.copy_(was)
+
+
+@pytest.mark.gpu
 def test_captured_again(cuda):
     """Tiles of window copies and a chunk in a graph: every replay gives what the eager call does, to
     the last bits of tiles taken in another order."""
