@@ -306,7 +306,8 @@ typedef struct oscarop_bounds_args_v1 {
   const int32_t* seq_lens;        /* [num_reqs] device: and after */
   int32_t num_reqs;               /* at most 65535, as KV heads */
   int32_t reserved;
-  int64_t max_new;                /* the most new tokens of a request: sizes the launch */
+  int64_t max_new;                /* the most new tokens of a request: sizes the launch (0: none); pages
+                                     of a request that grew by more take turns */
   void* bounds;                   /* fp16 [num_blocks][Hk][2][D], 16-byte aligned */
 } oscarop_bounds_args_v1;
 

@@ -7,8 +7,9 @@
 // 64 bits, and so are their sums unless the terms lie 2^30 apart: pages are told apart by
 // their real order, whatever order the sums are taken in.
 //
-//   bounds_kernel   one workgroup per page: the codes of its tokens, each token's four values from a
-//                   table, packed minimum and maximum
+//   bounds_kernel   one workgroup per page (several in turn where a request grew by more than
+//                   max_new): the codes of its tokens, each token's four values from a table,
+//                   packed minimum and maximum
 //   select_kernel   eight lanes a page, the bounds in registers, the queries in LDS in 64 bits; the
 //                   last workgroup of a (request, KV head) finds the budget-th largest score by
 //                   radix selection and writes the chosen columns in their order
@@ -56,59 +57,61 @@ __global__ __launch_bounds__(kThreads) void bounds_kernel(oscarop_bounds_args_v1
   const int bs = (int)A.cache.block_size;
   const int64_t before = A.lengths[r], after = A.seq_lens[r];
   if (before < 0 || after <= before || (after - 1) / bs >= A.block_table_cols) return;
-  const int64_t col = before / bs + blockIdx.x;
-  if (col * bs >= after) return;
-  const int page = A.block_table[r * A.block_table_stride + col];
-  if (page < 0 || page >= A.cache.num_blocks) return;
-  const int held = after - col * bs < bs ? (int)(after - col * bs) : bs;
-  const uint8_t* base = A.cache.k + (int64_t)page * A.cache.k_stride[0] + (int64_t)h * A.cache.k_stride[2];
-  const int64_t ks1 = A.cache.k_stride[1];
-  const int c = tid % CH, group = tid / CH;
-  f16x2 low[8], high[8];
+  __shared__ unsigned s_part[GROUPS][CH][17];
+  // one page, unless a request grew by more than the launch was sized for
+  for (int64_t col = before / bs + blockIdx.x; col * bs < after; col += gridDim.x) {
+    const int page = A.block_table[r * A.block_table_stride + col];
+    if (page < 0 || page >= A.cache.num_blocks) continue;
+    const int held = after - col * bs < bs ? (int)(after - col * bs) : bs;
+    const uint8_t* base = A.cache.k + (int64_t)page * A.cache.k_stride[0] + (int64_t)h * A.cache.k_stride[2];
+    const int64_t ks1 = A.cache.k_stride[1];
+    const int c = tid % CH, group = tid / CH;
+    f16x2 low[8], high[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) low[k] = as_f16x2(0x7c007c00u), high[k] = as_f16x2(0xfc00fc00u);
-  constexpr int BATCH = 128 / GROUPS;  // slots of a thread in flight: a page of 128 tokens at once
-  for (int t0 = group; t0 < held; t0 += BATCH * GROUPS) {
-    unsigned consts[BATCH], w[BATCH];
+    for (int k = 0; k < 8; ++k) low[k] = as_f16x2(0x7c007c00u), high[k] = as_f16x2(0xfc00fc00u);
+    constexpr int BATCH = 128 / GROUPS;  // slots of a thread in flight: a page of 128 tokens at once
+    for (int t0 = group; t0 < held; t0 += BATCH * GROUPS) {
+      unsigned consts[BATCH], w[BATCH];
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      // (behind the page's tokens: the thread's first one again)
-      const uint8_t* slot = base + (t0 + u * GROUPS < held ? t0 + u * GROUPS : t0) * ks1;
-      consts[u] = *(const unsigned*)slot;
-      w[u] = *(const unsigned*)(slot + 32 + 4 * c);
-    }
+      for (int u = 0; u < BATCH; ++u) {
+        // (behind the page's tokens: the thread's first one again)
+        const uint8_t* slot = base + (t0 + u * GROUPS < held ? t0 + u * GROUPS : t0) * ks1;
+        consts[u] = *(const unsigned*)slot;
+        w[u] = *(const unsigned*)(slot + 32 + 4 * c);
+      }
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      unsigned lo, hi;
-      value_table<OSCAR_F16>(consts[u], lo, hi);
+      for (int u = 0; u < BATCH; ++u) {
+        unsigned lo, hi;
+        value_table<OSCAR_F16>(consts[u], lo, hi);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        // channels k and k + 8 of the chunk
-        const unsigned y = (w[u] >> (2 * k)) & 0x00030003u;
-        const f16x2 v = as_f16x2(__builtin_amdgcn_perm(hi, lo, y * 0x202u + 0x01000100u));
-        low[k] = pk_min(low[k], v);
-        high[k] = pk_max(high[k], v);
+        for (int k = 0; k < 8; ++k) {
+          // channels k and k + 8 of the chunk
+          const unsigned y = (w[u] >> (2 * k)) & 0x00030003u;
+          const f16x2 v = as_f16x2(__builtin_amdgcn_perm(hi, lo, y * 0x202u + 0x01000100u));
+          low[k] = pk_min(low[k], v);
+          high[k] = pk_max(high[k], v);
+        }
       }
     }
-  }
-  __shared__ unsigned s_part[GROUPS][CH][17];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    s_part[group][c][k] = as_u32(low[k]);
-    s_part[group][c][8 + k] = as_u32(high[k]);
-  }
-  __syncthreads();
-  uint16_t* out = (uint16_t*)A.bounds + (((int64_t)page * A.cache.num_kv_heads + h) * 2) * D;
-  if (tid < D) {
-    const int chunk = tid / 16, k = tid % 16;
-    f16x2 v = as_f16x2(s_part[0][chunk][k]);
-    for (int g = 1; g < GROUPS; ++g) {
-      const f16x2 o = as_f16x2(s_part[g][chunk][k]);
-      v = k < 8 ? pk_min(v, o) : pk_max(v, o);
+    for (int k = 0; k < 8; ++k) {
+      s_part[group][c][k] = as_u32(low[k]);
+      s_part[group][c][8 + k] = as_u32(high[k]);
     }
-    uint16_t* row = out + (k < 8 ? 0 : D) + 16 * chunk + (k & 7);
-    row[0] = (uint16_t)as_u32(v);
-    row[8] = (uint16_t)(as_u32(v) >> 16);
+    __syncthreads();
+    uint16_t* out = (uint16_t*)A.bounds + (((int64_t)page * A.cache.num_kv_heads + h) * 2) * D;
+    if (tid < D) {
+      const int chunk = tid / 16, k = tid % 16;
+      f16x2 v = as_f16x2(s_part[0][chunk][k]);
+      for (int g = 1; g < GROUPS; ++g) {
+        const f16x2 o = as_f16x2(s_part[g][chunk][k]);
+        v = k < 8 ? pk_min(v, o) : pk_max(v, o);
+      }
+      uint16_t* row = out + (k < 8 ? 0 : D) + 16 * chunk + (k & 7);
+      row[0] = (uint16_t)as_u32(v);
+      row[8] = (uint16_t)(as_u32(v) >> 16);
+    }
+    __syncthreads();  // s_part is rewritten for the next page
   }
 }
 

@@ -1284,8 +1284,9 @@ def page_bounds(k_cache, bounds, block_table, lengths, seq_lens, *, max_new: int
     bounds [blocks, Hk, 2, D] fp16: the least and the largest key that a page holds, for each
     KV head and channel, of the keys as their slots hold them.  Request r had lengths[r] tokens
     in the cache and has seq_lens[r] now (int32 on the device): its pages from the one of token
-    lengths[r] on are looked at again, those of a request that did not grow are not.  max_new:
-    the most new tokens of a request.  Call it after the step's store; after an eviction with
+    lengths[r] on are looked at again, those of a request that did not grow are not.  max_new: the
+    most new tokens of a request, which sizes the launch (a request that grew by more is served as
+    well, its pages in turn).  Call it after the step's store; after an eviction with
     lengths 0 (kept tokens have moved)."""
     index = _device_index(k_cache, bounds, block_table, lengths, seq_lens)
     cache = _cache_values(k_cache, k_cache, head_dim)
@@ -1299,7 +1300,7 @@ def page_bounds(k_cache, bounds, block_table, lengths, seq_lens, *, max_new: int
     if table.ndim != 2 or table.shape[0] < reqs:
         raise ValueError("Missing request block-table rows")
     a = _BOUNDS(*cache, table.data_ptr(), table.stride(0), *table.shape, lengths.data_ptr(), seq_lens.data_ptr(), reqs, 0,
-                max_new, bounds.data_ptr())
+                max(max_new, 1), bounds.data_ptr())
     _launch("oscarop_page_bounds_v1", index, a)
     return bounds
 
