@@ -29,7 +29,8 @@
 // Values: K is the reference's bf16 or fp16 of fp16(code * scale + zero), V fp16(...)
 // unrounded, the window's FP32 copies likewise; P fp16, up to 2^15, the reference m 2^7 below the
 // largest score at its last move, so that keys of 2^-21 of the largest still keep 11 bits.  The chunk's
-// V in bf16 have a wider range than fp16: chunk tiles multiply it by P in two bf16 parts.  A
+// V in bf16 have a wider range than fp16: chunk tiles multiply it by P in two bf16 parts, P at most 2^-16
+// so that no sum of finite values overflows.  A
 // value of the chunk that is not finite goes into LDS as zero and is added afterwards, to the
 // rows alone that see its node.
 //
@@ -67,6 +68,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kBelow = 7.f;    // the reference below the maximum where it moves to,
 constexpr float kMost = 15.f;    // and how far above it a score may come (log2 units)
+// The same for tiles of a bf16 chunk, whose values reach 2^128: probabilities of at most 2^-16 keep the sums
+// of an item's 2^15 keys below it (as two bf16 parts they lose nothing), and the merge's weights of at most
+// 2^-12 the sums of its items.
+constexpr float kChunk = -16.f;
+constexpr float kWeight = 1.f / 4096.f;
 typedef short __attribute__((ext_vector_type(4))) i16x4;
 
 template <int D>
@@ -321,8 +327,9 @@ __device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uin
         if (seen && (x & kInf) == kInf) O[b][r] = fmaf(p, QT == OSCAR_BF16 ? bf16_bits_to_f32(x) : f16_bits_to_f32(x), O[b][r]);
       }
   };
-  // p = exp2(score - reference); the reference moves, and O with it, where a score comes 2^15 above it
-  auto softmax = [&]() {
+  // p = exp2(score - reference); the reference moves, and O with it, where a score comes 2^most above it, to
+  // 2^below under that
+  auto softmax = [&](float below, float most) {
     float mx = -INFINITY;
 #pragma unroll
     for (int a = 0; a < C::KSUB; ++a)
@@ -330,9 +337,9 @@ __device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uin
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[a][r]);
     if (!kScaled) mx *= c_score;
     mx = fmaxf(mx, swap_halves(mx));
-    const bool up = mx > m_run + kMost;
+    const bool up = mx > m_run + most;
     if (__builtin_expect_with_probability(__any(up) != 0, 0, 0.999)) {
-      const float to = up ? mx - kBelow : m_run;
+      const float to = up ? mx - below : m_run;
       const float f = !up ? 1.f : (m_run == -INFINITY ? 0.f : exp2f(m_run - to));
       l_run *= f;
       m_run = to;
@@ -478,7 +485,7 @@ __device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uin
         if (K == 1) next();
         qk(j & 1);
         __builtin_amdgcn_sched_barrier(0);
-        softmax();
+        softmax(kBelow, kMost);
         half();
         __builtin_amdgcn_sched_barrier(0);
         pv(j & 1);
@@ -499,7 +506,8 @@ __device__ __forceinline__ void run_item(const TreeParams& P, const Item& I, uin
       __syncthreads();
       qk(0);
       mask(t);
-      softmax();
+      const bool chunk = QT == OSCAR_BF16 && t >= htiles;
+      softmax(chunk ? kChunk : kBelow, chunk ? kChunk : kMost);
     };
     int j = 0;
     if (I.first < htiles) {  // the ragged end
@@ -626,7 +634,7 @@ __global__ __launch_bounds__(kMergeThreads) void tree_merge_kernel(TreeParams P)
     L *= f;
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const float w = l[u] == -INFINITY ? 0.f : exp2f(l[u] - top);
+      const float w = l[u] == -INFINITY ? 0.f : exp2f(l[u] - top) * kWeight;
       L += w;
       acc += w > 0.f ? x[u] * w : f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -640,7 +648,7 @@ __global__ __launch_bounds__(kMergeThreads) void tree_merge_kernel(TreeParams P)
   float* out = A.out_rot + (token * A.num_q_heads + head) * D + e;
   *(float2*)out = make_float2(acc[0], acc[2]);
   *(float2*)(out + 4) = make_float2(acc[1], acc[3]);
-  if (col == 0) A.lse[token * A.num_q_heads + head] = nan ? NAN : (some ? (M + log2f(L)) * kLn2 : -INFINITY);
+  if (col == 0) A.lse[token * A.num_q_heads + head] = nan ? NAN : (some ? (M + log2f(L / kWeight)) * kLn2 : -INFINITY);
 }
 
 template <int D>
