@@ -3,9 +3,11 @@
 // A query's product with any key of a page is at most
 //   sum_d max(q_d low_d, q_d high_d) = sum_d (q_d m_d + |q_d| w_d),
 // low and high being the least and the largest key of the page in channel d, m = (low + high) / 2
-// and w = (high - low) / 2.  The products of 8 or 11 bits of a query with 12 of m or w are exact in
-// 64 bits, and so are their sums unless the terms lie 2^30 apart: pages are told apart by
-// their real order, whatever order the sums are taken in.
+// and w = (high - low) / 2, of the keys as their slots hold them, fp16.  m and w have up to 41 bits, a query
+// 8 or 11: their products are exact in 64 bits.  A sum's order is the same for every page and form of the
+// kernel, so that equal bounds give equal scores; it is off by 13 (D 128) or 21 (D 256) additions'
+// rounding at most, 21 2^-53 sum_d (|q_d m_d| + |q_d| w_d), and exact where the terms' bits all
+// fit in 53 (values of one range mostly).
 //
 //   bounds_kernel   one workgroup per page (several in turn where a request grew by more than
 //                   max_new): the codes of its tokens, each token's four values from a table,

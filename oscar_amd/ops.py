@@ -1364,9 +1364,12 @@ def select_pages(q, bounds, block_table, plan: SelectPlan) -> tuple:
 
     q [N, Hq, D] bf16 or fp16, rotated as the cache; bounds: page_bounds(...).  A page's
     score is the largest, over the request's queries and the KV head's query heads, of
-    sum_d max(q_d low_d, q_d high_d), which no key of the page exceeds; summed in 64 bits.  Equal
-    scores: the earlier page; one with a bound or a query that is not finite counts as the
-    largest.  A history of at most budget pages is chosen whole."""
+    sum_d max(q_d low_d, q_d high_d), summed in 64 bits in a fixed order (2^-48 of its terms' sizes at
+    most off).  Equal scores: the earlier page; one with a bound or a query that is not finite counts as the
+    largest.  It is no less than the product with any of the page's keys as its slots hold them, fp16(x);
+    what attention reads can be larger: bf16(fp16(x)) with bf16 queries (2^-9 of a key), and copies in the
+    FP32 window, which are not clipped and stay behind the last pages until their seats are
+    written again.  A history of at most budget pages is chosen whole."""
     index = _device_index(q, bounds, block_table, plan.qsl)
     code = _DTYPES.get(q.dtype)
     if code is None or code == OSCAR_F32:
