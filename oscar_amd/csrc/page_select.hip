@@ -534,7 +534,7 @@ extern "C" int oscarop_select_v1(const oscarop_select_args_v1* args, void* strea
   dim3 grid(1, (unsigned)a.num_kv_heads, (unsigned)a.num_reqs);
   bool by_rows = true;
   if (need > 0) {
-    if (!a.q || !a.bounds || a.num_blocks < 1) return fail(-22, "oscarop_select_v1: missing pointer");
+    if ((a.num_tokens > 0 && !a.q) || !a.bounds || a.num_blocks < 1) return fail(-22, "oscarop_select_v1: missing pointer");
     if ((a.q_stride_token & 7) || ((uintptr_t)a.q & 15) || ((uintptr_t)a.bounds & 15))
       return fail(-22, "oscarop_select_v1: q rows and bounds must be 16-byte aligned");
     if (a.workspace_bytes < need || !a.workspace || ((uintptr_t)a.workspace & 15))

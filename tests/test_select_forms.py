@@ -92,6 +92,20 @@ def test_scales_that_change_along_a_history(cuda, steps, shape, dtype):
     assert lse.isfinite().all()
 
 
+@pytest.mark.gpu
+def test_a_step_without_queries(cuda):
+    """A list of requests none of which has a row: every page scores alike, the earlier ones are chosen, and
+    there is nothing to attend to."""
+    g = torch.Generator().manual_seed(3)
+    table = torch.randperm(80, generator=g).to(torch.int32).view(2, 40)
+    q = torch.zeros(0, 6, 256, dtype=torch.bfloat16)
+    plan, chosen, _ = choose(cuda, q, random_bounds(g, 80, 1, 256), table, [0, 0, 0], [5000, 300], hk=1, d=256, budget=6)
+    k_cache = torch.zeros(80, 128, 1, 256, dtype=torch.int8, device=cuda)
+    none = torch.zeros(0, 1, 256, dtype=torch.bfloat16, device=cuda)
+    out, lse = ops.attention_selected(q.to(cuda), none, none, k_cache, k_cache, chosen, plan, 0.1, head_dim=256)
+    assert out.shape == (0, 6, 256) and lse.shape == (0, 6)
+
+
 def test_slopes_are_refused_by_name():
     """Arguments that pass every other check."""
     lib, a = _lib.load(), attn_args().attn
