@@ -261,8 +261,8 @@ int oscarop_tree_mask_v1(const oscarop_tree_args_v1* args, void* stream);
  * mask's words are not seen).  A row that sees no key gets zeros and lse -inf.  No
  * alibi_slopes (a node's distance is its depth, not its row); scale > 0.  History keys are
  * q_dtype(fp16(x)), history values fp16(x), the chunk's as they are; probabilities are rounded to
- * fp16 for the history, to two bf16 parts for a bf16 chunk; sums and the softmax are fp32.  The
- * same plan gives the same bits. */
+ * fp16 for the history and an fp16 chunk, to two bf16 parts for a bf16 one; sums and the softmax are fp32,
+ * and no sum of finite values overflows (chunks of up to 2^17 rows).  The same plan gives the same bits. */
 #define OSCAROP_TREE_ITEM_INTS 12
 
 typedef struct oscarop_tree_sizes_v1 {
@@ -368,7 +368,8 @@ int oscarop_select_v1(const oscarop_select_args_v1* args, void* stream);
  * lengths and the plan are those of the chosen tokens.  History keys are q_dtype(fp16(x)), history
  * values fp16(x) (full tiles of codes: x itself), the chunk's as they are; probabilities are rounded to
  * fp16 times a value's scale in full tiles of codes, to two parts in q_dtype elsewhere; sums and the softmax
- * are fp32.  A value that is not finite reaches no query that does not see its token.  No alibi_slopes (the chosen pages' distances are
+ * are fp32 and hold probabilities of up to 2^8, as the decode's: with n keys, values of the chunk beyond
+ * 1e36 / n can overflow them.  A value that is not finite reaches no query that does not see its token.  No alibi_slopes (the chosen pages' distances are
  * not the table's); scale > 0. */
 int oscarop_attn_selected_v1(const oscar_attn_args_v1* args, const oscarop_score_v1* score, int64_t table_stride_head,
                              void* stream);

@@ -158,7 +158,7 @@ struct TileRegs {
 // scored variants walk an item's tiles from its last to its first: the reference maximum
 // of a row settles on the near tiles instead of moving (and O with it) tile by tile.
 // OWN: each KV head reads a block table of its own, the pages chosen for it (oscarop_attn_selected_v1).
-// 8 requests of 48 pages and 24 rows 16.0 us, 16 of 64 pages and 6 rows 23.7: the plain decode of as many
+// 8 requests of 48 pages and 24 rows 17.0 us, 16 of 64 pages and 6 rows 23.7: the plain decode of as many
 // tokens, about 8 us of prologue, drain and merge with it, and 0.3 to 0.7 for values that are not finite.
 // Its slow tiles hold history values as fp16(x) for bf16 queries as well (the plain ones as the reference
 // rounds them, bf16(fp16(x))): 0 to 0.8 us of 36 to 49; one request of 5 pages 2.0e-3 -> 1.7e-3 off,

@@ -35,7 +35,7 @@
 // rows alone that see its node.
 //
 // What bounds it: 8 requests of 24576 tokens with 32 nodes (192 rows, D 256) take 61 to 63 us, 0.62
-// PFLOP/s in 39 GFLOP: 24 tiles a workgroup at 2.0 us and 12 us before and after them, of which
+// PFLOP/s in 39 GFLOP: 25 tiles a workgroup at 2.0 us and 12 us before and after them, of which
 // 50 MB of partials; their merge takes another 10 us.  A tile's products alone take 1.0 us at the 2.0 to
 // 2.1 GHz that the matrix units leave the clock, its softmax and unpacking (about 255 vector
 // instructions a wave) as long again, and the two overlap in part (252 rows: the matrix unit busy for 36%
